@@ -348,6 +348,110 @@ int ojx_e8r_gemv_grouped(const ojx_e8t_gemv_job* jobs, const ojx_e8t_gemv_job* j
                          int njobs, const void* x, void* y, int64_t M, int64_t gs, int dtype,
                          void* stream);
 
+/* ---- 8-bit paged key / value cache, its attention, token log probabilities ----
+ *
+ * What a decoder of packed linears keeps and answers with.  A cache of `num_blocks` blocks of
+ * `block_size` tokens (16, 32, 64, 128 or 256) for `kv_heads` heads of `head_dim` (1..256)
+ * elements, stored as Dp = head_dim rounded up to a multiple of 64:
+ *   k_codes, v_codes  int8 [num_blocks][kv_heads][block_size * Dp], 16-byte aligned.  Within
+ *       one block and head the tokens lie in groups of 16 (16 * Dp bytes each); key d of token
+ *       t (0..15) of a group is byte
+ *           (d / 64) * 1024 + (t / 4) * 256 + (d % 64 / 16) * 64 + (t % 4) * 16 + d % 16,
+ *       value d of token t is byte d * 16 + t: the operand order of the matrix instructions
+ *       that read them.
+ *   scales            float [num_blocks][kv_heads][2], the keys' and the values': an element
+ *       is code * scale, code in -127..127.  Scales are finite and not negative.
+ * Block tables map block i of request r's tokens to a block of the cache; an entry outside
+ * [0, num_blocks) is no block: its tokens are neither written nor seen. */
+
+/* The next step of `requests` requests: request r holds seq_lens[r] tokens and gets
+ * new_lens[r] more (negative counts as 0).  Blocks that the new tokens begin are taken from the
+ * top of the stack free_blocks[0 .. *num_free), in request order, and written to block_tables
+ * [requests][table_ld], of which table_width columns may be used (a request longer than that
+ * gets no further block).  Results:
+ *   slots [tokens]        block * block_size + offset of each new token, -1 without a block
+ *   positions [tokens]    its place in the request;  request_ids [tokens]  its request
+ *   query_starts [requests + 1]   first token of each request;  seq_lens_out [requests]
+ *   num_free_out [1]      what is left on the stack; negative: so many blocks were missing, and
+ *                         the entries of the last ones are -1
+ * Tokens past the new lengths' sum are padding: slot, position and request -1.  The stack itself
+ * and num_free are not written, so a call may be repeated.  No output overlaps an input. */
+int ojx_kv8_plan(const int32_t* seq_lens, const int32_t* new_lens, int64_t requests,
+                 int32_t* block_tables, int64_t table_ld, int64_t table_width,
+                 const int32_t* free_blocks, int64_t free_capacity, const int32_t* num_free,
+                 int64_t block_size, int64_t tokens, int64_t* slots, int32_t* positions,
+                 int32_t* request_ids, int32_t* query_starts, int32_t* seq_lens_out,
+                 int32_t* num_free_out, void* stream);
+
+/* Writes keys and values of `tokens` new tokens into the cache.  k, v: [tokens][kv_heads]
+ * [head_dim] in dtype, with strides (elements) between tokens and between heads.  Tokens of one
+ * block are neighbours in `slots` and at rising offsets without a gap, each block in one run of
+ * the call; slots outside the cache are skipped.  A block's scale is the largest |element| of the
+ * run over 127; where the run begins inside the block, its earlier tokens keep their place: the
+ * scale is then not less than the old one and, where it grew, the earlier codes are rounded
+ * again.  Infinite elements become +-127 times the scale, NaN 0; neither takes part in the
+ * scale, nor does a run whose largest element is under 2^-100 (it is written as zeros). */
+int ojx_kv8_append(int8_t* k_codes, int8_t* v_codes, float* scales, int64_t num_blocks,
+                   int64_t kv_heads, int64_t block_size, int64_t head_dim, const void* k,
+                   int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                   int64_t v_token_stride, int64_t v_head_stride, int dtype,
+                   const int64_t* slots, int64_t tokens, void* stream);
+
+/* The values of whole blocks: k_out, v_out [n][block_size][kv_heads][head_dim] in dtype, 16-byte
+ * aligned, and their scales, scales_out [n][kv_heads][2]; an index outside the cache gives
+ * zeros. */
+int ojx_kv8_read(const int8_t* k_codes, const int8_t* v_codes, const float* scales,
+                 int64_t num_blocks, int64_t kv_heads, int64_t block_size, int64_t head_dim,
+                 const int32_t* blocks, int64_t n, int dtype, void* k_out, void* v_out,
+                 float* scales_out, void* stream);
+
+/* Causal attention of the newest tokens over the cache: token i of request r's n newest (its
+ * rows query_starts[r] .. query_starts[r + 1] of q) sits at seq_lens[r] - n + i and sees the keys
+ * up to itself, with window > 0 only the window nearest of them.  query_starts NULL: one token a
+ * request.  q, out: [tokens][heads][head_dim] in dtype (strides of q in elements, out
+ * contiguous), heads a multiple of kv_heads, consecutive heads sharing one.  lse (may be NULL):
+ * float [tokens][heads], the natural logarithm of the softmax's sum.  A row that sees nothing
+ * gets zeros and -inf; a row of q with NaN or infinities gets NaN.  max_query_len and
+ * max_seq_len: no request has more (they size the launch; tokens beyond them are not computed).
+ * The workspace holds partial results of a split over the keys; a smaller one (or none) only
+ * lowers the split. */
+int ojx_kv8_attention_workspace_bytes(int64_t tokens, int64_t requests, int64_t heads,
+                                      int64_t kv_heads, int64_t head_dim, int64_t window,
+                                      int64_t max_query_len, int64_t max_seq_len, int dtype,
+                                      size_t* bytes);
+int ojx_kv8_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                      int64_t tokens, int64_t heads, int dtype, const int8_t* k_codes,
+                      const int8_t* v_codes, const float* scales, int64_t num_blocks,
+                      int64_t kv_heads, int64_t block_size, int64_t head_dim,
+                      const int32_t* block_tables, int64_t table_ld, int64_t table_width,
+                      const int32_t* seq_lens, const int32_t* query_starts, int64_t requests,
+                      int64_t max_query_len, int64_t max_seq_len, float softmax_scale,
+                      int64_t window, void* out, float* lse, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* Log probabilities from logits [rows][vocab] (row stride ld elements): logprob [rows] of the
+ * token ids[row] (0 where it is outside [0, vocab)), entropy [rows], lse [rows], stats [rows][2]
+ * = (largest logit, log of the sum of exp(logit - largest)), whose sum lse is before rounding, and
+ * the top_k (0..64, at most vocab) largest in falling order, equal ones by rising token:
+ * top_logprobs, top_ids [rows][top_k].  Everything in fp32.  A row of -inf only has lse -inf, entropy 0 and log
+ * probabilities -inf; NaN or +inf in a row makes its results NaN (NaN counts as the largest). */
+int ojx_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int64_t top_k, int dtype,
+                                       size_t* bytes);
+int ojx_token_logprobs(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int dtype,
+                       const int64_t* ids, int64_t top_k, float* logprob, float* entropy,
+                       float* lse, float* stats, float* top_logprobs, int64_t* top_ids,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* grad_logits [rows][vocab] (contiguous, in dtype): for p = exp(logits - lse), from stats,
+ *   grad = grad_logprob (1[id] - p) - grad_entropy p (log p + entropy) + grad_lse p
+ *          + sum_i grad_top[i] (1[top_ids[i]] - p),
+ * each gradient pointer NULL for none. */
+int ojx_token_logprobs_bwd(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int dtype,
+                           const int64_t* ids, const float* entropy, const float* stats,
+                           int64_t top_k, const int64_t* top_ids, const float* grad_logprob,
+                           const float* grad_entropy, const float* grad_lse,
+                           const float* grad_top, void* grad_logits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

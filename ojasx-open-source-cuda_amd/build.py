@@ -31,7 +31,11 @@ SOURCES = [
     "e8t_qat.hip",
     "e8t_noalloc.hip",
     "e8t_lora.hip",
+    "kv8_cache.hip",
+    "kv8_attention.hip",
+    "token_logprobs.hip",
     "e8t_capi.cpp",
+    "serve_capi.cpp",
 ]
 
 HIPCC = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"

@@ -17,6 +17,7 @@
 #include "../../include/ojasx_e8t.h"
 #include "e8t_device.h"
 #include "e8t_internal.h"
+#include "serve.h"
 
 namespace {
 
@@ -75,8 +76,18 @@ int done(hipError_t e, const char* what) {
 
 }  // namespace
 
+// What the other entry points share of the above.
 namespace ojx {
 int api_fail(int code, const char* msg) { return fail(code, "%s", msg); }
+int api_failf(int code, const char* fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
+    va_end(ap);
+    return code;
+}
+int api_check_device() { return check_device(); }
+int api_done(hipError_t e, const char* what) { return done(e, what); }
 }  // namespace ojx
 
 // The prefill MFMA GEMM with its tile configuration and K split.  The split's fp32 partial

@@ -7,7 +7,7 @@ operation runs in hand-written HIP kernels for gfx950 (libojasx_e8t.so, C ABI in
 include/ojasx_e8t.h) registered as ``torch.ops.ojasx_e8t.*``.
 """
 
-from . import grouped, hardware, ops, optim_state
+from . import grouped, hardware, kv8, ops, optim_state, serve_ops
 from .lattice import (
     E8LatticeLinear,
     E8QuantizationAwareLinear,
@@ -25,6 +25,8 @@ from .lattice import (
     fwht_block32,
     pack_model_e8,
 )
+from .kv8 import KV8Cache
+from .logprobs import TokenLogprobs, token_logprobs
 from .streaming import StreamingE8LoadReport, load_hf_checkpoint_e8, pack_weight_rowwise
 
 __version__ = "0.1.0"
@@ -32,8 +34,13 @@ __version__ = "0.1.0"
 __all__ = [
     "grouped",
     "hardware",
+    "kv8",
     "ops",
     "optim_state",
+    "serve_ops",
+    "KV8Cache",
+    "TokenLogprobs",
+    "token_logprobs",
     "E8LatticeLinear",
     "E8QuantizationAwareLinear",
     "_E8STEFunction",

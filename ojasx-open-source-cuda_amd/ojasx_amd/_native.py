@@ -54,6 +54,14 @@ EXPORTS = (
     "ojx_e8_ste_quantize",
     "ojx_e8_cs_project_dt",
     "ojx_e8_ste_quantize_dt",
+    "ojx_kv8_plan",
+    "ojx_kv8_append",
+    "ojx_kv8_read",
+    "ojx_kv8_attention_workspace_bytes",
+    "ojx_kv8_attention",
+    "ojx_token_logprobs_workspace_bytes",
+    "ojx_token_logprobs",
+    "ojx_token_logprobs_bwd",
 )
 
 
@@ -176,6 +184,24 @@ def lib() -> ctypes.CDLL:
             L.ojx_e8_cs_project_dt.argtypes = [_P, _INT, _I64, _P, _P]
             L.ojx_e8_ste_quantize_dt.restype = _INT
             L.ojx_e8_ste_quantize_dt.argtypes = [_P, _INT, _I64, _P, _P]
+            for name, args in (
+                    ("ojx_kv8_plan", [_P, _P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _I64]
+                     + [_P] * 7),
+                    ("ojx_kv8_append", [_P, _P, _P] + [_I64] * 4
+                     + [_P, _I64, _I64, _P, _I64, _I64, _INT, _P, _I64, _P]),
+                    ("ojx_kv8_read", [_P, _P, _P] + [_I64] * 4 + [_P, _I64, _INT, _P, _P, _P, _P]),
+                    ("ojx_kv8_attention_workspace_bytes", [_I64] * 8 + [_INT, _P]),
+                    ("ojx_kv8_attention", [_P, _I64, _I64, _I64, _I64, _INT, _P, _P, _P]
+                     + [_I64] * 4 + [_P, _I64, _I64, _P, _P, _I64, _I64, _I64, _F32, _I64, _P, _P,
+                                     _P, _SZ, _P]),
+                    ("ojx_token_logprobs_workspace_bytes", [_I64, _I64, _I64, _INT, _P]),
+                    ("ojx_token_logprobs", [_P, _I64, _I64, _I64, _INT, _P, _I64, _P, _P, _P, _P,
+                                            _P, _P, _P, _SZ, _P]),
+                    ("ojx_token_logprobs_bwd", [_P, _I64, _I64, _I64, _INT, _P, _P, _P, _I64]
+                     + [_P] * 7)):
+                fn = getattr(L, name)
+                fn.restype = _INT
+                fn.argtypes = args
             _lib = L
     return _lib
 
