@@ -50,9 +50,11 @@ COMMON = ["-x", "hip", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
 
 # Per-file code generation options.  The decode GEMV keeps its MFMA results in ordinary
 # VGPRs: its post-scaled kernel reads every result with VALU FMAs, and the accumulator
-# register form would add a v_accvgpr_read per read and raise the register total.
+# register form would add a v_accvgpr_read per read and raise the register total.  So does the
+# cache's attention, whose integer products are all read by VALU conversions.
 EXTRA = {
     "e8t_gemv.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "kv8_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

@@ -133,18 +133,727 @@ __global__ __launch_bounds__(64) void row_kernel(AttnArgs a) {
             some ? (bad ? nan : (m + log2f(l)) * kLn2) : -INFINITY;
 }
 
+
+// ---------------------------------------------------------------- tiles of rows on int8 products
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr float kFixed = 32512.f;  // largest fixed-point value: 127 * 256 with its low part 0
+constexpr float kMagic = 12582912.f + 128.f;  // 1.5 * 2^23: the sum's low bits are the integer
+constexpr float kLeastScale = 0x1p-100f;
+constexpr int kMaxSplits = 64;
+
+// How a launch cuts its work.  An item is a tile of rows of one request (tok tokens of it, or
+// part of one token's heads where a key head has more than a tile's rows) and one key head; with
+// splits > 1 its keys are shared out and the partial results joined by a second launch.
+struct Cut {
+    int rows;    // rows of a tile
+    int tok;     // tokens of a tile
+    int subs;    // tiles of one token's heads of a key head
+    int tiles;   // tiles (upper bound), without subs and key heads
+    int splits;
+    int least;   // fewest 64-key tiles of a split
+    int small;   // requests of at most so many tokens belong to the launch that splits keys
+    float* part;   // [splits][items][rows][dp]
+    float2* ml;    // [splits][items][rows]
+};
+
+struct Item {
+    int head, sub, tile, split;
+    int r, tok0, ntok;   // request, the tile's tokens in it
+    int q0;              // first row of q of the request
+    int group;           // query heads of a key head
+    int rows;            // rows in use
+    int len;             // the request's tokens, newest included
+    int before;          // the tile's first token's place
+};
+
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Largest over the four lanes of a column (lanes n, n + 16, n + 32, n + 48).
+__device__ __forceinline__ float col_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float col_sum(float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+// The item of workgroup `id` (without its split); false: none.
+template <bool ROWS>
+__device__ __forceinline__ bool find_item(const AttnArgs& a, const Cut& c, int id, Item& it) {
+    it.head = id % a.shape.kv_heads;
+    id /= a.shape.kv_heads;
+    it.sub = id % c.subs;
+    it.tile = id / c.subs;
+    it.group = a.shape.heads / a.shape.kv_heads;
+    int q0, q1;
+    if constexpr (!ROWS) {
+        it.r = it.tile;
+        q0 = a.query_starts ? a.query_starts[it.r] : it.r;
+        q1 = a.query_starts ? a.query_starts[it.r + 1] : it.r + 1;
+        it.tok0 = 0;
+        if (q1 - q0 > c.small) return false;
+    } else {
+        // request r's tiles begin at query_starts[r] / tok + r: room for each one's last, partly
+        // filled tile without a sum over the requests; 64 requests are looked at at a time
+        int lo = 0, n = a.shape.requests;
+        const int lane = threadIdx.x & 63;
+        while (n > 0) {
+            const int step = (n + 63) >> 6;
+            const int i = lo + lane * step;
+            const bool at = lane * step < n && a.query_starts[i] / c.tok + i <= it.tile;
+            const int last = 63 - __builtin_clzll(__ballot(at) | 1);
+            lo += last * step;
+            n = step == 1 ? 0 : min(step, n - last * step);
+        }
+        it.r = lo;
+        q0 = a.query_starts[lo];
+        q1 = a.query_starts[lo + 1];
+        it.tok0 = (it.tile - (q0 / c.tok + lo)) * c.tok;
+        if (q1 - q0 <= c.small || it.tok0 < 0) return false;
+    }
+    const int newest = q1 - q0;
+    it.ntok = min(min(newest, a.shape.max_query) - it.tok0, c.tok);
+    if (it.ntok <= 0) return false;
+    // no rows outside q, whatever query_starts says
+    if (q0 < 0 || q0 + it.tok0 + it.ntok > a.shape.tokens) return false;
+    it.q0 = q0;
+    it.rows = c.subs > 1 ? min(it.group - it.sub * c.rows, c.rows) : it.ntok * it.group;
+    it.len = max(0, min(a.seq_lens[it.r], a.shape.max_seq));
+    it.before = a.seq_lens[it.r] - newest + it.tok0;
+    return true;
+}
+
+// Token (within the tile) and query head of a row of an item.
+__device__ __forceinline__ void row_at(const AttnArgs& a, const Cut& c, const Item& it, int row,
+                                       int& tok, int& head) {
+    tok = c.subs > 1 ? 0 : row / it.group;
+    head = it.head * it.group + (c.subs > 1 ? it.sub * c.rows + row : row - tok * it.group);
+}
+
+template <int DT> __device__ __forceinline__ void load8(const void* p, int64_t e, float (&x)[8]) {
+    if constexpr (DT == kF32) {
+        const float4* w = reinterpret_cast<const float4*>(static_cast<const float*>(p) + e);
+        const float4 lo = w[0], hi = w[1];
+        x[0] = lo.x; x[1] = lo.y; x[2] = lo.z; x[3] = lo.w;
+        x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
+    } else {
+        const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + e);
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = DT == kBF16 ? bf16_bits_to_f32(u[i] & 0xFFFFu) : f16_bits_to_f32(u[i] & 0xFFFFu);
+            x[2 * i + 1] = DT == kBF16 ? bf16_bits_to_f32(u[i] >> 16) : f16_bits_to_f32(u[i] >> 16);
+        }
+    }
+}
+
+// The high and low bytes of four fixed-point values, each the low 16 bits of a float kMagic was
+// added to: value = 256 * high + low, both signed bytes.
+__device__ __forceinline__ void limbs(const float (&t)[4], int& high, int& low) {
+    const uint32_t t0 = __float_as_uint(t[0]), t1 = __float_as_uint(t[1]);
+    const uint32_t t2 = __float_as_uint(t[2]), t3 = __float_as_uint(t[3]);
+    const uint32_t a = __builtin_amdgcn_perm(t1, t0, 0x05010400u);  // t0.b0 t1.b0 t0.b1 t1.b1
+    const uint32_t b = __builtin_amdgcn_perm(t3, t2, 0x05010400u);
+    low = (int)(__builtin_amdgcn_perm(b, a, 0x05040100u) ^ 0x80808080u);
+    high = (int)__builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+
+__device__ __forceinline__ v4i times256(v4i x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = (int)((uint32_t)x[i] << 8);
+    return x;
+}
+
+__device__ __forceinline__ v4i product(v4i a, v4i b, v4i c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+}
+
+template <int DT>
+__device__ __forceinline__ void store_row4(void* out, int64_t e, int n, bool vec, const float (&v)[4]) {
+    if (vec && n >= 4) {
+        if constexpr (DT == kF32) {
+            *reinterpret_cast<float4*>(static_cast<float*>(out) + e) =
+                make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+            uint32_t b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                b[i] = DT == kBF16 ? f32_to_bf16_bits(v[i]) : f32_to_f16_bits(v[i]);
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + e) =
+                make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < n) store_from_f32<DT>(out, e + i, v[i]);
+}
+
+__device__ __forceinline__ bool out_vector(const AttnArgs& a) {
+    return a.shape.d % 4 == 0 && ((uintptr_t)a.out & 15) == 0;
+}
+
+// Rows of one item over a range of its keys, on the matrix unit in whole numbers: a score is
+// 256 (qh.k) + (ql.k) with the row's q in 16-bit fixed point against its own largest element,
+// 64 keys at a time; the weights of 64 keys are 16-bit fixed point against their largest
+// weight * (value scale), so codes of keys and values enter as they lie in memory.  Tile t of
+// the four score products takes 4 keys of each group of 16: a lane then holds the 16 scores of
+// one group, whose weights are the second operand of the value products as they come.
+//
+// ROWS false: the workgroup's waves share the keys of one tile of 16 NQ rows and join their
+// results in LDS.  ROWS true: each wave has 16 NQ rows of its own.
+template <int DT, int DC, int NQ, bool ROWS>
+__global__ __launch_bounds__(kThreads) void tile_kernel(AttnArgs a, Cut c) {
+    constexpr int DP = 64 * DC, DM = DP / 16;
+    constexpr int LD = DP + 4;
+    __shared__ float joined[ROWS ? 1 : kWaves * 16 * NQ * LD];
+    __shared__ float wave_m[kWaves][16 * NQ], wave_l[kWaves][16 * NQ];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
+    const int items = c.tiles * c.subs * a.shape.kv_heads;
+    Item it;
+    it.split = blockIdx.x / items;
+    const int id = blockIdx.x - it.split * items;
+    if (!find_item<ROWS>(a, c, id, it)) return;
+    const KvCache& cache = a.cache;
+
+    // rows of this lane's columns
+    const int row0 = ROWS ? wave * 16 * NQ : 0;
+    int hi[NQ], lo[NQ];
+    float qs[NQ];
+    bool live[NQ], bad[NQ];
+    v4i qh[NQ][DC], ql[NQ][DC];
+    const bool vec = a.shape.d % 8 == 0 && ((uintptr_t)a.q.p & 15) == 0 &&
+                     a.q.token % (DT == kF32 ? 4 : 8) == 0 && a.q.head % (DT == kF32 ? 4 : 8) == 0;
+    const float to_log2 = a.scale * kLog2e;
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        const int row = row0 + 16 * q + n;
+        live[q] = row < it.rows;
+        int tok, head;
+        row_at(a, c, it, live[q] ? row : 0, tok, head);
+        const int pos = it.before + tok;
+        hi[q] = max(0, min(pos + 1, it.len));
+        lo[q] = a.shape.window ? max(0, pos + 1 - a.shape.window) : 0;
+        const int64_t e = (int64_t)(it.q0 + it.tok0 + tok) * a.q.token + head * a.q.head;
+        float x[DC][16], m = 0.f;
+        bool odd = false;
+#pragma unroll
+        for (int k = 0; k < DC; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int d = 64 * k + 16 * g + 8 * h;
+                float y[8];
+                if (vec && d < a.shape.d) {
+                    load8<DT>(a.q.p, e + d, y);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        y[i] = d + i < a.shape.d ? load_as_f32<DT>(a.q.p, e + d + i) : 0.f;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    odd |= !(fabsf(y[i]) < INFINITY);
+                    x[k][8 * h + i] = y[i] * to_log2;
+                    m = fmaxf(m, fabsf(x[k][8 * h + i]));
+                }
+            }
+        m = col_max(m);
+        // a product with the scale may overflow where q itself is finite; so far out only NaN is right
+        bad[q] = col_max(odd || !(m < INFINITY) ? 1.f : 0.f) > 0.f;
+        const float up = m >= kLeastScale && !bad[q] ? kFixed / m : 0.f;
+        qs[q] = up > 0.f ? m * (1.f / kFixed) : 0.f;
+#pragma unroll
+        for (int k = 0; k < DC; ++k)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                float t[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    t[i] = bad[q] ? kMagic : __builtin_fmaf(x[k][4 * w + i], up, kMagic);
+                int high, low;
+                limbs(t, high, low);
+                qh[q][k][w] = high;
+                ql[q][k][w] = low;
+            }
+    }
+
+    // 64-key tiles: the item's, the split's of them, the wave's of those
+    const int last = it.before + it.ntok - 1;  // newest token of the tile
+    int first_key = a.shape.window ? max(0, it.before + 1 - a.shape.window) : 0;
+    int end_key = max(0, min(last + 1, it.len));
+    const int t_first = first_key >> 6, t_end = (end_key + 63) >> 6;
+    const int per = max(c.least, (t_end - t_first + c.splits - 1) / c.splits);
+    int t0 = t_first + it.split * per, t1 = min(t_end, t0 + per);
+    int step = 1;
+    if constexpr (ROWS) {
+        // this wave's rows only
+        int ta, tb, unused;
+        const int rows_here = min(it.rows - row0, 16 * NQ);
+        row_at(a, c, it, rows_here > 0 ? row0 : 0, ta, unused);
+        row_at(a, c, it, rows_here > 0 ? row0 + rows_here - 1 : 0, tb, unused);
+        if (a.shape.window) t0 = max(t0, max(0, it.before + ta + 1 - a.shape.window) >> 6);
+        t1 = rows_here > 0 ? min(t1, (max(0, min(it.before + tb + 1, it.len)) + 63) >> 6) : t0;
+    } else {
+        t0 += wave;
+        step = kWaves;
+    }
+
+    v4f o[NQ][DM];
+    float m_run[NQ], l_run[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        m_run[q] = -INFINITY;
+        l_run[q] = 0.f;
+#pragma unroll
+        for (int i = 0; i < DM; ++i) o[q][i] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+
+    const int32_t* table = a.tables + it.r * a.table_ld;
+    const int block = 1 << cache.log_block;
+    const int64_t head_bytes = cache.head_bytes();
+    // The block of 16 keys from `key` on (-1: none), and their bytes' offset.
+    auto group_block = [&](int key) {
+        const int i = key >> cache.log_block;
+        return key < end_key && i < a.width ? table[i] : -1;
+    };
+    auto group_at = [&](int b, int key) {
+        const int safe = b >= 0 && b < cache.blocks ? b : 0;
+        return ((int64_t)safe * cache.heads + it.head) * head_bytes +
+               ((key & (block - 1)) >> 4) * (16 * DP);
+    };
+    const int key_k = (n >> 2) * 16, key_v = g * 16;
+    const int in_k = g * 64 + (n & 3) * 16, in_v = n * 16;
+    v4i kf[4][DC], vf[DM];
+    float2 sc = make_float2(0.f, 0.f);
+    auto load_keys = [&](int b, int j0) {
+        const int8_t* p = cache.k + group_at(b, j0 + key_k) + in_k;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int k = 0; k < DC; ++k)
+                kf[t][k] = *reinterpret_cast<const v4i*>(p + (4 * k + t) * 256);
+    };
+    auto load_values = [&](int b, int j0) {
+        const int8_t* p = cache.v + group_at(b, j0 + key_v) + in_v;
+#pragma unroll
+        for (int i = 0; i < DM; ++i) vf[i] = *reinterpret_cast<const v4i*>(p + i * 256);
+    };
+    auto load_scales = [&](int b) {
+        const int safe = b >= 0 && b < cache.blocks ? b : 0;
+        return *reinterpret_cast<const float2*>(cache.scales + cache.scale_at(safe, it.head));
+    };
+    int bk = -1, bv = -1, bk_next = -1, bv_next = -1;
+    if (t0 < t1) {
+        bk = group_block(t0 * 64 + key_k);
+        bv = group_block(t0 * 64 + key_v);
+        bk_next = group_block((t0 + step) * 64 + key_k);
+        bv_next = group_block((t0 + step) * 64 + key_v);
+        load_keys(bk, t0 * 64);
+        sc = load_scales(bv);
+        load_values(bv, t0 * 64);
+    }
+    for (int t = t0; t < t1; t += step) {
+        const int j0 = t * 64;
+        v4i s[NQ][4];
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[q][i] = v4i{0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < DC; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[q][i] = product(kf[i][k], qh[q][k], s[q][i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[q][i] = times256(s[q][i]);
+#pragma unroll
+            for (int k = 0; k < DC; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[q][i] = product(kf[i][k], ql[q][k], s[q][i]);
+        }
+        const bool valid = bv >= 0 && bv < cache.blocks;
+        const float ks = sc.x, vs = sc.y;
+        const bool more = t + step < t1;
+        const int bv_now = bv_next;
+        if (more) {
+            load_keys(bk_next, j0 + 64 * step);
+            sc = load_scales(bv_next);
+            bv = bv_next;
+            bk_next = group_block(j0 + 128 * step + key_k);
+            bv_next = group_block(j0 + 128 * step + key_v);
+        }
+        const float v_scale = fmaxf(vs, kLeastScale);
+        const float lv = __builtin_amdgcn_logf(v_scale), rv = __builtin_amdgcn_rcpf(v_scale);
+        bool whole = valid;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+            whole &= !live[q] || (lo[q] <= j0 && hi[q] >= j0 + 64);
+        whole = __all(whole);
+        const bool no_value = __any(vs == 0.f);
+        v4i ph[NQ], pl[NQ];
+        float beta[NQ];
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            const float f = qs[q] * ks;
+            // keys this row sees, from bit 0 on
+            uint32_t seen = 0xFFFFu;
+            if (!whole) {
+                const int h = hi[q] - (j0 + key_v), w = lo[q] - (j0 + key_v);
+                seen = h <= 0 || !valid ? 0u : h >= 16 ? 0xFFFFu : (1u << h) - 1u;
+                seen &= w <= 0 ? 0xFFFFu : w >= 16 ? 0u : ~((1u << w) - 1u);
+            }
+            int top = INT32_MIN;
+            if (whole) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) top = max(top, s[q][i][r]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        top = max(top, seen >> (4 * i + r) & 1 ? s[q][i][r] : INT32_MIN);
+            }
+            float m = __builtin_fmaf((float)top, f, lv);
+            m = seen ? m : -INFINITY;
+            m = col_max(m);
+            const float base = lv - (m == -INFINITY ? 0.f : m);
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float p[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float e = fast_exp2(__builtin_fmaf((float)s[q][i][r], f, base));
+                    if (!whole) e = seen >> (4 * i + r) & 1 ? e : 0.f;
+                    sum += e;
+                    if (no_value) e = vs == 0.f ? 0.f : e;
+                    p[r] = __builtin_fmaf(e, kFixed, kMagic);
+                }
+                int high, low;
+                limbs(p, high, low);
+                ph[q][i] = high;
+                pl[q][i] = low;
+            }
+            const float next = fmaxf(m_run[q], m);
+            const float keep = next == -INFINITY ? 1.f : fast_exp2(m_run[q] - next);
+            const float part = next == -INFINITY ? 0.f : fast_exp2(m - next);
+            l_run[q] = __builtin_fmaf(l_run[q], keep, sum * rv * part);
+            beta[q] = part * (1.f / kFixed);
+            if (!__all(m_run[q] == next)) {
+#pragma unroll
+                for (int i = 0; i < DM; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[q][i][r] *= keep;
+            }
+            m_run[q] = next;
+        }
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int i0 = 0; i0 < DM; i0 += 4) {
+                v4i x[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = product(vf[i0 + i], ph[q], v4i{0, 0, 0, 0});
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = product(vf[i0 + i], pl[q], times256(x[i]));
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        o[q][i0 + i][r] = __builtin_fmaf((float)x[i][r], beta[q], o[q][i0 + i][r]);
+            }
+        if (more) load_values(bv_now, j0 + 64 * step);
+    }
+
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) l_run[q] = col_sum(l_run[q]);
+    const bool out_vec = out_vector(a);
+    const float nan = __uint_as_float(0x7FC00000u);
+    const int64_t item_rows = ((int64_t)it.split * items + id) * c.rows;
+    if constexpr (ROWS) {
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            if (!live[q]) continue;
+            const int row = row0 + 16 * q + n;
+            const float l = l_run[q];
+            if (c.splits > 1) {
+                if (g == 0) c.ml[item_rows + row] = make_float2(bad[q] && l > 0.f ? nan : m_run[q], l);
+                if (!(l > 0.f)) continue;
+                float* p = c.part + (item_rows + row) * DP + 4 * g;
+#pragma unroll
+                for (int i = 0; i < DM; ++i) *reinterpret_cast<v4f*>(p + 16 * i) = o[q][i];
+                continue;
+            }
+            int tok, head;
+            row_at(a, c, it, row, tok, head);
+            const int64_t at = (int64_t)(it.q0 + it.tok0 + tok) * a.shape.heads + head;
+            const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+            for (int i = 0; i < DM; ++i) {
+                float v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = bad[q] && l > 0.f ? nan : o[q][i][r] * inv;
+                const int d = 16 * i + 4 * g;
+                store_row4<DT>(a.out, at * a.shape.d + d, a.shape.d - d, out_vec, v);
+            }
+            if (a.lse && g == 0)
+                a.lse[at] = !(l > 0.f) ? -INFINITY : bad[q] ? nan : (m_run[q] + log2f(l)) * kLn2;
+        }
+    } else {
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+            if (g == 0) {
+                wave_m[wave][16 * q + n] = m_run[q];
+                wave_l[wave][16 * q + n] = l_run[q];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            const int row = 16 * q + n;
+            float m = wave_m[0][row];
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) m = fmaxf(m, wave_m[w][row]);
+            const float keep = m_run[q] == -INFINITY ? 0.f : fast_exp2(m_run[q] - m);
+            if (live[q]) {
+                float* p = joined + (wave * 16 * NQ + row) * LD + 4 * g;
+#pragma unroll
+                for (int i = 0; i < DM; ++i) *reinterpret_cast<v4f*>(p + 16 * i) = o[q][i] * keep;
+            }
+            // the joined sum, in every wave
+            float l = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w)
+                l += wave_m[w][row] == -INFINITY ? 0.f
+                                                 : wave_l[w][row] * fast_exp2(wave_m[w][row] - m);
+            l_run[q] = l;
+            m_run[q] = m;
+        }
+        __syncthreads();
+        if (wave == 0 && g == 0) {
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) {
+                wave_m[0][16 * q + n] = bad[q] && l_run[q] > 0.f ? nan : m_run[q];
+                wave_l[0][16 * q + n] = l_run[q];
+            }
+        }
+        __syncthreads();
+        for (int u = threadIdx.x; u < it.rows * (DP / 4); u += kThreads) {
+            const int row = u / (DP / 4), d = (u - row * (DP / 4)) * 4;
+            const float m = wave_m[0][row], l = wave_l[0][row];
+            v4f sum = *reinterpret_cast<const v4f*>(joined + row * LD + d);
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w)
+                sum += *reinterpret_cast<const v4f*>(joined + (w * 16 * NQ + row) * LD + d);
+            if (c.splits > 1) {
+                if (d == 0) c.ml[item_rows + row] = make_float2(m, l);
+                if (l > 0.f) *reinterpret_cast<v4f*>(c.part + (item_rows + row) * DP + d) = sum;
+                continue;
+            }
+            int tok, head;
+            row_at(a, c, it, row, tok, head);
+            const int64_t at = (int64_t)(it.q0 + it.tok0 + tok) * a.shape.heads + head;
+            const float inv = l > 0.f ? 1.f / l : 0.f;
+            float v[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = m != m ? nan : sum[r] * inv;
+            if (d < a.shape.d) store_row4<DT>(a.out, at * a.shape.d + d, a.shape.d - d, out_vec, v);
+            if (a.lse && d == 0)
+                a.lse[at] = !(l > 0.f) ? -INFINITY : m != m ? nan : (m + log2f(l)) * kLn2;
+        }
+    }
+}
+
+// Joins the splits of an item, a wave per row: lane s has split s's maximum and sum.
+template <int DT, int DC, bool ROWS>
+__global__ __launch_bounds__(kThreads) void join_kernel(AttnArgs a, Cut c) {
+    constexpr int DP = 64 * DC;
+    const int lane = threadIdx.x & 63;
+    const int items = c.tiles * c.subs * a.shape.kv_heads;
+    Item it;
+    if (!find_item<ROWS>(a, c, blockIdx.x, it)) return;
+    const float nan = __uint_as_float(0x7FC00000u);
+    for (int row = blockIdx.y * kWaves + (threadIdx.x >> 6); row < it.rows;
+         row += gridDim.y * kWaves) {
+        const int64_t at0 = (int64_t)blockIdx.x * c.rows + row, stride = (int64_t)items * c.rows;
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (lane < c.splits) ml = c.ml[at0 + lane * stride];
+        const bool some = ml.y > 0.f;
+        const bool bad = __any(some && ml.x != ml.x);
+        float m = some && !bad ? ml.x : -INFINITY;
+#pragma unroll
+        for (int s = 32; s; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
+        const float keep = some && !bad ? fast_exp2(ml.x - m) : 0.f;
+        float l = keep * ml.y;
+#pragma unroll
+        for (int s = 32; s; s >>= 1) l += __shfl_xor(l, s);
+        float sum[DC];
+#pragma unroll
+        for (int i = 0; i < DC; ++i) sum[i] = 0.f;
+        uint64_t used = __ballot(some && !bad);
+        while (used) {
+            const int s = __builtin_ctzll(used);
+            used &= used - 1;
+            const float f = __shfl(keep, s);
+            const float* p = c.part + (at0 + s * stride) * DP + lane;
+#pragma unroll
+            for (int i = 0; i < DC; ++i) sum[i] = __builtin_fmaf(p[64 * i], f, sum[i]);
+        }
+        int tok, head;
+        row_at(a, c, it, row, tok, head);
+        const int64_t at = (int64_t)(it.q0 + it.tok0 + tok) * a.shape.heads + head;
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+        for (int i = 0; i < DC; ++i) {
+            const int d = lane + 64 * i;
+            if (d < a.shape.d) store_from_f32<DT>(a.out, at * a.shape.d + d, bad ? nan : sum[i] * inv);
+        }
+        if (a.lse && lane == 0)
+            a.lse[at] = bad ? nan : l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+    }
+}
+
+// ---------------------------------------------------------------- how a call is cut
+
+int64_t item_count(const Cut& c, const AttnShape& s) {
+    return (int64_t)c.tiles * c.subs * s.kv_heads;
+}
+
+// 64-key tiles of the longest range that rows of `tok` tokens see.
+int64_t key_tiles(const AttnShape& s, int tok) {
+    int64_t keys = s.max_seq;
+    if (s.window && s.window + tok < keys) keys = s.window + tok;
+    return (keys + 63) / 64 + 1;
+}
+
+void set_splits(Cut& c, const AttnShape& s, int64_t target, int least) {
+    const int64_t items = item_count(c, s), tiles = key_tiles(s, c.tok);
+    int64_t n = items > 0 ? (target + items - 1) / items : 1;
+    if (n > (tiles + least - 1) / least) n = (tiles + least - 1) / least;
+    if (n > kMaxSplits) n = kMaxSplits;
+    c.splits = n < 1 ? 1 : (int)n;
+    c.least = least;
+}
+
+// Rows of a request that the key-splitting launch takes: up to two 16-row columns.
+int key_rows(const AttnShape& s) {
+    const int64_t group = s.heads / s.kv_heads;
+    const int64_t most = group * (s.max_query < 32 / group ? s.max_query : 32 / group);
+    return (group <= 16 && most <= 16) ? 16 : 32;
+}
+
+Cut key_cut(const AttnShape& s) {
+    const int group = s.heads / s.kv_heads;
+    Cut c{};
+    c.rows = key_rows(s);
+    c.tok = group <= c.rows ? c.rows / group : 1;
+    c.subs = group <= c.rows ? 1 : (group + c.rows - 1) / c.rows;
+    c.tiles = s.requests;
+    c.small = c.tok;
+    set_splits(c, s, 8192, 4);
+    return c;
+}
+
+constexpr int kRowTile = 32 * kWaves;
+
+Cut row_cut(const AttnShape& s, int small) {
+    const int group = s.heads / s.kv_heads;
+    Cut c{};
+    c.rows = kRowTile;
+    c.tok = group <= c.rows ? c.rows / group : 1;
+    c.subs = group <= c.rows ? 1 : (group + c.rows - 1) / c.rows;
+    c.tiles = s.tokens / c.tok + s.requests;
+    c.small = small;
+    set_splits(c, s, 512, 16);
+    return c;
+}
+
+bool has_key_launch(const AttnShape& s, const Cut& key) {
+    // all requests of the longest length: every one is the other launch's
+    return s.max_query <= key.small || (int64_t)s.requests * s.max_query != s.tokens;
+}
+
+size_t cut_bytes(const Cut& c, const AttnShape& s) {
+    if (c.splits <= 1) return 0;
+    const size_t rows = (size_t)c.splits * item_count(c, s) * c.rows;
+    return rows * ((s.d + 63) / 64 * 64 * sizeof(float) + sizeof(float2));
+}
+
+template <int DT, int DC>
+hipError_t run(const AttnArgs& a, Cut c, bool by_rows, void* ws, size_t ws_bytes, hipStream_t stream) {
+    const int64_t items = item_count(c, a.shape);
+    if (items == 0) return hipSuccess;
+    if (c.splits > 1) {
+        const size_t per = cut_bytes(c, a.shape) / c.splits;
+        const size_t fit = ws ? ws_bytes / per : 0;
+        if ((size_t)c.splits > fit) c.splits = fit < 2 ? 1 : (int)fit;
+        c.part = static_cast<float*>(ws);
+        c.ml = reinterpret_cast<float2*>(c.part + (size_t)c.splits * items * c.rows * 64 * DC);
+    }
+    if (items * c.splits > 0x7FFFFFFF) return hipErrorInvalidValue;
+    const dim3 g((unsigned)(items * c.splits)), b(kThreads);
+    if (by_rows) tile_kernel<DT, DC, 2, true><<<g, b, 0, stream>>>(a, c);
+    else if (c.rows == 16) tile_kernel<DT, DC, 1, false><<<g, b, 0, stream>>>(a, c);
+    else tile_kernel<DT, DC, 2, false><<<g, b, 0, stream>>>(a, c);
+    if (c.splits > 1) {
+        const dim3 gj((unsigned)items, by_rows ? 8 : 1);
+        if (by_rows) join_kernel<DT, DC, true><<<gj, b, 0, stream>>>(a, c);
+        else join_kernel<DT, DC, false><<<gj, b, 0, stream>>>(a, c);
+    }
+    return hipGetLastError();
+}
+
+template <int DT>
+hipError_t run(const AttnArgs& a, const Cut& c, bool by_rows, void* ws, size_t ws_bytes,
+               hipStream_t stream) {
+    switch (a.cache.dp / 64) {
+        case 1: return run<DT, 1>(a, c, by_rows, ws, ws_bytes, stream);
+        case 2: return run<DT, 2>(a, c, by_rows, ws, ws_bytes, stream);
+        case 3: return run<DT, 3>(a, c, by_rows, ws, ws_bytes, stream);
+        default: return run<DT, 4>(a, c, by_rows, ws, ws_bytes, stream);
+    }
+}
+
 }  // namespace
 
-size_t kv8_attention_bytes(const AttnShape& s) { return 0; }
+size_t kv8_attention_bytes(const AttnShape& s) {
+    if (s.dtype == kF32 || s.tokens == 0 || s.requests == 0) return 0;
+    const Cut key = key_cut(s);
+    size_t n = has_key_launch(s, key) ? cut_bytes(key, s) : 0;
+    if (s.max_query > key.small) {
+        const size_t r = cut_bytes(row_cut(s, key.small), s);
+        n = r > n ? r : n;  // one after the other on the stream
+    }
+    return n;
+}
 
-hipError_t launch_kv8_attention(const AttnArgs& a, void* ws, size_t ws_bytes, hipStream_t stream) {
-    const int64_t rows = (int64_t)a.shape.tokens * a.shape.heads;
-    if (rows > 0x7FFFFFFF) return hipErrorInvalidValue;
-    const dim3 g((unsigned)rows), b(64);
-    if (a.shape.dtype == kF32) row_kernel<kF32><<<g, b, 0, stream>>>(a);
-    else if (a.shape.dtype == kF16) row_kernel<kF16><<<g, b, 0, stream>>>(a);
-    else row_kernel<kBF16><<<g, b, 0, stream>>>(a);
-    return hipGetLastError();
+hipError_t launch_kv8_attention(const AttnArgs& args, void* ws, size_t ws_bytes,
+                                hipStream_t stream) {
+    AttnArgs a = args;
+    if (a.cache.blocks == 0) a.shape.max_seq = 0;  // nothing to see
+    if (a.shape.dtype == kF32) {
+        const int64_t rows = (int64_t)a.shape.tokens * a.shape.heads;
+        if (rows > 0x7FFFFFFF) return hipErrorInvalidValue;
+        row_kernel<kF32><<<(unsigned)rows, 64, 0, stream>>>(a);
+        return hipGetLastError();
+    }
+    const Cut key = key_cut(a.shape);
+    hipError_t e = hipSuccess;
+    if (has_key_launch(a.shape, key))
+        e = a.shape.dtype == kF16 ? run<kF16>(a, key, false, ws, ws_bytes, stream)
+                                  : run<kBF16>(a, key, false, ws, ws_bytes, stream);
+    if (e == hipSuccess && a.shape.max_query > key.small) {
+        const Cut rows = row_cut(a.shape, key.small);
+        e = a.shape.dtype == kF16 ? run<kF16>(a, rows, true, ws, ws_bytes, stream)
+                                  : run<kBF16>(a, rows, true, ws, ws_bytes, stream);
+    }
+    return e;
 }
 
 }  // namespace ojx
