@@ -17,6 +17,9 @@ namespace ojx {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kPlainMax = 1e30f;
 
 // fp32 bits in rising order as unsigned, -0 as +0, NaN above everything.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -44,12 +47,14 @@ template <class T, class F> __device__ T block_reduce(T v, T* shared, F f) {
     return v;
 }
 
-// One workgroup per row, one pass for the maximum, one for the sums, one per alternative.
+// ---------------------------------------------------------------- rows out of the ordinary
+
+// A row with NaN or infinities, or whose largest logit is beyond +-kPlainMax (all of it masked
+// by a type's lowest value, say): one workgroup, one pass for the maximum, one for the sums,
+// one per alternative.
 template <int DT>
-__global__ __launch_bounds__(kThreads) void row_kernel(LogprobArgs a) {
-    __shared__ float sf[kThreads / 64];
-    __shared__ uint64_t sk[kThreads / 64];
-    const int row = blockIdx.x, v = a.vocab;
+__device__ __noinline__ void odd_row(const LogprobArgs& a, int row, float* sf, uint64_t* sk) {
+    const int v = a.vocab;
     const int64_t x0 = row * a.ld;
     auto add = [](float p, float q) { return p + q; };
     auto most = [](float p, float q) { return fmaxf(p, q); };
@@ -80,11 +85,10 @@ __global__ __launch_bounds__(kThreads) void row_kernel(LogprobArgs a) {
     if (threadIdx.x == 0) {
         const int64_t id = a.ids[row];
         const bool in = id >= 0 && id < v;
-        const float x = in ? load_as_f32<DT>(a.x, x0 + id) : 0.f;
         a.lse[row] = bad ? nan : m + ls;
         a.stats[2 * (int64_t)row] = bad ? nan : m;
         a.stats[2 * (int64_t)row + 1] = ls;
-        a.logprob[row] = in ? log_p(x) : 0.f;
+        a.logprob[row] = in ? log_p(load_as_f32<DT>(a.x, x0 + id)) : 0.f;
         a.entropy[row] = bad ? nan : none ? 0.f : ls - u / s;
     }
     uint64_t last = ~0ull;
@@ -96,19 +100,312 @@ __global__ __launch_bounds__(kThreads) void row_kernel(LogprobArgs a) {
         }
         last = block_reduce(best, sk, [](uint64_t p, uint64_t q) { return p > q ? p : q; });
         if (threadIdx.x == 0) {
-            const float x = unordered((uint32_t)(last >> 32));
             const int64_t o = (int64_t)row * a.top + i;
             a.top_ids[o] = 0xFFFFFFFFu - (uint32_t)last;
-            a.top_lp[o] = log_p(x);
+            a.top_lp[o] = log_p(unordered((uint32_t)(last >> 32)));
         }
     }
 }
 
-// One workgroup per row: p for every logit, then the tokens that a gradient names.
+// ---------------------------------------------------------------- one pass over a row
+
+// Sums of some of a row's logits in binary units: r a reference near the largest of them times
+// log2(e), s = sum 2^t and u = sum t 2^t over t = x log2(e) - r.  r is only a reference: its own
+// rounding does not enter.  m is the largest logit itself.
+struct Sums {
+    float r, s, u, m;
+};
+
+// The larger of two, NaN if either is (v_maximum3_f32).
+__device__ __forceinline__ float or_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// t below which 2^t is zero: keeps t 2^t from becoming -inf * 0 at masked logits.
+__device__ __forceinline__ float term(float x, float base) {
+    return fmaxf(__builtin_fmaf(x, kLog2e, -base), -200.f);
+}
+
+__device__ __forceinline__ void rescale(Sums& a, float base) {
+    const float d = fmaxf(a.r - base, -200.f), f = __builtin_amdgcn_exp2f(d);
+    a.u = f * __builtin_fmaf(d, a.s, a.u);
+    a.s *= f;
+}
+
+__device__ __forceinline__ Sums merge(Sums a, Sums b) {
+    const float r = fmaxf(a.r, b.r), base = r == -INFINITY ? 0.f : r;
+    rescale(a, base);
+    rescale(b, base);
+    return Sums{r, a.s + b.s, a.u + b.u, or_nan(a.m, b.m)};
+}
+
+__device__ __forceinline__ Sums merge_wave(Sums a) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1)
+        a = merge(a, Sums{__shfl_xor(a.r, o), __shfl_xor(a.s, o), __shfl_xor(a.u, o),
+                          __shfl_xor(a.m, o)});
+    return a;
+}
+
+__device__ __forceinline__ bool ordinary(const Sums& a) {
+    return a.m > -kPlainMax && a.m < kPlainMax;  // not NaN
+}
+
+// The k best keys that a wave has seen, the i-th in lane i.
+struct Best {
+    uint64_t key;   // 0: none yet
+    float least;    // the k-th one's logit; -inf while there are fewer
+    bool full;
+};
+
+__device__ __forceinline__ uint64_t read_lane(uint64_t v, int lane) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+    const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane);
+    return (uint64_t)hi << 32 | lo;
+}
+
+__device__ __forceinline__ void insert(Best& b, uint64_t key, int k, int lane) {
+    if (key <= read_lane(b.key, k - 1)) return;
+    const int at = __popcll(__ballot(b.key > key));
+    const uint64_t up = __shfl_up(b.key, 1);
+    b.key = lane < at ? b.key : lane == at ? key : up;
+}
+
+// The k-th largest of the lanes' values (0 where fewer than k lanes have one above 0).
+__device__ __forceinline__ uint32_t kth_of_lanes(uint32_t v, int k) {
+    uint32_t t = 0;
+#pragma unroll 1
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t c = t | 1u << bit;
+        if (__popcll(__ballot(v >= c)) >= k) t = c;
+    }
+    return t;
+}
+
+constexpr int kLaneLogits = 32;                  // logits of a lane in one batch
+constexpr int kBatch = 64 * kLaneLogits;         // of a wave
+constexpr int kGroups = kThreads / 64;
+constexpr int kMaxRowSplits = 64;
+
+template <int DT> struct Batch {
+    static constexpr int kVec = DT == kF32 ? 4 : 8;  // logits of 16 bytes
+    static constexpr int kVecs = kLaneLogits / kVec;
+    uint4 w[kVecs];
+
+    // logit i of the lane in the row, for batch b of a row that begins `shift` logits after an
+    // address that is a multiple of 16 bytes
+    static __device__ __forceinline__ int index(int b, int i, int lane, int shift) {
+        return ((b * kVecs + i / kVec) * 64 + lane) * kVec + i % kVec - shift;
+    }
+
+    // Vectors that reach over an end of the row are put together from its logits and -inf.
+    __device__ __forceinline__ void load(const void* x, int64_t x0, int v, int b, int lane,
+                                         int shift) {
+#pragma unroll
+        for (int n = 0; n < kVecs; ++n) {
+            const int j = index(b, n * kVec, lane, shift);
+            if (j >= 0 && j + kVec <= v) {
+                if constexpr (DT == kF32)
+                    w[n] = *reinterpret_cast<const uint4*>(static_cast<const float*>(x) + x0 + j);
+                else
+                    w[n] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + x0 + j);
+            } else {
+                uint32_t u[4];
+                constexpr uint32_t low = DT == kF32 ? 0xFF800000u : DT == kF16 ? 0xFC00u : 0xFF80u;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (DT == kF32) {
+                        const bool in = j + i >= 0 && j + i < v;
+                        u[i] = in ? static_cast<const uint32_t*>(x)[x0 + j + i] : low;
+                    } else {
+                        const uint16_t* h = static_cast<const uint16_t*>(x) + x0;
+                        const int p = j + 2 * i;
+                        const uint32_t lo = p >= 0 && p < v ? h[p] : low;
+                        const uint32_t hi = p + 1 >= 0 && p + 1 < v ? h[p + 1] : low;
+                        u[i] = lo | hi << 16;
+                    }
+                }
+                w[n] = make_uint4(u[0], u[1], u[2], u[3]);
+            }
+        }
+    }
+
+    __device__ __forceinline__ float get(int i) const {
+        const uint4& q = w[i / kVec];
+        const int n = i % kVec;
+        const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+        if constexpr (DT == kF32) return __uint_as_float(u[n]);
+        else if constexpr (DT == kF16) return f16_bits_to_f32(n & 1 ? u[n >> 1] >> 16 : u[n >> 1] & 0xFFFFu);
+        else return __uint_as_float(n & 1 ? u[n >> 1] & 0xFFFF0000u : u[n >> 1] << 16);
+    }
+};
+
+// Takes a batch's candidates into the wave's best k.  Batches come by rising token, so a later
+// logit that only equals the k-th one loses.  Where more than k lanes have a candidate, the
+// k-th largest of the lanes' maxima is a bound under which none can stay: about k candidates
+// are left whatever the row's order.
 template <int DT>
-__global__ __launch_bounds__(kThreads) void grad_kernel(LogprobGradArgs a) {
-    const int row = blockIdx.x, v = a.vocab;
+__device__ __forceinline__ void take(Best& best, const Batch<DT>& x, float lane_max, int b, int k,
+                                     int lane, int shift) {
+    const bool may = !best.full || lane_max > best.least;
+    const uint64_t lanes = __ballot(may);
+    if (!lanes) return;
+    uint32_t cut = 0;
+    if (__popcll(lanes) > k) cut = kth_of_lanes(may ? ordered(lane_max) : 0u, k);
+#pragma unroll
+    for (int i = 0; i < kLaneLogits; ++i) {
+        const float f = x.get(i);
+        uint64_t c = __ballot((!best.full || f > best.least) && ordered(f) >= cut);
+        const uint64_t key = key_of(f, Batch<DT>::index(b, i, lane, shift));
+        while (c) {
+            const int from = __builtin_ctzll(c);
+            c &= c - 1;
+            insert(best, read_lane(key, from), k, lane);
+        }
+    }
+    const uint64_t last = read_lane(best.key, k - 1);
+    best.full = last != 0;
+    best.least = best.full ? unordered((uint32_t)(last >> 32)) : -INFINITY;
+}
+
+// A row's results from its sums and the waves' best keys (keys[kGroups][top] in LDS, behind a
+// barrier).
+template <int DT>
+__device__ void finish(const LogprobArgs& a, int row, const Sums& t, const uint64_t* keys,
+                       float* sf, uint64_t* sk) {
+    if (!ordinary(t)) return odd_row<DT>(a, row, sf, sk);
+    const float l2 = log2f(t.s);
+    const float ls = (l2 - __builtin_fmaf(t.m, kLog2e, -t.r)) * kLn2;
+    auto log_p = [&](float x) { return x == -INFINITY ? x : (x - t.m) - ls; };
+    if (threadIdx.x == 0) {
+        const int64_t id = a.ids[row];
+        const bool in = id >= 0 && id < a.vocab;
+        a.lse[row] = t.m + ls;
+        a.stats[2 * (int64_t)row] = t.m;
+        a.stats[2 * (int64_t)row + 1] = ls;
+        a.logprob[row] = in ? log_p(load_as_f32<DT>(a.x, row * a.ld + id)) : 0.f;
+        a.entropy[row] = (l2 - t.u / t.s) * kLn2;
+    }
+    // a key's rank among the waves' is its place
+    for (int i = threadIdx.x; i < kGroups * a.top; i += kThreads) {
+        const uint64_t k = keys[i];
+        int rank = 0;
+        for (int j = 0; j < kGroups * a.top; ++j) rank += keys[j] > k;
+        if (rank < a.top) {
+            const int64_t o = (int64_t)row * a.top + rank;
+            a.top_ids[o] = 0xFFFFFFFFu - (uint32_t)k;
+            a.top_lp[o] = log_p(unordered((uint32_t)(k >> 32)));
+        }
+    }
+}
+
+// Partial results of a row's splits: sums, then k keys each.
+struct Parts {
+    Sums* sums;      // [rows][splits]
+    uint64_t* keys;  // [rows][splits][top]
+    int splits;
+};
+
+// A workgroup reads a row, or with splits > 1 a part of it, once: every wave keeps its sums and
+// its best k.
+template <int DT, bool TOP>
+__global__ __launch_bounds__(kThreads) void pass_kernel(LogprobArgs a, Parts p) {
+    __shared__ Sums sums[kGroups];
+    __shared__ uint64_t keys[TOP ? kGroups * kTopMax : 1];
+    __shared__ float sf[kGroups];
+    __shared__ uint64_t sk[kGroups];
+    using B = Batch<DT>;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits;
+    const int64_t x0 = row * a.ld;
+    const int size = DT == kF32 ? 4 : 2;
+    const int shift = (int)((((uintptr_t)a.x + x0 * size) & 15) / size);
+    const int batches = (int)(((int64_t)a.vocab + shift + kBatch - 1) / kBatch);
+    const int per = (batches + p.splits - 1) / p.splits;
+    const int end = min(batches, (split + 1) * per);
+    Sums t{-INFINITY, 0.f, 0.f, -INFINITY};
+    Best best{0, -INFINITY, false};
+    B x;
+    int b = split * per + wave;
+    if (b < end) x.load(a.x, x0, a.vocab, b, lane, shift);
+    for (; b < end; b += kGroups) {
+        B next;
+        if (b + kGroups < end) next.load(a.x, x0, a.vocab, b + kGroups, lane, shift);
+        float m = x.get(0);
+#pragma unroll
+        for (int i = 1; i < kLaneLogits; ++i) m = or_nan(m, x.get(i));
+        const float r = fmaxf(t.r, m < -kPlainMax ? -INFINITY : m * kLog2e);
+        const float base = r == -INFINITY ? 0.f : r;
+        rescale(t, base);
+        t.r = r;
+        t.m = or_nan(t.m, m);  // NaN would be lost in term()
+#pragma unroll
+        for (int i = 0; i < kLaneLogits; ++i) {
+            const float d = term(x.get(i), base), e = __builtin_amdgcn_exp2f(d);
+            t.s += e;
+            t.u = __builtin_fmaf(d, e, t.u);
+        }
+        if constexpr (TOP) take<DT>(best, x, m, b, a.top, lane, shift);
+        x = next;
+    }
+    t = merge_wave(t);
+    if (lane == 0) sums[wave] = t;
+    if (TOP && lane < a.top) keys[wave * a.top + lane] = best.key;
+    __syncthreads();
+    t = merge(merge(sums[0], sums[1]), merge(sums[2], sums[3]));
+    if (p.splits == 1) return finish<DT>(a, row, t, keys, sf, sk);
+    const int64_t at = (int64_t)row * p.splits + split;
+    if (threadIdx.x == 0) p.sums[at] = t;
+    if constexpr (TOP) {
+        // the waves' lists in order, for the next kernel
+        for (int i = threadIdx.x; i < kGroups * a.top; i += kThreads) {
+            const uint64_t k = keys[i];
+            int rank = 0;
+            for (int j = 0; j < kGroups * a.top; ++j) rank += keys[j] > k || (keys[j] == k && j < i);
+            if (rank < a.top) p.keys[at * a.top + rank] = k;
+        }
+    }
+}
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) void join_kernel(LogprobArgs a, Parts p) {
+    __shared__ uint64_t keys[kGroups * kTopMax];
+    __shared__ float sf[kGroups];
+    __shared__ uint64_t sk[kGroups];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.x;
+    Sums t{-INFINITY, 0.f, 0.f, -INFINITY};
+    if (lane < p.splits) t = p.sums[(int64_t)row * p.splits + lane];
+    t = merge_wave(t);
+    if (a.top > 0) {
+        Best b{0, 0.f, false};
+        for (int s = wave; s < p.splits; s += kGroups) {
+            const uint64_t* from = p.keys + ((int64_t)row * p.splits + s) * a.top;
+            const uint64_t k = lane < a.top ? from[lane] : 0;
+            uint64_t c = __ballot(k > read_lane(b.key, a.top - 1));
+            while (c) {
+                const int i = __builtin_ctzll(c);
+                c &= c - 1;
+                insert(b, read_lane(k, i), a.top, lane);
+            }
+        }
+        if (lane < a.top) keys[wave * a.top + lane] = b.key;
+    }
+    __syncthreads();
+    finish<DT>(a, row, t, keys, sf, sk);
+}
+
+// ---------------------------------------------------------------- gradient
+
+constexpr int kGradLogits = 8 * kThreads;  // of a workgroup's step, 16 bytes a thread and more
+
+// A workgroup writes the gradient of a part of a row, then goes over the tokens that a gradient
+// names and that lie in its part.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void grad_kernel(LogprobGradArgs a, int splits, int per) {
+    constexpr int VE = Batch<DT>::kVec;
+    const int row = blockIdx.x / splits, split = blockIdx.x - row * splits, v = a.vocab;
     const int64_t x0 = row * a.ld, g0 = (int64_t)row * v;
+    const int size = DT == kF32 ? 4 : 2;
+    const int shift = (int)((((uintptr_t)a.x + x0 * size) & 15) / size);
+    const bool same = shift == (int)((((uintptr_t)a.gx + g0 * size) & 15) / size);
     const int64_t id = a.ids[row];
     const bool in = id >= 0 && id < v;
     const float g_id = in && a.g_lp ? a.g_lp[row] : 0.f;
@@ -117,22 +414,58 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(LogprobGradArgs a) {
     const float h = a.entropy[row];
     float g_all = g_id - (a.g_lse ? a.g_lse[row] : 0.f);
     for (int i = 0; i < a.top; ++i) g_all += a.g_top[(int64_t)row * a.top + i];
-    auto grad = [&](int64_t j) {
-        const float x = load_as_f32<DT>(a.x, x0 + j);
-        const float lp = (x - m) - ls;
-        const float p = x == -INFINITY ? 0.f : expf(lp);
-        return -p * (g_all + (p > 0.f ? g_h * (lp + h) : 0.f));
+    // -p (g_all + g_h (log p + h)); the log probability bounded as in term(), where p is 0; a
+    // row with NaN has it in the factor
+    const float c0 = m == m ? -__builtin_fmaf(g_h, h, g_all) : m, c1 = -g_h;
+    const bool none = m == -INFINITY;
+    auto grad = [&](float x) {
+        const float lp = none ? -200.f : fmaxf((x - m) - ls, -200.f);
+        const float p = __builtin_amdgcn_exp2f(lp * kLog2e);
+        return p * __builtin_fmaf(c1, lp, c0);
     };
-    for (int j = threadIdx.x; j < v; j += kThreads) store_from_f32<DT>(a.gx, g0 + j, grad(j));
+    // the part: logits [j0, j1) on the row's 16-byte grid
+    const int64_t j0 = (int64_t)split * per - shift, j1 = j0 + per;
+    for (int64_t j = j0 + (int64_t)threadIdx.x * VE; j < j1 && j < v; j += kThreads * VE) {
+        if (same && j >= 0 && j + VE <= v) {
+            if constexpr (DT == kF32) {
+                const float4 x = *reinterpret_cast<const float4*>(static_cast<const float*>(a.x) + x0 + j);
+                *reinterpret_cast<float4*>(static_cast<float*>(a.gx) + g0 + j) =
+                    make_float4(grad(x.x), grad(x.y), grad(x.z), grad(x.w));
+            } else {
+                const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + x0 + j);
+                const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+                uint32_t o[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float lo, hi;
+                    if constexpr (DT == kF16) {
+                        lo = f16_bits_to_f32(u[i] & 0xFFFFu);
+                        hi = f16_bits_to_f32(u[i] >> 16);
+                        o[i] = f32_to_f16_bits(grad(lo)) | f32_to_f16_bits(grad(hi)) << 16;
+                    } else {
+                        lo = __uint_as_float(u[i] << 16);
+                        hi = __uint_as_float(u[i] & 0xFFFF0000u);
+                        o[i] = bf16_bits_hw(grad(lo)) | bf16_bits_hw(grad(hi)) << 16;
+                    }
+                }
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.gx) + g0 + j) =
+                    make_uint4(o[0], o[1], o[2], o[3]);
+            }
+        } else {
+            for (int i = 0; i < VE; ++i)
+                if (j + i >= 0 && j + i < v)
+                    store_from_f32<DT>(a.gx, g0 + j + i, grad(load_as_f32<DT>(a.x, x0 + j + i)));
+        }
+    }
     __syncthreads();
-    // Named tokens, each once: with its own gradient and those of equal names.
+    // Named tokens: each once for all its names, with its own gradient added.
     for (int i = threadIdx.x; i <= a.top; i += kThreads) {
         const int64_t j = i < a.top ? a.top_ids[(int64_t)row * a.top + i] : id;
-        if (j < 0 || j >= v) continue;
+        if (j < 0 || j >= v || j < j0 || j >= j1) continue;
         float g = in && j == id ? g_id : 0.f;
         for (int n = 0; n < a.top; ++n)
             if (a.top_ids[(int64_t)row * a.top + n] == j) g += a.g_top[(int64_t)row * a.top + n];
-        store_from_f32<DT>(a.gx, g0 + j, grad(j) + g);
+        store_from_f32<DT>(a.gx, g0 + j, grad(load_as_f32<DT>(a.x, x0 + j)) + g);
     }
 }
 
@@ -142,21 +475,60 @@ template <class F> void by_dtype(int dtype, F f) {
     else f(std::integral_constant<int, kBF16>{});
 }
 
+// Splits of a row: until the workgroups fill the GPU twice, none under a batch per wave.
+int row_splits(int rows, int vocab) {
+    const int64_t most = ((int64_t)vocab + kBatch * kGroups - 1) / (kBatch * kGroups);
+    int64_t n = rows > 0 ? 2048 / rows : 1;
+    if (n > most) n = most;
+    if (n > kMaxRowSplits) n = kMaxRowSplits;
+    return n < 1 ? 1 : (int)n;
+}
+
+size_t parts_bytes(int rows, int splits, int top) {
+    return splits > 1 ? (size_t)rows * splits * (sizeof(Sums) + top * sizeof(uint64_t)) : 0;
+}
+
 }  // namespace
 
-size_t token_logprobs_bytes(int rows, int vocab, int top, int dtype) { return 0; }
+size_t token_logprobs_bytes(int rows, int vocab, int top, int dtype) {
+    return parts_bytes(rows, row_splits(rows, vocab), top);
+}
 
 hipError_t launch_token_logprobs(const LogprobArgs& a, void* ws, size_t ws_bytes,
                                  hipStream_t stream) {
+    Parts p{};
+    p.splits = row_splits(a.rows, a.vocab);
+    if (p.splits > 1) {
+        const size_t per = (size_t)a.rows * (sizeof(Sums) + a.top * sizeof(uint64_t));
+        const size_t fit = ws ? ws_bytes / per : 0;
+        if ((size_t)p.splits > fit) p.splits = fit < 2 ? 1 : (int)fit;
+    }
+    p.sums = static_cast<Sums*>(ws);
+    p.keys = reinterpret_cast<uint64_t*>(p.sums + (size_t)a.rows * p.splits);
+    const int64_t grid = (int64_t)a.rows * p.splits;
+    if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
     by_dtype(a.dtype, [&](auto dt) {
-        row_kernel<decltype(dt)::value><<<a.rows, kThreads, 0, stream>>>(a);
+        constexpr int DT = decltype(dt)::value;
+        if (a.top > 0) pass_kernel<DT, true><<<(unsigned)grid, kThreads, 0, stream>>>(a, p);
+        else pass_kernel<DT, false><<<(unsigned)grid, kThreads, 0, stream>>>(a, p);
+        if (p.splits > 1) join_kernel<DT><<<a.rows, kThreads, 0, stream>>>(a, p);
     });
     return hipGetLastError();
 }
 
 hipError_t launch_token_logprobs_bwd(const LogprobGradArgs& a, hipStream_t stream) {
+    int64_t splits = a.rows > 0 ? 4096 / a.rows : 1;
+    const int64_t most = ((int64_t)a.vocab + kGradLogits - 1) / kGradLogits;
+    splits = splits < 1 ? 1 : splits > most ? most : splits;
+    // parts of whole steps; the row's shift may need one more logit's step
+    int64_t per = ((int64_t)a.vocab + 8 + splits - 1) / splits;
+    per = (per + kGradLogits - 1) / kGradLogits * kGradLogits;
+    splits = ((int64_t)a.vocab + 8 + per - 1) / per;
+    const int64_t grid = a.rows * splits;
+    if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
     by_dtype(a.dtype, [&](auto dt) {
-        grad_kernel<decltype(dt)::value><<<a.rows, kThreads, 0, stream>>>(a);
+        grad_kernel<decltype(dt)::value>
+            <<<(unsigned)grid, kThreads, 0, stream>>>(a, (int)splits, (int)per);
     });
     return hipGetLastError();
 }
