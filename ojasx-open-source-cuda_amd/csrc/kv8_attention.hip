@@ -299,110 +299,197 @@ __device__ __forceinline__ bool out_vector(const AttnArgs& a) {
     return a.shape.d % 4 == 0 && ((uintptr_t)a.out & 15) == 0;
 }
 
-// Rows of one item over a range of its keys, on the matrix unit in whole numbers: a score is
-// 256 (qh.k) + (ql.k) with the row's q in 16-bit fixed point against its own largest element,
-// 64 keys at a time; the weights of 64 keys are 16-bit fixed point against their largest
-// weight * (value scale), so codes of keys and values enter as they lie in memory.  Tile t of
-// the four score products takes 4 keys of each group of 16: a lane then holds the 16 scores of
-// one group, whose weights are the second operand of the value products as they come.
-//
-// ROWS false: the workgroup's waves share the keys of one tile of 16 NQ rows and join their
-// results in LDS.  ROWS true: each wave has 16 NQ rows of its own.
-template <int DT, int DC, int NQ, bool ROWS>
-__global__ __launch_bounds__(kThreads) void tile_kernel(AttnArgs a, Cut c) {
+// The query rows of a lane's columns: fixed-point operands of the score products, bounds of the
+// keys that a row sees.
+template <int DC, int NQ> struct Rows {
+    int hi[NQ], lo[NQ];
+    float qs[NQ];  // a row's unit times scale * log2(e): a whole-number score times it and the
+                   // key scale is the exponent
+    bool live[NQ], bad[NQ];
+    v4i qh[NQ][DC], ql[NQ][DC];
+
+    template <int DT>
+    __device__ __forceinline__ void load(const AttnArgs& a, const Cut& c, const Item& it, int row0,
+                                         int g, int n) {
+        constexpr int unit = DT == kF32 ? 4 : 8;
+        const bool vec = a.shape.d % 8 == 0 && ((uintptr_t)a.q.p & 15) == 0 &&
+                         a.q.token % unit == 0 && a.q.head % unit == 0;
+        const float to_log2 = a.scale * kLog2e;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            const int row = row0 + 16 * q + n;
+            live[q] = row < it.rows;
+            int tok, head;
+            row_at(a, c, it, live[q] ? row : 0, tok, head);
+            const int pos = it.before + tok;
+            hi[q] = max(0, min(pos + 1, it.len));
+            lo[q] = a.shape.window ? max(0, pos + 1 - a.shape.window) : 0;
+            const int64_t e = (int64_t)(it.q0 + it.tok0 + tok) * a.q.token + head * a.q.head;
+            float x[DC][16], m = 0.f;
+#pragma unroll
+            for (int k = 0; k < DC; ++k)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int d = 64 * k + 16 * g + 8 * h;
+                    float y[8];
+                    if (vec && d < a.shape.d) {
+                        load8<DT>(a.q.p, e + d, y);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            y[i] = d + i < a.shape.d ? load_as_f32<DT>(a.q.p, e + d + i) : 0.f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        x[k][8 * h + i] = y[i] * to_log2;
+                        m = __builtin_elementwise_maximum(m, fabsf(x[k][8 * h + i]));  // keeps NaN
+                    }
+                }
+            m = col_max(m < INFINITY ? m : INFINITY);
+            // also where only the product with the scale overflows: so far out only NaN is right
+            bad[q] = m == INFINITY;
+            const float up = m >= kLeastScale && !bad[q] ? kFixed / m : 0.f;
+            qs[q] = up > 0.f ? m * (1.f / kFixed) : 0.f;
+#pragma unroll
+            for (int k = 0; k < DC; ++k)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    float t[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        t[i] = bad[q] ? kMagic : __builtin_fmaf(x[k][4 * w + i], up, kMagic);
+                    int high, low;
+                    limbs(t, high, low);
+                    qh[q][k][w] = high;
+                    ql[q][k][w] = low;
+                }
+        }
+    }
+
+    // Whether every row sees the 64 keys from j0 on.
+    __device__ __forceinline__ bool see_all(int j0) const {
+        bool all = true;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) all &= !live[q] || (lo[q] <= j0 && hi[q] >= j0 + 64);
+        return all;
+    }
+
+    // Those of the 16 keys from `key` on that row q sees, from bit 0 on.
+    __device__ __forceinline__ uint32_t seen(int q, int key) const {
+        const int h = hi[q] - key, w = lo[q] - key;
+        const uint32_t below = h <= 0 ? 0u : h >= 16 ? 0xFFFFu : (1u << h) - 1u;
+        return below & (w <= 0 ? 0xFFFFu : w >= 16 ? 0u : ~((1u << w) - 1u));
+    }
+};
+
+// Largest of a lane's 16 scores, those that `seen` names where MASKED.
+template <bool MASKED> __device__ __forceinline__ int largest(const v4i (&s)[4], uint32_t seen) {
+    int top = INT32_MIN;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            top = max(top, !MASKED || seen >> (4 * i + r) & 1 ? s[i][r] : INT32_MIN);
+    return top;
+}
+
+// The block of a group of 16 keys (-1: none) and its bytes' offset.
+struct Pages {
+    const int32_t* table;
+    int width, log_block, blocks, heads, head, end;
+    int64_t head_bytes;
+
+    __device__ __forceinline__ Pages(const AttnArgs& a, const Item& it, int end_key)
+        : table(a.tables + it.r * a.table_ld), width(a.width), log_block(a.cache.log_block),
+          blocks(a.cache.blocks), heads(a.cache.heads), head(it.head), end(end_key),
+          head_bytes(a.cache.head_bytes()) {}
+    __device__ __forceinline__ int block(int key) const {
+        const int i = key >> log_block;
+        return key < end && i < width ? table[i] : -1;
+    }
+    __device__ __forceinline__ bool valid(int b) const { return b >= 0 && b < blocks; }
+    __device__ __forceinline__ int64_t index(int b) const {  // of (block, head)
+        return (int64_t)(valid(b) ? b : 0) * heads + head;
+    }
+    __device__ __forceinline__ int64_t at(int b, int key, int dp) const {
+        return index(b) * head_bytes + ((key & ((1 << log_block) - 1)) >> 4) * (16 * dp);
+    }
+};
+
+// What an item's rows see together, as 64-key tiles, and the split's part of them.
+__device__ __forceinline__ void key_range(const AttnArgs& a, const Cut& c, const Item& it, int& t0,
+                                          int& t1, int& end_key) {
+    const int first = a.shape.window ? max(0, it.before + 1 - a.shape.window) : 0;
+    end_key = max(0, min(it.before + it.ntok, it.len));
+    const int from = first >> 6, to = (end_key + 63) >> 6;
+    const int per = max(c.least, (to - from + c.splits - 1) / c.splits);
+    t0 = from + it.split * per;
+    t1 = min(to, t0 + per);
+}
+
+// Few rows over many keys, on the matrix unit in whole numbers: a score is 256 (qh.k) + (ql.k)
+// with the row's q in 16-bit fixed point against its own largest element, 64 keys at a time;
+// the weights of 64 keys are 16-bit fixed point against their largest weight * (value scale), so
+// codes of keys and values enter as they lie in memory: what the cache costs is its bytes.
+// Tile t of the four score products takes 4 keys of each group of 16: a lane then holds the 16
+// scores of one group (one block: one pair of scales), and their weights are the second operand
+// of the value products as they come.  The workgroup's waves take every fourth 64 keys of a
+// 16 NQ row tile and join their results in LDS.
+template <int DT, int DC, int NQ>
+__global__ __launch_bounds__(kThreads) void key_kernel(AttnArgs a, Cut c) {
     constexpr int DP = 64 * DC, DM = DP / 16;
     constexpr int LD = DP + 4;
-    __shared__ float joined[ROWS ? 1 : kWaves * 16 * NQ * LD];
+    __shared__ float joined[kWaves * 16 * NQ * LD];
     __shared__ float wave_m[kWaves][16 * NQ], wave_l[kWaves][16 * NQ];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
     const int items = c.tiles * c.subs * a.shape.kv_heads;
     Item it;
     it.split = blockIdx.x / items;
     const int id = blockIdx.x - it.split * items;
-    if (!find_item<ROWS>(a, c, id, it)) return;
-    const KvCache& cache = a.cache;
-
-    // rows of this lane's columns
-    const int row0 = ROWS ? wave * 16 * NQ : 0;
-    int hi[NQ], lo[NQ];
-    float qs[NQ];
-    bool live[NQ], bad[NQ];
-    v4i qh[NQ][DC], ql[NQ][DC];
-    const bool vec = a.shape.d % 8 == 0 && ((uintptr_t)a.q.p & 15) == 0 &&
-                     a.q.token % (DT == kF32 ? 4 : 8) == 0 && a.q.head % (DT == kF32 ? 4 : 8) == 0;
-    const float to_log2 = a.scale * kLog2e;
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-        const int row = row0 + 16 * q + n;
-        live[q] = row < it.rows;
-        int tok, head;
-        row_at(a, c, it, live[q] ? row : 0, tok, head);
-        const int pos = it.before + tok;
-        hi[q] = max(0, min(pos + 1, it.len));
-        lo[q] = a.shape.window ? max(0, pos + 1 - a.shape.window) : 0;
-        const int64_t e = (int64_t)(it.q0 + it.tok0 + tok) * a.q.token + head * a.q.head;
-        float x[DC][16], m = 0.f;
-        bool odd = false;
-#pragma unroll
-        for (int k = 0; k < DC; ++k)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int d = 64 * k + 16 * g + 8 * h;
-                float y[8];
-                if (vec && d < a.shape.d) {
-                    load8<DT>(a.q.p, e + d, y);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        y[i] = d + i < a.shape.d ? load_as_f32<DT>(a.q.p, e + d + i) : 0.f;
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    odd |= !(fabsf(y[i]) < INFINITY);
-                    x[k][8 * h + i] = y[i] * to_log2;
-                    m = fmaxf(m, fabsf(x[k][8 * h + i]));
-                }
-            }
-        m = col_max(m);
-        // a product with the scale may overflow where q itself is finite; so far out only NaN is right
-        bad[q] = col_max(odd || !(m < INFINITY) ? 1.f : 0.f) > 0.f;
-        const float up = m >= kLeastScale && !bad[q] ? kFixed / m : 0.f;
-        qs[q] = up > 0.f ? m * (1.f / kFixed) : 0.f;
-#pragma unroll
-        for (int k = 0; k < DC; ++k)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                float t[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    t[i] = bad[q] ? kMagic : __builtin_fmaf(x[k][4 * w + i], up, kMagic);
-                int high, low;
-                limbs(t, high, low);
-                qh[q][k][w] = high;
-                ql[q][k][w] = low;
-            }
+    if (!find_item<false>(a, c, id, it)) return;
+    const int64_t item_rows = ((int64_t)it.split * items + id) * c.rows;
+    int t0, t1, end_key;
+    key_range(a, c, it, t0, t1, end_key);
+    if (t0 >= t1 && c.splits > 1) {  // nothing of this split's
+        if ((int)threadIdx.x < it.rows) c.ml[item_rows + threadIdx.x] = make_float2(-INFINITY, 0.f);
+        return;
     }
+    t0 += wave;
 
-    // 64-key tiles: the item's, the split's of them, the wave's of those
-    const int last = it.before + it.ntok - 1;  // newest token of the tile
-    int first_key = a.shape.window ? max(0, it.before + 1 - a.shape.window) : 0;
-    int end_key = max(0, min(last + 1, it.len));
-    const int t_first = first_key >> 6, t_end = (end_key + 63) >> 6;
-    const int per = max(c.least, (t_end - t_first + c.splits - 1) / c.splits);
-    int t0 = t_first + it.split * per, t1 = min(t_end, t0 + per);
-    int step = 1;
-    if constexpr (ROWS) {
-        // this wave's rows only
-        int ta, tb, unused;
-        const int rows_here = min(it.rows - row0, 16 * NQ);
-        row_at(a, c, it, rows_here > 0 ? row0 : 0, ta, unused);
-        row_at(a, c, it, rows_here > 0 ? row0 + rows_here - 1 : 0, tb, unused);
-        if (a.shape.window) t0 = max(t0, max(0, it.before + ta + 1 - a.shape.window) >> 6);
-        t1 = rows_here > 0 ? min(t1, (max(0, min(it.before + tb + 1, it.len)) + 63) >> 6) : t0;
-    } else {
-        t0 += wave;
-        step = kWaves;
+    // the first keys and values are on their way before the queries
+    const Pages pages(a, it, end_key);
+    const int key_k = (n >> 2) * 16, key_v = g * 16;
+    const int in_k = g * 64 + (n & 3) * 16, in_v = n * 16;
+    v4i kf[4][DC], vf[DM];
+    float2 sc = make_float2(0.f, 0.f);
+    auto load_keys = [&](int b, int j0) {
+        const int8_t* p = a.cache.k + pages.at(b, j0 + key_k, DP) + in_k;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int k = 0; k < DC; ++k)
+                kf[t][k] = *reinterpret_cast<const v4i*>(p + (4 * k + t) * 256);
+    };
+    auto load_values = [&](int b, int j0) {
+        const int8_t* p = a.cache.v + pages.at(b, j0 + key_v, DP) + in_v;
+#pragma unroll
+        for (int i = 0; i < DM; ++i) vf[i] = *reinterpret_cast<const v4i*>(p + i * 256);
+    };
+    auto load_scales = [&](int b) {
+        return *reinterpret_cast<const float2*>(a.cache.scales + 2 * pages.index(b));
+    };
+    int bv = -1, bk_next = -1, bv_next = -1;
+    if (t0 < t1) {
+        const int bk = pages.block(t0 * 64 + key_k);
+        bv = pages.block(t0 * 64 + key_v);
+        bk_next = pages.block((t0 + kWaves) * 64 + key_k);
+        bv_next = pages.block((t0 + kWaves) * 64 + key_v);
+        load_keys(bk, t0 * 64);
+        sc = load_scales(bv);
+        load_values(bv, t0 * 64);
     }
+    Rows<DC, NQ> rows;
+    rows.template load<DT>(a, c, it, 0, g, n);
 
     v4f o[NQ][DM];
     float m_run[NQ], l_run[NQ];
@@ -413,52 +500,7 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(AttnArgs a, Cut c) {
 #pragma unroll
         for (int i = 0; i < DM; ++i) o[q][i] = v4f{0.f, 0.f, 0.f, 0.f};
     }
-
-    const int32_t* table = a.tables + it.r * a.table_ld;
-    const int block = 1 << cache.log_block;
-    const int64_t head_bytes = cache.head_bytes();
-    // The block of 16 keys from `key` on (-1: none), and their bytes' offset.
-    auto group_block = [&](int key) {
-        const int i = key >> cache.log_block;
-        return key < end_key && i < a.width ? table[i] : -1;
-    };
-    auto group_at = [&](int b, int key) {
-        const int safe = b >= 0 && b < cache.blocks ? b : 0;
-        return ((int64_t)safe * cache.heads + it.head) * head_bytes +
-               ((key & (block - 1)) >> 4) * (16 * DP);
-    };
-    const int key_k = (n >> 2) * 16, key_v = g * 16;
-    const int in_k = g * 64 + (n & 3) * 16, in_v = n * 16;
-    v4i kf[4][DC], vf[DM];
-    float2 sc = make_float2(0.f, 0.f);
-    auto load_keys = [&](int b, int j0) {
-        const int8_t* p = cache.k + group_at(b, j0 + key_k) + in_k;
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int k = 0; k < DC; ++k)
-                kf[t][k] = *reinterpret_cast<const v4i*>(p + (4 * k + t) * 256);
-    };
-    auto load_values = [&](int b, int j0) {
-        const int8_t* p = cache.v + group_at(b, j0 + key_v) + in_v;
-#pragma unroll
-        for (int i = 0; i < DM; ++i) vf[i] = *reinterpret_cast<const v4i*>(p + i * 256);
-    };
-    auto load_scales = [&](int b) {
-        const int safe = b >= 0 && b < cache.blocks ? b : 0;
-        return *reinterpret_cast<const float2*>(cache.scales + cache.scale_at(safe, it.head));
-    };
-    int bk = -1, bv = -1, bk_next = -1, bv_next = -1;
-    if (t0 < t1) {
-        bk = group_block(t0 * 64 + key_k);
-        bv = group_block(t0 * 64 + key_v);
-        bk_next = group_block((t0 + step) * 64 + key_k);
-        bv_next = group_block((t0 + step) * 64 + key_v);
-        load_keys(bk, t0 * 64);
-        sc = load_scales(bv);
-        load_values(bv, t0 * 64);
-    }
-    for (int t = t0; t < t1; t += step) {
+    for (int t = t0; t < t1; t += kWaves) {
         const int j0 = t * 64;
         v4i s[NQ][4];
 #pragma unroll
@@ -468,92 +510,71 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(AttnArgs a, Cut c) {
 #pragma unroll
             for (int k = 0; k < DC; ++k)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[q][i] = product(kf[i][k], qh[q][k], s[q][i]);
+                for (int i = 0; i < 4; ++i) s[q][i] = product(kf[i][k], rows.qh[q][k], s[q][i]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[q][i] = times256(s[q][i]);
 #pragma unroll
             for (int k = 0; k < DC; ++k)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[q][i] = product(kf[i][k], ql[q][k], s[q][i]);
+                for (int i = 0; i < 4; ++i) s[q][i] = product(kf[i][k], rows.ql[q][k], s[q][i]);
         }
-        const bool valid = bv >= 0 && bv < cache.blocks;
-        const float ks = sc.x, vs = sc.y;
-        const bool more = t + step < t1;
+        const bool valid = pages.valid(bv);
+        const float ks = sc.x, v_scale = fmaxf(sc.y, kLeastScale);
+        const bool more = t + kWaves < t1;
         const int bv_now = bv_next;
         if (more) {
-            load_keys(bk_next, j0 + 64 * step);
+            load_keys(bk_next, j0 + 64 * kWaves);
             sc = load_scales(bv_next);
             bv = bv_next;
-            bk_next = group_block(j0 + 128 * step + key_k);
-            bv_next = group_block(j0 + 128 * step + key_v);
+            bk_next = pages.block(j0 + 128 * kWaves + key_k);
+            bv_next = pages.block(j0 + 128 * kWaves + key_v);
         }
-        const float v_scale = fmaxf(vs, kLeastScale);
         const float lv = __builtin_amdgcn_logf(v_scale), rv = __builtin_amdgcn_rcpf(v_scale);
-        bool whole = valid;
-#pragma unroll
-        for (int q = 0; q < NQ; ++q)
-            whole &= !live[q] || (lo[q] <= j0 && hi[q] >= j0 + 64);
-        whole = __all(whole);
-        const bool no_value = __any(vs == 0.f);
         v4i ph[NQ], pl[NQ];
         float beta[NQ];
+        auto weigh = [&](auto masked) {
+            constexpr bool MASKED = decltype(masked)::value;
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-            const float f = qs[q] * ks;
-            // keys this row sees, from bit 0 on
-            uint32_t seen = 0xFFFFu;
-            if (!whole) {
-                const int h = hi[q] - (j0 + key_v), w = lo[q] - (j0 + key_v);
-                seen = h <= 0 || !valid ? 0u : h >= 16 ? 0xFFFFu : (1u << h) - 1u;
-                seen &= w <= 0 ? 0xFFFFu : w >= 16 ? 0u : ~((1u << w) - 1u);
-            }
-            int top = INT32_MIN;
-            if (whole) {
+            for (int q = 0; q < NQ; ++q) {
+                const float f = rows.qs[q] * ks;
+                uint32_t seen = 0xFFFFu;
+                if constexpr (MASKED) seen = valid ? rows.seen(q, j0 + key_v) : 0u;
+                float m = __builtin_fmaf((float)largest<MASKED>(s[q], seen), f, lv);
+                if constexpr (MASKED) m = seen ? m : -INFINITY;
+                m = col_max(m);
+                const float base = lv - (MASKED && m == -INFINITY ? 0.f : m);
+                float sum = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 4; ++i) {
+                    float p[4];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) top = max(top, s[q][i][r]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        top = max(top, seen >> (4 * i + r) & 1 ? s[q][i][r] : INT32_MIN);
-            }
-            float m = __builtin_fmaf((float)top, f, lv);
-            m = seen ? m : -INFINITY;
-            m = col_max(m);
-            const float base = lv - (m == -INFINITY ? 0.f : m);
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float p[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float e = fast_exp2(__builtin_fmaf((float)s[q][i][r], f, base));
-                    if (!whole) e = seen >> (4 * i + r) & 1 ? e : 0.f;
-                    sum += e;
-                    if (no_value) e = vs == 0.f ? 0.f : e;
-                    p[r] = __builtin_fmaf(e, kFixed, kMagic);
+                    for (int r = 0; r < 4; ++r) {
+                        float e = fast_exp2(__builtin_fmaf((float)s[q][i][r], f, base));
+                        if constexpr (MASKED) e = seen >> (4 * i + r) & 1 ? e : 0.f;
+                        sum += e;
+                        p[r] = __builtin_fmaf(e, kFixed, kMagic);
+                    }
+                    int high, low;
+                    limbs(p, high, low);
+                    ph[q][i] = high;
+                    pl[q][i] = low;
                 }
-                int high, low;
-                limbs(p, high, low);
-                ph[q][i] = high;
-                pl[q][i] = low;
-            }
-            const float next = fmaxf(m_run[q], m);
-            const float keep = next == -INFINITY ? 1.f : fast_exp2(m_run[q] - next);
-            const float part = next == -INFINITY ? 0.f : fast_exp2(m - next);
-            l_run[q] = __builtin_fmaf(l_run[q], keep, sum * rv * part);
-            beta[q] = part * (1.f / kFixed);
-            if (!__all(m_run[q] == next)) {
+                const float next = fmaxf(m_run[q], m);
+                const float keep = next == -INFINITY ? 1.f : fast_exp2(m_run[q] - next);
+                const float part = next == -INFINITY ? 0.f : fast_exp2(m - next);
+                l_run[q] = __builtin_fmaf(l_run[q], keep, sum * rv * part);
+                beta[q] = part * (1.f / kFixed);
+                if (!__all(m_run[q] == next)) {
 #pragma unroll
-                for (int i = 0; i < DM; ++i)
+                    for (int i = 0; i < DM; ++i)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) o[q][i][r] *= keep;
+                        for (int r = 0; r < 4; ++r) o[q][i][r] *= keep;
+                }
+                m_run[q] = next;
             }
-            m_run[q] = next;
-        }
+        };
+        if (__all(valid && rows.see_all(j0))) weigh(std::false_type{});
+        else weigh(std::true_type{});
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
 #pragma unroll
@@ -569,104 +590,317 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(AttnArgs a, Cut c) {
                     for (int r = 0; r < 4; ++r)
                         o[q][i0 + i][r] = __builtin_fmaf((float)x[i][r], beta[q], o[q][i0 + i][r]);
             }
-        if (more) load_values(bv_now, j0 + 64 * step);
+        if (more) load_values(bv_now, j0 + 64 * kWaves);
     }
 
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) l_run[q] = col_sum(l_run[q]);
     const bool out_vec = out_vector(a);
     const float nan = __uint_as_float(0x7FC00000u);
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        l_run[q] = col_sum(l_run[q]);
+        if (g == 0) {
+            wave_m[wave][16 * q + n] = m_run[q];
+            wave_l[wave][16 * q + n] = l_run[q];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        const int row = 16 * q + n;
+        float m = wave_m[0][row];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) m = fmaxf(m, wave_m[w][row]);
+        const float keep = m_run[q] == -INFINITY ? 0.f : fast_exp2(m_run[q] - m);
+        if (rows.live[q]) {
+            float* p = joined + (wave * 16 * NQ + row) * LD + 4 * g;
+#pragma unroll
+            for (int i = 0; i < DM; ++i) *reinterpret_cast<v4f*>(p + 16 * i) = o[q][i] * keep;
+        }
+        // the joined sum, in every wave
+        float l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w)
+            l += wave_m[w][row] == -INFINITY ? 0.f
+                                             : wave_l[w][row] * fast_exp2(wave_m[w][row] - m);
+        l_run[q] = l;
+        m_run[q] = m;
+    }
+    __syncthreads();
+    if (wave == 0 && g == 0) {
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            wave_m[0][16 * q + n] = rows.bad[q] && l_run[q] > 0.f ? nan : m_run[q];
+            wave_l[0][16 * q + n] = l_run[q];
+        }
+    }
+    __syncthreads();
+    for (int u = threadIdx.x; u < it.rows * (DP / 4); u += kThreads) {
+        const int row = u / (DP / 4), d = (u - row * (DP / 4)) * 4;
+        const float m = wave_m[0][row], l = wave_l[0][row];
+        v4f sum = *reinterpret_cast<const v4f*>(joined + row * LD + d);
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w)
+            sum += *reinterpret_cast<const v4f*>(joined + (w * 16 * NQ + row) * LD + d);
+        if (c.splits > 1) {
+            if (d == 0) c.ml[item_rows + row] = make_float2(m, l);
+            if (l > 0.f) *reinterpret_cast<v4f*>(c.part + (item_rows + row) * DP + d) = sum;
+            continue;
+        }
+        int tok, head;
+        row_at(a, c, it, row, tok, head);
+        const int64_t at = (int64_t)(it.q0 + it.tok0 + tok) * a.shape.heads + head;
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        float v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = m != m ? nan : sum[r] * inv;
+        if (d < a.shape.d) store_row4<DT>(a.out, at * a.shape.d + d, a.shape.d - d, out_vec, v);
+        if (a.lse && d == 0)
+            a.lse[at] = !(l > 0.f) ? -INFINITY : m != m ? nan : (m + log2f(l)) * kLn2;
+    }
+}
+
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+// Four codes as fp16, exactly: the byte with its sign flipped is code + 128, under the exponent
+// of 1024 it reads 1152 + code.
+__device__ __forceinline__ void halves_of(uint32_t codes, uint32_t& a, uint32_t& b) {
+    const uint32_t u = codes ^ 0x80808080u;
+    const v2h bias = {(_Float16)1152.f, (_Float16)1152.f};
+    const uint32_t lo = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);
+    const uint32_t hi = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
+    a = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, lo) - bias);
+    b = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, hi) - bias);
+}
+
+// Many rows: each wave has 32 of its own, and the workgroup goes through the keys together, 64 at
+// a time through two buffers in LDS.  Vector instructions bound it, so they are what the layout
+// saves: scores as in key_kernel (no conversion of keys; q's second byte costs matrix
+// instructions, which are not the bound), but the weights as fp16 on fp16 values, converted once
+// for the workgroup on their way into LDS: the products then add up in fp32 in the matrix unit,
+// where whole-number products would cost three vector instructions for every result of every 64
+// keys.  The reference of the weights is raised only when one would pass 2^kHeadroom times it, so
+// the sums are scaled again rarely.
+constexpr float kHeadroom = 8.f;
+
+template <int DT, int DC>
+__global__ __launch_bounds__(kThreads, DC <= 2 ? 2 : 1) void row_tile_kernel(AttnArgs a, Cut c) {
+    constexpr int NQ = 2, DP = 64 * DC, DM = DP / 16;
+    constexpr int kGroup = 16 * DP + 64;  // bytes of 16 keys: groups begin in different banks
+    __shared__ __align__(16) int8_t keys[2][4 * kGroup];
+    __shared__ __align__(16) _Float16 values[2][64 * DP];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
+    const int items = c.tiles * c.subs * a.shape.kv_heads;
+    Item it;
+    it.split = blockIdx.x / items;
+    const int id = blockIdx.x - it.split * items;
+    if (!find_item<true>(a, c, id, it)) return;
     const int64_t item_rows = ((int64_t)it.split * items + id) * c.rows;
-    if constexpr (ROWS) {
+    int t0, t1, end_key;
+    key_range(a, c, it, t0, t1, end_key);
+    if (t0 >= t1 && c.splits > 1) {
+        if ((int)threadIdx.x < it.rows) c.ml[item_rows + threadIdx.x] = make_float2(-INFINITY, 0.f);
+        return;
+    }
+    const Pages pages(a, it, end_key);
+
+    // Thread's pieces (16 bytes) of a tile: piece u of DP a group of 16 keys.
+    v4i kr[DC], vr[DC];
+    int next_block[DC];
+    auto piece_key = [&](int i) { return (int)(threadIdx.x + kThreads * i) / DP * 16; };
+    auto piece_in = [&](int i) { return (int)(threadIdx.x + kThreads * i) % DP; };
+    auto find = [&](int t) {
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-            if (!live[q]) continue;
-            const int row = row0 + 16 * q + n;
-            const float l = l_run[q];
-            if (c.splits > 1) {
-                if (g == 0) c.ml[item_rows + row] = make_float2(bad[q] && l > 0.f ? nan : m_run[q], l);
-                if (!(l > 0.f)) continue;
-                float* p = c.part + (item_rows + row) * DP + 4 * g;
+        for (int i = 0; i < DC; ++i) next_block[i] = pages.block(t * 64 + piece_key(i));
+    };
+    auto fetch = [&](int t) {
 #pragma unroll
-                for (int i = 0; i < DM; ++i) *reinterpret_cast<v4f*>(p + 16 * i) = o[q][i];
-                continue;
-            }
-            int tok, head;
-            row_at(a, c, it, row, tok, head);
-            const int64_t at = (int64_t)(it.q0 + it.tok0 + tok) * a.shape.heads + head;
-            const float inv = l > 0.f ? 1.f / l : 0.f;
-#pragma unroll
-            for (int i = 0; i < DM; ++i) {
-                float v[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = bad[q] && l > 0.f ? nan : o[q][i][r] * inv;
-                const int d = 16 * i + 4 * g;
-                store_row4<DT>(a.out, at * a.shape.d + d, a.shape.d - d, out_vec, v);
-            }
-            if (a.lse && g == 0)
-                a.lse[at] = !(l > 0.f) ? -INFINITY : bad[q] ? nan : (m_run[q] + log2f(l)) * kLn2;
+        for (int i = 0; i < DC; ++i) {
+            const int64_t at = pages.at(next_block[i], t * 64 + piece_key(i), DP) + piece_in(i) * 16;
+            kr[i] = *reinterpret_cast<const v4i*>(a.cache.k + at);
+            vr[i] = *reinterpret_cast<const v4i*>(a.cache.v + at);
         }
-    } else {
+    };
+    // values: [d / 16][half of the group's 16 keys][group][d % 16][8 keys]
+    auto put = [&](int buf) {
 #pragma unroll
-        for (int q = 0; q < NQ; ++q)
-            if (g == 0) {
-                wave_m[wave][16 * q + n] = m_run[q];
-                wave_l[wave][16 * q + n] = l_run[q];
-            }
-        __syncthreads();
+        for (int i = 0; i < DC; ++i) {
+            const int group = piece_key(i) >> 4, in = piece_in(i);
+            *reinterpret_cast<v4i*>(keys[buf] + group * kGroup + in * 16) = kr[i];
+            uint32_t w[8];
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-            const int row = 16 * q + n;
-            float m = wave_m[0][row];
-#pragma unroll
-            for (int w = 1; w < kWaves; ++w) m = fmaxf(m, wave_m[w][row]);
-            const float keep = m_run[q] == -INFINITY ? 0.f : fast_exp2(m_run[q] - m);
-            if (live[q]) {
-                float* p = joined + (wave * 16 * NQ + row) * LD + 4 * g;
-#pragma unroll
-                for (int i = 0; i < DM; ++i) *reinterpret_cast<v4f*>(p + 16 * i) = o[q][i] * keep;
-            }
-            // the joined sum, in every wave
-            float l = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w)
-                l += wave_m[w][row] == -INFINITY ? 0.f
-                                                 : wave_l[w][row] * fast_exp2(wave_m[w][row] - m);
-            l_run[q] = l;
-            m_run[q] = m;
+            for (int j = 0; j < 4; ++j) halves_of((uint32_t)vr[i][j], w[2 * j], w[2 * j + 1]);
+            uint4* p = reinterpret_cast<uint4*>(values[buf]) + (in >> 4) * 128 + group * 16 + (in & 15);
+            p[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            p[64] = make_uint4(w[4], w[5], w[6], w[7]);
         }
-        __syncthreads();
-        if (wave == 0 && g == 0) {
+    };
+    int bv = -1, bv_next = -1;
+    float2 sc = make_float2(0.f, 0.f), sc_next = sc;
+    auto load_scales = [&](int b) {
+        return *reinterpret_cast<const float2*>(a.cache.scales + 2 * pages.index(b));
+    };
+    const int key_v = g * 16;
+    if (t0 < t1) {
+        find(t0);
+        bv = pages.block(t0 * 64 + key_v);
+        fetch(t0);
+        sc = load_scales(bv);
+        find(t0 + 1);
+        bv_next = pages.block((t0 + 1) * 64 + key_v);
+    }
+    const int row0 = wave * 16 * NQ;
+    Rows<DC, NQ> rows;
+    rows.template load<DT>(a, c, it, row0, g, n);
+    // tiles that this wave's rows see
+    int w0 = t1, w1 = t0;
+    {
+        const int here = min(it.rows - row0, 16 * NQ);
+        if (here > 0) {
+            int ta, tb, unused;
+            row_at(a, c, it, row0, ta, unused);
+            row_at(a, c, it, row0 + here - 1, tb, unused);
+            w0 = a.shape.window ? max(0, it.before + ta + 1 - a.shape.window) >> 6 : t0;
+            w1 = (max(0, min(it.before + tb + 1, it.len)) + 63) >> 6;
+        }
+    }
+
+    v4f o[NQ][DM];
+    float ref[NQ], l_run[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        ref[q] = -INFINITY;
+        l_run[q] = 0.f;
+#pragma unroll
+        for (int i = 0; i < DM; ++i) o[q][i] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    if (t0 < t1) put(0);
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        const int buf = (t - t0) & 1, j0 = t * 64;
+        const bool more = t + 1 < t1;
+        if (more) {
+            fetch(t + 1);
+            sc_next = load_scales(bv_next);
+            find(t + 2);
+        }
+        if (t >= w0 && t < w1) {
+            v4i s[NQ][4];
+#pragma unroll
+            for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[q][i] = v4i{0, 0, 0, 0};
+            const int8_t* kp = keys[buf] + (n >> 2) * kGroup + g * 64 + (n & 3) * 16;
+            v4i kf[4][DC];
+#pragma unroll
+            for (int k = 0; k < DC; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    kf[i][k] = *reinterpret_cast<const v4i*>(kp + (4 * k + i) * 256);
 #pragma unroll
             for (int q = 0; q < NQ; ++q) {
-                wave_m[0][16 * q + n] = bad[q] && l_run[q] > 0.f ? nan : m_run[q];
-                wave_l[0][16 * q + n] = l_run[q];
+#pragma unroll
+                for (int k = 0; k < DC; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[q][i] = product(kf[i][k], rows.qh[q][k], s[q][i]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[q][i] = times256(s[q][i]);
+#pragma unroll
+                for (int k = 0; k < DC; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[q][i] = product(kf[i][k], rows.ql[q][k], s[q][i]);
             }
+            const bool valid = pages.valid(bv);
+            const float ks = sc.x, v_scale = fmaxf(sc.y, kLeastScale);
+            const float lv = __builtin_amdgcn_logf(v_scale), rv = __builtin_amdgcn_rcpf(v_scale);
+            v8h p[NQ][2];
+            auto weigh = [&](auto masked) {
+                constexpr bool MASKED = decltype(masked)::value;
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+                    const float f = rows.qs[q] * ks;
+                    uint32_t seen = 0xFFFFu;
+                    if constexpr (MASKED) seen = valid ? rows.seen(q, j0 + key_v) : 0u;
+                    float m = __builtin_fmaf((float)largest<MASKED>(s[q], seen), f, lv);
+                    if constexpr (MASKED) m = seen ? m : -INFINITY;
+                    if (!__all(m <= ref[q] + kHeadroom)) {
+                        m = col_max(m);
+                        const float next = m > ref[q] + kHeadroom ? m : ref[q];
+                        const float keep = next == -INFINITY ? 1.f : fast_exp2(ref[q] - next);
+                        l_run[q] *= keep;
+#pragma unroll
+                        for (int i = 0; i < DM; ++i)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) o[q][i][r] *= keep;
+                        ref[q] = next;
+                    }
+                    const float base = lv - (MASKED && ref[q] == -INFINITY ? 0.f : ref[q]);
+                    float sum = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            float e = fast_exp2(__builtin_fmaf((float)s[q][i][r], f, base));
+                            if constexpr (MASKED) e = seen >> (4 * i + r) & 1 ? e : 0.f;
+                            sum += e;
+                            p[q][i >> 1][4 * (i & 1) + r] = (_Float16)e;
+                        }
+                    l_run[q] = __builtin_fmaf(sum, rv, l_run[q]);
+                }
+            };
+            if (__all(valid && rows.see_all(j0))) weigh(std::false_type{});
+            else weigh(std::true_type{});
+            const v8h* vp = reinterpret_cast<const v8h*>(values[buf]) + lane;
+#pragma unroll
+            for (int i = 0; i < DM; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const v8h v = vp[(2 * i + h) * 64];
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q)
+                        o[q][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[q][h], o[q][i], 0, 0, 0);
+                }
+        }
+        if (more) {
+            put(buf ^ 1);
+            sc = sc_next;
+            bv = bv_next;
+            bv_next = pages.block((t + 2) * 64 + key_v);
         }
         __syncthreads();
-        for (int u = threadIdx.x; u < it.rows * (DP / 4); u += kThreads) {
-            const int row = u / (DP / 4), d = (u - row * (DP / 4)) * 4;
-            const float m = wave_m[0][row], l = wave_l[0][row];
-            v4f sum = *reinterpret_cast<const v4f*>(joined + row * LD + d);
+    }
+
+    const bool out_vec = out_vector(a);
+    const float nan = __uint_as_float(0x7FC00000u);
 #pragma unroll
-            for (int w = 1; w < kWaves; ++w)
-                sum += *reinterpret_cast<const v4f*>(joined + (w * 16 * NQ + row) * LD + d);
-            if (c.splits > 1) {
-                if (d == 0) c.ml[item_rows + row] = make_float2(m, l);
-                if (l > 0.f) *reinterpret_cast<v4f*>(c.part + (item_rows + row) * DP + d) = sum;
-                continue;
-            }
-            int tok, head;
-            row_at(a, c, it, row, tok, head);
-            const int64_t at = (int64_t)(it.q0 + it.tok0 + tok) * a.shape.heads + head;
-            const float inv = l > 0.f ? 1.f / l : 0.f;
+    for (int q = 0; q < NQ; ++q) {
+        const float l = col_sum(l_run[q]);
+        if (!rows.live[q]) continue;
+        const int row = row0 + 16 * q + n;
+        if (c.splits > 1) {
+            if (g == 0)
+                c.ml[item_rows + row] = make_float2(rows.bad[q] && l > 0.f ? nan : ref[q], l);
+            if (!(l > 0.f)) continue;
+            float* p = c.part + (item_rows + row) * DP + 4 * g;
+#pragma unroll
+            for (int i = 0; i < DM; ++i) *reinterpret_cast<v4f*>(p + 16 * i) = o[q][i];
+            continue;
+        }
+        int tok, head;
+        row_at(a, c, it, row, tok, head);
+        const int64_t at = (int64_t)(it.q0 + it.tok0 + tok) * a.shape.heads + head;
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+        for (int i = 0; i < DM; ++i) {
             float v[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = m != m ? nan : sum[r] * inv;
-            if (d < a.shape.d) store_row4<DT>(a.out, at * a.shape.d + d, a.shape.d - d, out_vec, v);
-            if (a.lse && d == 0)
-                a.lse[at] = !(l > 0.f) ? -INFINITY : m != m ? nan : (m + log2f(l)) * kLn2;
+            for (int r = 0; r < 4; ++r) v[r] = rows.bad[q] && l > 0.f ? nan : o[q][i][r] * inv;
+            const int d = 16 * i + 4 * g;
+            if (d < a.shape.d)
+                store_row4<DT>(a.out, at * a.shape.d + d, a.shape.d - d, out_vec, v);
         }
+        if (a.lse && g == 0)
+            a.lse[at] = !(l > 0.f) ? -INFINITY : rows.bad[q] ? nan : (ref[q] + log2f(l)) * kLn2;
     }
 }
 
@@ -798,9 +1032,9 @@ hipError_t run(const AttnArgs& a, Cut c, bool by_rows, void* ws, size_t ws_bytes
     }
     if (items * c.splits > 0x7FFFFFFF) return hipErrorInvalidValue;
     const dim3 g((unsigned)(items * c.splits)), b(kThreads);
-    if (by_rows) tile_kernel<DT, DC, 2, true><<<g, b, 0, stream>>>(a, c);
-    else if (c.rows == 16) tile_kernel<DT, DC, 1, false><<<g, b, 0, stream>>>(a, c);
-    else tile_kernel<DT, DC, 2, false><<<g, b, 0, stream>>>(a, c);
+    if (by_rows) row_tile_kernel<DT, DC><<<g, b, 0, stream>>>(a, c);
+    else if (c.rows == 16) key_kernel<DT, DC, 1><<<g, b, 0, stream>>>(a, c);
+    else key_kernel<DT, DC, 2><<<g, b, 0, stream>>>(a, c);
     if (c.splits > 1) {
         const dim3 gj((unsigned)items, by_rows ? 8 : 1);
         if (by_rows) join_kernel<DT, DC, true><<<gj, b, 0, stream>>>(a, c);

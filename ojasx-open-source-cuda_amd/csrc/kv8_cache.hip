@@ -306,48 +306,310 @@ __device__ void append_run(const KvCache& c, const KvRows& src, bool values, int
     }
 }
 
-// A wave looks for run starts among `window` tokens and writes each run for one head, keys or
-// values.  Runs end where the slots leave the block or skip.
-template <int DT, bool VEC>
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a),
+                                                                  __builtin_bit_cast(u16x2, b)));
+}
+
+template <int DT> __device__ __forceinline__ float half_to_f32(uint32_t bits) {
+    return DT == kBF16 ? bf16_bits_to_f32(bits) : f16_bits_to_f32(bits);
+}
+
+// x times the inverse scale, rounded, as the low byte of a float: 1.5 * 2^23 is added to the
+// rounded product (not fused with it), whose nearest integer then is the sum's low bits.
+__device__ __forceinline__ uint32_t byte_float(float x, float inverse) {
+#pragma clang fp contract(off)
+    const float f = x * inverse;
+    return __float_as_uint(f + 12582912.f);
+}
+
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    const uint32_t ab = __builtin_amdgcn_perm(b, a, 0x0C0C0400u);
+    const uint32_t cd = __builtin_amdgcn_perm(d, c, 0x04000C0Cu);
+    return ab | cd;
+}
+
+// Codes of eight 16-bit elements; `plain`: all of the run's are finite.
+template <int DT>
+__device__ __forceinline__ uint2 codes8(const uint4& q, float inverse, bool plain) {
+    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = half_to_f32<DT>(u[i] & 0xFFFFu);
+        x[2 * i + 1] = half_to_f32<DT>(u[i] >> 16);
+    }
+    if (!plain)
+        return make_uint2(pack4(code_of(x[0], inverse), code_of(x[1], inverse),
+                                code_of(x[2], inverse), code_of(x[3], inverse)),
+                          pack4(code_of(x[4], inverse), code_of(x[5], inverse),
+                                code_of(x[6], inverse), code_of(x[7], inverse)));
+    uint32_t c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = byte_float(x[i], inverse);
+    return make_uint2(low_bytes(c[0], c[1], c[2], c[3]), low_bytes(c[4], c[5], c[6], c[7]));
+}
+
+__device__ __forceinline__ uint32_t recode4(uint32_t w, float ratio) {
+    return pack4(recode(byte_of(w, 0), ratio), recode(byte_of(w, 1), ratio),
+                 recode(byte_of(w, 2), ratio), recode(byte_of(w, 3), ratio));
+}
+
+// u / d for u < 2^16: `inverse` is 2^32 / d rounded up.
+__device__ __forceinline__ uint32_t inverse_of(int d) { return 0xFFFFFFFFu / (uint32_t)d + 1u; }
+__device__ __forceinline__ int quotient(int u, uint32_t inverse, int d) {
+    return d == 1 ? u : (int)__umulhi((uint32_t)u, inverse);
+}
+
+// Earlier codes of a block and head for its new scale, a few loads of 16 bytes in flight: keys
+// of `off` tokens, or value words of `quads` 4-token groups.
+__device__ __forceinline__ void recode_keys(int8_t* base, int off, int d, int dp, float ratio,
+                                            int first, int step) {
+    const int chunks = (d + 15) >> 4, total = off * chunks;
+    const uint32_t inv = inverse_of(chunks);
+    for (int i0 = first; i0 < total; i0 += 4 * step) {
+        uint4* p[4];
+        uint4 o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = min(i0 + j * step, total - 1), t = quotient(i, inv, chunks);
+            p[j] = reinterpret_cast<uint4*>(base + key_at(t, i - t * chunks, dp));
+            o[j] = *p[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (i0 + j * step < total)
+                *p[j] = make_uint4(recode4(o[j].x, ratio), recode4(o[j].y, ratio),
+                                   recode4(o[j].z, ratio), recode4(o[j].w, ratio));
+    }
+}
+
+__device__ __forceinline__ void recode_values(int8_t* base, int quads, int d, int dp, float ratio,
+                                              int first, int step) {
+    const int groups = (quads + 3) >> 2, total = groups * d;
+    const uint32_t inv = inverse_of(d);
+    for (int i0 = first; i0 < total; i0 += 4 * step) {
+        uint32_t* p[4];
+        uint4 o[4];
+        int words[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = min(i0 + j * step, total - 1), g = quotient(i, inv, d);
+            p[j] = reinterpret_cast<uint32_t*>(base + g * 16 * dp + (i - g * d) * 16);
+            o[j] = *reinterpret_cast<const uint4*>(p[j]);
+            words[j] = i0 + j * step < total ? quads - 4 * g : 0;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint4 v = make_uint4(recode4(o[j].x, ratio), recode4(o[j].y, ratio),
+                                       recode4(o[j].z, ratio), recode4(o[j].w, ratio));
+            if (words[j] >= 4) {
+                *reinterpret_cast<uint4*>(p[j]) = v;
+            } else {  // the rest of the group is written elsewhere
+                if (words[j] > 0) p[j][0] = v.x;
+                if (words[j] > 1) p[j][1] = v.y;
+                if (words[j] > 2) p[j][2] = v.z;
+            }
+        }
+    }
+}
+
+// append_run for 16-bit rows on a 16-byte grid, with the run held in registers between its
+// maximum and its codes: HOLD loads of eight elements a lane, all in flight at once.  `waves`
+// waves share a run (their maxima meet in LDS).  Values are taken as 4 tokens by 8 d, whose
+// bytes a lane turns into 8 words of 4 tokens; words that the run does not fill are read first.
+template <int DT, int HOLD, int WAVES>
+__device__ void append_held(const KvCache& c, const KvRows& src, bool values, int head, int64_t t0,
+                            int n, int block, int off, int lane, int wave, uint32_t* shared) {
+    const uint16_t* x0 = static_cast<const uint16_t*>(src.p) + t0 * src.token + head * src.head;
+    const int d8 = c.d >> 3, first = wave * 64 + lane;
+    const uint32_t inv8 = inverse_of(d8);
+    const int q0 = off >> 2, quads = ((off + n - 1) >> 2) - q0 + 1;
+    const int units = values ? quads * d8 : n * d8;
+    float* sp = c.scales + c.scale_at(block, head) + values;
+    const float before = off > 0 ? *sp : 0.f;
+    int8_t* base = (values ? c.v : c.k) + c.at(block, head);
+    // value word (quad q, d) of the block
+    auto value_at = [&](int q, int d) { return base + (q >> 2) * 16 * c.dp + d * 16 + (q & 3) * 4; };
+    uint4 w[HOLD];
+    uint32_t m = 0;
+    if (!values) {
+#pragma unroll
+        for (int i = 0; i < HOLD; ++i) {
+            const int u = first + i * 64 * WAVES;
+            w[i] = make_uint4(0, 0, 0, 0);
+            if (u < units) {
+                const int t = quotient(u, inv8, d8);
+                w[i] = *reinterpret_cast<const uint4*>(x0 + t * src.token + (u - t * d8) * 8);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < HOLD; i += 4) {
+            const int u = first + (i >> 2) * 64 * WAVES;
+            const int q = quotient(u, inv8, d8), d = (u - q * d8) * 8;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int t = 4 * (q0 + q) + j - off;
+                w[i + j] = make_uint4(0, 0, 0, 0);
+                if (u < units && t >= 0 && t < n)
+                    w[i + j] = *reinterpret_cast<const uint4*>(x0 + t * src.token + d);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < HOLD; ++i) {
+        const uint32_t a = max_pair(w[i].x & 0x7FFF7FFFu, w[i].y & 0x7FFF7FFFu);
+        const uint32_t b = max_pair(w[i].z & 0x7FFF7FFFu, w[i].w & 0x7FFF7FFFu);
+        m = max_pair(m, max_pair(a, b));
+    }
+    // largest over the run of `bits`, pairs of 16 bits
+    auto run_max = [&](uint32_t v) {
+        uint32_t b = max(v & 0xFFFFu, v >> 16);
+#pragma unroll
+        for (int o = 32; o; o >>= 1) b = max(b, (uint32_t)__shfl_xor((int)b, o));
+        if constexpr (WAVES > 1) {
+            __syncthreads();
+            if (lane == 0) shared[wave] = b;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) b = max(b, shared[i]);
+        }
+        return b;
+    };
+    constexpr uint32_t inf = DT == kBF16 ? 0x7F80u : 0x7C00u;
+    uint32_t top = run_max(m);
+    const bool plain = top < inf;
+    if (!plain) {  // finite elements only
+        m = 0;
+#pragma unroll
+        for (int i = 0; i < HOLD; ++i) {
+            const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t lo = u[j] & 0x7FFFu, hi = u[j] >> 16 & 0x7FFFu;
+                m = max(m, lo < inf ? lo : 0u);
+                m = max(m, hi < inf ? hi : 0u);
+            }
+        }
+        top = run_max(m);
+    }
+    float largest = half_to_f32<DT>(top);
+    largest = largest < kTinyAmax ? 0.f : largest;
+    const float scale = fmaxf(before, largest * (1.f / 127.f));
+    const float inverse = scale > 0.f ? 1.f / scale : 0.f;
+    const float ratio = scale > 0.f ? before / scale : 0.f;
+    const bool again = off > 0 && scale > before;
+    if (lane == 0 && wave == 0) *sp = scale;
+    if (!values) {
+        if (again) recode_keys(base, off, c.d, c.dp, ratio, first, 64 * WAVES);
+#pragma unroll
+        for (int i = 0; i < HOLD; ++i) {
+            const int u = first + i * 64 * WAVES;
+            if (u >= units) break;
+            const int t = quotient(u, inv8, d8), ch = u - t * d8;
+            *reinterpret_cast<uint2*>(base + key_at(off + t, ch >> 1, c.dp) + (ch & 1) * 8) =
+                codes8<DT>(w[i], inverse, plain);
+        }
+        return;
+    }
+    if (again) recode_values(base, q0, c.d, c.dp, ratio, first, 64 * WAVES);
+#pragma unroll
+    for (int i = 0; i < HOLD; i += 4) {
+        const int u = first + (i >> 2) * 64 * WAVES;
+        if (u >= units) break;
+        const int q = quotient(u, inv8, d8), d = (u - q * d8) * 8;
+        uint32_t row[4][2];
+        uint32_t fresh = 0;  // bytes of a word that the run fills
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint2 b = codes8<DT>(w[i + j], inverse, plain);
+            row[j][0] = b.x;
+            row[j][1] = b.y;
+            const int t = 4 * (q0 + q) + j - off;
+            fresh |= t >= 0 && t < n ? 0xFFu << (8 * j) : 0u;
+        }
+        int8_t* p = value_at(q0 + q, d);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            // 4 tokens of 4 d -> 4 d of 4 tokens
+            const uint32_t a = __builtin_amdgcn_perm(row[1][h], row[0][h], 0x05010400u);
+            const uint32_t b = __builtin_amdgcn_perm(row[3][h], row[2][h], 0x05010400u);
+            const uint32_t e = __builtin_amdgcn_perm(row[1][h], row[0][h], 0x07030602u);
+            const uint32_t f = __builtin_amdgcn_perm(row[3][h], row[2][h], 0x07030602u);
+            const uint32_t v[4] = {__builtin_amdgcn_perm(b, a, 0x05040100u),
+                                   __builtin_amdgcn_perm(b, a, 0x07060302u),
+                                   __builtin_amdgcn_perm(f, e, 0x05040100u),
+                                   __builtin_amdgcn_perm(f, e, 0x07060302u)};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t* o = reinterpret_cast<uint32_t*>(p + (4 * h + j) * 16);
+                uint32_t keep = 0;
+                if (fresh != 0xFFFFFFFFu) {
+                    keep = *o;
+                    if (again) {
+                        // bytes before the run; those after it stay
+                        const uint32_t r = recode4(keep, ratio);
+                        const uint32_t old = fresh ? (fresh & (0u - fresh)) - 1u : 0xFFFFFFFFu;
+                        keep = (r & old) | (keep & ~old);
+                    }
+                }
+                *o = (v[j] & fresh) | (keep & ~fresh);
+            }
+        }
+    }
+}
+
+// A wave (WAVES > 1: a workgroup) looks for run starts among `window` tokens and writes each run
+// for one head, keys or values.  Runs end where the slots leave the block or skip.
+template <int DT, bool VEC, int HOLD, int WAVES>
 __global__ __launch_bounds__(kAppendWaves * kWave) void append_kernel(
     KvCache c, KvRows k, KvRows v, const int64_t* __restrict__ slots, int tokens, int window,
     int64_t units) {
-    const int lane = threadIdx.x & 63;
-    const int64_t u = (int64_t)blockIdx.x * kAppendWaves + (threadIdx.x >> 6);
+    __shared__ uint32_t shared[WAVES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t u = WAVES > 1 ? blockIdx.x : (int64_t)blockIdx.x * kAppendWaves + wave;
     if (u >= units) return;
     const int parts = 2 * c.heads;
     const int64_t w = u / parts;
     const int part = (int)(u - w * parts), head = part >> 1;
     const int64_t end = (int64_t)c.blocks << c.log_block;
     const int block = 1 << c.log_block;
-    const int64_t t = w * window + lane;
-    int64_t slot = -1, prev = -1;
-    if (lane < window && t < tokens) {
-        slot = slots[t];
-        if (t > 0) prev = slots[t - 1];
-    }
-    const bool start = slot >= 0 && slot < end &&
-                       (prev != slot - 1 || (slot & (block - 1)) == 0);
-    uint64_t heads = __ballot(start);
+    // lane i has the slot of token base + i - 1: the window's and what may follow it
+    const int64_t base = w * window, t = base + lane - 1;
+    int64_t slot = -1;
+    if (t >= 0 && t < tokens) slot = slots[t];
+    const int64_t prev = __shfl_up(slot, 1);
+    const bool in = slot >= 0 && slot < end;
+    const bool follows = in && lane > 0 && prev == slot - 1 && (slot & (block - 1)) != 0;
+    const uint64_t more = __ballot(follows);
+    uint64_t heads = __ballot(in && !follows && lane > 0 && lane <= window);
     while (heads) {
         const int i = __builtin_ctzll(heads);
         heads &= heads - 1;
-        const int64_t t0 = w * window + i;
+        const int64_t t0 = base + i - 1;
         const int64_t s0 = __shfl(slot, i);
         const int off = (int)(s0 & (block - 1));
-        int n = 0;
-        for (; n < block - off;) {  // tokens that follow it in the block
-            const int64_t tn = t0 + n + lane;
-            const bool next = n + lane < block - off && tn < tokens && slots[tn] == s0 + n + lane;
-            const uint64_t miss = ~__ballot(next);
-            if (miss) {
-                n += __builtin_ctzll(miss);
-                break;
+        const uint64_t after = i < 63 ? ~(more >> (i + 1)) : ~0ull;
+        int n = 1 + __builtin_ctzll(after);
+        if (i + n == 64) {  // it may go on past what the lanes hold
+            while (n < block - off) {
+                const int64_t tn = t0 + n + lane;
+                const bool next = n + lane < block - off && tn < tokens && slots[tn] == s0 + n + lane;
+                const uint64_t miss = ~__ballot(next);
+                n += miss ? __builtin_ctzll(miss) : kWave;
+                if (miss) break;
             }
-            n += kWave;
         }
-        append_run<DT, VEC>(c, part & 1 ? v : k, part & 1, head, t0, n,
-                            (int)(s0 >> c.log_block), off, lane);
+        const int at = (int)(s0 >> c.log_block);
+        if constexpr (HOLD > 0)
+            append_held<DT, HOLD, WAVES>(c, part & 1 ? v : k, part & 1, head, t0, n, at, off, lane,
+                                         WAVES > 1 ? wave : 0, shared);
+        else
+            append_run<DT, VEC>(c, part & 1 ? v : k, part & 1, head, t0, n, at, off, lane);
     }
 }
 
@@ -361,43 +623,84 @@ template <int DT> __device__ __forceinline__ void store_value(void* p, int64_t i
 }
 
 constexpr int kReadThreads = 256;
+constexpr int kReadUnits = 4;  // per thread
 
-template <int DT>
+// Eight values from their codes (in the low byte of each of eight words), 16 bytes and more.
+template <int DT> __device__ __forceinline__ void store8(void* p, int64_t i, const int (&code)[8], float s) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        v[j] = (float)code[j] * s;
+        keep_f32(v[j]);
+    }
+    if constexpr (DT == kF32) {
+        float4* o = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
+        o[0] = make_float4(v[0], v[1], v[2], v[3]);
+        o[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            w[j] = DT == kF16 ? f32_to_f16_bits(v[2 * j]) | f32_to_f16_bits(v[2 * j + 1]) << 16
+                              : bf16_bits_hw(v[2 * j]) | bf16_bits_hw(v[2 * j + 1]) << 16;
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// One block's keys or values per blockIdx.x, a share of its units per blockIdx.y.  The output's
+// order (token, head, d) is the units': 8 d of a token's key, or of 4 tokens' values, whose
+// codes are 8 words of 4 tokens.  WIDE: d a multiple of 8, else a unit is a single element.
+template <int DT, bool WIDE>
 __global__ __launch_bounds__(kReadThreads) void read_kernel(KvCache c,
                                                             const int32_t* __restrict__ blocks,
                                                             void* k_out, void* v_out,
                                                             float* scales_out) {
-    const int parts = 2 * c.heads;
-    const int64_t i = blockIdx.x / parts;
-    const int part = blockIdx.x % parts, head = part >> 1, values = part & 1;
+    const int64_t i = blockIdx.x >> 1;
+    const int values = blockIdx.x & 1;
     const int b = blocks[i], size = 1 << c.log_block;
     const bool in = b >= 0 && b < c.blocks;
-    const float s = in ? c.scales[c.scale_at(b, head) + values] : 0.f;
-    const int8_t* base = (values ? c.v : c.k) + (in ? c.at(b, head) : 0);
+    const int8_t* base = (values ? c.v : c.k) + (in ? c.at(b, 0) : 0);
+    const float* scales = c.scales + (in ? c.scale_at(b, 0) : 0) + values;
     void* out = values ? v_out : k_out;
-    if (threadIdx.x == 0) scales_out[(i * c.heads + head) * 2 + values] = s;
-    // output element of (token, d)
-    const int64_t o0 = ((i << c.log_block) * c.heads + head) * c.d, ot = (int64_t)c.heads * c.d;
-    if (!values) {
-        const int chunks = (c.d + 15) >> 4;
-        for (int u = threadIdx.x; u < size * chunks; u += kReadThreads) {
-            const int t = u / chunks, ch = u - t * chunks;
-            uint4 o = make_uint4(0, 0, 0, 0);
-            if (in) o = *reinterpret_cast<const uint4*>(base + key_at(t, ch, c.dp));
-            const uint32_t w[4] = {o.x, o.y, o.z, o.w};
-            for (int j = 0; j < 16 && ch * 16 + j < c.d; ++j)
-                store_value<DT>(out, o0 + t * ot + ch * 16 + j, byte_of(w[j >> 2], j & 3), s);
-        }
-        return;
-    }
-    for (int u = threadIdx.x; u < (size >> 4) * c.d; u += kReadThreads) {
-        const int g = u / c.d, d = u - g * c.d;
-        uint4 o = make_uint4(0, 0, 0, 0);
-        if (in) o = *reinterpret_cast<const uint4*>(base + (int64_t)g * 16 * c.dp + d * 16);
-        const uint32_t w[4] = {o.x, o.y, o.z, o.w};
+    const int per = WIDE ? c.d >> 3 : c.d;
+    const int row = c.heads * per;
+    const int units = (WIDE && values ? size >> 2 : size) * row;
+    const int64_t head_bytes = c.head_bytes(), o0 = ((i << c.log_block) * c.heads) * c.d;
+    const int64_t ot = (int64_t)c.heads * c.d;
+    if (blockIdx.y == 0)
+        for (int h = threadIdx.x; h < c.heads; h += kReadThreads)
+            scales_out[(i * c.heads + h) * 2 + values] = in ? scales[2 * h] : 0.f;
+#pragma unroll 4
+    for (int u = blockIdx.y * kReadThreads + threadIdx.x; u < units; u += gridDim.y * kReadThreads) {
+        const int t = u / row, e = u - t * row, h = e / per, x = e - h * per;
+        const int8_t* p = base + h * head_bytes;
+        const float s = in ? scales[2 * h] : 0.f;
+        if constexpr (!WIDE) {
+            const int at = values ? (t >> 4) * 16 * c.dp + x * 16 + (t & 15)
+                                  : key_at(t, x >> 4, c.dp) + (x & 15);
+            store_value<DT>(out, o0 + t * ot + e, in ? p[at] : 0, s);
+        } else if (!values) {
+            uint2 w = make_uint2(0, 0);
+            if (in) w = *reinterpret_cast<const uint2*>(p + key_at(t, x >> 1, c.dp) + (x & 1) * 8);
+            int code[8];
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-            store_value<DT>(out, o0 + (g * 16 + j) * ot + d, byte_of(w[j >> 2], j & 3), s);
+            for (int j = 0; j < 8; ++j) code[j] = byte_of(j < 4 ? w.x : w.y, j & 3);
+            store8<DT>(out, o0 + t * ot + h * c.d + x * 8, code, s);
+        } else {
+            uint32_t w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                w[j] = in ? *reinterpret_cast<const uint32_t*>(p + (t >> 2) * 16 * c.dp +
+                                                              (x * 8 + j) * 16 + (t & 3) * 4)
+                          : 0u;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                int code[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) code[j] = byte_of(w[j], n);
+                store8<DT>(out, o0 + (4 * t + n) * ot + h * c.d + x * 8, code, s);
+            }
+        }
     }
 }
 
@@ -417,20 +720,37 @@ hipError_t launch_kv8_plan(const PlanArgs& a, hipStream_t stream) {
 
 hipError_t launch_kv8_append(const KvCache& c, const KvRows& k, const KvRows& v, int dtype,
                              const int64_t* slots, int tokens, hipStream_t stream) {
+    const int64_t held = (int64_t)c.d << c.log_block;
+    const bool vec = rows_vector(k, dtype) && rows_vector(v, dtype);
+    // Rows that a run is held in registers of: 16-bit ones on a 16-byte grid.  fp32 caches'
+    // inputs and odd rows are read twice instead, the second time from the cache.
+    const bool hold = vec && dtype != kF32 && c.d % 8 == 0 && held <= 32768;
+    const bool shared = hold && held > 8192;  // the workgroup's waves share a run
     // A window per token fills the GPU for a decode step, whose tokens all begin runs; with
     // many tokens most of such waves would find none.
     const int window = (int64_t)tokens * 2 * c.heads <= 16384 ? 1 : 16;
     const int64_t units = ((int64_t)tokens + window - 1) / window * 2 * c.heads;
-    const int64_t grid = (units + kAppendWaves - 1) / kAppendWaves;
+    const int64_t grid = shared ? units : (units + kAppendWaves - 1) / kAppendWaves;
     if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
-    const bool vec = rows_vector(k, dtype) && rows_vector(v, dtype);
     const dim3 g((unsigned)grid), b(kAppendWaves * kWave);
     auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
+        if constexpr (DT != kF32) {
+            if (shared)
+                append_kernel<DT, true, 16, kAppendWaves>
+                    <<<g, b, 0, stream>>>(c, k, v, slots, tokens, window, units);
+            else if (hold && held > 2048)
+                append_kernel<DT, true, 16, 1>
+                    <<<g, b, 0, stream>>>(c, k, v, slots, tokens, window, units);
+            else if (hold)
+                append_kernel<DT, true, 4, 1>
+                    <<<g, b, 0, stream>>>(c, k, v, slots, tokens, window, units);
+            if (hold) return;
+        }
         if (vec)
-            append_kernel<DT, true><<<g, b, 0, stream>>>(c, k, v, slots, tokens, window, units);
+            append_kernel<DT, true, 0, 1><<<g, b, 0, stream>>>(c, k, v, slots, tokens, window, units);
         else
-            append_kernel<DT, false><<<g, b, 0, stream>>>(c, k, v, slots, tokens, window, units);
+            append_kernel<DT, false, 0, 1><<<g, b, 0, stream>>>(c, k, v, slots, tokens, window, units);
     };
     if (dtype == kF32) go(std::integral_constant<int, kF32>{});
     else if (dtype == kF16) go(std::integral_constant<int, kF16>{});
@@ -440,12 +760,20 @@ hipError_t launch_kv8_append(const KvCache& c, const KvRows& k, const KvRows& v,
 
 hipError_t launch_kv8_read(const KvCache& c, const int32_t* blocks, int n, int dtype, void* k_out,
                            void* v_out, float* scales_out, hipStream_t stream) {
-    const int64_t grid = (int64_t)n * 2 * c.heads;
-    if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
-    const dim3 g((unsigned)grid), b(kReadThreads);
-    if (dtype == kF32) read_kernel<kF32><<<g, b, 0, stream>>>(c, blocks, k_out, v_out, scales_out);
-    else if (dtype == kF16) read_kernel<kF16><<<g, b, 0, stream>>>(c, blocks, k_out, v_out, scales_out);
-    else read_kernel<kBF16><<<g, b, 0, stream>>>(c, blocks, k_out, v_out, scales_out);
+    const bool wide = c.d % 8 == 0;
+    const int64_t units = ((int64_t)c.heads * (wide ? c.d / 8 : c.d)) << c.log_block;
+    int64_t shares = (units + kReadThreads * kReadUnits - 1) / (kReadThreads * kReadUnits);
+    if (shares > 1024) shares = 1024;
+    if ((int64_t)n * 2 > 0x7FFFFFFF) return hipErrorInvalidValue;
+    const dim3 g((unsigned)(2 * n), (unsigned)shares), b(kReadThreads);
+    auto go = [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        if (wide) read_kernel<DT, true><<<g, b, 0, stream>>>(c, blocks, k_out, v_out, scales_out);
+        else read_kernel<DT, false><<<g, b, 0, stream>>>(c, blocks, k_out, v_out, scales_out);
+    };
+    if (dtype == kF32) go(std::integral_constant<int, kF32>{});
+    else if (dtype == kF16) go(std::integral_constant<int, kF16>{});
+    else go(std::integral_constant<int, kBF16>{});
     return hipGetLastError();
 }
 
