@@ -382,16 +382,33 @@ template <int DC, int NQ> struct Rows {
     }
 };
 
-// Largest of a lane's 16 scores, those that `seen` names where MASKED.
-template <bool MASKED> __device__ __forceinline__ int largest(const v4i (&s)[4], uint32_t seen) {
-    int top = INT32_MIN;
+// A lane's 16 whole-number scores as floats, and -inf in the place of those without a bit in
+// `seen`: a step of its own for the tiles that need it, so the weights' code is the same for all.
+__device__ __forceinline__ void to_float(const v4i (&s)[4], v4f (&x)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            top = max(top, !MASKED || seen >> (4 * i + r) & 1 ? s[i][r] : INT32_MIN);
+        for (int r = 0; r < 4; ++r) x[i][r] = (float)s[i][r];
+}
+__device__ __forceinline__ void hide(v4f (&x)[4], uint32_t seen) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[i][r] = seen >> (4 * i + r) & 1 ? x[i][r] : -INFINITY;
+}
+__device__ __forceinline__ float largest(const v4f (&x)[4]) {
+    float top = x[0][0];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, x[i][r]);
     return top;
 }
+
+// A reference below every score (and no infinity, whose differences would be NaN), and the least
+// factor of a score: times -inf it stays -inf.
+constexpr float kNone = -1e30f;
+constexpr float kLeastFactor = 0x1p-120f;
 
 // The block of a group of 16 keys (-1: none) and its bytes' offset.
 struct Pages {
@@ -495,7 +512,7 @@ __global__ __launch_bounds__(kThreads) void key_kernel(AttnArgs a, Cut c) {
     float m_run[NQ], l_run[NQ];
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
-        m_run[q] = -INFINITY;
+        m_run[q] = kNone;
         l_run[q] = 0.f;
 #pragma unroll
         for (int i = 0; i < DM; ++i) o[q][i] = v4f{0.f, 0.f, 0.f, 0.f};
@@ -530,65 +547,61 @@ __global__ __launch_bounds__(kThreads) void key_kernel(AttnArgs a, Cut c) {
             bv_next = pages.block(j0 + 128 * kWaves + key_v);
         }
         const float lv = __builtin_amdgcn_logf(v_scale), rv = __builtin_amdgcn_rcpf(v_scale);
+        v4f x[NQ][4];
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) to_float(s[q], x[q]);
+        if (!__all(valid && rows.see_all(j0))) {
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) hide(x[q], valid ? rows.seen(q, j0 + key_v) : 0u);
+        }
         v4i ph[NQ], pl[NQ];
         float beta[NQ];
-        auto weigh = [&](auto masked) {
-            constexpr bool MASKED = decltype(masked)::value;
 #pragma unroll
-            for (int q = 0; q < NQ; ++q) {
-                const float f = rows.qs[q] * ks;
-                uint32_t seen = 0xFFFFu;
-                if constexpr (MASKED) seen = valid ? rows.seen(q, j0 + key_v) : 0u;
-                float m = __builtin_fmaf((float)largest<MASKED>(s[q], seen), f, lv);
-                if constexpr (MASKED) m = seen ? m : -INFINITY;
-                m = col_max(m);
-                const float base = lv - (MASKED && m == -INFINITY ? 0.f : m);
-                float sum = 0.f;
+        for (int q = 0; q < NQ; ++q) {
+            const float f = fmaxf(rows.qs[q] * ks, kLeastFactor);
+            const float m = fmaxf(col_max(__builtin_fmaf(largest(x[q]), f, lv)), kNone);
+            const float base = lv - m;
+            float sum = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float p[4];
+            for (int i = 0; i < 4; ++i) {
+                float p[4];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        float e = fast_exp2(__builtin_fmaf((float)s[q][i][r], f, base));
-                        if constexpr (MASKED) e = seen >> (4 * i + r) & 1 ? e : 0.f;
-                        sum += e;
-                        p[r] = __builtin_fmaf(e, kFixed, kMagic);
-                    }
-                    int high, low;
-                    limbs(p, high, low);
-                    ph[q][i] = high;
-                    pl[q][i] = low;
+                for (int r = 0; r < 4; ++r) {
+                    const float e = fast_exp2(__builtin_fmaf(x[q][i][r], f, base));
+                    sum += e;
+                    p[r] = __builtin_fmaf(e, kFixed, kMagic);
                 }
-                const float next = fmaxf(m_run[q], m);
-                const float keep = next == -INFINITY ? 1.f : fast_exp2(m_run[q] - next);
-                const float part = next == -INFINITY ? 0.f : fast_exp2(m - next);
-                l_run[q] = __builtin_fmaf(l_run[q], keep, sum * rv * part);
-                beta[q] = part * (1.f / kFixed);
-                if (!__all(m_run[q] == next)) {
-#pragma unroll
-                    for (int i = 0; i < DM; ++i)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) o[q][i][r] *= keep;
-                }
-                m_run[q] = next;
+                int high, low;
+                limbs(p, high, low);
+                ph[q][i] = high;
+                pl[q][i] = low;
             }
-        };
-        if (__all(valid && rows.see_all(j0))) weigh(std::false_type{});
-        else weigh(std::true_type{});
+            const float next = fmaxf(m_run[q], m);
+            const float keep = fast_exp2(m_run[q] - next), part = fast_exp2(m - next);
+            l_run[q] = __builtin_fmaf(l_run[q], keep, sum * rv * part);
+            beta[q] = part * (1.f / kFixed);
+            if (!__all(m_run[q] == next)) {
+#pragma unroll
+                for (int i = 0; i < DM; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[q][i][r] *= keep;
+            }
+            m_run[q] = next;
+        }
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
 #pragma unroll
             for (int i0 = 0; i0 < DM; i0 += 4) {
-                v4i x[4];
+                v4i w[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = product(vf[i0 + i], ph[q], v4i{0, 0, 0, 0});
+                for (int i = 0; i < 4; ++i) w[i] = product(vf[i0 + i], ph[q], v4i{0, 0, 0, 0});
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = product(vf[i0 + i], pl[q], times256(x[i]));
+                for (int i = 0; i < 4; ++i) w[i] = product(vf[i0 + i], pl[q], times256(w[i]));
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        o[q][i0 + i][r] = __builtin_fmaf((float)x[i][r], beta[q], o[q][i0 + i][r]);
+                        o[q][i0 + i][r] = __builtin_fmaf((float)w[i][r], beta[q], o[q][i0 + i][r]);
             }
         if (more) load_values(bv_now, j0 + 64 * kWaves);
     }
@@ -610,7 +623,7 @@ __global__ __launch_bounds__(kThreads) void key_kernel(AttnArgs a, Cut c) {
         float m = wave_m[0][row];
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) m = fmaxf(m, wave_m[w][row]);
-        const float keep = m_run[q] == -INFINITY ? 0.f : fast_exp2(m_run[q] - m);
+        const float keep = fast_exp2(m_run[q] - m);
         if (rows.live[q]) {
             float* p = joined + (wave * 16 * NQ + row) * LD + 4 * g;
 #pragma unroll
@@ -620,8 +633,7 @@ __global__ __launch_bounds__(kThreads) void key_kernel(AttnArgs a, Cut c) {
         float l = 0.f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w)
-            l += wave_m[w][row] == -INFINITY ? 0.f
-                                             : wave_l[w][row] * fast_exp2(wave_m[w][row] - m);
+            l = __builtin_fmaf(wave_l[w][row], fast_exp2(wave_m[w][row] - m), l);
         l_run[q] = l;
         m_run[q] = m;
     }
@@ -769,7 +781,7 @@ __global__ __launch_bounds__(kThreads, DC <= 2 ? 2 : 1) void row_tile_kernel(Att
     float ref[NQ], l_run[NQ];
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
-        ref[q] = -INFINITY;
+        ref[q] = kNone;
         l_run[q] = 0.f;
 #pragma unroll
         for (int i = 0; i < DM; ++i) o[q][i] = v4f{0.f, 0.f, 0.f, 0.f};
@@ -791,65 +803,62 @@ __global__ __launch_bounds__(kThreads, DC <= 2 ? 2 : 1) void row_tile_kernel(Att
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[q][i] = v4i{0, 0, 0, 0};
             const int8_t* kp = keys[buf] + (n >> 2) * kGroup + g * 64 + (n & 3) * 16;
-            v4i kf[4][DC];
 #pragma unroll
-            for (int k = 0; k < DC; ++k)
+            for (int i = 0; i < 4; ++i) {
+                v4i kf[DC];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    kf[i][k] = *reinterpret_cast<const v4i*>(kp + (4 * k + i) * 256);
-#pragma unroll
-            for (int q = 0; q < NQ; ++q) {
+                for (int k = 0; k < DC; ++k) kf[k] = *reinterpret_cast<const v4i*>(kp + (4 * k + i) * 256);
 #pragma unroll
                 for (int k = 0; k < DC; ++k)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[q][i] = product(kf[i][k], rows.qh[q][k], s[q][i]);
+                    for (int q = 0; q < NQ; ++q) s[q][i] = product(kf[k], rows.qh[q][k], s[q][i]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[q][i] = times256(s[q][i]);
+                for (int q = 0; q < NQ; ++q) s[q][i] = times256(s[q][i]);
 #pragma unroll
                 for (int k = 0; k < DC; ++k)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[q][i] = product(kf[i][k], rows.ql[q][k], s[q][i]);
+                    for (int q = 0; q < NQ; ++q) s[q][i] = product(kf[k], rows.ql[q][k], s[q][i]);
             }
+            __builtin_amdgcn_sched_barrier(0);
             const bool valid = pages.valid(bv);
             const float ks = sc.x, v_scale = fmaxf(sc.y, kLeastScale);
             const float lv = __builtin_amdgcn_logf(v_scale), rv = __builtin_amdgcn_rcpf(v_scale);
+            v4f x[NQ][4];
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) to_float(s[q], x[q]);
+            if (!__all(valid && rows.see_all(j0))) {
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) hide(x[q], valid ? rows.seen(q, j0 + key_v) : 0u);
+            }
             v8h p[NQ][2];
-            auto weigh = [&](auto masked) {
-                constexpr bool MASKED = decltype(masked)::value;
 #pragma unroll
-                for (int q = 0; q < NQ; ++q) {
-                    const float f = rows.qs[q] * ks;
-                    uint32_t seen = 0xFFFFu;
-                    if constexpr (MASKED) seen = valid ? rows.seen(q, j0 + key_v) : 0u;
-                    float m = __builtin_fmaf((float)largest<MASKED>(s[q], seen), f, lv);
-                    if constexpr (MASKED) m = seen ? m : -INFINITY;
-                    if (!__all(m <= ref[q] + kHeadroom)) {
-                        m = col_max(m);
-                        const float next = m > ref[q] + kHeadroom ? m : ref[q];
-                        const float keep = next == -INFINITY ? 1.f : fast_exp2(ref[q] - next);
-                        l_run[q] *= keep;
+            for (int q = 0; q < NQ; ++q) {
+                const float f = fmaxf(rows.qs[q] * ks, kLeastFactor);
+                float m = __builtin_fmaf(largest(x[q]), f, lv);
+                if (!__all(m <= ref[q] + kHeadroom)) {
+                    m = col_max(m);
+                    const float next = m > ref[q] + kHeadroom ? m : ref[q];
+                    const float keep = fast_exp2(ref[q] - next);
+                    l_run[q] *= keep;
 #pragma unroll
-                        for (int i = 0; i < DM; ++i)
+                    for (int i = 0; i < DM; ++i)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) o[q][i][r] *= keep;
-                        ref[q] = next;
-                    }
-                    const float base = lv - (MASKED && ref[q] == -INFINITY ? 0.f : ref[q]);
-                    float sum = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            float e = fast_exp2(__builtin_fmaf((float)s[q][i][r], f, base));
-                            if constexpr (MASKED) e = seen >> (4 * i + r) & 1 ? e : 0.f;
-                            sum += e;
-                            p[q][i >> 1][4 * (i & 1) + r] = (_Float16)e;
-                        }
-                    l_run[q] = __builtin_fmaf(sum, rv, l_run[q]);
+                        for (int r = 0; r < 4; ++r) o[q][i][r] *= keep;
+                    ref[q] = next;
                 }
-            };
-            if (__all(valid && rows.see_all(j0))) weigh(std::false_type{});
-            else weigh(std::true_type{});
+                const float base = lv - ref[q];
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float e = fast_exp2(__builtin_fmaf(x[q][i][r], f, base));
+                        sum += e;
+                        p[q][i >> 1][4 * (i & 1) + r] = (_Float16)e;
+                    }
+                l_run[q] = __builtin_fmaf(sum, rv, l_run[q]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
             const v8h* vp = reinterpret_cast<const v8h*>(values[buf]) + lane;
 #pragma unroll
             for (int i = 0; i < DM; ++i)
