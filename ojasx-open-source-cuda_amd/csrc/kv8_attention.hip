@@ -452,17 +452,21 @@ __device__ __forceinline__ void key_range(const AttnArgs& a, const Cut& c, const
 // scores of one group (one block: one pair of scales), and their weights are the second operand
 // of the value products as they come.  The workgroup's waves take every fourth 64 keys of a
 // 16 NQ row tile and join their results in LDS.
+template <int DC, int NQ> struct KeyShared {
+    static constexpr int kLd = 64 * DC + 4;
+    float joined[kWaves * 16 * NQ * kLd];
+    float m[kWaves][16 * NQ], l[kWaves][16 * NQ];
+};
+
 template <int DT, int DC, int NQ>
-__global__ __launch_bounds__(kThreads) void key_kernel(AttnArgs a, Cut c) {
-    constexpr int DP = 64 * DC, DM = DP / 16;
-    constexpr int LD = DP + 4;
-    __shared__ float joined[kWaves * 16 * NQ * LD];
-    __shared__ float wave_m[kWaves][16 * NQ], wave_l[kWaves][16 * NQ];
+__device__ __forceinline__ void key_item(const AttnArgs& a, const Cut& c, int block,
+                                         KeyShared<DC, NQ>& sh) {
+    constexpr int DP = 64 * DC, DM = DP / 16, LD = KeyShared<DC, NQ>::kLd;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
     const int items = c.tiles * c.subs * a.shape.kv_heads;
     Item it;
-    it.split = blockIdx.x / items;
-    const int id = blockIdx.x - it.split * items;
+    it.split = block / items;
+    const int id = block - it.split * items;
     if (!find_item<false>(a, c, id, it)) return;
     const int64_t item_rows = ((int64_t)it.split * items + id) * c.rows;
     int t0, t1, end_key;
@@ -612,20 +616,20 @@ __global__ __launch_bounds__(kThreads) void key_kernel(AttnArgs a, Cut c) {
     for (int q = 0; q < NQ; ++q) {
         l_run[q] = col_sum(l_run[q]);
         if (g == 0) {
-            wave_m[wave][16 * q + n] = m_run[q];
-            wave_l[wave][16 * q + n] = l_run[q];
+            sh.m[wave][16 * q + n] = m_run[q];
+            sh.l[wave][16 * q + n] = l_run[q];
         }
     }
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
         const int row = 16 * q + n;
-        float m = wave_m[0][row];
+        float m = sh.m[0][row];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) m = fmaxf(m, wave_m[w][row]);
+        for (int w = 1; w < kWaves; ++w) m = fmaxf(m, sh.m[w][row]);
         const float keep = fast_exp2(m_run[q] - m);
         if (rows.live[q]) {
-            float* p = joined + (wave * 16 * NQ + row) * LD + 4 * g;
+            float* p = sh.joined + (wave * 16 * NQ + row) * LD + 4 * g;
 #pragma unroll
             for (int i = 0; i < DM; ++i) *reinterpret_cast<v4f*>(p + 16 * i) = o[q][i] * keep;
         }
@@ -633,7 +637,7 @@ __global__ __launch_bounds__(kThreads) void key_kernel(AttnArgs a, Cut c) {
         float l = 0.f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w)
-            l = __builtin_fmaf(wave_l[w][row], fast_exp2(wave_m[w][row] - m), l);
+            l = __builtin_fmaf(sh.l[w][row], fast_exp2(sh.m[w][row] - m), l);
         l_run[q] = l;
         m_run[q] = m;
     }
@@ -641,18 +645,18 @@ __global__ __launch_bounds__(kThreads) void key_kernel(AttnArgs a, Cut c) {
     if (wave == 0 && g == 0) {
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
-            wave_m[0][16 * q + n] = rows.bad[q] && l_run[q] > 0.f ? nan : m_run[q];
-            wave_l[0][16 * q + n] = l_run[q];
+            sh.m[0][16 * q + n] = rows.bad[q] && l_run[q] > 0.f ? nan : m_run[q];
+            sh.l[0][16 * q + n] = l_run[q];
         }
     }
     __syncthreads();
     for (int u = threadIdx.x; u < it.rows * (DP / 4); u += kThreads) {
         const int row = u / (DP / 4), d = (u - row * (DP / 4)) * 4;
-        const float m = wave_m[0][row], l = wave_l[0][row];
-        v4f sum = *reinterpret_cast<const v4f*>(joined + row * LD + d);
+        const float m = sh.m[0][row], l = sh.l[0][row];
+        v4f sum = *reinterpret_cast<const v4f*>(sh.joined + row * LD + d);
 #pragma unroll
         for (int w = 1; w < kWaves; ++w)
-            sum += *reinterpret_cast<const v4f*>(joined + (w * 16 * NQ + row) * LD + d);
+            sum += *reinterpret_cast<const v4f*>(sh.joined + (w * 16 * NQ + row) * LD + d);
         if (c.splits > 1) {
             if (d == 0) c.ml[item_rows + row] = make_float2(m, l);
             if (l > 0.f) *reinterpret_cast<v4f*>(c.part + (item_rows + row) * DP + d) = sum;
@@ -695,17 +699,22 @@ __device__ __forceinline__ void halves_of(uint32_t codes, uint32_t& a, uint32_t&
 // the sums are scaled again rarely.
 constexpr float kHeadroom = 8.f;
 
+template <int DC> struct RowShared {
+    // bytes of 16 keys: groups begin in different banks
+    static constexpr int kGroup = 16 * 64 * DC + 64;
+    int8_t keys[2][4 * kGroup];
+    _Float16 values[2][64 * 64 * DC];
+};
+
 template <int DT, int DC>
-__global__ __launch_bounds__(kThreads, DC <= 2 ? 2 : 1) void row_tile_kernel(AttnArgs a, Cut c) {
-    constexpr int NQ = 2, DP = 64 * DC, DM = DP / 16;
-    constexpr int kGroup = 16 * DP + 64;  // bytes of 16 keys: groups begin in different banks
-    __shared__ __align__(16) int8_t keys[2][4 * kGroup];
-    __shared__ __align__(16) _Float16 values[2][64 * DP];
+__device__ __forceinline__ void row_item(const AttnArgs& a, const Cut& c, int block,
+                                         RowShared<DC>& sh) {
+    constexpr int NQ = 2, DP = 64 * DC, DM = DP / 16, kGroup = RowShared<DC>::kGroup;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
     const int items = c.tiles * c.subs * a.shape.kv_heads;
     Item it;
-    it.split = blockIdx.x / items;
-    const int id = blockIdx.x - it.split * items;
+    it.split = block / items;
+    const int id = block - it.split * items;
     if (!find_item<true>(a, c, id, it)) return;
     const int64_t item_rows = ((int64_t)it.split * items + id) * c.rows;
     int t0, t1, end_key;
@@ -738,11 +747,11 @@ __global__ __launch_bounds__(kThreads, DC <= 2 ? 2 : 1) void row_tile_kernel(Att
 #pragma unroll
         for (int i = 0; i < DC; ++i) {
             const int group = piece_key(i) >> 4, in = piece_in(i);
-            *reinterpret_cast<v4i*>(keys[buf] + group * kGroup + in * 16) = kr[i];
+            *reinterpret_cast<v4i*>(sh.keys[buf] + group * kGroup + in * 16) = kr[i];
             uint32_t w[8];
 #pragma unroll
             for (int j = 0; j < 4; ++j) halves_of((uint32_t)vr[i][j], w[2 * j], w[2 * j + 1]);
-            uint4* p = reinterpret_cast<uint4*>(values[buf]) + (in >> 4) * 128 + group * 16 + (in & 15);
+            uint4* p = reinterpret_cast<uint4*>(sh.values[buf]) + (in >> 4) * 128 + group * 16 + (in & 15);
             p[0] = make_uint4(w[0], w[1], w[2], w[3]);
             p[64] = make_uint4(w[4], w[5], w[6], w[7]);
         }
@@ -802,7 +811,7 @@ __global__ __launch_bounds__(kThreads, DC <= 2 ? 2 : 1) void row_tile_kernel(Att
             for (int q = 0; q < NQ; ++q)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[q][i] = v4i{0, 0, 0, 0};
-            const int8_t* kp = keys[buf] + (n >> 2) * kGroup + g * 64 + (n & 3) * 16;
+            const int8_t* kp = sh.keys[buf] + (n >> 2) * kGroup + g * 64 + (n & 3) * 16;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 v4i kf[DC];
@@ -859,7 +868,7 @@ __global__ __launch_bounds__(kThreads, DC <= 2 ? 2 : 1) void row_tile_kernel(Att
                 l_run[q] = __builtin_fmaf(sum, rv, l_run[q]);
             }
             __builtin_amdgcn_sched_barrier(0);
-            const v8h* vp = reinterpret_cast<const v8h*>(values[buf]) + lane;
+            const v8h* vp = reinterpret_cast<const v8h*>(sh.values[buf]) + lane;
 #pragma unroll
             for (int i = 0; i < DM; ++i)
 #pragma unroll
@@ -913,23 +922,44 @@ __global__ __launch_bounds__(kThreads, DC <= 2 ? 2 : 1) void row_tile_kernel(Att
     }
 }
 
-// Joins the splits of an item, a wave per row: lane s has split s's maximum and sum.
+// What a launch does: every block of a batch whose requests all have few rows (Few1, Few2: up to
+// 16 or 32) or all have many is of one kind; in a mixed batch the first `row_blocks` take the
+// requests of many rows, the others those of up to 16.
+enum class Mix { Few1, Few2, Many, Both };
+
+template <int DT, int DC, Mix MIX>
+__global__ __launch_bounds__(kThreads, DC <= 2 && MIX != Mix::Few2 ? 2 : 1) void attend_kernel(
+    AttnArgs a, Cut key, Cut row, int row_blocks) {
+    constexpr int NQ = MIX == Mix::Few2 ? 2 : 1;
+    constexpr size_t few = MIX == Mix::Many ? 0 : sizeof(KeyShared<DC, NQ>);
+    constexpr size_t many = MIX == Mix::Many || MIX == Mix::Both ? sizeof(RowShared<DC>) : 0;
+    __shared__ __align__(16) char lds[few > many ? few : many];
+    if constexpr (MIX == Mix::Many || MIX == Mix::Both) {
+        if (MIX == Mix::Many || (int)blockIdx.x < row_blocks)
+            return row_item<DT, DC>(a, row, blockIdx.x, *reinterpret_cast<RowShared<DC>*>(lds));
+    }
+    if constexpr (MIX != Mix::Many)
+        key_item<DT, DC, NQ>(a, key, blockIdx.x - row_blocks,
+                             *reinterpret_cast<KeyShared<DC, NQ>*>(lds));
+}
+
+// Joins the splits of an item's rows from `first` on, a wave per row: lane s has split s's maximum
+// and sum.
 template <int DT, int DC, bool ROWS>
-__global__ __launch_bounds__(kThreads) void join_kernel(AttnArgs a, Cut c) {
+__device__ __forceinline__ void join_item(const AttnArgs& a, const Cut& c, int id, int first, int step) {
     constexpr int DP = 64 * DC;
     const int lane = threadIdx.x & 63;
     const int items = c.tiles * c.subs * a.shape.kv_heads;
     Item it;
-    if (!find_item<ROWS>(a, c, blockIdx.x, it)) return;
+    if (!find_item<ROWS>(a, c, id, it)) return;
     const float nan = __uint_as_float(0x7FC00000u);
-    for (int row = blockIdx.y * kWaves + (threadIdx.x >> 6); row < it.rows;
-         row += gridDim.y * kWaves) {
-        const int64_t at0 = (int64_t)blockIdx.x * c.rows + row, stride = (int64_t)items * c.rows;
-        float2 ml = make_float2(-INFINITY, 0.f);
+    for (int row = first + (threadIdx.x >> 6); row < it.rows; row += step) {
+        const int64_t at0 = (int64_t)id * c.rows + row, stride = (int64_t)items * c.rows;
+        float2 ml = make_float2(kNone, 0.f);
         if (lane < c.splits) ml = c.ml[at0 + lane * stride];
         const bool some = ml.y > 0.f;
         const bool bad = __any(some && ml.x != ml.x);
-        float m = some && !bad ? ml.x : -INFINITY;
+        float m = some && !bad ? ml.x : kNone;
 #pragma unroll
         for (int s = 32; s; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
         const float keep = some && !bad ? fast_exp2(ml.x - m) : 0.f;
@@ -939,14 +969,22 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttnArgs a, Cut c) {
         float sum[DC];
 #pragma unroll
         for (int i = 0; i < DC; ++i) sum[i] = 0.f;
-        uint64_t used = __ballot(some && !bad);
-        while (used) {
-            const int s = __builtin_ctzll(used);
-            used &= used - 1;
-            const float f = __shfl(keep, s);
-            const float* p = c.part + (at0 + s * stride) * DP + lane;
+        const uint64_t used = __ballot(some && !bad);
+        const float* p = c.part + at0 * DP + lane;
+        // four splits' loads at a time; one without keys has written nothing
+        for (int s0 = 0; s0 < c.splits; s0 += 4) {
+            float v[4][DC];
 #pragma unroll
-            for (int i = 0; i < DC; ++i) sum[i] = __builtin_fmaf(p[64 * i], f, sum[i]);
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < DC; ++i)
+                    v[j][i] = used >> (s0 + j) & 1 ? p[(s0 + j) * stride * DP + 64 * i] : 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float f = __shfl(keep, s0 + j);
+#pragma unroll
+                for (int i = 0; i < DC; ++i) sum[i] = __builtin_fmaf(v[j][i], f, sum[i]);
+            }
         }
         int tok, head;
         row_at(a, c, it, row, tok, head);
@@ -962,7 +1000,27 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttnArgs a, Cut c) {
     }
 }
 
+constexpr int kRowJoins = 8;  // workgroups of an item of many rows
+
+template <int DT, int DC>
+__global__ __launch_bounds__(kThreads) void join_kernel(AttnArgs a, Cut key, Cut row, int row_blocks) {
+    const int b = blockIdx.x;
+    if (b < row_blocks)
+        return join_item<DT, DC, true>(a, row, b / kRowJoins, b % kRowJoins * kWaves,
+                                       kRowJoins * kWaves);
+    join_item<DT, DC, false>(a, key, b - row_blocks, 0, kWaves);
+}
+
 // ---------------------------------------------------------------- how a call is cut
+
+constexpr int kRowTile = 32 * kWaves;
+constexpr int64_t kKeyBlocks = 4096, kRowBlocks = 512;
+
+struct Plan {
+    Mix mix;
+    Cut key, row;
+    bool has_key, has_row;
+};
 
 int64_t item_count(const Cut& c, const AttnShape& s) {
     return (int64_t)c.tiles * c.subs * s.kv_heads;
@@ -971,95 +1029,110 @@ int64_t item_count(const Cut& c, const AttnShape& s) {
 // 64-key tiles of the longest range that rows of `tok` tokens see.
 int64_t key_tiles(const AttnShape& s, int tok) {
     int64_t keys = s.max_seq;
-    if (s.window && s.window + tok < keys) keys = s.window + tok;
+    if (s.window && (int64_t)s.window + tok < keys) keys = s.window + tok;
     return (keys + 63) / 64 + 1;
 }
 
-void set_splits(Cut& c, const AttnShape& s, int64_t target, int least) {
+void set_cut(Cut& c, const AttnShape& s, int rows, int tiles_more) {
+    const int group = s.heads / s.kv_heads;
+    c.rows = rows;
+    c.tok = group <= rows ? rows / group : 1;
+    c.subs = group <= rows ? 1 : (group + rows - 1) / rows;
+    c.tiles = s.requests + (tiles_more ? s.tokens / c.tok : 0);
+}
+
+void set_splits(Cut& c, const AttnShape& s, int64_t blocks, int64_t least) {
     const int64_t items = item_count(c, s), tiles = key_tiles(s, c.tok);
-    int64_t n = items > 0 ? (target + items - 1) / items : 1;
+    int64_t n = items > 0 ? (blocks + items - 1) / items : 1;
     if (n > (tiles + least - 1) / least) n = (tiles + least - 1) / least;
     if (n > kMaxSplits) n = kMaxSplits;
     c.splits = n < 1 ? 1 : (int)n;
-    c.least = least;
+    c.least = (int)least;
 }
 
-// Rows of a request that the key-splitting launch takes: up to two 16-row columns.
-int key_rows(const AttnShape& s) {
-    const int64_t group = s.heads / s.kv_heads;
-    const int64_t most = group * (s.max_query < 32 / group ? s.max_query : 32 / group);
-    return (group <= 16 && most <= 16) ? 16 : 32;
-}
-
-Cut key_cut(const AttnShape& s) {
+Plan plan_of(const AttnShape& s) {
+    Plan p{};
     const int group = s.heads / s.kv_heads;
-    Cut c{};
-    c.rows = key_rows(s);
-    c.tok = group <= c.rows ? c.rows / group : 1;
-    c.subs = group <= c.rows ? 1 : (group + c.rows - 1) / c.rows;
-    c.tiles = s.requests;
-    c.small = c.tok;
-    set_splits(c, s, 8192, 4);
-    return c;
+    const int64_t most = (int64_t)s.max_query * group;  // rows of a request and key head
+    const bool one = s.max_query <= 1;
+    p.mix = most <= 16 || (one && group % 32 >= 1 && group % 32 <= 16) ? Mix::Few1
+            : most <= 32 || one                                       ? Mix::Few2
+            // all requests of the longest length?
+            : (int64_t)s.requests * s.max_query == s.tokens ? Mix::Many
+                                                            : Mix::Both;
+    p.has_key = p.mix != Mix::Many;
+    p.has_row = p.mix == Mix::Many || p.mix == Mix::Both;
+    if (p.has_key) {
+        set_cut(p.key, s, p.mix == Mix::Few2 ? 32 : 16, 0);
+        p.key.small = p.mix == Mix::Both ? p.key.tok : INT32_MAX;
+        // Splits down to one tile a wave where the batch is too small to fill the GPU (one token
+        // over 2048 keys: 9.7 us at 4 tiles a split, 12.6 at 16, 17.2 unsplit), eight a wave where
+        // it does (64 tokens over up to 16000: 132 us at 32, 157 at 4, whose waves mostly start
+        // up and join).
+        int64_t least = item_count(p.key, s) * key_tiles(s, p.key.tok) / 2048;
+        least = least < 4 ? 4 : least > 32 ? 32 : least;
+        set_splits(p.key, s, kKeyBlocks, least);
+    }
+    if (p.has_row) {
+        set_cut(p.row, s, kRowTile, 1);
+        p.row.small = p.has_key ? p.key.small : 0;
+        // Only what does not fill the GPU is split: prompts of 6000 tokens in all take 439 us with
+        // 512 blocks, 487 cut to 2048.
+        set_splits(p.row, s, kRowBlocks, 16);
+    }
+    return p;
 }
 
-constexpr int kRowTile = 32 * kWaves;
-
-Cut row_cut(const AttnShape& s, int small) {
-    const int group = s.heads / s.kv_heads;
-    Cut c{};
-    c.rows = kRowTile;
-    c.tok = group <= c.rows ? c.rows / group : 1;
-    c.subs = group <= c.rows ? 1 : (group + c.rows - 1) / c.rows;
-    c.tiles = s.tokens / c.tok + s.requests;
-    c.small = small;
-    set_splits(c, s, 512, 16);
-    return c;
-}
-
-bool has_key_launch(const AttnShape& s, const Cut& key) {
-    // all requests of the longest length: every one is the other launch's
-    return s.max_query <= key.small || (int64_t)s.requests * s.max_query != s.tokens;
-}
-
-size_t cut_bytes(const Cut& c, const AttnShape& s) {
-    if (c.splits <= 1) return 0;
-    const size_t rows = (size_t)c.splits * item_count(c, s) * c.rows;
+size_t split_bytes(const Cut& c, const AttnShape& s) {  // of one split
+    const size_t rows = (size_t)item_count(c, s) * c.rows;
     return rows * ((s.d + 63) / 64 * 64 * sizeof(float) + sizeof(float2));
 }
 
+size_t cut_bytes(const Cut& c, const AttnShape& s) {
+    return c.splits > 1 ? c.splits * split_bytes(c, s) : 0;
+}
+
+// The cut's part of the workspace, which it moves past; fewer splits where it is too small.
+void place(Cut& c, const AttnShape& s, char*& ws, size_t& left) {
+    if (c.splits <= 1) return;
+    const size_t per = split_bytes(c, s), fit = left / per;
+    if ((size_t)c.splits > fit) c.splits = fit < 2 ? 1 : (int)fit;
+    if (c.splits <= 1) return;
+    const size_t rows = (size_t)c.splits * item_count(c, s) * c.rows;
+    c.part = reinterpret_cast<float*>(ws);
+    c.ml = reinterpret_cast<float2*>(c.part + rows * ((s.d + 63) / 64 * 64));
+    ws += c.splits * per;
+    left -= c.splits * per;
+}
+
 template <int DT, int DC>
-hipError_t run(const AttnArgs& a, Cut c, bool by_rows, void* ws, size_t ws_bytes, hipStream_t stream) {
-    const int64_t items = item_count(c, a.shape);
-    if (items == 0) return hipSuccess;
-    if (c.splits > 1) {
-        const size_t per = cut_bytes(c, a.shape) / c.splits;
-        const size_t fit = ws ? ws_bytes / per : 0;
-        if ((size_t)c.splits > fit) c.splits = fit < 2 ? 1 : (int)fit;
-        c.part = static_cast<float*>(ws);
-        c.ml = reinterpret_cast<float2*>(c.part + (size_t)c.splits * items * c.rows * 64 * DC);
+hipError_t run(const AttnArgs& a, const Plan& p, hipStream_t stream) {
+    const int64_t row_blocks = p.has_row ? item_count(p.row, a.shape) * p.row.splits : 0;
+    const int64_t key_blocks = p.has_key ? item_count(p.key, a.shape) * p.key.splits : 0;
+    if (row_blocks + key_blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
+    const dim3 g((unsigned)(row_blocks + key_blocks)), b(kThreads);
+    const int rb = (int)row_blocks;
+    switch (p.mix) {
+        case Mix::Few1: attend_kernel<DT, DC, Mix::Few1><<<g, b, 0, stream>>>(a, p.key, p.row, rb); break;
+        case Mix::Few2: attend_kernel<DT, DC, Mix::Few2><<<g, b, 0, stream>>>(a, p.key, p.row, rb); break;
+        case Mix::Many: attend_kernel<DT, DC, Mix::Many><<<g, b, 0, stream>>>(a, p.key, p.row, rb); break;
+        case Mix::Both: attend_kernel<DT, DC, Mix::Both><<<g, b, 0, stream>>>(a, p.key, p.row, rb); break;
     }
-    if (items * c.splits > 0x7FFFFFFF) return hipErrorInvalidValue;
-    const dim3 g((unsigned)(items * c.splits)), b(kThreads);
-    if (by_rows) row_tile_kernel<DT, DC><<<g, b, 0, stream>>>(a, c);
-    else if (c.rows == 16) key_kernel<DT, DC, 1><<<g, b, 0, stream>>>(a, c);
-    else key_kernel<DT, DC, 2><<<g, b, 0, stream>>>(a, c);
-    if (c.splits > 1) {
-        const dim3 gj((unsigned)items, by_rows ? 8 : 1);
-        if (by_rows) join_kernel<DT, DC, true><<<gj, b, 0, stream>>>(a, c);
-        else join_kernel<DT, DC, false><<<gj, b, 0, stream>>>(a, c);
-    }
+    const int64_t row_joins = p.has_row && p.row.splits > 1 ? item_count(p.row, a.shape) * kRowJoins : 0;
+    const int64_t key_joins = p.has_key && p.key.splits > 1 ? item_count(p.key, a.shape) : 0;
+    if (row_joins + key_joins > 0x7FFFFFFF) return hipErrorInvalidValue;
+    if (row_joins + key_joins > 0)
+        join_kernel<DT, DC><<<(unsigned)(row_joins + key_joins), b, 0, stream>>>(a, p.key, p.row,
+                                                                               (int)row_joins);
     return hipGetLastError();
 }
 
-template <int DT>
-hipError_t run(const AttnArgs& a, const Cut& c, bool by_rows, void* ws, size_t ws_bytes,
-               hipStream_t stream) {
+template <int DT> hipError_t run(const AttnArgs& a, const Plan& p, hipStream_t stream) {
     switch (a.cache.dp / 64) {
-        case 1: return run<DT, 1>(a, c, by_rows, ws, ws_bytes, stream);
-        case 2: return run<DT, 2>(a, c, by_rows, ws, ws_bytes, stream);
-        case 3: return run<DT, 3>(a, c, by_rows, ws, ws_bytes, stream);
-        default: return run<DT, 4>(a, c, by_rows, ws, ws_bytes, stream);
+        case 1: return run<DT, 1>(a, p, stream);
+        case 2: return run<DT, 2>(a, p, stream);
+        case 3: return run<DT, 3>(a, p, stream);
+        default: return run<DT, 4>(a, p, stream);
     }
 }
 
@@ -1067,13 +1140,8 @@ hipError_t run(const AttnArgs& a, const Cut& c, bool by_rows, void* ws, size_t w
 
 size_t kv8_attention_bytes(const AttnShape& s) {
     if (s.dtype == kF32 || s.tokens == 0 || s.requests == 0) return 0;
-    const Cut key = key_cut(s);
-    size_t n = has_key_launch(s, key) ? cut_bytes(key, s) : 0;
-    if (s.max_query > key.small) {
-        const size_t r = cut_bytes(row_cut(s, key.small), s);
-        n = r > n ? r : n;  // one after the other on the stream
-    }
-    return n;
+    const Plan p = plan_of(s);
+    return (p.has_key ? cut_bytes(p.key, s) : 0) + (p.has_row ? cut_bytes(p.row, s) : 0);
 }
 
 hipError_t launch_kv8_attention(const AttnArgs& args, void* ws, size_t ws_bytes,
@@ -1086,17 +1154,12 @@ hipError_t launch_kv8_attention(const AttnArgs& args, void* ws, size_t ws_bytes,
         row_kernel<kF32><<<(unsigned)rows, 64, 0, stream>>>(a);
         return hipGetLastError();
     }
-    const Cut key = key_cut(a.shape);
-    hipError_t e = hipSuccess;
-    if (has_key_launch(a.shape, key))
-        e = a.shape.dtype == kF16 ? run<kF16>(a, key, false, ws, ws_bytes, stream)
-                                  : run<kBF16>(a, key, false, ws, ws_bytes, stream);
-    if (e == hipSuccess && a.shape.max_query > key.small) {
-        const Cut rows = row_cut(a.shape, key.small);
-        e = a.shape.dtype == kF16 ? run<kF16>(a, rows, true, ws, ws_bytes, stream)
-                                  : run<kBF16>(a, rows, true, ws, ws_bytes, stream);
-    }
-    return e;
+    Plan p = plan_of(a.shape);
+    char* at = static_cast<char*>(ws);
+    size_t left = ws ? ws_bytes : 0;
+    if (p.has_key) place(p.key, a.shape, at, left);
+    if (p.has_row) place(p.row, a.shape, at, left);
+    return a.shape.dtype == kF16 ? run<kF16>(a, p, stream) : run<kBF16>(a, p, stream);
 }
 
 }  // namespace ojx
