@@ -25,6 +25,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <string>
 
@@ -399,6 +400,269 @@ PyObject* decode(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------- cache, log probabilities
+
+bool kv_block(int64_t b) { return b == 16 || b == 32 || b == 64 || b == 128 || b == 256; }
+
+bool ints(const Tensor& t, at::ScalarType type, int64_t n) {
+    return t.scalar_type() == type && t.dim() == 1 && t.numel() == n && t.is_contiguous();
+}
+
+// A cache's tensors as the ops take them, for heads of size d.
+bool cache_ok(const Tensor& k, const Tensor& v, const Tensor& scales, int64_t d) {
+    return k.scalar_type() == at::kChar && v.scalar_type() == at::kChar &&
+           scales.scalar_type() == at::kFloat && k.dim() == 4 && k.sizes() == v.sizes() &&
+           scales.dim() == 3 && scales.size(0) == k.size(0) && scales.size(1) == k.size(1) &&
+           scales.size(2) == 2 && k.is_contiguous() && v.is_contiguous() &&
+           scales.is_contiguous() && kv_block(k.size(2)) && d >= 1 && d <= 256 &&
+           k.size(3) == (d + 63) / 64 * 64 && v.device() == k.device() &&
+           scales.device() == k.device();
+}
+
+PyObject* tuple_of(Tensor* ts, int n) {
+    PyObject* out = PyTuple_New(n);
+    if (!out) throw python_error();
+    for (int i = 0; i < n; ++i) PyTuple_SET_ITEM(out, i, THPVariable_Wrap(std::move(ts[i])));
+    return out;
+}
+
+bool all_plain(PyObject* const* argv, int n) {
+    if (!plain_state()) return false;
+    for (int i = 0; i < n; ++i)
+        if (!plain(argv[i])) return false;
+    return true;
+}
+
+// kv8_plan(seq_lens, new_lens, tables, free, num_free, block_size, tokens): the op's results
+PyObject* kv8_plan(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 7, "kv8_plan");
+    const Args a{argv, n};
+    if (!all_plain(argv, 5)) Py_RETURN_NONE;
+    const Tensor &seq = a.t(0), &fresh = a.t(1), &tables = a.t(2), &free = a.t(3), &left = a.t(4);
+    const int64_t block = a.i64(5), tokens = a.i64(6), r = seq.numel();
+    if (!ints(seq, at::kInt, r) || !ints(fresh, at::kInt, r) ||
+        !ints(free, at::kInt, free.numel()) || !ints(left, at::kInt, 1) ||
+        tables.scalar_type() != at::kInt || tables.dim() != 2 || tables.size(0) != r ||
+        (tables.numel() > 0 && tables.stride(1) != 1) || !kv_block(block) || tokens < 0 ||
+        fresh.device() != seq.device() || tables.device() != seq.device() ||
+        free.device() != seq.device() || left.device() != seq.device())
+        Py_RETURN_NONE;
+    RECORD_FUNCTION("ojasx_e8t::kv8_plan", std::vector<c10::IValue>());
+    Unlocked unlocked;
+    const c10::DeviceGuard on_device(seq.device());
+    const auto i32 = seq.options();
+    Tensor out[] = {at::empty({tokens}, i32.dtype(at::kLong)), at::empty({tokens}, i32),
+                    at::empty({tokens}, i32), at::empty({r + 1}, i32), at::empty({r}, i32),
+                    at::empty({1}, i32)};
+    check(ojx_kv8_plan((const int32_t*)data(seq), (const int32_t*)data(fresh), r,
+                       (int32_t*)data(tables), tables.stride(0), tables.size(1),
+                       (const int32_t*)data(free), free.numel(), (const int32_t*)data(left), block,
+                       tokens, (int64_t*)data(out[0]), (int32_t*)data(out[1]),
+                       (int32_t*)data(out[2]), (int32_t*)data(out[3]), (int32_t*)data(out[4]),
+                       (int32_t*)data(out[5]), current_stream(seq.device())),
+          "kv8_plan");
+    torch::autograd::impl::bump_version(tables);
+    unlocked.lock();
+    return tuple_of(out, 6);
+    END_HANDLE_TH_ERRORS
+}
+
+// kv8_append(k, v, slots, k_codes, v_codes, scales): True
+PyObject* kv8_append(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 6, "kv8_append");
+    const Args a{argv, n};
+    if (!all_plain(argv, 6)) Py_RETURN_NONE;
+    const Tensor &k = a.t(0), &v = a.t(1), &slots = a.t(2), &kc = a.t(3), &vc = a.t(4),
+                 &scales = a.t(5);
+    const int dt = dtype_code(k.scalar_type());
+    if (dt < 0 || v.scalar_type() != k.scalar_type() || k.dim() != 3 || k.sizes() != v.sizes() ||
+        k.stride(2) != 1 || v.stride(2) != 1 || !cache_ok(kc, vc, scales, k.size(2)) ||
+        k.size(1) != kc.size(1) || !ints(slots, at::kLong, k.size(0)) ||
+        k.device() != kc.device() || v.device() != kc.device() || slots.device() != kc.device())
+        Py_RETURN_NONE;
+    RECORD_FUNCTION("ojasx_e8t::kv8_append", std::vector<c10::IValue>());
+    Unlocked unlocked;
+    const c10::DeviceGuard on_device(kc.device());
+    check(ojx_kv8_append((int8_t*)data(kc), (int8_t*)data(vc), (float*)data(scales), kc.size(0),
+                         kc.size(1), kc.size(2), k.size(2), data(k), k.stride(0), k.stride(1),
+                         data(v), v.stride(0), v.stride(1), dt, (const int64_t*)data(slots),
+                         k.size(0), current_stream(kc.device())),
+          "kv8_append");
+    for (const Tensor* t : {&kc, &vc, &scales}) torch::autograd::impl::bump_version(*t);
+    unlocked.lock();
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// kv8_read(k_codes, v_codes, scales, blocks, head_dim, dtype): (k, v, scales), dtype a code of
+// the C ABI
+PyObject* kv8_read(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 6, "kv8_read");
+    const Args a{argv, n};
+    if (!all_plain(argv, 4)) Py_RETURN_NONE;
+    const Tensor &kc = a.t(0), &vc = a.t(1), &scales = a.t(2), &blocks = a.t(3);
+    const int64_t d = a.i64(4), m = blocks.numel();
+    const int dt = (int)a.i64(5);
+    if (dt < 0 || dt > 2 || !cache_ok(kc, vc, scales, d) || !ints(blocks, at::kInt, m) ||
+        blocks.device() != kc.device())
+        Py_RETURN_NONE;
+    RECORD_FUNCTION("ojasx_e8t::kv8_read", std::vector<c10::IValue>());
+    Unlocked unlocked;
+    const c10::DeviceGuard on_device(kc.device());
+    const at::ScalarType types[] = {at::kFloat, at::kHalf, at::kBFloat16};
+    const auto opt = kc.options().dtype(types[dt]);
+    Tensor out[] = {at::empty({m, kc.size(2), kc.size(1), d}, opt),
+                    at::empty({m, kc.size(2), kc.size(1), d}, opt),
+                    at::empty({m, kc.size(1), 2}, scales.options())};
+    check(ojx_kv8_read((const int8_t*)data(kc), (const int8_t*)data(vc),
+                       (const float*)data(scales), kc.size(0), kc.size(1), kc.size(2), d,
+                       (const int32_t*)data(blocks), m, dt, data(out[0]), data(out[1]),
+                       (float*)data(out[2]), current_stream(kc.device())),
+          "kv8_read");
+    unlocked.lock();
+    return tuple_of(out, 3);
+    END_HANDLE_TH_ERRORS
+}
+
+// kv8_attention(q, k_codes, v_codes, scales, tables, seq_lens, query_starts | None, scale, window,
+// max_query_len, max_seq_len, return_lse): (out, lse | empty)
+PyObject* kv8_attention(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 12, "kv8_attention");
+    const Args a{argv, n};
+    if (!all_plain(argv, 6) || (argv[6] != Py_None && !plain(argv[6]))) Py_RETURN_NONE;
+    const Tensor &q = a.t(0), &kc = a.t(1), &vc = a.t(2), &scales = a.t(3), &tables = a.t(4),
+                 &lens = a.t(5);
+    const Tensor starts = argv[6] == Py_None ? Tensor() : a.t(6);
+    const int dt = dtype_code(q.scalar_type());
+    const int64_t r = lens.numel(), window = a.i64(8), most = a.i64(9), longest = a.i64(10);
+    const double scale = a.f64(7);
+    if (dt < 0 || q.dim() != 3 || q.stride(2) != 1 || !cache_ok(kc, vc, scales, q.size(2)) ||
+        !ints(lens, at::kInt, r) || (starts.defined() && !ints(starts, at::kInt, r + 1)) ||
+        tables.scalar_type() != at::kInt || tables.dim() != 2 || tables.size(0) != r ||
+        (tables.numel() > 0 && tables.stride(1) != 1) || q.device() != kc.device() ||
+        tables.device() != kc.device() || lens.device() != kc.device() ||
+        (starts.defined() && starts.device() != kc.device()) ||
+        (c10::GradMode::is_enabled() && records(q)))
+        Py_RETURN_NONE;
+    RECORD_FUNCTION("ojasx_e8t::kv8_attention", std::vector<c10::IValue>());
+    Unlocked unlocked;
+    const c10::DeviceGuard on_device(kc.device());
+    const int64_t t = q.size(0), heads = q.size(1), d = q.size(2);
+    const bool with_lse = a.flag(11);
+    Tensor out[] = {at::empty({t, heads, d}, q.options()),
+                    at::empty({with_lse ? t : 0, heads}, scales.options())};
+    size_t bytes = 0;
+    check(ojx_kv8_attention_workspace_bytes(t, r, heads, kc.size(1), d, window, most, longest, dt,
+                                            &bytes),
+          "kv8_attention_workspace_bytes");
+    const Tensor ws = workspace(bytes, q);
+    check(ojx_kv8_attention(data(q), q.stride(0), q.stride(1), t, heads, dt,
+                            (const int8_t*)data(kc), (const int8_t*)data(vc),
+                            (const float*)data(scales), kc.size(0), kc.size(1), kc.size(2), d,
+                            (const int32_t*)data(tables), tables.stride(0), tables.size(1),
+                            (const int32_t*)data(lens), (const int32_t*)data(starts), r, most,
+                            longest, (float)scale, window, data(out[0]),
+                            with_lse ? (float*)data(out[1]) : nullptr, data(ws), bytes,
+                            current_stream(kc.device())),
+          "kv8_attention");
+    unlocked.lock();
+    return tuple_of(out, 2);
+    END_HANDLE_TH_ERRORS
+}
+
+// Logits [..., V] as rows with neighbouring logits, without a copy; ids as they lie.
+bool logits_ok(const Tensor& x, const Tensor& ids) {
+    if (x.dim() < 1 || x.size(-1) < 1 || ids.scalar_type() != at::kLong || !ids.is_contiguous() ||
+        ids.device() != x.device() || ids.dim() != x.dim() - 1)
+        return false;
+    for (int64_t i = 0; i < ids.dim(); ++i)
+        if (ids.size(i) != x.size(i)) return false;
+    return x.is_contiguous() || (x.dim() == 2 && x.stride(1) == 1 && x.stride(0) >= x.size(1));
+}
+int64_t row_stride(const Tensor& x) { return x.is_contiguous() ? x.size(-1) : x.stride(0); }
+
+// token_logprobs(logits, ids, top_k): the op's results
+PyObject* token_logprobs(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 3, "token_logprobs");
+    const Args a{argv, n};
+    if (!all_plain(argv, 2)) Py_RETURN_NONE;
+    const Tensor &x = a.t(0), &ids = a.t(1);
+    const int64_t top = a.i64(2);
+    const int dt = dtype_code(x.scalar_type());
+    if (dt < 0 || !logits_ok(x, ids) || top < 0 || top > 64 || top > x.size(-1) ||
+        (c10::GradMode::is_enabled() && records(x)))
+        Py_RETURN_NONE;
+    RECORD_FUNCTION("ojasx_e8t::token_logprobs", std::vector<c10::IValue>());
+    Unlocked unlocked;
+    const c10::DeviceGuard on_device(x.device());
+    const int64_t v = x.size(-1), rows = ids.numel();
+    const auto f32 = x.options().dtype(at::kFloat);
+    std::vector<int64_t> shape(ids.sizes().begin(), ids.sizes().end()), tops = shape, two = shape;
+    tops.push_back(top);
+    two.push_back(2);
+    Tensor out[] = {at::empty(shape, f32), at::empty(shape, f32), at::empty(shape, f32),
+                    at::empty(tops, f32), at::empty(tops, ids.options()), at::empty(two, f32)};
+    size_t bytes = 0;
+    check(ojx_token_logprobs_workspace_bytes(rows, v, top, dt, &bytes),
+          "token_logprobs_workspace_bytes");
+    const Tensor ws = workspace(bytes, x);
+    check(ojx_token_logprobs(data(x), row_stride(x), rows, v, dt, (const int64_t*)data(ids), top,
+                             (float*)data(out[0]), (float*)data(out[1]), (float*)data(out[2]),
+                             (float*)data(out[5]), (float*)data(out[3]), (int64_t*)data(out[4]),
+                             data(ws), bytes, current_stream(x.device())),
+          "token_logprobs");
+    unlocked.lock();
+    return tuple_of(out, 6);
+    END_HANDLE_TH_ERRORS
+}
+
+// token_logprobs_bwd(logits, ids, entropy, stats, top_ids, grad_logprob | None, grad_entropy |
+// None, grad_lse | None, grad_top | None): the logits' gradient
+PyObject* token_logprobs_bwd(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 9, "token_logprobs_bwd");
+    const Args a{argv, n};
+    if (!all_plain(argv, 5) || c10::GradMode::is_enabled()) Py_RETURN_NONE;
+    const Tensor &x = a.t(0), &ids = a.t(1), &h = a.t(2), &stats = a.t(3), &top_ids = a.t(4);
+    const int dt = dtype_code(x.scalar_type());
+    const int64_t rows = ids.numel(), top = top_ids.dim() ? top_ids.size(-1) : 0;
+    auto floats = [&](const Tensor& t, int64_t count) {
+        return t.scalar_type() == at::kFloat && t.is_contiguous() && t.numel() == count &&
+               t.device() == x.device();
+    };
+    if (dt < 0 || !logits_ok(x, ids) || !floats(h, rows) || !floats(stats, 2 * rows) ||
+        top_ids.scalar_type() != at::kLong || top_ids.dim() != ids.dim() + 1 ||
+        top_ids.numel() != rows * top || !top_ids.is_contiguous() ||
+        top_ids.device() != x.device())
+        Py_RETURN_NONE;
+    Tensor g[4];
+    for (int i = 0; i < 4; ++i) {
+        if (argv[5 + i] == Py_None) continue;
+        if (!plain(argv[5 + i])) Py_RETURN_NONE;
+        g[i] = a.t(5 + i);
+        if (!floats(g[i], i < 3 ? rows : rows * top)) Py_RETURN_NONE;
+    }
+    RECORD_FUNCTION("ojasx_e8t::token_logprobs_bwd", std::vector<c10::IValue>());
+    Unlocked unlocked;
+    const c10::DeviceGuard on_device(x.device());
+    Tensor gx = at::empty(x.sizes(), x.options());
+    check(ojx_token_logprobs_bwd(data(x), row_stride(x), rows, x.size(-1), dt,
+                                 (const int64_t*)data(ids), (const float*)data(h),
+                                 (const float*)data(stats), top, (const int64_t*)data(top_ids),
+                                 (const float*)data(g[0]), (const float*)data(g[1]),
+                                 (const float*)data(g[2]), (const float*)data(g[3]), data(gx),
+                                 current_stream(x.device())),
+          "token_logprobs_bwd");
+    unlocked.lock();
+    return THPVariable_Wrap(std::move(gx));
+    END_HANDLE_TH_ERRORS
+}
+
 // plain(tensor, ...): whether a Function over these tensors is plain eager work (grad aside)
 PyObject* is_plain(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -416,6 +680,12 @@ PyMethodDef kMethods[] = {
     {"linear_lora_bwd", (PyCFunction)(void*)linear_lora_bwd, METH_FASTCALL, nullptr},
     {"encode", (PyCFunction)(void*)encode, METH_FASTCALL, nullptr},
     {"decode", (PyCFunction)(void*)decode, METH_FASTCALL, nullptr},
+    {"kv8_plan", (PyCFunction)(void*)kv8_plan, METH_FASTCALL, nullptr},
+    {"kv8_append", (PyCFunction)(void*)kv8_append, METH_FASTCALL, nullptr},
+    {"kv8_read", (PyCFunction)(void*)kv8_read, METH_FASTCALL, nullptr},
+    {"kv8_attention", (PyCFunction)(void*)kv8_attention, METH_FASTCALL, nullptr},
+    {"token_logprobs", (PyCFunction)(void*)token_logprobs, METH_FASTCALL, nullptr},
+    {"token_logprobs_bwd", (PyCFunction)(void*)token_logprobs_bwd, METH_FASTCALL, nullptr},
     {"is_plain", (PyCFunction)(void*)is_plain, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

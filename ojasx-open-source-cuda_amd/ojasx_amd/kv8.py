@@ -19,7 +19,13 @@ from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 
+from . import _native as N
 from . import serve_ops as S
+
+
+def _eager(name: str, *args):
+    """The call in native code where it is plain eager work, else None (csrc/e8t_torch.cpp)."""
+    return None if torch.compiler.is_compiling() else getattr(N.eager(), name)(*args)
 
 
 class KV8Plan(NamedTuple):
@@ -44,8 +50,8 @@ def plan(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torch.Ten
     ``new_lens`` or more (a padded batch); of more new tokens only the first ``num_tokens`` get
     their place.
     """
-    return KV8Plan(*S.kv8_plan(seq_lens, new_lens, block_tables, free_blocks, num_free, block_size,
-                               num_tokens))
+    args = (seq_lens, new_lens, block_tables, free_blocks, num_free, block_size, num_tokens)
+    return KV8Plan(*(_eager("kv8_plan", *args) or S.kv8_plan(*args)))
 
 
 def append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_codes: torch.Tensor,
@@ -55,14 +61,18 @@ def append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_codes: torch
     A block's scale covers the largest element it was given; where a later token raises it, the
     codes that are there already are rounded again.  Slots outside the cache (-1) are skipped.
     """
-    S.kv8_append(k, v, slots, k_codes, v_codes, scales)
+    args = (k, v, slots, k_codes, v_codes, scales)
+    if _eager("kv8_append", *args) is None:
+        S.kv8_append(*args)
 
 
 def read(k_codes: torch.Tensor, v_codes: torch.Tensor, scales: torch.Tensor, blocks: torch.Tensor,
          head_dim: int, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Keys and values of whole blocks, ``[n, block_size, kv heads, head size]`` in ``dtype``, and
     the blocks' scales ``[n, kv heads, 2]``."""
-    return S.kv8_read(k_codes, v_codes, scales, blocks, head_dim, dtype)
+    args = (k_codes, v_codes, scales, blocks, head_dim)
+    out = _eager("kv8_read", *args, N.DTYPE_CODE.get(dtype, -1))
+    return S.kv8_read(*args, dtype) if out is None else out
 
 
 def attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, scales: torch.Tensor,
@@ -86,8 +96,9 @@ def attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, sca
         max_query_len = 1 if query_starts is None else q.shape[0]
     if max_seq_len is None:
         max_seq_len = block_tables.shape[-1] * k_codes.shape[2]
-    out, lse = S.kv8_attention(q, k_codes, v_codes, scales, block_tables, seq_lens, query_starts,
-                               scale, window, max_query_len, max_seq_len, return_lse)
+    args = (q, k_codes, v_codes, scales, block_tables, seq_lens, query_starts, float(scale), window,
+            max_query_len, max_seq_len, return_lse)
+    out, lse = _eager("kv8_attention", *args) or S.kv8_attention(*args)
     return (out, lse) if return_lse else out
 
 
