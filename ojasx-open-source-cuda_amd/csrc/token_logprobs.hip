@@ -53,7 +53,7 @@ template <class T, class F> __device__ T block_reduce(T v, T* shared, F f) {
 // by a type's lowest value, say): one workgroup, one pass for the maximum, one for the sums,
 // one per alternative.
 template <int DT>
-__device__ __noinline__ void odd_row(const LogprobArgs& a, int row, float* sf, uint64_t* sk) {
+__device__ __forceinline__ void odd_row(const LogprobArgs& a, int row, float* sf, uint64_t* sk) {
     const int v = a.vocab;
     const int64_t x0 = row * a.ld;
     auto add = [](float p, float q) { return p + q; };
@@ -169,11 +169,12 @@ __device__ __forceinline__ void insert(Best& b, uint64_t key, int k, int lane) {
     b.key = lane < at ? b.key : lane == at ? key : up;
 }
 
-// The k-th largest of the lanes' values (0 where fewer than k lanes have one above 0).
-__device__ __forceinline__ uint32_t kth_of_lanes(uint32_t v, int k) {
+// A bound that k lanes' values reach: their k-th largest in its `BITS` leading bits, the others 0
+// (0 where fewer than k lanes have a value above 0).
+template <int BITS> __device__ __forceinline__ uint32_t kth_of_lanes(uint32_t v, int k) {
     uint32_t t = 0;
 #pragma unroll 1
-    for (int bit = 31; bit >= 0; --bit) {
+    for (int bit = 31; bit >= 32 - BITS; --bit) {
         const uint32_t c = t | 1u << bit;
         if (__popcll(__ballot(v >= c)) >= k) t = c;
     }
@@ -248,12 +249,19 @@ __device__ __forceinline__ void take(Best& best, const Batch<DT>& x, float lane_
     const bool may = !best.full || lane_max > best.least;
     const uint64_t lanes = __ballot(may);
     if (!lanes) return;
-    uint32_t cut = 0;
-    if (__popcll(lanes) > k) cut = kth_of_lanes(may ? ordered(lane_max) : 0u, k);
+    float cut = -INFINITY;
+    if (__popcll(lanes) >= k) {
+        // sign, exponent and fraction of the type; fp32 in full
+        constexpr int bits = DT == kBF16 ? 16 : DT == kF16 ? 19 : 32;
+        const uint32_t t = kth_of_lanes<bits>(may ? ordered(lane_max) : 0u, k);
+        if (t > 0x007FFFFFu) cut = unordered(t);  // above -inf
+    }
+    const uint64_t open = best.full ? 0ull : ~0ull;
 #pragma unroll
     for (int i = 0; i < kLaneLogits; ++i) {
         const float f = x.get(i);
-        uint64_t c = __ballot((!best.full || f > best.least) && ordered(f) >= cut);
+        uint64_t c = __ballot(f >= cut) & (__ballot(f > best.least) | open);
+        if (!c) continue;
         const uint64_t key = key_of(f, Batch<DT>::index(b, i, lane, shift));
         while (c) {
             const int from = __builtin_ctzll(c);
@@ -375,10 +383,12 @@ __global__ __launch_bounds__(kThreads) void join_kernel(LogprobArgs a, Parts p) 
     if (lane < p.splits) t = p.sums[(int64_t)row * p.splits + lane];
     t = merge_wave(t);
     if (a.top > 0) {
-        Best b{0, 0.f, false};
-        for (int s = wave; s < p.splits; s += kGroups) {
-            const uint64_t* from = p.keys + ((int64_t)row * p.splits + s) * a.top;
-            const uint64_t k = lane < a.top ? from[lane] : 0;
+        // every split's list is in order; the first is the wave's to begin with
+        const uint64_t* from = p.keys + ((int64_t)row * p.splits + wave) * a.top + lane;
+        Best b{wave < p.splits && lane < a.top ? *from : 0, 0.f, false};
+        for (int s = wave + kGroups; s < p.splits; s += kGroups) {
+            from += kGroups * a.top;
+            const uint64_t k = lane < a.top ? *from : 0;
             uint64_t c = __ballot(k > read_lane(b.key, a.top - 1));
             while (c) {
                 const int i = __builtin_ctzll(c);
