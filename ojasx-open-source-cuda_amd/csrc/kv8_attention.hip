@@ -173,16 +173,6 @@ struct Item {
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Largest over the four lanes of a column (lanes n, n + 16, n + 32, n + 48).
-__device__ __forceinline__ float col_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
-}
-__device__ __forceinline__ float col_sum(float v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
-}
-
 // The item of workgroup `id` (without its split); false: none.
 template <bool ROWS>
 __device__ __forceinline__ bool find_item(const AttnArgs& a, const Cut& c, int id, Item& it) {
@@ -960,12 +950,9 @@ __device__ __forceinline__ void join_item(const AttnArgs& a, const Cut& c, int i
         const bool some = ml.y > 0.f;
         const bool bad = __any(some && ml.x != ml.x);
         float m = some && !bad ? ml.x : kNone;
-#pragma unroll
-        for (int s = 32; s; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
+        m = wave_max(m);
         const float keep = some && !bad ? fast_exp2(ml.x - m) : 0.f;
-        float l = keep * ml.y;
-#pragma unroll
-        for (int s = 32; s; s >>= 1) l += __shfl_xor(l, s);
+        const float l = wave_sum(keep * ml.y);
         float sum[DC];
 #pragma unroll
         for (int i = 0; i < DC; ++i) sum[i] = 0.f;

@@ -148,12 +148,6 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
 constexpr int kAppendWaves = 4;
 constexpr float kTinyAmax = 0x1p-100f;
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
-}
-
 template <int DT> __device__ __forceinline__ float elem(const void* p, int64_t i) {
     return load_as_f32<DT>(p, i);
 }
@@ -468,9 +462,7 @@ __device__ void append_held(const KvCache& c, const KvRows& src, bool values, in
     }
     // largest over the run of `bits`, pairs of 16 bits
     auto run_max = [&](uint32_t v) {
-        uint32_t b = max(v & 0xFFFFu, v >> 16);
-#pragma unroll
-        for (int o = 32; o; o >>= 1) b = max(b, (uint32_t)__shfl_xor((int)b, o));
+        uint32_t b = wave_max((uint32_t)max(v & 0xFFFFu, v >> 16));
         if constexpr (WAVES > 1) {
             __syncthreads();
             if (lane == 0) shared[wave] = b;
@@ -670,36 +662,64 @@ __global__ __launch_bounds__(kReadThreads) void read_kernel(KvCache c,
     if (blockIdx.y == 0)
         for (int h = threadIdx.x; h < c.heads; h += kReadThreads)
             scales_out[(i * c.heads + h) * 2 + values] = in ? scales[2 * h] : 0.f;
-#pragma unroll 4
-    for (int u = blockIdx.y * kReadThreads + threadIdx.x; u < units; u += gridDim.y * kReadThreads) {
-        const int t = u / row, e = u - t * row, h = e / per, x = e - h * per;
-        const int8_t* p = base + h * head_bytes;
-        const float s = in ? scales[2 * h] : 0.f;
-        if constexpr (!WIDE) {
-            const int at = values ? (t >> 4) * 16 * c.dp + x * 16 + (t & 15)
-                                  : key_at(t, x >> 4, c.dp) + (x & 15);
-            store_value<DT>(out, o0 + t * ot + e, in ? p[at] : 0, s);
-        } else if (!values) {
-            uint2 w = make_uint2(0, 0);
-            if (in) w = *reinterpret_cast<const uint2*>(p + key_at(t, x >> 1, c.dp) + (x & 1) * 8);
+    const int first = blockIdx.y * kReadThreads + threadIdx.x, step = gridDim.y * kReadThreads;
+    // (token or quad, head, place in the head) of unit u
+    auto split = [&](int u, int& t, int& h, int& x) {
+        t = u / row;
+        const int e = u - t * row;
+        h = e / per;
+        x = e - h * per;
+    };
+    if (!WIDE || values) {
+        for (int u = first; u < units; u += step) {
+            int t, h, x;
+            split(u, t, h, x);
+            const int8_t* p = base + h * head_bytes;
+            const float s = in ? scales[2 * h] : 0.f;
+            const int64_t o = o0 + h * c.d;
+            if constexpr (!WIDE) {
+                const int at = values ? (t >> 4) * 16 * c.dp + x * 16 + (t & 15)
+                                      : key_at(t, x >> 4, c.dp) + (x & 15);
+                store_value<DT>(out, o + t * ot + x, in ? p[at] : 0, s);
+            } else {
+                uint32_t w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    w[j] = in ? *reinterpret_cast<const uint32_t*>(p + (t >> 2) * 16 * c.dp +
+                                                                  (x * 8 + j) * 16 + (t & 3) * 4)
+                              : 0u;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    int code[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) code[j] = byte_of(w[j], n);
+                    store8<DT>(out, o + (4 * t + n) * ot + x * 8, code, s);
+                }
+            }
+        }
+        return;
+    }
+    for (int u0 = first; u0 < units; u0 += kReadUnits * step) {
+        uint2 w[kReadUnits];
+        float s[kReadUnits];
+        int64_t o[kReadUnits];
+#pragma unroll
+        for (int i = 0; i < kReadUnits; ++i) {
+            int t, h, x;
+            split(min(u0 + i * step, units - 1), t, h, x);
+            w[i] = make_uint2(0, 0);
+            if (in)
+                w[i] = *reinterpret_cast<const uint2*>(base + h * head_bytes +
+                                                       key_at(t, x >> 1, c.dp) + (x & 1) * 8);
+            s[i] = in ? scales[2 * h] : 0.f;
+            o[i] = o0 + t * ot + h * c.d + x * 8;
+        }
+#pragma unroll
+        for (int i = 0; i < kReadUnits; ++i) {
             int code[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) code[j] = byte_of(j < 4 ? w.x : w.y, j & 3);
-            store8<DT>(out, o0 + t * ot + h * c.d + x * 8, code, s);
-        } else {
-            uint32_t w[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                w[j] = in ? *reinterpret_cast<const uint32_t*>(p + (t >> 2) * 16 * c.dp +
-                                                              (x * 8 + j) * 16 + (t & 3) * 4)
-                          : 0u;
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                int code[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) code[j] = byte_of(w[j], n);
-                store8<DT>(out, o0 + (4 * t + n) * ot + h * c.d + x * 8, code, s);
-            }
+            for (int j = 0; j < 8; ++j) code[j] = byte_of(j < 4 ? w[i].x : w[i].y, j & 3);
+            if (u0 + i * step < units) store8<DT>(out, o[i], code, s[i]);
         }
     }
 }

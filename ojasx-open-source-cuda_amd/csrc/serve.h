@@ -10,6 +10,60 @@
 
 namespace ojx {
 
+// ---------------------------------------------------------------- sums over lanes
+
+// v of the lane N places round in its row of 16.
+template <int N> __device__ __forceinline__ float row_turn(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v),
+                                                                 0x120 + N, 0xF, 0xF, true));
+}
+
+// a, b = the lower and the upper lane's v of each pair (l, l + 16) or (l, l + 32), in both lanes:
+// v_permlane*_swap exchanges the odd rows (the upper half) of its first operand with the even
+// rows (the lower half) of its second.  Its wait after a vector write stands with it.
+__device__ __forceinline__ void pair16(float v, float& a, float& b) {
+    a = b = v;
+    asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+}
+__device__ __forceinline__ void pair32(float v, float& a, float& b) {
+    a = b = v;
+    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+}
+
+// Over the lanes n, n + 16, n + 32, n + 48.
+__device__ __forceinline__ float col_max(float v) {
+    float a, b;
+    pair16(v, a, b);
+    pair32(fmaxf(a, b), a, b);
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float col_sum(float v) {
+    float a, b;
+    pair16(v, a, b);
+    pair32(a + b, a, b);
+    return a + b;
+}
+
+// Over the wave, in every lane.
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, row_turn<8>(v));
+    v = fmaxf(v, row_turn<4>(v));
+    v = fmaxf(v, row_turn<2>(v));
+    return col_max(fmaxf(v, row_turn<1>(v)));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    v += row_turn<8>(v);
+    v += row_turn<4>(v);
+    v += row_turn<2>(v);
+    return col_sum(v + row_turn<1>(v));
+}
+
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+    return v;
+}
+
 // e8t_capi.cpp: the calling thread's error message, the arch check and a launch's status
 int api_failf(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 int api_check_device();

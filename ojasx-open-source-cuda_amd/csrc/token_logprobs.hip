@@ -138,11 +138,11 @@ __device__ __forceinline__ Sums merge(Sums a, Sums b) {
 }
 
 __device__ __forceinline__ Sums merge_wave(Sums a) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1)
-        a = merge(a, Sums{__shfl_xor(a.r, o), __shfl_xor(a.s, o), __shfl_xor(a.u, o),
-                          __shfl_xor(a.m, o)});
-    return a;
+    const bool bad = __any(a.m != a.m);
+    const float r = wave_max(a.r);
+    rescale(a, r == -INFINITY ? 0.f : r);
+    const float m = wave_max(a.m);
+    return Sums{r, wave_sum(a.s), wave_sum(a.u), bad ? __uint_as_float(0x7FC00000u) : m};
 }
 
 __device__ __forceinline__ bool ordinary(const Sums& a) {
@@ -169,16 +169,55 @@ __device__ __forceinline__ void insert(Best& b, uint64_t key, int k, int lane) {
     b.key = lane < at ? b.key : lane == at ? key : up;
 }
 
-// A bound that k lanes' values reach: their k-th largest in its `BITS` leading bits, the others 0
-// (0 where fewer than k lanes have a value above 0).
-template <int BITS> __device__ __forceinline__ uint32_t kth_of_lanes(uint32_t v, int k) {
-    uint32_t t = 0;
-#pragma unroll 1
-    for (int bit = 31; bit >= 32 - BITS; --bit) {
-        const uint32_t c = t | 1u << bit;
-        if (__popcll(__ballot(v >= c)) >= k) t = c;
+// A wave's candidates on their way into its best k.
+constexpr int kPool = 256;
+struct Pool {
+    uint64_t keys[kPool];
+    uint64_t sorted[64];
+    float maxima[64];
+};
+
+// The k-th largest of the lanes' values: the least of those that fewer than k exceed.
+__device__ __forceinline__ float kth_of_lanes(float v, int k, int lane, Pool& pool) {
+    pool.maxima[lane] = v;
+    __builtin_amdgcn_wave_barrier();
+    int above = 0;
+#pragma unroll
+    for (int j = 0; j < 64; j += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(pool.maxima + j);
+        above += f.x > v;
+        above += f.y > v;
+        above += f.z > v;
+        above += f.w > v;
     }
-    return t;
+    return -wave_max(above < k ? -v : -INFINITY);
+}
+
+// Takes the first n of the pool into the best k: a few one by one (about 200 cycles each), more
+// by their ranks among all of them and the k.
+__device__ __forceinline__ void settle(Best& b, Pool& pool, int n, int k, int lane) {
+    __builtin_amdgcn_wave_barrier();
+    if (n <= 4) {
+        for (int i = 0; i < n; ++i) insert(b, read_lane(pool.keys[i], 0), k, lane);
+    } else {
+        const int all = n + k;  // the best so far behind the new
+        if (lane < k) pool.keys[n + lane] = b.key;
+        if (lane < k) pool.sorted[lane] = 0;
+        __builtin_amdgcn_wave_barrier();
+        for (int i0 = 0; i0 < all; i0 += 64) {
+            const uint64_t mine = i0 + lane < all ? pool.keys[i0 + lane] : 0;
+            int rank = 0;
+#pragma unroll 8
+            for (int j = 0; j < all; ++j) rank += pool.keys[j] > mine;
+            if (mine != 0 && rank < k) pool.sorted[rank] = mine;
+        }
+        __builtin_amdgcn_wave_barrier();
+        b.key = lane < k ? pool.sorted[lane] : 0;
+        __builtin_amdgcn_wave_barrier();
+    }
+    const uint64_t last = read_lane(b.key, k - 1);
+    b.full = last != 0;
+    b.least = b.full ? unordered((uint32_t)(last >> 32)) : -INFINITY;
 }
 
 constexpr int kLaneLogits = 32;                  // logits of a lane in one batch
@@ -200,6 +239,14 @@ template <int DT> struct Batch {
     // Vectors that reach over an end of the row are put together from its logits and -inf.
     __device__ __forceinline__ void load(const void* x, int64_t x0, int v, int b, int lane,
                                          int shift) {
+        // a batch within the row: the same for all lanes, and nothing to check
+        if (b * kBatch >= shift && (int64_t)(b + 1) * kBatch - shift <= v) {
+            const char* p = static_cast<const char*>(x) +
+                            (x0 + index(b, 0, lane, shift)) * (16 / kVec);
+#pragma unroll
+            for (int n = 0; n < kVecs; ++n) w[n] = *reinterpret_cast<const uint4*>(p + n * 1024);
+            return;
+        }
 #pragma unroll
         for (int n = 0; n < kVecs; ++n) {
             const int j = index(b, n * kVec, lane, shift);
@@ -229,6 +276,14 @@ template <int DT> struct Batch {
         }
     }
 
+    // Logits read from here on are converted anew: kept as floats they would cost a register each.
+    __device__ __forceinline__ void drop_floats() {
+        if constexpr (DT != kF32)
+#pragma unroll
+            for (int n = 0; n < kVecs; ++n)
+                asm("" : "+v"(w[n].x), "+v"(w[n].y), "+v"(w[n].z), "+v"(w[n].w));
+    }
+
     __device__ __forceinline__ float get(int i) const {
         const uint4& q = w[i / kVec];
         const int n = i % kVec;
@@ -240,63 +295,73 @@ template <int DT> struct Batch {
 };
 
 // Takes a batch's candidates into the wave's best k.  Batches come by rising token, so a later
-// logit that only equals the k-th one loses.  Where more than k lanes have a candidate, the
-// k-th largest of the lanes' maxima is a bound under which none can stay: about k candidates
-// are left whatever the row's order.
+// logit that only equals the k-th one loses.  Where many lanes have a candidate (all at first), the
+// k-th largest of the lanes' maxima is a bound under which none can stay: about k candidates are
+// left whatever the row's order.
 template <int DT>
 __device__ __forceinline__ void take(Best& best, const Batch<DT>& x, float lane_max, int b, int k,
-                                     int lane, int shift) {
+                                     int lane, int shift, Pool& pool) {
     const bool may = !best.full || lane_max > best.least;
     const uint64_t lanes = __ballot(may);
     if (!lanes) return;
     float cut = -INFINITY;
-    if (__popcll(lanes) >= k) {
-        // sign, exponent and fraction of the type; fp32 in full
-        constexpr int bits = DT == kBF16 ? 16 : DT == kF16 ? 19 : 32;
-        const uint32_t t = kth_of_lanes<bits>(may ? ordered(lane_max) : 0u, k);
-        if (t > 0x007FFFFFu) cut = unordered(t);  // above -inf
-    }
-    const uint64_t open = best.full ? 0ull : ~0ull;
+    const int many = __popcll(lanes);
+    if (many >= k && (many > k + 12 || !best.full))
+        cut = kth_of_lanes(may ? lane_max : -INFINITY, k, lane, pool);
+    uint64_t open = best.full ? 0ull : ~0ull;
+    int n = 0;
 #pragma unroll
     for (int i = 0; i < kLaneLogits; ++i) {
         const float f = x.get(i);
-        uint64_t c = __ballot(f >= cut) & (__ballot(f > best.least) | open);
+        const uint64_t c = __ballot(f >= cut) & (__ballot(f > best.least) | open);
         if (!c) continue;
-        const uint64_t key = key_of(f, Batch<DT>::index(b, i, lane, shift));
-        while (c) {
-            const int from = __builtin_ctzll(c);
-            c &= c - 1;
-            insert(best, read_lane(key, from), k, lane);
+        if (n + __popcll(c) + k > kPool) {
+            settle(best, pool, n, k, lane);
+            n = 0;
         }
+        const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(c >> 32),
+                                                     __builtin_amdgcn_mbcnt_lo((uint32_t)c, 0));
+        if (c >> lane & 1) pool.keys[at] = key_of(f, Batch<DT>::index(b, i, lane, shift));
+        n += __popcll(c);
     }
-    const uint64_t last = read_lane(best.key, k - 1);
-    best.full = last != 0;
-    best.least = best.full ? unordered((uint32_t)(last >> 32)) : -INFINITY;
+    if (n) settle(best, pool, n, k, lane);
 }
 
-// A row's results from its sums and the waves' best keys (keys[kGroups][top] in LDS, behind a
-// barrier).
+// A row's given token: read ahead of its use.
+struct Asked {
+    int64_t id;
+    bool in;
+    float x;
+};
+template <int DT> __device__ __forceinline__ Asked asked_of(const LogprobArgs& a, int row) {
+    Asked t;
+    t.id = a.ids[row];
+    t.in = t.id >= 0 && t.id < a.vocab;
+    t.x = t.in ? load_as_f32<DT>(a.x, row * a.ld + t.id) : 0.f;
+    return t;
+}
+
+// A row's results from its sums and n keys in LDS (behind a barrier), its best among them.
 template <int DT>
-__device__ void finish(const LogprobArgs& a, int row, const Sums& t, const uint64_t* keys,
-                       float* sf, uint64_t* sk) {
+__device__ __forceinline__ void finish(const LogprobArgs& a, int row, const Sums& t, const Asked& asked,
+                                       const uint64_t* keys, int n, float* sf, uint64_t* sk) {
     if (!ordinary(t)) return odd_row<DT>(a, row, sf, sk);
     const float l2 = log2f(t.s);
     const float ls = (l2 - __builtin_fmaf(t.m, kLog2e, -t.r)) * kLn2;
     auto log_p = [&](float x) { return x == -INFINITY ? x : (x - t.m) - ls; };
     if (threadIdx.x == 0) {
-        const int64_t id = a.ids[row];
-        const bool in = id >= 0 && id < a.vocab;
         a.lse[row] = t.m + ls;
         a.stats[2 * (int64_t)row] = t.m;
         a.stats[2 * (int64_t)row + 1] = ls;
-        a.logprob[row] = in ? log_p(load_as_f32<DT>(a.x, row * a.ld + id)) : 0.f;
+        a.logprob[row] = asked.in ? log_p(asked.x) : 0.f;
         a.entropy[row] = (l2 - t.u / t.s) * kLn2;
     }
-    // a key's rank among the waves' is its place
-    for (int i = threadIdx.x; i < kGroups * a.top; i += kThreads) {
+    // a key's rank is its place
+    for (int i = threadIdx.x; i < n; i += kThreads) {
         const uint64_t k = keys[i];
         int rank = 0;
-        for (int j = 0; j < kGroups * a.top; ++j) rank += keys[j] > k;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) rank += keys[j] > k;
         if (rank < a.top) {
             const int64_t o = (int64_t)row * a.top + rank;
             a.top_ids[o] = 0xFFFFFFFFu - (uint32_t)k;
@@ -317,6 +382,7 @@ struct Parts {
 template <int DT, bool TOP>
 __global__ __launch_bounds__(kThreads) void pass_kernel(LogprobArgs a, Parts p) {
     __shared__ Sums sums[kGroups];
+    __shared__ Pool pool[TOP ? kGroups : 1];
     __shared__ uint64_t keys[TOP ? kGroups * kTopMax : 1];
     __shared__ float sf[kGroups];
     __shared__ uint64_t sk[kGroups];
@@ -333,10 +399,8 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(LogprobArgs a, Parts p) 
     Best best{0, -INFINITY, false};
     B x;
     int b = split * per + wave;
-    if (b < end) x.load(a.x, x0, a.vocab, b, lane, shift);
     for (; b < end; b += kGroups) {
-        B next;
-        if (b + kGroups < end) next.load(a.x, x0, a.vocab, b + kGroups, lane, shift);
+        x.load(a.x, x0, a.vocab, b, lane, shift);
         float m = x.get(0);
 #pragma unroll
         for (int i = 1; i < kLaneLogits; ++i) m = or_nan(m, x.get(i));
@@ -351,15 +415,16 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(LogprobArgs a, Parts p) 
             t.s += e;
             t.u = __builtin_fmaf(d, e, t.u);
         }
-        if constexpr (TOP) take<DT>(best, x, m, b, a.top, lane, shift);
-        x = next;
+        if constexpr (TOP) x.drop_floats();
+        if constexpr (TOP) take<DT>(best, x, m, b, a.top, lane, shift, pool[wave]);
     }
     t = merge_wave(t);
     if (lane == 0) sums[wave] = t;
     if (TOP && lane < a.top) keys[wave * a.top + lane] = best.key;
     __syncthreads();
     t = merge(merge(sums[0], sums[1]), merge(sums[2], sums[3]));
-    if (p.splits == 1) return finish<DT>(a, row, t, keys, sf, sk);
+    if (p.splits == 1)
+        return finish<DT>(a, row, t, asked_of<DT>(a, row), keys, TOP ? kGroups * a.top : 0, sf, sk);
     const int64_t at = (int64_t)row * p.splits + split;
     if (threadIdx.x == 0) p.sums[at] = t;
     if constexpr (TOP) {
@@ -367,6 +432,7 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(LogprobArgs a, Parts p) 
         for (int i = threadIdx.x; i < kGroups * a.top; i += kThreads) {
             const uint64_t k = keys[i];
             int rank = 0;
+#pragma unroll 8
             for (int j = 0; j < kGroups * a.top; ++j) rank += keys[j] > k || (keys[j] == k && j < i);
             if (rank < a.top) p.keys[at * a.top + rank] = k;
         }
@@ -379,16 +445,21 @@ __global__ __launch_bounds__(kThreads) void join_kernel(LogprobArgs a, Parts p) 
     __shared__ float sf[kGroups];
     __shared__ uint64_t sk[kGroups];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.x;
+    const Asked asked = asked_of<DT>(a, row);
+    const int n = p.splits * a.top;
+    const uint64_t* from = p.keys + (int64_t)row * n;
+    const bool few = n <= kGroups * kTopMax;
+    if (few && (int)threadIdx.x < n) keys[threadIdx.x] = from[threadIdx.x];
     Sums t{-INFINITY, 0.f, 0.f, -INFINITY};
     if (lane < p.splits) t = p.sums[(int64_t)row * p.splits + lane];
     t = merge_wave(t);
-    if (a.top > 0) {
+    if (!few) {
         // every split's list is in order; the first is the wave's to begin with
-        const uint64_t* from = p.keys + ((int64_t)row * p.splits + wave) * a.top + lane;
-        Best b{wave < p.splits && lane < a.top ? *from : 0, 0.f, false};
+        const uint64_t* list = from + wave * a.top + lane;
+        Best b{wave < p.splits && lane < a.top ? *list : 0, 0.f, false};
         for (int s = wave + kGroups; s < p.splits; s += kGroups) {
-            from += kGroups * a.top;
-            const uint64_t k = lane < a.top ? *from : 0;
+            list += kGroups * a.top;
+            const uint64_t k = lane < a.top ? *list : 0;
             uint64_t c = __ballot(k > read_lane(b.key, a.top - 1));
             while (c) {
                 const int i = __builtin_ctzll(c);
@@ -399,7 +470,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(LogprobArgs a, Parts p) 
         if (lane < a.top) keys[wave * a.top + lane] = b.key;
     }
     __syncthreads();
-    finish<DT>(a, row, t, keys, sf, sk);
+    finish<DT>(a, row, t, asked, keys, few ? n : kGroups * a.top, sf, sk);
 }
 
 // ---------------------------------------------------------------- gradient
