@@ -144,38 +144,46 @@ constexpr int kThreads = 64 * kWaves;
 constexpr float kFixed = 32512.f;  // largest fixed-point value: 127 * 256 with its low part 0
 constexpr float kMagic = 12582912.f + 128.f;  // 1.5 * 2^23: the sum's low bits are the integer
 constexpr float kLeastScale = 0x1p-100f;
-constexpr int kMaxSplits = 64;
 
 // How a launch cuts its work.  An item is a tile of rows of one request (tok tokens of it, or
-// part of one token's heads where a key head has more than a tile's rows) and one key head; with
-// splits > 1 its keys are shared out and the partial results joined by a second launch.
+// part of one token's heads where a key head has more than a tile's rows) and one key head.  Items
+// of more than `per` 64-key tiles are done in parts by several workgroups, joined by a second
+// launch; of the two kinds, the last items may be cut finer than the first `whole`.
 struct Cut {
-    int rows;    // rows of a tile
-    int tok;     // tokens of a tile
-    int subs;    // tiles of one token's heads of a key head
-    int tiles;   // tiles (upper bound), without subs and key heads
-    int splits;
-    int least;   // fewest 64-key tiles of a split
-    int small;   // requests of at most so many tokens belong to the launch that splits keys
-    float* part;   // [splits][items][rows][dp]
-    float2* ml;    // [splits][items][rows]
+    int rows;      // rows of a tile
+    int tok;       // tokens of a tile
+    int subs;      // tiles of one token's heads of a key head
+    int tiles;     // tiles (upper bound), without subs and key heads
+    int small;     // requests of at most so many tokens belong to the launch that splits keys
+    int items, whole;
+    int per[2];    // 64-key tiles of a part, at most
+    int parts[2];  // parts of an item, at most (the launch's workgroups for each)
+    float* part;   // [stored parts][rows][dp]
+    float2* ml;    // [stored parts][rows]
 };
 
 struct Item {
-    int head, sub, tile, split;
+    int id, split;       // of the launch: the item, and which of its parts
+    int head, sub, tile;
     int r, tok0, ntok;   // request, the tile's tokens in it
     int q0;              // first row of q of the request
     int group;           // query heads of a key head
     int rows;            // rows in use
     int len;             // the request's tokens, newest included
     int before;          // the tile's first token's place
+    int parts;
+    int t0, t1;          // 64-key tiles of the part
+    int end_key;         // end of the keys that any of its rows sees
+    int64_t stored;      // first row of the part's results, of several
 };
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The item of workgroup `id` (without its split); false: none.
+// The item `id` in its part `split`; false: none.
 template <bool ROWS>
-__device__ __forceinline__ bool find_item(const AttnArgs& a, const Cut& c, int id, Item& it) {
+__device__ __forceinline__ bool find_item(const AttnArgs& a, const Cut& c, int id, int split, Item& it) {
+    it.id = id;
+    it.split = split;
     it.head = id % a.shape.kv_heads;
     id /= a.shape.kv_heads;
     it.sub = id % c.subs;
@@ -216,7 +224,30 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, const Cut& c, int i
     it.rows = c.subs > 1 ? min(it.group - it.sub * c.rows, c.rows) : it.ntok * it.group;
     it.len = max(0, min(a.seq_lens[it.r], a.shape.max_seq));
     it.before = a.seq_lens[it.r] - newest + it.tok0;
+    const int first = a.shape.window ? max(0, it.before + 1 - a.shape.window) : 0;
+    it.end_key = max(0, min(it.before + it.ntok, it.len));
+    const int kind = it.id < c.whole ? 0 : 1;
+    const int from = first >> 6, to = max(from, (it.end_key + 63) >> 6);
+    it.parts = max(1, min(c.parts[kind], (to - from + c.per[kind] - 1) / c.per[kind]));
+    if (it.split >= it.parts) return false;
+    const int per = (to - from + it.parts - 1) / it.parts;
+    it.t0 = from + it.split * per;
+    it.t1 = min(to, it.t0 + per);
+    const int64_t at = kind == 0 ? (int64_t)it.split * c.whole + it.id
+                                 : (c.parts[0] > 1 ? (int64_t)c.parts[0] * c.whole : 0) +
+                                       (int64_t)it.split * (c.items - c.whole) + it.id - c.whole;
+    it.stored = at * c.rows;
     return true;
+}
+
+// The item and part of a workgroup: parts of an item lie apart, so they run at the same time.
+template <bool ROWS>
+__device__ __forceinline__ bool block_item(const AttnArgs& a, const Cut& c, int block, Item& it) {
+    const int first = c.whole * c.parts[0];
+    if (block < first) return find_item<ROWS>(a, c, block % c.whole, block / c.whole, it);
+    block -= first;
+    const int rest = c.items - c.whole;
+    return find_item<ROWS>(a, c, c.whole + block % rest, block / rest, it);
 }
 
 // Token (within the tile) and query head of a row of an item.
@@ -406,9 +437,9 @@ struct Pages {
     int width, log_block, blocks, heads, head, end;
     int64_t head_bytes;
 
-    __device__ __forceinline__ Pages(const AttnArgs& a, const Item& it, int end_key)
+    __device__ __forceinline__ Pages(const AttnArgs& a, const Item& it)
         : table(a.tables + it.r * a.table_ld), width(a.width), log_block(a.cache.log_block),
-          blocks(a.cache.blocks), heads(a.cache.heads), head(it.head), end(end_key),
+          blocks(a.cache.blocks), heads(a.cache.heads), head(it.head), end(it.end_key),
           head_bytes(a.cache.head_bytes()) {}
     __device__ __forceinline__ int block(int key) const {
         const int i = key >> log_block;
@@ -422,17 +453,6 @@ struct Pages {
         return index(b) * head_bytes + ((key & ((1 << log_block) - 1)) >> 4) * (16 * dp);
     }
 };
-
-// What an item's rows see together, as 64-key tiles, and the split's part of them.
-__device__ __forceinline__ void key_range(const AttnArgs& a, const Cut& c, const Item& it, int& t0,
-                                          int& t1, int& end_key) {
-    const int first = a.shape.window ? max(0, it.before + 1 - a.shape.window) : 0;
-    end_key = max(0, min(it.before + it.ntok, it.len));
-    const int from = first >> 6, to = (end_key + 63) >> 6;
-    const int per = max(c.least, (to - from + c.splits - 1) / c.splits);
-    t0 = from + it.split * per;
-    t1 = min(to, t0 + per);
-}
 
 // Few rows over many keys, on the matrix unit in whole numbers: a score is 256 (qh.k) + (ql.k)
 // with the row's q in 16-bit fixed point against its own largest element, 64 keys at a time;
@@ -453,22 +473,12 @@ __device__ __forceinline__ void key_item(const AttnArgs& a, const Cut& c, int bl
                                          KeyShared<DC, NQ>& sh) {
     constexpr int DP = 64 * DC, DM = DP / 16, LD = KeyShared<DC, NQ>::kLd;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
-    const int items = c.tiles * c.subs * a.shape.kv_heads;
     Item it;
-    it.split = block / items;
-    const int id = block - it.split * items;
-    if (!find_item<false>(a, c, id, it)) return;
-    const int64_t item_rows = ((int64_t)it.split * items + id) * c.rows;
-    int t0, t1, end_key;
-    key_range(a, c, it, t0, t1, end_key);
-    if (t0 >= t1 && c.splits > 1) {  // nothing of this split's
-        if ((int)threadIdx.x < it.rows) c.ml[item_rows + threadIdx.x] = make_float2(-INFINITY, 0.f);
-        return;
-    }
-    t0 += wave;
+    if (!block_item<false>(a, c, block, it)) return;
+    const int t0 = it.t0 + wave, t1 = it.t1;
 
     // the first keys and values are on their way before the queries
-    const Pages pages(a, it, end_key);
+    const Pages pages(a, it);
     const int key_k = (n >> 2) * 16, key_v = g * 16;
     const int in_k = g * 64 + (n & 3) * 16, in_v = n * 16;
     v4i kf[4][DC], vf[DM];
@@ -647,9 +657,9 @@ __device__ __forceinline__ void key_item(const AttnArgs& a, const Cut& c, int bl
 #pragma unroll
         for (int w = 1; w < kWaves; ++w)
             sum += *reinterpret_cast<const v4f*>(sh.joined + (w * 16 * NQ + row) * LD + d);
-        if (c.splits > 1) {
-            if (d == 0) c.ml[item_rows + row] = make_float2(m, l);
-            if (l > 0.f) *reinterpret_cast<v4f*>(c.part + (item_rows + row) * DP + d) = sum;
+        if (it.parts > 1) {
+            if (d == 0) c.ml[it.stored + row] = make_float2(m, l);
+            if (l > 0.f) *reinterpret_cast<v4f*>(c.part + (it.stored + row) * DP + d) = sum;
             continue;
         }
         int tok, head;
@@ -701,19 +711,10 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Cut& c, int bl
                                          RowShared<DC>& sh) {
     constexpr int NQ = 2, DP = 64 * DC, DM = DP / 16, kGroup = RowShared<DC>::kGroup;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
-    const int items = c.tiles * c.subs * a.shape.kv_heads;
     Item it;
-    it.split = block / items;
-    const int id = block - it.split * items;
-    if (!find_item<true>(a, c, id, it)) return;
-    const int64_t item_rows = ((int64_t)it.split * items + id) * c.rows;
-    int t0, t1, end_key;
-    key_range(a, c, it, t0, t1, end_key);
-    if (t0 >= t1 && c.splits > 1) {
-        if ((int)threadIdx.x < it.rows) c.ml[item_rows + threadIdx.x] = make_float2(-INFINITY, 0.f);
-        return;
-    }
-    const Pages pages(a, it, end_key);
+    if (!block_item<true>(a, c, block, it)) return;
+    const int t0 = it.t0, t1 = it.t1;
+    const Pages pages(a, it);
 
     // Thread's pieces (16 bytes) of a tile: piece u of DP a group of 16 keys.
     v4i kr[DC], vr[DC];
@@ -885,11 +886,11 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Cut& c, int bl
         const float l = col_sum(l_run[q]);
         if (!rows.live[q]) continue;
         const int row = row0 + 16 * q + n;
-        if (c.splits > 1) {
+        if (it.parts > 1) {
             if (g == 0)
-                c.ml[item_rows + row] = make_float2(rows.bad[q] && l > 0.f ? nan : ref[q], l);
+                c.ml[it.stored + row] = make_float2(rows.bad[q] && l > 0.f ? nan : ref[q], l);
             if (!(l > 0.f)) continue;
-            float* p = c.part + (item_rows + row) * DP + 4 * g;
+            float* p = c.part + (it.stored + row) * DP + 4 * g;
 #pragma unroll
             for (int i = 0; i < DM; ++i) *reinterpret_cast<v4f*>(p + 16 * i) = o[q][i];
             continue;
@@ -933,20 +934,20 @@ __global__ __launch_bounds__(kThreads, DC <= 2 && MIX != Mix::Few2 ? 2 : 1) void
                              *reinterpret_cast<KeyShared<DC, NQ>*>(lds));
 }
 
-// Joins the splits of an item's rows from `first` on, a wave per row: lane s has split s's maximum
+// Joins the parts of an item's rows from `first` on, a wave per row: lane s has part s's maximum
 // and sum.
 template <int DT, int DC, bool ROWS>
 __device__ __forceinline__ void join_item(const AttnArgs& a, const Cut& c, int id, int first, int step) {
     constexpr int DP = 64 * DC;
     const int lane = threadIdx.x & 63;
-    const int items = c.tiles * c.subs * a.shape.kv_heads;
     Item it;
-    if (!find_item<ROWS>(a, c, id, it)) return;
+    if (!find_item<ROWS>(a, c, id, 0, it) || it.parts <= 1) return;
+    const int64_t stride = (int64_t)(id < c.whole ? c.whole : c.items - c.whole) * c.rows;
     const float nan = __uint_as_float(0x7FC00000u);
     for (int row = first + (threadIdx.x >> 6); row < it.rows; row += step) {
-        const int64_t at0 = (int64_t)id * c.rows + row, stride = (int64_t)items * c.rows;
+        const int64_t at0 = it.stored + row;
         float2 ml = make_float2(kNone, 0.f);
-        if (lane < c.splits) ml = c.ml[at0 + lane * stride];
+        if (lane < it.parts) ml = c.ml[at0 + lane * stride];
         const bool some = ml.y > 0.f;
         const bool bad = __any(some && ml.x != ml.x);
         float m = some && !bad ? ml.x : kNone;
@@ -958,8 +959,8 @@ __device__ __forceinline__ void join_item(const AttnArgs& a, const Cut& c, int i
         for (int i = 0; i < DC; ++i) sum[i] = 0.f;
         const uint64_t used = __ballot(some && !bad);
         const float* p = c.part + at0 * DP + lane;
-        // four splits' loads at a time; one without keys has written nothing
-        for (int s0 = 0; s0 < c.splits; s0 += 4) {
+        // four parts' loads at a time; where a part has no key for a row it has written nothing
+        for (int s0 = 0; s0 < it.parts; s0 += 4) {
             float v[4][DC];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -992,26 +993,24 @@ constexpr int kRowJoins = 8;  // workgroups of an item of many rows
 template <int DT, int DC>
 __global__ __launch_bounds__(kThreads) void join_kernel(AttnArgs a, Cut key, Cut row, int row_blocks) {
     const int b = blockIdx.x;
+    // items that can have parts: all, or the last ones
     if (b < row_blocks)
-        return join_item<DT, DC, true>(a, row, b / kRowJoins, b % kRowJoins * kWaves,
-                                       kRowJoins * kWaves);
-    join_item<DT, DC, false>(a, key, b - row_blocks, 0, kWaves);
+        return join_item<DT, DC, true>(a, row, (row.parts[0] > 1 ? 0 : row.whole) + b / kRowJoins,
+                                       b % kRowJoins * kWaves, kRowJoins * kWaves);
+    join_item<DT, DC, false>(a, key, (key.parts[0] > 1 ? 0 : key.whole) + b - row_blocks, 0, kWaves);
 }
 
 // ---------------------------------------------------------------- how a call is cut
 
 constexpr int kRowTile = 32 * kWaves;
-constexpr int64_t kKeyBlocks = 4096, kRowBlocks = 512;
+constexpr int kMaxParts = 64;
+constexpr int kUncut = 1 << 30;
 
 struct Plan {
     Mix mix;
     Cut key, row;
     bool has_key, has_row;
 };
-
-int64_t item_count(const Cut& c, const AttnShape& s) {
-    return (int64_t)c.tiles * c.subs * s.kv_heads;
-}
 
 // 64-key tiles of the longest range that rows of `tok` tokens see.
 int64_t key_tiles(const AttnShape& s, int tok) {
@@ -1020,25 +1019,25 @@ int64_t key_tiles(const AttnShape& s, int tok) {
     return (keys + 63) / 64 + 1;
 }
 
-void set_cut(Cut& c, const AttnShape& s, int rows, int tiles_more) {
+void set_cut(Cut& c, const AttnShape& s, int rows, bool by_rows) {
     const int group = s.heads / s.kv_heads;
     c.rows = rows;
     c.tok = group <= rows ? rows / group : 1;
     c.subs = group <= rows ? 1 : (group + rows - 1) / rows;
-    c.tiles = s.requests + (tiles_more ? s.tokens / c.tok : 0);
+    c.tiles = s.requests + (by_rows ? s.tokens / c.tok : 0);
 }
 
-void set_splits(Cut& c, const AttnShape& s, int64_t blocks, int64_t least) {
-    const int64_t items = item_count(c, s), tiles = key_tiles(s, c.tok);
-    int64_t n = items > 0 ? (blocks + items - 1) / items : 1;
-    if (n > (tiles + least - 1) / least) n = (tiles + least - 1) / least;
-    if (n > kMaxSplits) n = kMaxSplits;
-    c.splits = n < 1 ? 1 : (int)n;
-    c.least = (int)least;
+void set_parts(Cut& c, int kind, int64_t per, int64_t tiles) {
+    if (per * kMaxParts < tiles) per = (tiles + kMaxParts - 1) / kMaxParts;
+    const int64_t n = (tiles + per - 1) / per;
+    c.per[kind] = (int)per;
+    c.parts[kind] = n < 1 ? 1 : (int)n;
 }
 
-Plan plan_of(const AttnShape& s) {
-    Plan p{};
+int64_t at_least(int64_t a, int64_t b) { return a < b ? b : a; }
+
+// false: more items than a launch can number
+bool plan_of(const AttnShape& s, Plan& p) {
     const int group = s.heads / s.kv_heads;
     const int64_t most = (int64_t)s.max_query * group;  // rows of a request and key head
     const bool one = s.max_query <= 1;
@@ -1049,53 +1048,94 @@ Plan plan_of(const AttnShape& s) {
                                                             : Mix::Both;
     p.has_key = p.mix != Mix::Many;
     p.has_row = p.mix == Mix::Many || p.mix == Mix::Both;
+    auto count = [&](Cut& c) {
+        const int64_t n = (int64_t)c.tiles * c.subs * s.kv_heads;
+        c.items = (int)n;
+        return n <= (1 << 24);
+    };
     if (p.has_key) {
-        set_cut(p.key, s, p.mix == Mix::Few2 ? 32 : 16, 0);
-        p.key.small = p.mix == Mix::Both ? p.key.tok : INT32_MAX;
-        // Splits down to one tile a wave where the batch is too small to fill the GPU (one token
-        // over 2048 keys: 9.7 us at 4 tiles a split, 12.6 at 16, 17.2 unsplit), eight a wave where
-        // it does (64 tokens over up to 16000: 132 us at 32, 157 at 4, whose waves mostly start
-        // up and join).
-        int64_t least = item_count(p.key, s) * key_tiles(s, p.key.tok) / 2048;
-        least = least < 4 ? 4 : least > 32 ? 32 : least;
-        set_splits(p.key, s, kKeyBlocks, least);
+        Cut& c = p.key;
+        set_cut(c, s, p.mix == Mix::Few2 ? 32 : 16, false);
+        c.small = p.mix == Mix::Both ? c.tok : INT32_MAX;
+        if (!count(c)) return false;
+        // Parts down to one tile a wave where the batch is too small to fill the GPU (one token
+        // over 2048 keys: 9.7 us at 4 tiles a part, 12.6 at 16, 17.2 uncut), eight a wave where it
+        // does (64 tokens over up to 16000: 132 us at 32, 157 at 4, whose waves mostly start up
+        // and join).
+        const int64_t tiles = key_tiles(s, c.tok);
+        int64_t per = (c.items * tiles + 4095) / 4096;
+        per = per < 4 ? 4 : per > 32 ? 32 : per;
+        set_parts(c, 1, per, tiles);
+        c.parts[0] = 1;
+        c.per[0] = kUncut;
     }
     if (p.has_row) {
-        set_cut(p.row, s, kRowTile, 1);
-        p.row.small = p.has_key ? p.key.small : 0;
-        // Only what does not fill the GPU is split: prompts of 6000 tokens in all take 439 us with
-        // 512 blocks, 487 cut to 2048.
-        set_splits(p.row, s, kRowBlocks, 16);
+        Cut& c = p.row;
+        set_cut(c, s, kRowTile, true);
+        c.small = p.has_key ? p.key.small : 0;
+        if (!count(c)) return false;
+        // Workgroups at a time: two on each CU, one where a head needs more of its LDS and registers.
+        const int64_t slots = s.d <= 128 ? 512 : 256, tiles = key_tiles(s, c.tok);
+        // Items of over half a slot's share are cut, which costs a store and a load of their rows
+        // in fp32.
+        const int64_t share = at_least((c.items * tiles + 2 * slots - 1) / (2 * slots), 16);
+        set_parts(c, 0, share, tiles);
+        // The items that are left when the others have filled the slots some times over would leave
+        // part of them idle: they are cut into as many parts as fill them best.
+        c.whole = (int)(c.items >= slots ? c.items - c.items % slots : 0);
+        const int64_t rest = c.items - c.whole;
+        double best = 1e9;
+        int64_t cuts = 1;
+        for (int64_t n = 1; n <= 8; ++n) {
+            const double cost = (double)((rest * n + slots - 1) / slots) / n + 0.03 * n;
+            if (cost < best - 1e-9) {
+                best = cost;
+                cuts = n;
+            }
+        }
+        const int64_t finer = at_least((tiles + cuts - 1) / cuts, 16);
+        set_parts(c, 1, c.whole && finer < share ? finer : share, tiles);
     }
-    return p;
+    return true;
 }
 
-size_t split_bytes(const Cut& c, const AttnShape& s) {  // of one split
-    const size_t rows = (size_t)item_count(c, s) * c.rows;
-    return rows * ((s.d + 63) / 64 * 64 * sizeof(float) + sizeof(float2));
+int64_t blocks_of(const Cut& c) {
+    return (int64_t)c.whole * c.parts[0] + (int64_t)(c.items - c.whole) * c.parts[1];
 }
+
+int64_t items_in_parts(const Cut& c) {
+    return (c.parts[0] > 1 ? c.whole : 0) + (c.parts[1] > 1 ? c.items - c.whole : 0);
+}
+
+size_t stored_rows(const Cut& c) {
+    return ((c.parts[0] > 1 ? (size_t)c.whole * c.parts[0] : 0) +
+            (c.parts[1] > 1 ? (size_t)(c.items - c.whole) * c.parts[1] : 0)) * c.rows;
+}
+
+size_t row_bytes(const AttnShape& s) { return (s.d + 63) / 64 * 64 * sizeof(float); }
 
 size_t cut_bytes(const Cut& c, const AttnShape& s) {
-    return c.splits > 1 ? c.splits * split_bytes(c, s) : 0;
+    return stored_rows(c) * (row_bytes(s) + sizeof(float2));
 }
 
-// The cut's part of the workspace, which it moves past; fewer splits where it is too small.
+// The cut's part of the workspace, which it moves past; no parts where it does not fit.
 void place(Cut& c, const AttnShape& s, char*& ws, size_t& left) {
-    if (c.splits <= 1) return;
-    const size_t per = split_bytes(c, s), fit = left / per;
-    if ((size_t)c.splits > fit) c.splits = fit < 2 ? 1 : (int)fit;
-    if (c.splits <= 1) return;
-    const size_t rows = (size_t)c.splits * item_count(c, s) * c.rows;
+    const size_t need = cut_bytes(c, s);
+    if (need > left) {
+        c.parts[0] = c.parts[1] = 1;
+        c.per[0] = c.per[1] = kUncut;
+        return;
+    }
     c.part = reinterpret_cast<float*>(ws);
-    c.ml = reinterpret_cast<float2*>(c.part + rows * ((s.d + 63) / 64 * 64));
-    ws += c.splits * per;
-    left -= c.splits * per;
+    c.ml = reinterpret_cast<float2*>(ws + stored_rows(c) * row_bytes(s));
+    ws += need;
+    left -= need;
 }
 
 template <int DT, int DC>
 hipError_t run(const AttnArgs& a, const Plan& p, hipStream_t stream) {
-    const int64_t row_blocks = p.has_row ? item_count(p.row, a.shape) * p.row.splits : 0;
-    const int64_t key_blocks = p.has_key ? item_count(p.key, a.shape) * p.key.splits : 0;
+    const int64_t row_blocks = p.has_row ? blocks_of(p.row) : 0;
+    const int64_t key_blocks = p.has_key ? blocks_of(p.key) : 0;
     if (row_blocks + key_blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
     const dim3 g((unsigned)(row_blocks + key_blocks)), b(kThreads);
     const int rb = (int)row_blocks;
@@ -1105,8 +1145,8 @@ hipError_t run(const AttnArgs& a, const Plan& p, hipStream_t stream) {
         case Mix::Many: attend_kernel<DT, DC, Mix::Many><<<g, b, 0, stream>>>(a, p.key, p.row, rb); break;
         case Mix::Both: attend_kernel<DT, DC, Mix::Both><<<g, b, 0, stream>>>(a, p.key, p.row, rb); break;
     }
-    const int64_t row_joins = p.has_row && p.row.splits > 1 ? item_count(p.row, a.shape) * kRowJoins : 0;
-    const int64_t key_joins = p.has_key && p.key.splits > 1 ? item_count(p.key, a.shape) : 0;
+    const int64_t row_joins = p.has_row ? items_in_parts(p.row) * kRowJoins : 0;
+    const int64_t key_joins = p.has_key ? items_in_parts(p.key) : 0;
     if (row_joins + key_joins > 0x7FFFFFFF) return hipErrorInvalidValue;
     if (row_joins + key_joins > 0)
         join_kernel<DT, DC><<<(unsigned)(row_joins + key_joins), b, 0, stream>>>(a, p.key, p.row,
@@ -1126,8 +1166,8 @@ template <int DT> hipError_t run(const AttnArgs& a, const Plan& p, hipStream_t s
 }  // namespace
 
 size_t kv8_attention_bytes(const AttnShape& s) {
-    if (s.dtype == kF32 || s.tokens == 0 || s.requests == 0) return 0;
-    const Plan p = plan_of(s);
+    Plan p{};
+    if (s.dtype == kF32 || s.tokens == 0 || s.requests == 0 || !plan_of(s, p)) return 0;
     return (p.has_key ? cut_bytes(p.key, s) : 0) + (p.has_row ? cut_bytes(p.row, s) : 0);
 }
 
@@ -1141,7 +1181,8 @@ hipError_t launch_kv8_attention(const AttnArgs& args, void* ws, size_t ws_bytes,
         row_kernel<kF32><<<(unsigned)rows, 64, 0, stream>>>(a);
         return hipGetLastError();
     }
-    Plan p = plan_of(a.shape);
+    Plan p{};
+    if (!plan_of(a.shape, p)) return hipErrorInvalidValue;
     char* at = static_cast<char*>(ws);
     size_t left = ws ? ws_bytes : 0;
     if (p.has_key) place(p.key, a.shape, at, left);
