@@ -146,6 +146,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
 // ---------------------------------------------------------------- append
 
 constexpr int kAppendWaves = 4;
+constexpr int64_t kAppendBlocks = 1024;
 constexpr float kTinyAmax = 0x1p-100f;
 
 template <int DT> __device__ __forceinline__ float elem(const void* p, int64_t i) {
@@ -413,47 +414,63 @@ __device__ __forceinline__ void recode_values(int8_t* base, int quads, int d, in
 
 // append_run for 16-bit rows on a 16-byte grid, with the run held in registers between its
 // maximum and its codes: HOLD loads of eight elements a lane, all in flight at once.  `waves`
-// waves share a run (their maxima meet in LDS).  Values are taken as 4 tokens by 8 d, whose
-// bytes a lane turns into 8 words of 4 tokens; words that the run does not fill are read first.
+// waves share a run (their maxima meet in LDS).  Lanes are laid out as the cache is, so that a
+// store instruction fills whole stretches of it (a word in each of 40 lines took 37 us for
+// 21500 tokens of 8 x 80 fp16 where reads and writes alone take 17): a key unit is 16 d of one
+// token, lanes going through the 4 tokens of a quad first; a value unit is 8 d of a quad of
+// tokens, lanes going through the 4 quads of a group first, and its bytes become 8 words of 4
+// tokens.  Words that the run does not fill are read first.
 template <int DT, int HOLD, int WAVES>
-__device__ void append_held(const KvCache& c, const KvRows& src, bool values, int head, int64_t t0,
-                            int n, int block, int off, int lane, int wave, uint32_t* shared) {
+__device__ __forceinline__ void append_held(const KvCache& c, const KvRows& src, bool values, int head,
+                                            int64_t t0, int n, int block, int off, int lane, int wave,
+                                            uint32_t* shared) {
     const uint16_t* x0 = static_cast<const uint16_t*>(src.p) + t0 * src.token + head * src.head;
-    const int d8 = c.d >> 3, first = wave * 64 + lane;
-    const uint32_t inv8 = inverse_of(d8);
-    const int q0 = off >> 2, quads = ((off + n - 1) >> 2) - q0 + 1;
-    const int units = values ? quads * d8 : n * d8;
+    const int d8 = c.d >> 3, chunks = (c.d + 15) >> 4, first = wave * 64 + lane;
+    const int wide = values ? d8 : chunks;
+    const uint32_t inv = inverse_of(wide);
+    // quads of the block that units cover: for keys the run's, for values whole groups
+    const int q0 = values ? off >> 4 << 2 : off >> 2;
+    const int quads = (values ? ((off + n - 1) >> 4 << 2) + 4 : ((off + n - 1) >> 2) + 1) - q0;
+    const int units = quads * wide * (values ? 1 : 4);
     float* sp = c.scales + c.scale_at(block, head) + values;
     const float before = off > 0 ? *sp : 0.f;
     int8_t* base = (values ? c.v : c.k) + c.at(block, head);
-    // value word (quad q, d) of the block
-    auto value_at = [&](int q, int d) { return base + (q >> 2) * 16 * c.dp + d * 16 + (q & 3) * 4; };
+    // unit u: its place along d, and its quad of the block
+    auto unit_of = [&](int u, int& quad, int& place) {
+        const int w = u >> 2, i = quotient(w, inv, wide);
+        place = w - i * wide;
+        quad = q0 + (values ? 4 * i + (u & 3) : i);
+    };
     uint4 w[HOLD];
-    uint32_t m = 0;
     if (!values) {
 #pragma unroll
-        for (int i = 0; i < HOLD; ++i) {
-            const int u = first + i * 64 * WAVES;
-            w[i] = make_uint4(0, 0, 0, 0);
-            if (u < units) {
-                const int t = quotient(u, inv8, d8);
-                w[i] = *reinterpret_cast<const uint4*>(x0 + t * src.token + (u - t * d8) * 8);
-            }
+        for (int i = 0; i < HOLD; i += 2) {
+            const int u = first + (i >> 1) * 64 * WAVES;
+            int q, ch;
+            unit_of(u, q, ch);
+            const int t = 4 * q + (u & 3) - off;
+            const bool in = u < units && t >= 0 && t < n;
+            const uint16_t* p = x0 + t * src.token + ch * 16;
+            w[i] = w[i + 1] = make_uint4(0, 0, 0, 0);
+            if (in) w[i] = *reinterpret_cast<const uint4*>(p);
+            if (in && 2 * ch + 1 < d8) w[i + 1] = *reinterpret_cast<const uint4*>(p + 8);
         }
     } else {
 #pragma unroll
         for (int i = 0; i < HOLD; i += 4) {
             const int u = first + (i >> 2) * 64 * WAVES;
-            const int q = quotient(u, inv8, d8), d = (u - q * d8) * 8;
+            int q, d;
+            unit_of(u, q, d);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int t = 4 * (q0 + q) + j - off;
+                const int t = 4 * q + j - off;
                 w[i + j] = make_uint4(0, 0, 0, 0);
                 if (u < units && t >= 0 && t < n)
-                    w[i + j] = *reinterpret_cast<const uint4*>(x0 + t * src.token + d);
+                    w[i + j] = *reinterpret_cast<const uint4*>(x0 + t * src.token + d * 8);
             }
         }
     }
+    uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < HOLD; ++i) {
         const uint32_t a = max_pair(w[i].x & 0x7FFF7FFFu, w[i].y & 0x7FFF7FFFu);
@@ -462,7 +479,7 @@ __device__ void append_held(const KvCache& c, const KvRows& src, bool values, in
     }
     // largest over the run of `bits`, pairs of 16 bits
     auto run_max = [&](uint32_t v) {
-        uint32_t b = wave_max((uint32_t)max(v & 0xFFFFu, v >> 16));
+        uint32_t b = (uint32_t)wave_max((float)max(v & 0xFFFFu, v >> 16));
         if constexpr (WAVES > 1) {
             __syncthreads();
             if (lane == 0) shared[wave] = b;
@@ -499,12 +516,15 @@ __device__ void append_held(const KvCache& c, const KvRows& src, bool values, in
     if (!values) {
         if (again) recode_keys(base, off, c.d, c.dp, ratio, first, 64 * WAVES);
 #pragma unroll
-        for (int i = 0; i < HOLD; ++i) {
-            const int u = first + i * 64 * WAVES;
+        for (int i = 0; i < HOLD; i += 2) {
+            const int u = first + (i >> 1) * 64 * WAVES;
             if (u >= units) break;
-            const int t = quotient(u, inv8, d8), ch = u - t * d8;
-            *reinterpret_cast<uint2*>(base + key_at(off + t, ch >> 1, c.dp) + (ch & 1) * 8) =
-                codes8<DT>(w[i], inverse, plain);
+            int q, ch;
+            unit_of(u, q, ch);
+            const int t = 4 * q + (u & 3);
+            const uint2 lo = codes8<DT>(w[i], inverse, plain), hi = codes8<DT>(w[i + 1], inverse, plain);
+            if (t >= off && t < off + n)
+                *reinterpret_cast<uint4*>(base + key_at(t, ch, c.dp)) = make_uint4(lo.x, lo.y, hi.x, hi.y);
         }
         return;
     }
@@ -513,7 +533,8 @@ __device__ void append_held(const KvCache& c, const KvRows& src, bool values, in
     for (int i = 0; i < HOLD; i += 4) {
         const int u = first + (i >> 2) * 64 * WAVES;
         if (u >= units) break;
-        const int q = quotient(u, inv8, d8), d = (u - q * d8) * 8;
+        int q, d;
+        unit_of(u, q, d);
         uint32_t row[4][2];
         uint32_t fresh = 0;  // bytes of a word that the run fills
 #pragma unroll
@@ -521,10 +542,13 @@ __device__ void append_held(const KvCache& c, const KvRows& src, bool values, in
             const uint2 b = codes8<DT>(w[i + j], inverse, plain);
             row[j][0] = b.x;
             row[j][1] = b.y;
-            const int t = 4 * (q0 + q) + j - off;
-            fresh |= t >= 0 && t < n ? 0xFFu << (8 * j) : 0u;
+            const int t = 4 * q + j;
+            fresh |= t >= off && t < off + n ? 0xFFu << (8 * j) : 0u;
         }
-        int8_t* p = value_at(q0 + q, d);
+        // words of a group beside the run: of earlier tokens only to be rounded again
+        if (fresh == 0 && !(again && 4 * q < off)) continue;
+        int8_t* p = base + (q >> 2) * 16 * c.dp + d * 128 + (q & 3) * 4;
+        uint32_t word[8];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             // 4 tokens of 4 d -> 4 d of 4 tokens
@@ -537,19 +561,22 @@ __device__ void append_held(const KvCache& c, const KvRows& src, bool values, in
                                    __builtin_amdgcn_perm(f, e, 0x05040100u),
                                    __builtin_amdgcn_perm(f, e, 0x07060302u)};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t* o = reinterpret_cast<uint32_t*>(p + (4 * h + j) * 16);
-                uint32_t keep = 0;
-                if (fresh != 0xFFFFFFFFu) {
-                    keep = *o;
-                    if (again) {
-                        // bytes before the run; those after it stay
-                        const uint32_t r = recode4(keep, ratio);
-                        const uint32_t old = fresh ? (fresh & (0u - fresh)) - 1u : 0xFFFFFFFFu;
-                        keep = (r & old) | (keep & ~old);
-                    }
-                }
-                *o = (v[j] & fresh) | (keep & ~fresh);
+            for (int j = 0; j < 4; ++j) word[4 * h + j] = v[j];
+        }
+        uint32_t* o = reinterpret_cast<uint32_t*>(p);
+        if (fresh == 0xFFFFFFFFu) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[4 * j] = word[j];
+        } else {
+            // bytes before the run, to be rounded again; those after it stay
+            const uint32_t old = fresh ? (fresh & (0u - fresh)) - 1u : 0xFFFFFFFFu;
+            uint32_t keep[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) keep[j] = o[4 * j];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (again) keep[j] = (recode4(keep[j], ratio) & old) | (keep[j] & ~old);
+                o[4 * j] = (word[j] & fresh) | (keep[j] & ~fresh);
             }
         }
     }
@@ -558,13 +585,9 @@ __device__ void append_held(const KvCache& c, const KvRows& src, bool values, in
 // A wave (WAVES > 1: a workgroup) looks for run starts among `window` tokens and writes each run
 // for one head, keys or values.  Runs end where the slots leave the block or skip.
 template <int DT, bool VEC, int HOLD, int WAVES>
-__global__ __launch_bounds__(kAppendWaves * kWave) void append_kernel(
-    KvCache c, KvRows k, KvRows v, const int64_t* __restrict__ slots, int tokens, int window,
-    int64_t units) {
-    __shared__ uint32_t shared[WAVES];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t u = WAVES > 1 ? blockIdx.x : (int64_t)blockIdx.x * kAppendWaves + wave;
-    if (u >= units) return;
+__device__ __forceinline__ void append_unit(const KvCache& c, const KvRows& k, const KvRows& v,
+                                            const int64_t* __restrict__ slots, int tokens, int window,
+                                            int64_t u, int lane, int wave, uint32_t* shared) {
     const int parts = 2 * c.heads;
     const int64_t w = u / parts;
     const int part = (int)(u - w * parts), head = part >> 1;
@@ -603,6 +626,19 @@ __global__ __launch_bounds__(kAppendWaves * kWave) void append_kernel(
         else
             append_run<DT, VEC>(c, part & 1 ? v : k, part & 1, head, t0, n, at, off, lane);
     }
+}
+
+// Workgroups start at a few hundred a microsecond at most, so with many units each takes several.
+template <int DT, bool VEC, int HOLD, int WAVES>
+__global__ __launch_bounds__(kAppendWaves * kWave) void append_kernel(
+    KvCache c, KvRows k, KvRows v, const int64_t* __restrict__ slots, int tokens, int window,
+    int64_t units) {
+    __shared__ uint32_t shared[WAVES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t step = (int64_t)gridDim.x * (WAVES > 1 ? 1 : kAppendWaves);
+    for (int64_t u = WAVES > 1 ? blockIdx.x : (int64_t)blockIdx.x * kAppendWaves + wave; u < units;
+         u += step)
+        append_unit<DT, VEC, HOLD, WAVES>(c, k, v, slots, tokens, window, u, lane, wave, shared);
 }
 
 // ---------------------------------------------------------------- read
@@ -663,12 +699,15 @@ __global__ __launch_bounds__(kReadThreads) void read_kernel(KvCache c,
         for (int h = threadIdx.x; h < c.heads; h += kReadThreads)
             scales_out[(i * c.heads + h) * 2 + values] = in ? scales[2 * h] : 0.f;
     const int first = blockIdx.y * kReadThreads + threadIdx.x, step = gridDim.y * kReadThreads;
-    // (token or quad, head, place in the head) of unit u
+    // (token or quad, head, place in the head) of unit u; lanes go through a group's 4 quads of
+    // values first, whose bytes are neighbours
     auto split = [&](int u, int& t, int& h, int& x) {
-        t = u / row;
-        const int e = u - t * row;
+        const int w = WIDE && values ? u >> 2 : u;
+        t = w / row;
+        const int e = w - t * row;
         h = e / per;
         x = e - h * per;
+        if (WIDE && values) t = 4 * t + (u & 3);
     };
     if (!WIDE || values) {
         for (int u = first; u < units; u += step) {
@@ -750,8 +789,8 @@ hipError_t launch_kv8_append(const KvCache& c, const KvRows& k, const KvRows& v,
     // many tokens most of such waves would find none.
     const int window = (int64_t)tokens * 2 * c.heads <= 16384 ? 1 : 16;
     const int64_t units = ((int64_t)tokens + window - 1) / window * 2 * c.heads;
-    const int64_t grid = shared ? units : (units + kAppendWaves - 1) / kAppendWaves;
-    if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+    int64_t grid = shared ? units : (units + kAppendWaves - 1) / kAppendWaves;
+    grid = grid < kAppendBlocks ? grid : kAppendBlocks;
     const dim3 g((unsigned)grid), b(kAppendWaves * kWave);
     auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
@@ -783,7 +822,9 @@ hipError_t launch_kv8_read(const KvCache& c, const int32_t* blocks, int n, int d
     const bool wide = c.d % 8 == 0;
     const int64_t units = ((int64_t)c.heads * (wide ? c.d / 8 : c.d)) << c.log_block;
     int64_t shares = (units + kReadThreads * kReadUnits - 1) / (kReadThreads * kReadUnits);
-    if (shares > 1024) shares = 1024;
+    // some 2048 workgroups in all
+    const int64_t most = 1024 / (n < 1024 ? n : 1024);
+    shares = shares < most ? shares : most;
     if ((int64_t)n * 2 > 0x7FFFFFFF) return hipErrorInvalidValue;
     const dim3 g((unsigned)(2 * n), (unsigned)shares), b(kReadThreads);
     auto go = [&](auto dt) {

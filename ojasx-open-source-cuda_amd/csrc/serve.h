@@ -58,12 +58,6 @@ __device__ __forceinline__ float wave_sum(float v) {
     return col_sum(v + row_turn<1>(v));
 }
 
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
-    return v;
-}
-
 // e8t_capi.cpp: the calling thread's error message, the arch check and a launch's status
 int api_failf(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 int api_check_device();
