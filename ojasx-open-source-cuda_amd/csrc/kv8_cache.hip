@@ -18,31 +18,38 @@ constexpr int kWave = 64;
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanItems = 4;                            // requests per thread and pass
 constexpr int kPlanChunk = kPlanThreads * kPlanItems;    // requests per pass
-constexpr int kPlanTokens = kPlanThreads * 4;            // tokens per workgroup
+constexpr int kPlanTokens = kPlanThreads;                // tokens per workgroup
 
 __device__ __forceinline__ int sat32(int64_t v) { return v > 0x7FFFFFFF ? 0x7FFFFFFF : (int)v; }
 
+// Sums saturate: what lies past 2^32 - 1 is past every token and block anyway.
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) {
+    return __builtin_elementwise_add_sat(a, b);
+}
+
 // Exclusive sum of v over the workgroup; *total: the sum over all of it.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* totals, int64_t* total) {
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* totals, uint32_t* total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int64_t s = v;
+    uint32_t s = v;
 #pragma unroll
     for (int o = 1; o < kWave; o <<= 1) {
-        const int64_t up = __shfl_up(s, o);
-        if (lane >= o) s += up;
+        const uint32_t up = __shfl_up(s, o);
+        s = add_sat(s, lane >= o ? up : 0u);
     }
+    uint32_t before = __shfl_up(s, 1);
+    before = lane ? before : 0u;
     if (lane == 63) totals[wave] = s;
     __syncthreads();
-    int64_t before = 0, all = 0;
+    uint32_t all = 0;
 #pragma unroll
     for (int w = 0; w < kPlanThreads / kWave; ++w) {
-        const int64_t t = totals[w];
-        before += w < wave ? t : 0;
-        all += t;
+        const uint32_t t = totals[w];
+        before = add_sat(before, w < wave ? t : 0u);
+        all = add_sat(all, t);
     }
     __syncthreads();
     *total = all;
-    return before + s - v;
+    return before;
 }
 
 // Every workgroup sums up the requests by itself (a pass over kPlanChunk lengths is a few
@@ -50,49 +57,49 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* totals, int64_
 // one also writes the requests' results.
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
     __shared__ int starts[kPlanChunk], held[kPlanChunk], firsts[kPlanChunk];
-    __shared__ int64_t totals[kPlanThreads / kWave];
+    __shared__ uint32_t totals[kPlanThreads / kWave];
     const int block = 1 << a.log_block;
     const int64_t t0 = (int64_t)blockIdx.x * kPlanTokens, t1 = t0 + kPlanTokens;
+    const uint32_t tokens = a.tokens;
     const int nf = *a.num_free < a.capacity ? *a.num_free : a.capacity;
-    int64_t q_base = 0, need_base = 0;
+    uint32_t q_base = 0, need_base = 0;
     for (int64_t c = 0; c < a.requests; c += kPlanChunk) {
-        int64_t now[kPlanItems], old[kPlanItems], q = 0, need = 0, total;
+        int now[kPlanItems], old[kPlanItems];
+        uint32_t q = 0, need = 0, total;
         const int64_t r0 = c + (int64_t)threadIdx.x * kPlanItems;
 #pragma unroll
         for (int i = 0; i < kPlanItems; ++i) {
             const bool in = r0 + i < a.requests;
-            now[i] = in ? a.new_lens[r0 + i] : 0;
-            old[i] = in ? a.seq_lens[r0 + i] : 0;
-            now[i] = now[i] > 0 ? now[i] : 0;
-            old[i] = old[i] > 0 ? old[i] : 0;
-            q += now[i];
+            now[i] = in ? max(a.new_lens[r0 + i], 0) : 0;
+            old[i] = in ? max(a.seq_lens[r0 + i], 0) : 0;
+            q = add_sat(q, now[i]);
         }
-        int64_t start = q_base + block_scan(q, totals, &total);
-        const int64_t q_next = q_base + total;
+        uint32_t start = add_sat(q_base, block_scan(q, totals, &total));
+        const uint32_t q_next = add_sat(q_base, total);
 #pragma unroll
         for (int i = 0; i < kPlanItems; ++i) {
             // no more tokens than there is room for
-            const int64_t room = a.tokens - start;
-            const int64_t fit = now[i] < room ? now[i] : (room > 0 ? room : 0);
-            const int64_t have = (old[i] + block - 1) >> a.log_block;
+            const uint32_t at = min(start, tokens);
+            const int64_t fit = min((uint32_t)now[i], tokens - at);
+            const int64_t have = ((int64_t)old[i] + block - 1) >> a.log_block;
             const int64_t want = (old[i] + fit + block - 1) >> a.log_block;
             const int k = threadIdx.x * kPlanItems + i;
-            starts[k] = (int)(start < a.tokens ? start : a.tokens);
-            held[k] = sat32(old[i]);
+            starts[k] = (int)at;
+            held[k] = old[i];
             if (blockIdx.x == 0 && r0 + i < a.requests) {
-                a.query_starts[r0 + i] = starts[k];
+                a.query_starts[r0 + i] = (int)at;
                 a.seq_lens_out[r0 + i] = sat32(old[i] + fit);
             }
-            start += now[i];
-            now[i] = (want < a.width ? want : a.width) - (have < a.width ? have : a.width);
-            need += now[i];
+            start = add_sat(start, now[i]);
+            now[i] = (int)((want < a.width ? want : a.width) - (have < a.width ? have : a.width));
+            need = add_sat(need, now[i]);
         }
-        int64_t first = need_base + block_scan(need, totals, &total);
-        need_base += total;
+        uint32_t first = add_sat(need_base, block_scan(need, totals, &total));
+        need_base = add_sat(need_base, total);
 #pragma unroll
         for (int i = 0; i < kPlanItems; ++i) {
-            firsts[threadIdx.x * kPlanItems + i] = sat32(first);
-            first += now[i];
+            firsts[threadIdx.x * kPlanItems + i] = (int)min(first, 0x7FFFFFFFu);
+            first = add_sat(first, now[i]);
         }
         __syncthreads();
         // this workgroup's tokens among the pass's requests
@@ -138,7 +145,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         a.query_starts[a.requests] = (int)end;
-        const int64_t left = nf - need_base;
+        const int64_t left = (int64_t)nf - need_base;
         a.num_free_out[0] = left < -0x7FFFFFFF ? -0x7FFFFFFF : (int)left;
     }
 }
