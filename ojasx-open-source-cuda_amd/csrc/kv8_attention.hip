@@ -141,6 +141,12 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
+
+// Waves of a workgroup, and 16-row columns of a wave, where each wave has rows of its own: 128 rows
+// either way.  Heads of up to 128 leave registers for two columns a wave and two such workgroups
+// on a CU; larger ones take eight waves of one column, still two on a SIMD.
+constexpr int row_waves(int dc) { return dc <= 2 ? 4 : 8; }
+constexpr int row_columns(int dc) { return dc <= 2 ? 2 : 1; }
 constexpr float kFixed = 32512.f;  // largest fixed-point value: 127 * 256 with its low part 0
 constexpr float kMagic = 12582912.f + 128.f;  // 1.5 * 2^23: the sum's low bits are the integer
 constexpr float kLeastScale = 0x1p-100f;
@@ -154,6 +160,7 @@ struct Cut {
     int tok;       // tokens of a tile
     int subs;      // tiles of one token's heads of a key head
     int tiles;     // tiles (upper bound), without subs and key heads
+    int each;      // tiles of a request where every one has as many (few rows)
     int small;     // requests of at most so many tokens belong to the launch that splits keys
     int items, whole;
     int per[2];    // 64-key tiles of a part, at most
@@ -191,10 +198,10 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, const Cut& c, int i
     it.group = a.shape.heads / a.shape.kv_heads;
     int q0, q1;
     if constexpr (!ROWS) {
-        it.r = it.tile;
+        it.r = it.tile / c.each;
         q0 = a.query_starts ? a.query_starts[it.r] : it.r;
         q1 = a.query_starts ? a.query_starts[it.r + 1] : it.r + 1;
-        it.tok0 = 0;
+        it.tok0 = (it.tile - it.r * c.each) * c.tok;
         if (q1 - q0 > c.small) return false;
     } else {
         // request r's tiles begin at query_starts[r] / tok + r: room for each one's last, partly
@@ -460,18 +467,19 @@ struct Pages {
 // codes of keys and values enter as they lie in memory: what the cache costs is its bytes.
 // Tile t of the four score products takes 4 keys of each group of 16: a lane then holds the 16
 // scores of one group (one block: one pair of scales), and their weights are the second operand
-// of the value products as they come.  The workgroup's waves take every fourth 64 keys of a
-// 16 NQ row tile and join their results in LDS.
-template <int DC, int NQ> struct KeyShared {
+// of the value products as they come.  The workgroup's waves take turns at 64 keys of a 16-row tile
+// and join their results in LDS.  (Two tiles of rows for one pass over the keys would need more
+// than half of a SIMD's registers: two workgroups that share the keys in the L2 cache are faster.)
+template <int DC, int WAVES> struct KeyShared {
     static constexpr int kLd = 64 * DC + 4;
-    float joined[kWaves * 16 * NQ * kLd];
-    float m[kWaves][16 * NQ], l[kWaves][16 * NQ];
+    float joined[WAVES * 16 * kLd];
+    float m[WAVES][16], l[WAVES][16];
 };
 
-template <int DT, int DC, int NQ>
+template <int DT, int DC, int WAVES>
 __device__ __forceinline__ void key_item(const AttnArgs& a, const Cut& c, int block,
-                                         KeyShared<DC, NQ>& sh) {
-    constexpr int DP = 64 * DC, DM = DP / 16, LD = KeyShared<DC, NQ>::kLd;
+                                         KeyShared<DC, WAVES>& sh) {
+    constexpr int NQ = 1, DP = 64 * DC, DM = DP / 16, LD = KeyShared<DC, WAVES>::kLd;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
     Item it;
     if (!block_item<false>(a, c, block, it)) return;
@@ -503,8 +511,8 @@ __device__ __forceinline__ void key_item(const AttnArgs& a, const Cut& c, int bl
     if (t0 < t1) {
         const int bk = pages.block(t0 * 64 + key_k);
         bv = pages.block(t0 * 64 + key_v);
-        bk_next = pages.block((t0 + kWaves) * 64 + key_k);
-        bv_next = pages.block((t0 + kWaves) * 64 + key_v);
+        bk_next = pages.block((t0 + WAVES) * 64 + key_k);
+        bv_next = pages.block((t0 + WAVES) * 64 + key_v);
         load_keys(bk, t0 * 64);
         sc = load_scales(bv);
         load_values(bv, t0 * 64);
@@ -521,7 +529,7 @@ __device__ __forceinline__ void key_item(const AttnArgs& a, const Cut& c, int bl
 #pragma unroll
         for (int i = 0; i < DM; ++i) o[q][i] = v4f{0.f, 0.f, 0.f, 0.f};
     }
-    for (int t = t0; t < t1; t += kWaves) {
+    for (int t = t0; t < t1; t += WAVES) {
         const int j0 = t * 64;
         v4i s[NQ][4];
 #pragma unroll
@@ -541,14 +549,14 @@ __device__ __forceinline__ void key_item(const AttnArgs& a, const Cut& c, int bl
         }
         const bool valid = pages.valid(bv);
         const float ks = sc.x, v_scale = fmaxf(sc.y, kLeastScale);
-        const bool more = t + kWaves < t1;
+        const bool more = t + WAVES < t1;
         const int bv_now = bv_next;
         if (more) {
-            load_keys(bk_next, j0 + 64 * kWaves);
+            load_keys(bk_next, j0 + 64 * WAVES);
             sc = load_scales(bv_next);
             bv = bv_next;
-            bk_next = pages.block(j0 + 128 * kWaves + key_k);
-            bv_next = pages.block(j0 + 128 * kWaves + key_v);
+            bk_next = pages.block(j0 + 128 * WAVES + key_k);
+            bv_next = pages.block(j0 + 128 * WAVES + key_v);
         }
         const float lv = __builtin_amdgcn_logf(v_scale), rv = __builtin_amdgcn_rcpf(v_scale);
         v4f x[NQ][4];
@@ -607,7 +615,7 @@ __device__ __forceinline__ void key_item(const AttnArgs& a, const Cut& c, int bl
                     for (int r = 0; r < 4; ++r)
                         o[q][i0 + i][r] = __builtin_fmaf((float)w[i][r], beta[q], o[q][i0 + i][r]);
             }
-        if (more) load_values(bv_now, j0 + 64 * kWaves);
+        if (more) load_values(bv_now, j0 + 64 * WAVES);
     }
 
     const bool out_vec = out_vector(a);
@@ -626,7 +634,7 @@ __device__ __forceinline__ void key_item(const AttnArgs& a, const Cut& c, int bl
         const int row = 16 * q + n;
         float m = sh.m[0][row];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) m = fmaxf(m, sh.m[w][row]);
+        for (int w = 1; w < WAVES; ++w) m = fmaxf(m, sh.m[w][row]);
         const float keep = fast_exp2(m_run[q] - m);
         if (rows.live[q]) {
             float* p = sh.joined + (wave * 16 * NQ + row) * LD + 4 * g;
@@ -636,7 +644,7 @@ __device__ __forceinline__ void key_item(const AttnArgs& a, const Cut& c, int bl
         // the joined sum, in every wave
         float l = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w)
+        for (int w = 0; w < WAVES; ++w)
             l = __builtin_fmaf(sh.l[w][row], fast_exp2(sh.m[w][row] - m), l);
         l_run[q] = l;
         m_run[q] = m;
@@ -650,12 +658,12 @@ __device__ __forceinline__ void key_item(const AttnArgs& a, const Cut& c, int bl
         }
     }
     __syncthreads();
-    for (int u = threadIdx.x; u < it.rows * (DP / 4); u += kThreads) {
+    for (int u = threadIdx.x; u < it.rows * (DP / 4); u += 64 * WAVES) {
         const int row = u / (DP / 4), d = (u - row * (DP / 4)) * 4;
         const float m = sh.m[0][row], l = sh.l[0][row];
         v4f sum = *reinterpret_cast<const v4f*>(sh.joined + row * LD + d);
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w)
+        for (int w = 1; w < WAVES; ++w)
             sum += *reinterpret_cast<const v4f*>(sh.joined + (w * 16 * NQ + row) * LD + d);
         if (it.parts > 1) {
             if (d == 0) c.ml[it.stored + row] = make_float2(m, l);
@@ -689,7 +697,7 @@ __device__ __forceinline__ void halves_of(uint32_t codes, uint32_t& a, uint32_t&
     b = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, hi) - bias);
 }
 
-// Many rows: each wave has 32 of its own, and the workgroup goes through the keys together, 64 at
+// Many rows: each wave has 32 of its own (16 of large heads), and the workgroup goes through the keys together, 64 at
 // a time through two buffers in LDS.  Vector instructions bound it, so they are what the layout
 // saves: scores as in key_kernel (no conversion of keys; q's second byte costs matrix
 // instructions, which are not the bound), but the weights as fp16 on fp16 values, converted once
@@ -709,7 +717,13 @@ template <int DC> struct RowShared {
 template <int DT, int DC>
 __device__ __forceinline__ void row_item(const AttnArgs& a, const Cut& c, int block,
                                          RowShared<DC>& sh) {
-    constexpr int NQ = 2, DP = 64 * DC, DM = DP / 16, kGroup = RowShared<DC>::kGroup;
+    constexpr int NQ = row_columns(DC), DP = 64 * DC, DM = DP / 16, kGroup = RowShared<DC>::kGroup;
+    constexpr int kStep = 64 * row_waves(DC);          // threads
+    // pieces of 16 bytes in 64 keys, a thread's (the last of some threads where they do not come out even)
+    constexpr int kPieces = (4 * DP + kStep - 1) / kStep;
+    auto has_piece = [&](int i) {
+        return 4 * DP % kStep == 0 || (int)threadIdx.x + kStep * i < 4 * DP;
+    };
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
     Item it;
     if (!block_item<true>(a, c, block, it)) return;
@@ -717,17 +731,18 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Cut& c, int bl
     const Pages pages(a, it);
 
     // Thread's pieces (16 bytes) of a tile: piece u of DP a group of 16 keys.
-    v4i kr[DC], vr[DC];
-    int next_block[DC];
-    auto piece_key = [&](int i) { return (int)(threadIdx.x + kThreads * i) / DP * 16; };
-    auto piece_in = [&](int i) { return (int)(threadIdx.x + kThreads * i) % DP; };
+    v4i kr[kPieces], vr[kPieces];
+    int next_block[kPieces];
+    auto piece_key = [&](int i) { return (int)(threadIdx.x + kStep * i) / DP * 16; };
+    auto piece_in = [&](int i) { return (int)(threadIdx.x + kStep * i) % DP; };
     auto find = [&](int t) {
 #pragma unroll
-        for (int i = 0; i < DC; ++i) next_block[i] = pages.block(t * 64 + piece_key(i));
+        for (int i = 0; i < kPieces; ++i) next_block[i] = pages.block(t * 64 + piece_key(i));
     };
     auto fetch = [&](int t) {
 #pragma unroll
-        for (int i = 0; i < DC; ++i) {
+        for (int i = 0; i < kPieces; ++i) {
+            if (!has_piece(i)) continue;
             const int64_t at = pages.at(next_block[i], t * 64 + piece_key(i), DP) + piece_in(i) * 16;
             kr[i] = *reinterpret_cast<const v4i*>(a.cache.k + at);
             vr[i] = *reinterpret_cast<const v4i*>(a.cache.v + at);
@@ -736,7 +751,8 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Cut& c, int bl
     // values: [d / 16][half of the group's 16 keys][group][d % 16][8 keys]
     auto put = [&](int buf) {
 #pragma unroll
-        for (int i = 0; i < DC; ++i) {
+        for (int i = 0; i < kPieces; ++i) {
+            if (!has_piece(i)) continue;
             const int group = piece_key(i) >> 4, in = piece_in(i);
             *reinterpret_cast<v4i*>(sh.keys[buf] + group * kGroup + in * 16) = kr[i];
             uint32_t w[8];
@@ -913,25 +929,27 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Cut& c, int bl
     }
 }
 
-// What a launch does: every block of a batch whose requests all have few rows (Few1, Few2: up to
-// 16 or 32) or all have many is of one kind; in a mixed batch the first `row_blocks` take the
-// requests of many rows, the others those of up to 16.
-enum class Mix { Few1, Few2, Many, Both };
+// What a launch does: every block of a batch whose requests all have few rows or all have many is
+// of one kind; in a mixed batch the first `row_blocks` take the requests of many rows, the others
+// those of up to 16.
+enum class Mix { Few, Many, Both };
+
+constexpr int waves_of(int dc, Mix mix) { return mix == Mix::Few ? kWaves : row_waves(dc); }
 
 template <int DT, int DC, Mix MIX>
-__global__ __launch_bounds__(kThreads, DC <= 2 && MIX != Mix::Few2 ? 2 : 1) void attend_kernel(
-    AttnArgs a, Cut key, Cut row, int row_blocks) {
-    constexpr int NQ = MIX == Mix::Few2 ? 2 : 1;
-    constexpr size_t few = MIX == Mix::Many ? 0 : sizeof(KeyShared<DC, NQ>);
-    constexpr size_t many = MIX == Mix::Many || MIX == Mix::Both ? sizeof(RowShared<DC>) : 0;
+__global__ __launch_bounds__(64 * waves_of(DC, MIX), DC <= 2 || MIX != Mix::Few ? 2 : 1)
+void attend_kernel(AttnArgs a, Cut key, Cut row, int row_blocks) {
+    constexpr int waves = waves_of(DC, MIX);
+    constexpr size_t few = MIX == Mix::Many ? 0 : sizeof(KeyShared<DC, waves>);
+    constexpr size_t many = MIX == Mix::Few ? 0 : sizeof(RowShared<DC>);
     __shared__ __align__(16) char lds[few > many ? few : many];
-    if constexpr (MIX == Mix::Many || MIX == Mix::Both) {
+    if constexpr (MIX != Mix::Few) {
         if (MIX == Mix::Many || (int)blockIdx.x < row_blocks)
             return row_item<DT, DC>(a, row, blockIdx.x, *reinterpret_cast<RowShared<DC>*>(lds));
     }
     if constexpr (MIX != Mix::Many)
-        key_item<DT, DC, NQ>(a, key, blockIdx.x - row_blocks,
-                             *reinterpret_cast<KeyShared<DC, NQ>*>(lds));
+        key_item<DT, DC, waves>(a, key, blockIdx.x - row_blocks,
+                                *reinterpret_cast<KeyShared<DC, waves>*>(lds));
 }
 
 // Joins the parts of an item's rows from `first` on, a wave per row: lane s has part s's maximum
@@ -1002,7 +1020,8 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttnArgs a, Cut key, Cut
 
 // ---------------------------------------------------------------- how a call is cut
 
-constexpr int kRowTile = 32 * kWaves;
+constexpr int kRowTile = 128;
+constexpr int kFewRows = 32;
 constexpr int kMaxParts = 64;
 constexpr int kUncut = 1 << 30;
 
@@ -1019,12 +1038,14 @@ int64_t key_tiles(const AttnShape& s, int tok) {
     return (keys + 63) / 64 + 1;
 }
 
-void set_cut(Cut& c, const AttnShape& s, int rows, bool by_rows) {
+// each: tiles of every request; 0: as many as its tokens need.
+void set_cut(Cut& c, const AttnShape& s, int rows, int each) {
     const int group = s.heads / s.kv_heads;
     c.rows = rows;
     c.tok = group <= rows ? rows / group : 1;
     c.subs = group <= rows ? 1 : (group + rows - 1) / rows;
-    c.tiles = s.requests + (by_rows ? s.tokens / c.tok : 0);
+    c.each = each;
+    c.tiles = each ? s.requests * each : s.requests + s.tokens / c.tok;
 }
 
 void set_parts(Cut& c, int kind, int64_t per, int64_t tiles) {
@@ -1040,14 +1061,12 @@ int64_t at_least(int64_t a, int64_t b) { return a < b ? b : a; }
 bool plan_of(const AttnShape& s, Plan& p) {
     const int group = s.heads / s.kv_heads;
     const int64_t most = (int64_t)s.max_query * group;  // rows of a request and key head
-    const bool one = s.max_query <= 1;
-    p.mix = most <= 16 || (one && group % 32 >= 1 && group % 32 <= 16) ? Mix::Few1
-            : most <= 32 || one                                       ? Mix::Few2
+    p.mix = most <= kFewRows || s.max_query <= 1 ? Mix::Few
             // all requests of the longest length?
             : (int64_t)s.requests * s.max_query == s.tokens ? Mix::Many
                                                             : Mix::Both;
     p.has_key = p.mix != Mix::Many;
-    p.has_row = p.mix == Mix::Many || p.mix == Mix::Both;
+    p.has_row = p.mix != Mix::Few;
     auto count = [&](Cut& c) {
         const int64_t n = (int64_t)c.tiles * c.subs * s.kv_heads;
         c.items = (int)n;
@@ -1055,7 +1074,8 @@ bool plan_of(const AttnShape& s, Plan& p) {
     };
     if (p.has_key) {
         Cut& c = p.key;
-        set_cut(c, s, p.mix == Mix::Few2 ? 32 : 16, false);
+        const int tok = group <= 16 ? 16 / group : 1;
+        set_cut(c, s, 16, p.mix == Mix::Both || s.max_query < 1 ? 1 : (s.max_query + tok - 1) / tok);
         c.small = p.mix == Mix::Both ? c.tok : INT32_MAX;
         if (!count(c)) return false;
         // Parts down to one tile a wave where the batch is too small to fill the GPU (one token
@@ -1071,14 +1091,14 @@ bool plan_of(const AttnShape& s, Plan& p) {
     }
     if (p.has_row) {
         Cut& c = p.row;
-        set_cut(c, s, kRowTile, true);
+        set_cut(c, s, kRowTile, 0);
         c.small = p.has_key ? p.key.small : 0;
         if (!count(c)) return false;
         // Workgroups at a time: two on each CU, one where a head needs more of its LDS and registers.
         const int64_t slots = s.d <= 128 ? 512 : 256, tiles = key_tiles(s, c.tok);
         // Items of over half a slot's share are cut, which costs a store and a load of their rows
-        // in fp32.
-        const int64_t share = at_least((c.items * tiles + 2 * slots - 1) / (2 * slots), 16);
+        // in fp32; small batches down to a few tiles, each of which takes over a microsecond.
+        const int64_t share = at_least((c.items * tiles + 2 * slots - 1) / (2 * slots), 4);
         set_parts(c, 0, share, tiles);
         // The items that are left when the others have filled the slots some times over would leave
         // part of them idle: they are cut into as many parts as fill them best.
@@ -1137,20 +1157,24 @@ hipError_t run(const AttnArgs& a, const Plan& p, hipStream_t stream) {
     const int64_t row_blocks = p.has_row ? blocks_of(p.row) : 0;
     const int64_t key_blocks = p.has_key ? blocks_of(p.key) : 0;
     if (row_blocks + key_blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
-    const dim3 g((unsigned)(row_blocks + key_blocks)), b(kThreads);
-    const int rb = (int)row_blocks;
-    switch (p.mix) {
-        case Mix::Few1: attend_kernel<DT, DC, Mix::Few1><<<g, b, 0, stream>>>(a, p.key, p.row, rb); break;
-        case Mix::Few2: attend_kernel<DT, DC, Mix::Few2><<<g, b, 0, stream>>>(a, p.key, p.row, rb); break;
-        case Mix::Many: attend_kernel<DT, DC, Mix::Many><<<g, b, 0, stream>>>(a, p.key, p.row, rb); break;
-        case Mix::Both: attend_kernel<DT, DC, Mix::Both><<<g, b, 0, stream>>>(a, p.key, p.row, rb); break;
+    const int rb = (int)row_blocks, kb = (int)key_blocks;
+    constexpr int few = 64 * waves_of(DC, Mix::Few), many = 64 * waves_of(DC, Mix::Many);
+    bool both = p.mix == Mix::Both;
+    if constexpr (DC <= 2) {
+        if (both) attend_kernel<DT, DC, Mix::Both><<<rb + kb, many, 0, stream>>>(a, p.key, p.row, rb);
+    } else if (both) {
+        both = false;  // of large heads the few rows' code takes more registers: a launch each
     }
+    if (!both && p.has_row)
+        attend_kernel<DT, DC, Mix::Many><<<rb, many, 0, stream>>>(a, p.key, p.row, rb);
+    if (!both && p.has_key)
+        attend_kernel<DT, DC, Mix::Few><<<kb, few, 0, stream>>>(a, p.key, p.row, 0);
     const int64_t row_joins = p.has_row ? items_in_parts(p.row) * kRowJoins : 0;
     const int64_t key_joins = p.has_key ? items_in_parts(p.key) : 0;
     if (row_joins + key_joins > 0x7FFFFFFF) return hipErrorInvalidValue;
     if (row_joins + key_joins > 0)
-        join_kernel<DT, DC><<<(unsigned)(row_joins + key_joins), b, 0, stream>>>(a, p.key, p.row,
-                                                                               (int)row_joins);
+        join_kernel<DT, DC><<<(unsigned)(row_joins + key_joins), kThreads, 0, stream>>>(
+            a, p.key, p.row, (int)row_joins);
     return hipGetLastError();
 }
 
