@@ -23,7 +23,10 @@
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
 
@@ -55,12 +58,11 @@ bool plain_state() {
            !c10::impl::tls_local_dispatch_key_set().included_.has_any(kSpecialState);
 }
 
-bool plain(PyObject* o) {
-    if (!THPVariable_CheckExact(o)) return false;
-    const Tensor& t = THPVariable_Unpack(o);
+bool plain(const Tensor& t) {
     return t.defined() && t.layout() == at::kStrided && t.is_cuda() &&
            !t.key_set().has_any(kSpecialTensor) && !t._fw_grad(0).defined();
 }
+bool plain(PyObject* o) { return THPVariable_CheckExact(o) && plain(THPVariable_Unpack(o)); }
 
 int dtype_code(at::ScalarType t) {
     switch (t) {
@@ -585,81 +587,141 @@ bool logits_ok(const Tensor& x, const Tensor& ids) {
 }
 int64_t row_stride(const Tensor& x) { return x.is_contiguous() ? x.size(-1) : x.stride(0); }
 
+struct Logprobs {
+    Tensor out[6];  // the op's results
+
+    Logprobs(const Tensor& x, const Tensor& ids, int64_t top) {
+        const c10::DeviceGuard on_device(x.device());
+        const int dt = dtype_code(x.scalar_type());
+        const int64_t v = x.size(-1), rows = ids.numel();
+        const auto f32 = x.options().dtype(at::kFloat);
+        std::vector<int64_t> shape(ids.sizes().begin(), ids.sizes().end()), tops = shape,
+                             two = shape;
+        tops.push_back(top);
+        two.push_back(2);
+        for (int i = 0; i < 3; ++i) out[i] = at::empty(shape, f32);
+        out[3] = at::empty(tops, f32);
+        out[4] = at::empty(tops, ids.options());
+        out[5] = at::empty(two, f32);
+        size_t bytes = 0;
+        check(ojx_token_logprobs_workspace_bytes(rows, v, top, dt, &bytes),
+              "token_logprobs_workspace_bytes");
+        const Tensor ws = workspace(bytes, x);
+        check(ojx_token_logprobs(data(x), row_stride(x), rows, v, dt, (const int64_t*)data(ids),
+                                 top, (float*)data(out[0]), (float*)data(out[1]),
+                                 (float*)data(out[2]), (float*)data(out[5]), (float*)data(out[3]),
+                                 (int64_t*)data(out[4]), data(ws), bytes,
+                                 current_stream(x.device())),
+              "token_logprobs");
+    }
+};
+
+Tensor logprobs_gradient(const Tensor& x, const Tensor& ids, const Tensor& entropy,
+                         const Tensor& stats, const Tensor& top_ids, const Tensor* g) {
+    const c10::DeviceGuard on_device(x.device());
+    Tensor gx = at::empty(x.sizes(), x.options());
+    check(ojx_token_logprobs_bwd(data(x), row_stride(x), ids.numel(), x.size(-1),
+                                 dtype_code(x.scalar_type()), (const int64_t*)data(ids),
+                                 (const float*)data(entropy), (const float*)data(stats),
+                                 top_ids.size(-1), (const int64_t*)data(top_ids),
+                                 (const float*)data(g[0]), (const float*)data(g[1]),
+                                 (const float*)data(g[2]), (const float*)data(g[3]), data(gx),
+                                 current_stream(x.device())),
+          "token_logprobs_bwd");
+    return gx;
+}
+
+// The registered op's autograd formula as a node of the C++ engine: a Python one costs a call
+// of some rows 30 us more than its kernels run.
+struct RecordedLogprobs : torch::autograd::Function<RecordedLogprobs> {
+    using Context = torch::autograd::AutogradContext;
+    using List = torch::autograd::variable_list;
+
+    static List forward(Context* ctx, const Tensor& x, const Tensor& ids, int64_t top) {
+        Logprobs r(x, ids, top);
+        ctx->save_for_backward({x, ids, r.out[1], r.out[5], r.out[4]});
+        ctx->mark_non_differentiable({r.out[4]});
+        ctx->set_materialize_grads(false);
+        return {r.out[0], r.out[1], r.out[2], r.out[3], r.out[4]};
+    }
+
+    static List backward(Context* ctx, List grads) {
+        const List saved = ctx->get_saved_variables();
+        const Tensor& x = saved[0];
+        Tensor g[4];
+        bool any = false, known = plain_state() && plain(x), again = x.requires_grad();
+        for (int i = 0; i < 4; ++i) {
+            if (!grads[i].defined()) continue;
+            any = true;
+            again |= grads[i].requires_grad();
+            known &= plain(grads[i]) && grads[i].device() == x.device() &&
+                     grads[i].scalar_type() == at::kFloat;
+            g[i] = grads[i];
+        }
+        if (!any) return {Tensor(), Tensor(), Tensor()};
+        again &= c10::GradMode::is_enabled();
+        const at::AutoGradMode off(false);
+        Tensor gx;
+        if (known) {
+            for (Tensor& t : g)
+                if (t.defined()) t = t.contiguous();
+            RECORD_FUNCTION("ojasx_e8t::token_logprobs_bwd", std::vector<c10::IValue>());
+            gx = logprobs_gradient(x, saved[1], saved[2], saved[3], saved[4], g);
+        } else {
+            static const auto op =
+                c10::Dispatcher::singleton().findSchemaOrThrow("ojasx_e8t::token_logprobs_bwd", "");
+            std::vector<c10::IValue> stack(saved.begin(), saved.end());
+            for (const Tensor& t : g) stack.push_back(t.defined() ? c10::IValue(t) : c10::IValue());
+            op.callBoxed(stack);
+            gx = stack[0].toTensor();
+        }
+        if (again) {  // a graph of this gradient was asked for, which it has none of
+            const at::AutoGradMode on(true);
+            gx = gx.detach();
+            gx.set_requires_grad(true);
+            const auto refuse = std::make_shared<torch::autograd::DelayedError>(
+                "the gradient of token_logprobs cannot be differentiated", 1);
+            gx = (*refuse)({gx})[0];
+        }
+        return {gx, Tensor(), Tensor()};
+    }
+};
+
+// Whether token_logprobs(logits, ids, top_k) is a call on tensors as the kernels take them
+bool logprobs_ok(PyObject* const* argv, const Args& a) {
+    if (!all_plain(argv, 2)) return false;
+    const int64_t top = a.i64(2);
+    return dtype_code(a.t(0).scalar_type()) >= 0 && logits_ok(a.t(0), a.t(1)) && top >= 0 &&
+           top <= 64 && top <= a.t(0).size(-1);
+}
+
 // token_logprobs(logits, ids, top_k): the op's results
 PyObject* token_logprobs(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     expect(n, 3, "token_logprobs");
     const Args a{argv, n};
-    if (!all_plain(argv, 2)) Py_RETURN_NONE;
-    const Tensor &x = a.t(0), &ids = a.t(1);
+    if (!logprobs_ok(argv, a) || (c10::GradMode::is_enabled() && records(a.t(0)))) Py_RETURN_NONE;
     const int64_t top = a.i64(2);
-    const int dt = dtype_code(x.scalar_type());
-    if (dt < 0 || !logits_ok(x, ids) || top < 0 || top > 64 || top > x.size(-1) ||
-        (c10::GradMode::is_enabled() && records(x)))
-        Py_RETURN_NONE;
     RECORD_FUNCTION("ojasx_e8t::token_logprobs", std::vector<c10::IValue>());
     Unlocked unlocked;
-    const c10::DeviceGuard on_device(x.device());
-    const int64_t v = x.size(-1), rows = ids.numel();
-    const auto f32 = x.options().dtype(at::kFloat);
-    std::vector<int64_t> shape(ids.sizes().begin(), ids.sizes().end()), tops = shape, two = shape;
-    tops.push_back(top);
-    two.push_back(2);
-    Tensor out[] = {at::empty(shape, f32), at::empty(shape, f32), at::empty(shape, f32),
-                    at::empty(tops, f32), at::empty(tops, ids.options()), at::empty(two, f32)};
-    size_t bytes = 0;
-    check(ojx_token_logprobs_workspace_bytes(rows, v, top, dt, &bytes),
-          "token_logprobs_workspace_bytes");
-    const Tensor ws = workspace(bytes, x);
-    check(ojx_token_logprobs(data(x), row_stride(x), rows, v, dt, (const int64_t*)data(ids), top,
-                             (float*)data(out[0]), (float*)data(out[1]), (float*)data(out[2]),
-                             (float*)data(out[5]), (float*)data(out[3]), (int64_t*)data(out[4]),
-                             data(ws), bytes, current_stream(x.device())),
-          "token_logprobs");
+    Logprobs r(a.t(0), a.t(1), top);
     unlocked.lock();
-    return tuple_of(out, 6);
+    return tuple_of(r.out, 6);
     END_HANDLE_TH_ERRORS
 }
 
-// token_logprobs_bwd(logits, ids, entropy, stats, top_ids, grad_logprob | None, grad_entropy |
-// None, grad_lse | None, grad_top | None): the logits' gradient
-PyObject* token_logprobs_bwd(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+// token_logprobs_recorded(logits, ids, top_k): the op's results but the last, for autograd
+PyObject* token_logprobs_recorded(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    expect(n, 9, "token_logprobs_bwd");
+    expect(n, 3, "token_logprobs_recorded");
     const Args a{argv, n};
-    if (!all_plain(argv, 5) || c10::GradMode::is_enabled()) Py_RETURN_NONE;
-    const Tensor &x = a.t(0), &ids = a.t(1), &h = a.t(2), &stats = a.t(3), &top_ids = a.t(4);
-    const int dt = dtype_code(x.scalar_type());
-    const int64_t rows = ids.numel(), top = top_ids.dim() ? top_ids.size(-1) : 0;
-    auto floats = [&](const Tensor& t, int64_t count) {
-        return t.scalar_type() == at::kFloat && t.is_contiguous() && t.numel() == count &&
-               t.device() == x.device();
-    };
-    if (dt < 0 || !logits_ok(x, ids) || !floats(h, rows) || !floats(stats, 2 * rows) ||
-        top_ids.scalar_type() != at::kLong || top_ids.dim() != ids.dim() + 1 ||
-        top_ids.numel() != rows * top || !top_ids.is_contiguous() ||
-        top_ids.device() != x.device())
-        Py_RETURN_NONE;
-    Tensor g[4];
-    for (int i = 0; i < 4; ++i) {
-        if (argv[5 + i] == Py_None) continue;
-        if (!plain(argv[5 + i])) Py_RETURN_NONE;
-        g[i] = a.t(5 + i);
-        if (!floats(g[i], i < 3 ? rows : rows * top)) Py_RETURN_NONE;
-    }
-    RECORD_FUNCTION("ojasx_e8t::token_logprobs_bwd", std::vector<c10::IValue>());
+    if (!logprobs_ok(argv, a)) Py_RETURN_NONE;
+    const int64_t top = a.i64(2);
+    RECORD_FUNCTION("ojasx_e8t::token_logprobs", std::vector<c10::IValue>());
     Unlocked unlocked;
-    const c10::DeviceGuard on_device(x.device());
-    Tensor gx = at::empty(x.sizes(), x.options());
-    check(ojx_token_logprobs_bwd(data(x), row_stride(x), rows, x.size(-1), dt,
-                                 (const int64_t*)data(ids), (const float*)data(h),
-                                 (const float*)data(stats), top, (const int64_t*)data(top_ids),
-                                 (const float*)data(g[0]), (const float*)data(g[1]),
-                                 (const float*)data(g[2]), (const float*)data(g[3]), data(gx),
-                                 current_stream(x.device())),
-          "token_logprobs_bwd");
+    auto out = RecordedLogprobs::apply(a.t(0), a.t(1), top);
     unlocked.lock();
-    return THPVariable_Wrap(std::move(gx));
+    return tuple_of(out.data(), 5);
     END_HANDLE_TH_ERRORS
 }
 
@@ -685,7 +747,8 @@ PyMethodDef kMethods[] = {
     {"kv8_read", (PyCFunction)(void*)kv8_read, METH_FASTCALL, nullptr},
     {"kv8_attention", (PyCFunction)(void*)kv8_attention, METH_FASTCALL, nullptr},
     {"token_logprobs", (PyCFunction)(void*)token_logprobs, METH_FASTCALL, nullptr},
-    {"token_logprobs_bwd", (PyCFunction)(void*)token_logprobs_bwd, METH_FASTCALL, nullptr},
+    {"token_logprobs_recorded", (PyCFunction)(void*)token_logprobs_recorded, METH_FASTCALL,
+     nullptr},
     {"is_plain", (PyCFunction)(void*)is_plain, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -18,32 +18,6 @@ class TokenLogprobs(NamedTuple):
     top_ids: torch.Tensor       # int64 [..., top_k]; equal logits by rising token
 
 
-class _Recorded(torch.autograd.Function):
-    """token_logprobs recorded for plain eager calls (the registered op's own autograd formula,
-    without the ops' dispatch)."""
-
-    @staticmethod
-    def forward(ctx, logits, ids, top_k):
-        out = N.eager().token_logprobs(logits, ids, top_k)
-        if out is None:
-            out = S.token_logprobs(logits, ids, top_k)
-        lp, entropy, lse, top, top_ids, stats = out
-        ctx.save_for_backward(logits, ids, entropy, stats, top_ids)
-        ctx.mark_non_differentiable(top_ids)
-        ctx.set_materialize_grads(False)
-        return lp, entropy, lse, top, top_ids
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, *grads):
-        grads = grads[:4]
-        if all(g is None for g in grads):
-            return None, None, None
-        args = (*ctx.saved_tensors, *grads)
-        gx = N.eager().token_logprobs_bwd(*args)
-        return S.token_logprobs_bwd(*args) if gx is None else gx, None, None
-
-
 def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0) -> TokenLogprobs:
     """Of ``logits [..., vocabulary]`` and tokens ``ids [...]`` (int64), in one pass.
 
@@ -53,9 +27,8 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0) -> T
     differentiated); sums are in float32 whatever the logits' type.
     """
     if not torch.compiler.is_compiling():
-        out = N.eager().token_logprobs(logits, ids, top_k)  # None: to be recorded, or not plain
+        e = N.eager()  # None: with a gradient to record; not plain eager work at all
+        out = e.token_logprobs(logits, ids, top_k) or e.token_logprobs_recorded(logits, ids, top_k)
         if out is not None:
             return TokenLogprobs(*out[:5])
-        if N.eager().is_plain(logits, ids):
-            return TokenLogprobs(*_Recorded.apply(logits, ids, top_k))
     return TokenLogprobs(*S.token_logprobs(logits, ids, top_k)[:5])

@@ -3,6 +3,7 @@ the calls that have to take the registered op."""
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import kv8_plain as P
 import ojasx_amd
@@ -107,6 +108,47 @@ def test_calls_that_are_not_plain():
                              create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+def test_recorded_logprobs_in_autograd():
+    """The recorded call against the registered op's formula, as autograd meets it."""
+    ids = torch.tensor([3, -1, 100], device=DEV)
+    base = torch.randn(3, 300, device=DEV)
+
+    def both(use):
+        grads = []
+        for call in (ojasx_amd.token_logprobs, S.token_logprobs):
+            leaf = base.clone().requires_grad_(True)
+            use(leaf, lambda t, k=4: call(t, ids, k))
+            grads.append(leaf.grad)
+        assert torch.equal(*grads) and grads[0].abs().max() > 0
+
+    both(lambda t, f: f(t[:, :201])[0].sum().backward())                    # rows with a stride
+    both(lambda t, f: f(t.t().contiguous().t())[1].sum().backward())        # laid out across
+    both(lambda t, f: f(t)[3][:, ::2].sum().backward())                     # grads with holes
+    both(lambda t, f: (f(t)[0].sum() + f(t * 2)[2].sum()).backward())       # twice in a graph
+    both(lambda t, f: f(t)[0].backward(torch.ones(3, device=DEV).expand(3)))
+    both(lambda t, f: torch.utils.checkpoint.checkpoint(
+        lambda u: f(u)[0].sum(), t, use_reentrant=False).backward())
+
+    def twice(t, f):
+        y = f(t)[0].sum()
+        y.backward(retain_graph=True)
+        y.backward()
+    both(twice)
+
+    leaf = base.clone().requires_grad_(True)
+    out = ojasx_amd.token_logprobs(leaf, ids, 4)
+    assert out.logprob.requires_grad and not out.top_ids.requires_grad
+    work = leaf * 1
+    out = ojasx_amd.token_logprobs(work, ids)
+    work.add_(1)  # what the gradient is formed from
+    with pytest.raises(RuntimeError):
+        out.logprob.sum().backward()
+    out = ojasx_amd.token_logprobs(leaf.detach(), ids)
+    assert not out.logprob.requires_grad
+    with torch.no_grad():
+        assert not ojasx_amd.token_logprobs(leaf, ids).logprob.requires_grad
 
 
 def test_compiled_call_takes_the_op():
