@@ -19,122 +19,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// Request of token t: the last one that begins at or before it (tokens past the last
-// request's end have none: -1).
-__device__ __forceinline__ int request_of(const AttnArgs& a, int t) {
-    if (!a.query_starts) return t;
-    int l = 0, h = a.shape.requests;
-    while (h - l > 1) {
-        const int m = (l + h) >> 1;
-        if (a.query_starts[m] <= t) l = m; else h = m;
-    }
-    return a.query_starts[l] <= t && t < a.query_starts[l + 1] ? l : -1;
-}
-
-// ---------------------------------------------------------------- one row per wave
-
-// Everything in fp32, 64 keys at a time: a lane has a key for the scores and up to four d for
-// the values.
-template <int DT>
-__global__ __launch_bounds__(64) void row_kernel(AttnArgs a) {
-    __shared__ float q[256], p[64];
-    const KvCache& c = a.cache;
-    const int lane = threadIdx.x;
-    const int t = blockIdx.x / a.shape.heads, head = blockIdx.x % a.shape.heads;
-    const int r = request_of(a, t);
-    if (r < 0) return;
-    const int q0 = a.query_starts ? a.query_starts[r] : t;
-    const int q1 = a.query_starts ? a.query_starts[r + 1] : t + 1;
-    if (t - q0 >= a.shape.max_query) return;
-    const int len = min(a.seq_lens[r], a.shape.max_seq);
-    // keys [lo, hi)
-    const int hi = min(a.seq_lens[r] - (q1 - q0) + (t - q0) + 1, len);
-    const int lo = a.shape.window && hi > a.shape.window ? hi - a.shape.window : 0;
-    const int kvh = head / (a.shape.heads / a.shape.kv_heads);
-    bool bad = false;
-    for (int d = lane; d < c.dp; d += 64) {
-        const float x = d < c.d ? load_as_f32<DT>(a.q.p, t * a.q.token + head * a.q.head + d) : 0.f;
-        bad |= !(fabsf(x) < INFINITY);
-        q[d] = x * (a.scale * kLog2e);
-    }
-    bad = __any(bad);
-    __syncthreads();
-    float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    bool some = false;
-    const int32_t* row = a.tables + r * a.table_ld;
-    const int block = 1 << c.log_block;
-    for (int j0 = lo / 64 * 64; j0 < hi; j0 += 64) {
-        const int j = j0 + lane;
-        float s = -INFINITY, vs = 0.f;
-        int b = -1;
-        if (j >= lo && j < hi) b = row[j >> c.log_block];
-        if (b >= 0 && b < c.blocks) {
-            const int tok = j & (block - 1);
-            const int8_t* k = c.k + c.at(b, kvh) + (tok >> 4) * 16 * c.dp +
-                              ((tok & 15) >> 2) * 256 + (tok & 3) * 16;
-            float dot = 0.f;
-            for (int ch = 0; ch < c.dp >> 4; ++ch) {
-                const uint4 o = *reinterpret_cast<const uint4*>(k + (ch >> 2) * 1024 + (ch & 3) * 64);
-                const uint32_t w[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    dot = __builtin_fmaf((float)(int8_t)(w[i >> 2] >> (8 * (i & 3))), q[ch * 16 + i],
-                                         dot);
-            }
-            s = dot * c.scales[c.scale_at(b, kvh)];
-            vs = c.scales[c.scale_at(b, kvh) + 1];
-        }
-        some |= __any(b >= 0 && b < c.blocks);
-        float top = s;
-#pragma unroll
-        for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-        const float next = fmaxf(m, top);
-        const float keep = next == -INFINITY ? 1.f : exp2f(m - next);
-        float w = next == -INFINITY ? 0.f : exp2f(s - next);
-        m = next;
-        p[lane] = w * vs;
-#pragma unroll
-        for (int o = 32; o; o >>= 1) w += __shfl_xor(w, o);
-        l = l * keep + w;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] *= keep;
-        for (int g = 0; g < 4; ++g) {
-            // the 16 tokens share a block; those outside [lo, hi) have none
-            const uint64_t seen = __ballot(b >= 0 && b < c.blocks) >> (16 * g) & 0xFFFFu;
-            if (!seen) continue;
-            const int from = __shfl(b, 16 * g + __builtin_ctzll(seen));
-            const int tok = (j0 + 16 * g) & (block - 1);
-            const int8_t* v = c.v + c.at(from, kvh) + (tok >> 4) * 16 * c.dp;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int d = lane + 64 * i;
-                if (d >= c.d) continue;
-                const uint4 o = *reinterpret_cast<const uint4*>(v + d * 16);
-                const uint32_t w4[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-                for (int n = 0; n < 16; ++n)
-                    acc[i] = __builtin_fmaf(p[16 * g + n],
-                                            (float)(int8_t)(w4[n >> 2] >> (8 * (n & 3))), acc[i]);
-            }
-        }
-        __syncthreads();
-    }
-    const int64_t o0 = ((int64_t)t * a.shape.heads + head) * c.d;
-    const float nan = __uint_as_float(0x7FC00000u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int d = lane + 64 * i;
-        if (d < c.d)
-            store_from_f32<DT>(a.out, o0 + d, some ? (bad ? nan : acc[i] / l) : 0.f);
-    }
-    if (lane == 0 && a.lse)
-        a.lse[(int64_t)t * a.shape.heads + head] =
-            some ? (bad ? nan : (m + log2f(l)) * kLn2) : -INFINITY;
-}
-
-
-// ---------------------------------------------------------------- tiles of rows on int8 products
+// ---------------------------------------------------------------- items
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -163,6 +48,7 @@ struct Cut {
     int each;      // tiles of a request where every one has as many (few rows)
     int small;     // requests of at most so many tokens belong to the launch that splits keys
     int items, whole;
+    int joins;     // workgroups that join an item's parts
     int per[2];    // 64-key tiles of a part, at most
     int parts[2];  // parts of an item, at most (the launch's workgroups for each)
     float* part;   // [stored parts][rows][dp]
@@ -265,19 +151,12 @@ __device__ __forceinline__ void row_at(const AttnArgs& a, const Cut& c, const It
 }
 
 template <int DT> __device__ __forceinline__ void load8(const void* p, int64_t e, float (&x)[8]) {
-    if constexpr (DT == kF32) {
-        const float4* w = reinterpret_cast<const float4*>(static_cast<const float*>(p) + e);
-        const float4 lo = w[0], hi = w[1];
-        x[0] = lo.x; x[1] = lo.y; x[2] = lo.z; x[3] = lo.w;
-        x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
-    } else {
-        const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + e);
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + e);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = DT == kBF16 ? bf16_bits_to_f32(u[i] & 0xFFFFu) : f16_bits_to_f32(u[i] & 0xFFFFu);
-            x[2 * i + 1] = DT == kBF16 ? bf16_bits_to_f32(u[i] >> 16) : f16_bits_to_f32(u[i] >> 16);
-        }
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = DT == kBF16 ? bf16_bits_to_f32(u[i] & 0xFFFFu) : f16_bits_to_f32(u[i] & 0xFFFFu);
+        x[2 * i + 1] = DT == kBF16 ? bf16_bits_to_f32(u[i] >> 16) : f16_bits_to_f32(u[i] >> 16);
     }
 }
 
@@ -305,17 +184,12 @@ __device__ __forceinline__ v4i product(v4i a, v4i b, v4i c) {
 template <int DT>
 __device__ __forceinline__ void store_row4(void* out, int64_t e, int n, bool vec, const float (&v)[4]) {
     if (vec && n >= 4) {
-        if constexpr (DT == kF32) {
-            *reinterpret_cast<float4*>(static_cast<float*>(out) + e) =
-                make_float4(v[0], v[1], v[2], v[3]);
-        } else {
-            uint32_t b[4];
+        uint32_t b[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                b[i] = DT == kBF16 ? f32_to_bf16_bits(v[i]) : f32_to_f16_bits(v[i]);
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + e) =
-                make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
-        }
+        for (int i = 0; i < 4; ++i)
+            b[i] = DT == kBF16 ? f32_to_bf16_bits(v[i]) : f32_to_f16_bits(v[i]);
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + e) =
+            make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
         return;
     }
 #pragma unroll
@@ -339,9 +213,8 @@ template <int DC, int NQ> struct Rows {
     template <int DT>
     __device__ __forceinline__ void load(const AttnArgs& a, const Cut& c, const Item& it, int row0,
                                          int g, int n) {
-        constexpr int unit = DT == kF32 ? 4 : 8;
         const bool vec = a.shape.d % 8 == 0 && ((uintptr_t)a.q.p & 15) == 0 &&
-                         a.q.token % unit == 0 && a.q.head % unit == 0;
+                         a.q.token % 8 == 0 && a.q.head % 8 == 0;
         const float to_log2 = a.scale * kLog2e;
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
@@ -952,6 +825,192 @@ void attend_kernel(AttnArgs a, Cut key, Cut row, int row_blocks) {
                                 *reinterpret_cast<KeyShared<DC, waves>*>(lds));
 }
 
+// ---------------------------------------------------------------- fp32 rows
+
+// Queries in fp32 keep their 24 bits, which the int8 products do not hold: fp32 sums on the vector
+// units.  A workgroup has up to four rows of a key head, so a converted code serves all of them;
+// its waves take every fourth 64-key tile and are joined at the end.  For the scores a lane has a
+// key and q comes from scalar registers; for the values it has up to four d, and the weights pass
+// through LDS.
+constexpr int kFloatRows = kWaves;  // at the end a wave has a row
+constexpr float kLargest = 3e38f;
+
+template <int DC> struct FloatShared {
+    float p[kWaves][kFloatRows][64];
+    float o[kWaves][kFloatRows][64 * DC];
+    float m[kWaves][kFloatRows], l[kWaves][kFloatRows];
+};
+
+typedef const float __attribute__((address_space(4)))* scalar_floats;  // read by all lanes alike
+
+template <int DC, bool ROWS>
+__global__ __launch_bounds__(kThreads) void float_kernel(AttnArgs a, Cut c) {
+    constexpr int DP = 64 * DC, NR = kFloatRows;
+    __shared__ __align__(16) FloatShared<DC> sh;
+    const KvCache& kv = a.cache;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Item it;
+    if (!block_item<ROWS>(a, c, blockIdx.x, it)) return;
+    const float to_log2 = a.scale * kLog2e;
+    int hi[NR], lo[NR];
+    scalar_floats q[NR];
+    float m[NR], l[NR], acc[NR][DC];
+    int64_t at[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+        int tok, head;
+        row_at(a, c, it, r < it.rows ? r : 0, tok, head);
+        const int place = it.before + tok;
+        hi[r] = max(0, min(place + 1, it.len));
+        lo[r] = a.shape.window ? max(0, place + 1 - a.shape.window) : 0;
+        const int64_t token = it.q0 + it.tok0 + tok;
+        q[r] = (scalar_floats)(static_cast<const float*>(a.q.p) + token * a.q.token + head * a.q.head);
+        at[r] = token * a.shape.heads + head;
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+#pragma unroll
+        for (int i = 0; i < DC; ++i) acc[r][i] = 0.f;
+    }
+    const int32_t* pages = a.tables + it.r * a.table_ld;
+    const int inside = (1 << kv.log_block) - 1;
+    for (int t = it.t0 + wave; t < it.t1; t += kWaves) {
+        const int j = 64 * t + lane;
+        int b = j < it.end_key ? pages[j >> kv.log_block] : -1;
+        const bool have = b >= 0 && b < kv.blocks;
+        const uint64_t there = __ballot(have);
+        if (!there) continue;
+        if (!have) b = 0;  // read, not used
+        const int tok = j & inside;
+        const int8_t* k = kv.k + kv.at(b, it.head) + (tok >> 4) * 16 * DP + ((tok & 15) >> 2) * 256 +
+                          (tok & 3) * 16;
+        const float2 scales = *reinterpret_cast<const float2*>(kv.scales + kv.scale_at(b, it.head));
+        float s[NR] = {};
+        for (int d0 = 0; d0 < a.shape.d; d0 += 16) {
+            const uint4 w4 = *reinterpret_cast<const uint4*>(k + (d0 >> 6) * 1024 + (d0 & 63) * 4);
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+            float x[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = (float)(int8_t)(w[i >> 2] >> (8 * (i & 3)));
+            if (d0 + 16 <= a.shape.d) {
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[r] = __builtin_fmaf(x[i], q[r][d0 + i], s[r]);
+            } else {
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (d0 + i < a.shape.d) s[r] = __builtin_fmaf(x[i], q[r][d0 + i], s[r]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            const bool sees = have && j >= lo[r] && j < hi[r];
+            // finite, so a row that sees a key has a weight of 1; NaN becomes so too, and the row's
+            // end writes NaN
+            const float x = sees ? __builtin_amdgcn_fmed3f(s[r] * scales.x * to_log2, -kLargest, kLargest)
+                                 : -INFINITY;
+            const float next = fmaxf(m[r], wave_max(x));
+            const bool none = next == -INFINITY;
+            const float keep = none ? 1.f : exp2f(m[r] - next);
+            const float w = none ? 0.f : exp2f(x - next);
+            m[r] = next;
+            l[r] = __builtin_fmaf(l[r], keep, w);
+            sh.p[wave][r][lane] = w * scales.y;
+#pragma unroll
+            for (int i = 0; i < DC; ++i) acc[r][i] *= keep;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int g = 0; g < 4; ++g) {
+            // the 16 tokens share a block, whichever of them is there
+            const uint64_t those = there >> (16 * g) & 0xFFFFu;
+            if (!those) continue;
+            const int from = __builtin_amdgcn_readlane(b, 16 * g + __builtin_ctzll(those));
+            const int8_t* v = kv.v + kv.at(from, it.head) + (((64 * t + 16 * g) & inside) >> 4) * 16 * DP;
+            uint4 code[DC];
+#pragma unroll
+            for (int i = 0; i < DC; ++i)
+                code[i] = *reinterpret_cast<const uint4*>(v + (lane + 64 * i) * 16);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                float4 p[NR];
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+                    p[r] = *reinterpret_cast<const float4*>(&sh.p[wave][r][16 * g + 4 * n]);
+#pragma unroll
+                for (int i = 0; i < DC; ++i) {
+                    const uint32_t w = n == 0 ? code[i].x : n == 1 ? code[i].y
+                                     : n == 2 ? code[i].z : code[i].w;
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) {
+                        acc[r][i] = __builtin_fmaf(p[r].x, (float)(int8_t)w, acc[r][i]);
+                        acc[r][i] = __builtin_fmaf(p[r].y, (float)(int8_t)(w >> 8), acc[r][i]);
+                        acc[r][i] = __builtin_fmaf(p[r].z, (float)(int8_t)(w >> 16), acc[r][i]);
+                        acc[r][i] = __builtin_fmaf(p[r].w, (float)(int8_t)(w >> 24), acc[r][i]);
+                    }
+                }
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+        const float sum = wave_sum(l[r]);
+        if (lane == 0) {
+            sh.m[wave][r] = m[r];
+            sh.l[wave][r] = sum;
+        }
+#pragma unroll
+        for (int i = 0; i < DC; ++i) sh.o[wave][r][lane + 64 * i] = acc[r][i];
+    }
+    __syncthreads();
+    if (wave >= it.rows) return;
+    // row `wave`
+    int64_t mine = at[0];
+    scalar_floats mine_q = q[0];
+#pragma unroll
+    for (int r = 1; r < NR; ++r)
+        if (wave == r) {
+            mine = at[r];
+            mine_q = q[r];
+        }
+    bool bad = false;
+    for (int d = lane; d < a.shape.d; d += 64) bad |= !(fabsf(mine_q[d] * to_log2) < INFINITY);
+    bad = __any(bad);
+    float top = -INFINITY, sum = 0.f, o[DC] = {};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, sh.m[w][wave]);
+    const bool some = top != -INFINITY;
+    if (some) {
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float f = exp2f(sh.m[w][wave] - top);
+            sum = __builtin_fmaf(f, sh.l[w][wave], sum);
+#pragma unroll
+            for (int i = 0; i < DC; ++i) o[i] = __builtin_fmaf(f, sh.o[w][wave][lane + 64 * i], o[i]);
+        }
+    }
+    const float nan = __uint_as_float(0x7FC00000u);
+    if (it.parts > 1) {
+        if (lane == 0) c.ml[it.stored + wave] = make_float2(bad && some ? nan : top, sum);
+        if (!some) return;
+#pragma unroll
+        for (int i = 0; i < DC; ++i) c.part[(it.stored + wave) * DP + lane + 64 * i] = o[i];
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < DC; ++i) {
+        const int d = lane + 64 * i;
+        if (d < a.shape.d)
+            static_cast<float*>(a.out)[mine * a.shape.d + d] = !some ? 0.f : bad ? nan : o[i] / sum;
+    }
+    if (a.lse && lane == 0) a.lse[mine] = !some ? -INFINITY : bad ? nan : (top + log2f(sum)) * kLn2;
+}
+
+// ---------------------------------------------------------------- the parts' join
+
 // Joins the parts of an item's rows from `first` on, a wave per row: lane s has part s's maximum
 // and sum.
 template <int DT, int DC, bool ROWS>
@@ -1006,15 +1065,13 @@ __device__ __forceinline__ void join_item(const AttnArgs& a, const Cut& c, int i
     }
 }
 
-constexpr int kRowJoins = 8;  // workgroups of an item of many rows
-
 template <int DT, int DC>
 __global__ __launch_bounds__(kThreads) void join_kernel(AttnArgs a, Cut key, Cut row, int row_blocks) {
     const int b = blockIdx.x;
     // items that can have parts: all, or the last ones
     if (b < row_blocks)
-        return join_item<DT, DC, true>(a, row, (row.parts[0] > 1 ? 0 : row.whole) + b / kRowJoins,
-                                       b % kRowJoins * kWaves, kRowJoins * kWaves);
+        return join_item<DT, DC, true>(a, row, (row.parts[0] > 1 ? 0 : row.whole) + b / row.joins,
+                                       b % row.joins * kWaves, row.joins * kWaves);
     join_item<DT, DC, false>(a, key, (key.parts[0] > 1 ? 0 : key.whole) + b - row_blocks, 0, kWaves);
 }
 
@@ -1044,6 +1101,7 @@ void set_cut(Cut& c, const AttnShape& s, int rows, int each) {
     c.rows = rows;
     c.tok = group <= rows ? rows / group : 1;
     c.subs = group <= rows ? 1 : (group + rows - 1) / rows;
+    c.joins = rows < 32 ? 1 : rows / 16;
     c.each = each;
     c.tiles = each ? s.requests * each : s.requests + s.tokens / c.tok;
 }
@@ -1070,8 +1128,24 @@ bool plan_of(const AttnShape& s, Plan& p) {
     auto count = [&](Cut& c) {
         const int64_t n = (int64_t)c.tiles * c.subs * s.kv_heads;
         c.items = (int)n;
-        return n <= (1 << 24);
+        return n <= INT32_MAX;
     };
+    if (s.dtype == kF32) {
+        // Parts for some waves on every SIMD, of a tile a wave at least.
+        const bool single = s.max_query <= 1;
+        p.mix = single ? Mix::Few : Mix::Many;
+        p.has_key = single;
+        p.has_row = !single;
+        Cut& c = single ? p.key : p.row;
+        set_cut(c, s, kFloatRows, single ? 1 : 0);
+        c.small = single ? INT32_MAX : 0;
+        if (!count(c)) return false;
+        const int64_t tiles = key_tiles(s, c.tok);
+        set_parts(c, 1, at_least((c.items * tiles + 2047) / 2048, kWaves), tiles);
+        c.parts[0] = 1;
+        c.per[0] = kUncut;
+        return true;
+    }
     if (p.has_key) {
         Cut& c = p.key;
         const int tok = group <= 16 ? 16 / group : 1;
@@ -1158,18 +1232,26 @@ hipError_t run(const AttnArgs& a, const Plan& p, hipStream_t stream) {
     const int64_t key_blocks = p.has_key ? blocks_of(p.key) : 0;
     if (row_blocks + key_blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
     const int rb = (int)row_blocks, kb = (int)key_blocks;
-    constexpr int few = 64 * waves_of(DC, Mix::Few), many = 64 * waves_of(DC, Mix::Many);
-    bool both = p.mix == Mix::Both;
-    if constexpr (DC <= 2) {
-        if (both) attend_kernel<DT, DC, Mix::Both><<<rb + kb, many, 0, stream>>>(a, p.key, p.row, rb);
-    } else if (both) {
-        both = false;  // of large heads the few rows' code takes more registers: a launch each
+    if constexpr (DT == kF32) {
+        if (p.has_row)
+            float_kernel<DC, true><<<rb, kThreads, 0, stream>>>(a, p.row);
+        else
+            float_kernel<DC, false><<<kb, kThreads, 0, stream>>>(a, p.key);
+    } else {
+        constexpr int few = 64 * waves_of(DC, Mix::Few), many = 64 * waves_of(DC, Mix::Many);
+        bool both = p.mix == Mix::Both;
+        if constexpr (DC <= 2) {
+            if (both)
+                attend_kernel<DT, DC, Mix::Both><<<rb + kb, many, 0, stream>>>(a, p.key, p.row, rb);
+        } else if (both) {
+            both = false;  // of large heads the few rows' code takes more registers: a launch each
+        }
+        if (!both && p.has_row)
+            attend_kernel<DT, DC, Mix::Many><<<rb, many, 0, stream>>>(a, p.key, p.row, rb);
+        if (!both && p.has_key)
+            attend_kernel<DT, DC, Mix::Few><<<kb, few, 0, stream>>>(a, p.key, p.row, 0);
     }
-    if (!both && p.has_row)
-        attend_kernel<DT, DC, Mix::Many><<<rb, many, 0, stream>>>(a, p.key, p.row, rb);
-    if (!both && p.has_key)
-        attend_kernel<DT, DC, Mix::Few><<<kb, few, 0, stream>>>(a, p.key, p.row, 0);
-    const int64_t row_joins = p.has_row ? items_in_parts(p.row) * kRowJoins : 0;
+    const int64_t row_joins = p.has_row ? items_in_parts(p.row) * p.row.joins : 0;
     const int64_t key_joins = p.has_key ? items_in_parts(p.key) : 0;
     if (row_joins + key_joins > 0x7FFFFFFF) return hipErrorInvalidValue;
     if (row_joins + key_joins > 0)
@@ -1191,7 +1273,7 @@ template <int DT> hipError_t run(const AttnArgs& a, const Plan& p, hipStream_t s
 
 size_t kv8_attention_bytes(const AttnShape& s) {
     Plan p{};
-    if (s.dtype == kF32 || s.tokens == 0 || s.requests == 0 || !plan_of(s, p)) return 0;
+    if (s.tokens == 0 || s.requests == 0 || !plan_of(s, p)) return 0;
     return (p.has_key ? cut_bytes(p.key, s) : 0) + (p.has_row ? cut_bytes(p.row, s) : 0);
 }
 
@@ -1199,19 +1281,17 @@ hipError_t launch_kv8_attention(const AttnArgs& args, void* ws, size_t ws_bytes,
                                 hipStream_t stream) {
     AttnArgs a = args;
     if (a.cache.blocks == 0) a.shape.max_seq = 0;  // nothing to see
-    if (a.shape.dtype == kF32) {
-        const int64_t rows = (int64_t)a.shape.tokens * a.shape.heads;
-        if (rows > 0x7FFFFFFF) return hipErrorInvalidValue;
-        row_kernel<kF32><<<(unsigned)rows, 64, 0, stream>>>(a);
-        return hipGetLastError();
-    }
     Plan p{};
     if (!plan_of(a.shape, p)) return hipErrorInvalidValue;
     char* at = static_cast<char*>(ws);
     size_t left = ws ? ws_bytes : 0;
     if (p.has_key) place(p.key, a.shape, at, left);
     if (p.has_row) place(p.row, a.shape, at, left);
-    return a.shape.dtype == kF16 ? run<kF16>(a, p, stream) : run<kBF16>(a, p, stream);
+    switch (a.shape.dtype) {
+        case kF32: return run<kF32>(a, p, stream);
+        case kF16: return run<kF16>(a, p, stream);
+        default: return run<kBF16>(a, p, stream);
+    }
 }
 
 }  // namespace ojx
