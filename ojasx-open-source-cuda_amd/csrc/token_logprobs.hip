@@ -153,7 +153,6 @@ __device__ __forceinline__ bool ordinary(const Sums& a) {
 struct Best {
     uint64_t key;   // 0: none yet
     float least;    // the k-th one's logit; -inf while there are fewer
-    bool full;
 };
 
 __device__ __forceinline__ uint64_t read_lane(uint64_t v, int lane) {
@@ -216,14 +215,16 @@ __device__ __forceinline__ void settle(Best& b, Pool& pool, int n, int k, int la
         __builtin_amdgcn_wave_barrier();
     }
     const uint64_t last = read_lane(b.key, k - 1);
-    b.full = last != 0;
-    b.least = b.full ? unordered((uint32_t)(last >> 32)) : -INFINITY;
+    b.least = last != 0 ? unordered((uint32_t)(last >> 32)) : -INFINITY;
 }
 
 constexpr int kLaneLogits = 32;                  // logits of a lane in one batch
 constexpr int kBatch = 64 * kLaneLogits;         // of a wave
 constexpr int kGroups = kThreads / 64;
 constexpr int kMaxRowSplits = 64;
+// Lanes whose maximum is the bound of a batch's candidates, from which on their places are bounded
+// too: fewer hold at most one pool of equal logits.
+constexpr int kTied = kPool / kLaneLogits;
 
 template <int DT> struct Batch {
     static constexpr int kVec = DT == kF32 ? 4 : 8;  // logits of 16 bytes
@@ -294,35 +295,73 @@ template <int DT> struct Batch {
     }
 };
 
-// Takes a batch's candidates into the wave's best k.  Batches come by rising token, so a later
-// logit that only equals the k-th one loses.  Where many lanes have a candidate (all at first), the
-// k-th largest of the lanes' maxima is a bound under which none can stay: about k candidates are
-// left whatever the row's order.
+// The least float over x (of -inf: the lowest finite one).
+__device__ __forceinline__ float above(float x) { return unordered(ordered(x) + 1); }
+
+// Puts the lanes' keys (0: none) behind the pool's first n, which are taken first where they leave
+// no room.  Returns the number then there; `settled` tells of the best k's change.
+__device__ __forceinline__ int push(Best& b, Pool& pool, int n, bool on, uint64_t key, int k, int lane,
+                                    bool& settled) {
+    const uint64_t c = __ballot(on);
+    settled = n + __popcll(c) + k > kPool;
+    if (settled) {
+        settle(b, pool, n, k, lane);
+        n = 0;
+    }
+    const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(c >> 32),
+                                                 __builtin_amdgcn_mbcnt_lo((uint32_t)c, 0));
+    if (on) pool.keys[at] = key;
+    return n + __popcll(c);
+}
+
+// Takes a batch's candidates into the wave's best k: logits of at least `lo`.  Batches come by
+// rising token, so a later logit that only equals the k-th one loses; within a batch it may not.
+// Where many lanes have a candidate (all at first), the k-th largest of the lanes' maxima is a
+// bound under which none can stay: about k candidates are left whatever the row's order.  Logits
+// that equal this bound in many lanes (a row of one value, a mask of the type's lowest one) are
+// bounded by their places alike.  -inf is no candidate (finish adds what a row lacks), nor is the
+// padding beyond the row's ends.
 template <int DT>
-__device__ __forceinline__ void take(Best& best, const Batch<DT>& x, float lane_max, int b, int k,
+__device__ __forceinline__ void take(Best& best, Batch<DT>& x, float lane_max, int b, int k,
                                      int lane, int shift, Pool& pool) {
-    const bool may = !best.full || lane_max > best.least;
+    const bool may = lane_max > best.least;
     const uint64_t lanes = __ballot(may);
     if (!lanes) return;
-    float cut = -INFINITY;
-    const int many = __popcll(lanes);
-    if (many >= k && (many > k + 12 || !best.full))
-        cut = kth_of_lanes(may ? lane_max : -INFINITY, k, lane, pool);
-    uint64_t open = best.full ? 0ull : ~0ull;
+    float lo = above(best.least);
     int n = 0;
+    bool settled;
+    const int many = __popcll(lanes);
+    if (many >= k && (many > k + 12 || best.least == -INFINITY)) {
+        const float cut = kth_of_lanes(may ? lane_max : -INFINITY, k, lane, pool);
+        lo = fmaxf(lo, cut);
+        if (__popcll(__ballot(lane_max == cut)) > kTied) {
+            lo = above(cut);
+            constexpr int kVec = Batch<DT>::kVec;
+            uint32_t equal = 0;
+#pragma unroll
+            for (int i = 0; i < kLaneLogits; ++i) equal |= x.get(i) == cut ? 1u << i : 0u;
+            x.drop_floats();
+            // a lane's logits come by rising token, kVec together
+            auto place = [&](int i) { return (i / kVec * 64 + lane) * kVec + i % kVec; };
+            __builtin_amdgcn_wave_barrier();
+            const int last = (int)-kth_of_lanes(
+                equal ? -(float)place(__builtin_ctz(equal)) : -(float)kBatch, k, lane, pool);
+            __builtin_amdgcn_wave_barrier();
+            for (;;) {
+                const int i = __builtin_ctz(equal | 1u << 31);
+                const bool on = equal && place(i) <= last;
+                if (!__any(on)) break;
+                n = push(best, pool, n, on, key_of(cut, b * kBatch + place(i) - shift), k, lane, settled);
+                equal &= equal - 1;
+            }
+        }
+    }
 #pragma unroll
     for (int i = 0; i < kLaneLogits; ++i) {
         const float f = x.get(i);
-        const uint64_t c = __ballot(f >= cut) & (__ballot(f > best.least) | open);
-        if (!c) continue;
-        if (n + __popcll(c) + k > kPool) {
-            settle(best, pool, n, k, lane);
-            n = 0;
-        }
-        const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(c >> 32),
-                                                     __builtin_amdgcn_mbcnt_lo((uint32_t)c, 0));
-        if (c >> lane & 1) pool.keys[at] = key_of(f, Batch<DT>::index(b, i, lane, shift));
-        n += __popcll(c);
+        if (!__any(f >= lo)) continue;
+        n = push(best, pool, n, f >= lo, key_of(f, Batch<DT>::index(b, i, lane, shift)), k, lane, settled);
+        if (settled) lo = fmaxf(lo, best.least);
     }
     if (n) settle(best, pool, n, k, lane);
 }
@@ -356,17 +395,45 @@ __device__ __forceinline__ void finish(const LogprobArgs& a, int row, const Sums
         a.logprob[row] = asked.in ? log_p(asked.x) : 0.f;
         a.entropy[row] = (l2 - t.u / t.s) * kLn2;
     }
+    if (n == 0) return;
     // a key's rank is its place
+    bool lacks = false;
     for (int i = threadIdx.x; i < n; i += kThreads) {
         const uint64_t k = keys[i];
         int rank = 0;
 #pragma unroll 8
         for (int j = 0; j < n; ++j) rank += keys[j] > k;
-        if (rank < a.top) {
+        if (rank >= a.top) continue;
+        if (k != 0) {
             const int64_t o = (int64_t)row * a.top + rank;
             a.top_ids[o] = 0xFFFFFFFFu - (uint32_t)k;
             a.top_lp[o] = log_p(unordered((uint32_t)(k >> 32)));
+        } else {
+            lacks = true;
         }
+    }
+    if (!__syncthreads_or(lacks)) return;
+    // Fewer logits than alternatives: masked ones follow, by rising token.
+    int have = 0;
+    for (int j = 0; j < n; ++j) have += keys[j] != 0;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int j0 = 0; j0 < a.vocab && have < a.top; j0 += kThreads) {
+        const int j = j0 + threadIdx.x;
+        const bool masked = j < a.vocab && load_as_f32<DT>(a.x, row * a.ld + j) == -INFINITY;
+        const uint64_t those = __ballot(masked);
+        if (lane == 0) sk[wave] = __popcll(those);
+        __syncthreads();
+        int rank = have + __popcll(those & ((1ull << lane) - 1));
+        for (int w = 0; w < kGroups; ++w) {
+            if (w < wave) rank += (int)sk[w];
+            have += (int)sk[w];
+        }
+        if (masked && rank < a.top) {
+            const int64_t o = (int64_t)row * a.top + rank;
+            a.top_ids[o] = j;
+            a.top_lp[o] = -INFINITY;
+        }
+        __syncthreads();
     }
 }
 
@@ -396,7 +463,7 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(LogprobArgs a, Parts p) 
     const int per = (batches + p.splits - 1) / p.splits;
     const int end = min(batches, (split + 1) * per);
     Sums t{-INFINITY, 0.f, 0.f, -INFINITY};
-    Best best{0, -INFINITY, false};
+    Best best{0, -INFINITY};
     B x;
     int b = split * per + wave;
     for (; b < end; b += kGroups) {
@@ -456,7 +523,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(LogprobArgs a, Parts p) 
     if (!few) {
         // every split's list is in order; the first is the wave's to begin with
         const uint64_t* list = from + wave * a.top + lane;
-        Best b{wave < p.splits && lane < a.top ? *list : 0, 0.f, false};
+        Best b{wave < p.splits && lane < a.top ? *list : 0, 0.f};
         for (int s = wave + kGroups; s < p.splits; s += kGroups) {
             list += kGroups * a.top;
             const uint64_t k = lane < a.top ? *list : 0;

@@ -109,6 +109,30 @@ def test_masked_rows(dtype, v):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,v,top", [(1, 2054, 20), (2, 70001, 64), (300, 4100, 5)])
+def test_few_allowed_tokens(dtype, rows, v, top):
+    # fewer logits than alternatives, at the ends, together and far apart; the others masked
+    for low in (-math.inf, torch.finfo(dtype).min):
+        x = torch.full((rows, v), low)
+        x[0, [0, v // 2, v - 1]] = torch.tensor([1.0, 3.0, 2.0])
+        if rows > 1:
+            x[1, v - 3:] = 0.25
+            x[2:, 7::v // 4] = 0.5
+        _check(x.to(dtype), _ids(rows, v), top)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v", [2048, 9000])
+def test_equal_logits_among_rising_and_falling_ones(dtype, v):
+    # more candidates than are kept at a time, equal ones among them in both orders of place
+    j = torch.arange(v)
+    x = torch.stack([(j // 3 % 900).float(), (j // 64).float(), (j % 64).float(),
+                     -(j // 5 % 700).float(), (j // 40 * 7 % 64).float()]) / 32
+    _check(x.to(dtype), _ids(5, v), 64)
+    _check(x.to(dtype), _ids(5, v), 33)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("v", [9, 3000, 40000])
 def test_nan_and_infinity(dtype, v):
     x = _logits(3, v, dtype, v)
