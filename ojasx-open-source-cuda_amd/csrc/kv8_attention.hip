@@ -27,11 +27,12 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 
-// Waves of a workgroup, and 16-row columns of a wave, where each wave has rows of its own: 128 rows
-// either way.  Heads of up to 128 leave registers for two columns a wave and two such workgroups
-// on a CU; larger ones take eight waves of one column, still two on a SIMD.
-constexpr int row_waves(int dc) { return dc <= 2 ? 4 : 8; }
-constexpr int row_columns(int dc) { return dc <= 2 ? 2 : 1; }
+// Where each wave has rows of its own, a workgroup has 128 or 64.  Heads of up to 128 leave the
+// registers for two 16-row columns in each of four waves, or one (how a call is cut says when).
+// Larger ones have one: four waves at up to 192 (22 requests of up to 1796 tokens 170 us, 192 with
+// eight), eight over that (13 of up to 2038 tokens 249 us, 397 with four).
+constexpr int row_columns(int dc, int rows) { return dc <= 2 && rows == 128 ? 2 : 1; }
+constexpr int row_waves(int dc, int rows) { return rows / (16 * row_columns(dc, rows)); }
 constexpr float kFixed = 32512.f;  // largest fixed-point value: 127 * 256 with its low part 0
 constexpr float kMagic = 12582912.f + 128.f;  // 1.5 * 2^23: the sum's low bits are the integer
 constexpr float kLeastScale = 0x1p-100f;
@@ -570,9 +571,9 @@ __device__ __forceinline__ void halves_of(uint32_t codes, uint32_t& a, uint32_t&
     b = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, hi) - bias);
 }
 
-// Many rows: each wave has 32 of its own (16 of large heads), and the workgroup goes through the keys together, 64 at
-// a time through two buffers in LDS.  Vector instructions bound it, so they are what the layout
-// saves: scores as in key_kernel (no conversion of keys; q's second byte costs matrix
+// Many rows: each wave has 32 or 16 of its own, and the workgroup goes through the keys together,
+// 64 at a time through two buffers in LDS.  Vector instructions bound it, so they are what the layout
+// saves: scores as for few rows (no conversion of keys; q's second byte costs matrix
 // instructions, which are not the bound), but the weights as fp16 on fp16 values, converted once
 // for the workgroup on their way into LDS: the products then add up in fp32 in the matrix unit,
 // where whole-number products would cost three vector instructions for every result of every 64
@@ -587,11 +588,11 @@ template <int DC> struct RowShared {
     _Float16 values[2][64 * 64 * DC];
 };
 
-template <int DT, int DC>
+template <int DT, int DC, int ROWS>
 __device__ __forceinline__ void row_item(const AttnArgs& a, const Cut& c, int block,
                                          RowShared<DC>& sh) {
-    constexpr int NQ = row_columns(DC), DP = 64 * DC, DM = DP / 16, kGroup = RowShared<DC>::kGroup;
-    constexpr int kStep = 64 * row_waves(DC);          // threads
+    constexpr int NQ = row_columns(DC, ROWS), DP = 64 * DC, DM = DP / 16, kGroup = RowShared<DC>::kGroup;
+    constexpr int kStep = 64 * row_waves(DC, ROWS);    // threads
     // pieces of 16 bytes in 64 keys, a thread's (the last of some threads where they do not come out even)
     constexpr int kPieces = (4 * DP + kStep - 1) / kStep;
     auto has_piece = [&](int i) {
@@ -807,18 +808,20 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Cut& c, int bl
 // those of up to 16.
 enum class Mix { Few, Many, Both };
 
-constexpr int waves_of(int dc, Mix mix) { return mix == Mix::Few ? kWaves : row_waves(dc); }
+constexpr int waves_of(int dc, Mix mix, int rows) {
+    return mix == Mix::Few ? kWaves : row_waves(dc, rows);
+}
 
-template <int DT, int DC, Mix MIX>
-__global__ __launch_bounds__(64 * waves_of(DC, MIX), DC <= 2 || MIX != Mix::Few ? 2 : 1)
+template <int DT, int DC, Mix MIX, int ROWS>
+__global__ __launch_bounds__(64 * waves_of(DC, MIX, ROWS), DC <= 2 || MIX != Mix::Few ? 2 : 1)
 void attend_kernel(AttnArgs a, Cut key, Cut row, int row_blocks) {
-    constexpr int waves = waves_of(DC, MIX);
+    constexpr int waves = waves_of(DC, MIX, ROWS);
     constexpr size_t few = MIX == Mix::Many ? 0 : sizeof(KeyShared<DC, waves>);
     constexpr size_t many = MIX == Mix::Few ? 0 : sizeof(RowShared<DC>);
     __shared__ __align__(16) char lds[few > many ? few : many];
     if constexpr (MIX != Mix::Few) {
         if (MIX == Mix::Many || (int)blockIdx.x < row_blocks)
-            return row_item<DT, DC>(a, row, blockIdx.x, *reinterpret_cast<RowShared<DC>*>(lds));
+            return row_item<DT, DC, ROWS>(a, row, blockIdx.x, *reinterpret_cast<RowShared<DC>*>(lds));
     }
     if constexpr (MIX != Mix::Many)
         key_item<DT, DC, waves>(a, key, blockIdx.x - row_blocks,
@@ -1077,7 +1080,6 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttnArgs a, Cut key, Cut
 
 // ---------------------------------------------------------------- how a call is cut
 
-constexpr int kRowTile = 128;
 constexpr int kFewRows = 32;
 constexpr int kMaxParts = 64;
 constexpr int kUncut = 1 << 30;
@@ -1165,11 +1167,20 @@ bool plan_of(const AttnShape& s, Plan& p) {
     }
     if (p.has_row) {
         Cut& c = p.row;
-        set_cut(c, s, kRowTile, 0);
+        // Workgroups at a time: two on each CU, one where a head needs more of its LDS.
+        const int64_t slots = s.d <= 192 ? 512 : 256;
+        // Tiles of 128 rows read and convert the keys for more rows (four chunks of up to 2048
+        // tokens: 411 us, 535 at 64 rows); those of 64 are through theirs sooner, so they are for
+        // batches of few tiles a slot (7 requests of 62 to 550 tokens: 14.8 us, 30.2 at 128).
+        // Around 16 tiles a slot both come out alike.
+        int64_t tiles = 0;
+        for (int rows = s.d <= 128 || s.d > 192 ? 128 : 64;; rows = 64) {
+            set_cut(c, s, rows, 0);
+            if (!count(c)) return false;
+            tiles = key_tiles(s, c.tok);
+            if (rows == 64 || s.d > 192 || c.items * tiles >= 16 * slots) break;
+        }
         c.small = p.has_key ? p.key.small : 0;
-        if (!count(c)) return false;
-        // Workgroups at a time: two on each CU, one where a head needs more of its LDS and registers.
-        const int64_t slots = s.d <= 128 ? 512 : 256, tiles = key_tiles(s, c.tok);
         // Items of over half a slot's share are cut, which costs a store and a load of their rows
         // in fp32; small batches down to a few tiles, each of which takes over a microsecond.
         const int64_t share = at_least((c.items * tiles + 2 * slots - 1) / (2 * slots), 4);
@@ -1226,6 +1237,24 @@ void place(Cut& c, const AttnShape& s, char*& ws, size_t& left) {
     left -= need;
 }
 
+template <int DT, int DC, int ROWS>
+void attend(const AttnArgs& a, const Plan& p, int row_blocks, int key_blocks, hipStream_t stream) {
+    constexpr int few = 64 * waves_of(DC, Mix::Few, ROWS), many = 64 * waves_of(DC, Mix::Many, ROWS);
+    bool both = p.mix == Mix::Both;
+    if constexpr (DC <= 2) {
+        if (both)
+            attend_kernel<DT, DC, Mix::Both, ROWS>
+                <<<row_blocks + key_blocks, many, 0, stream>>>(a, p.key, p.row, row_blocks);
+    } else if (both) {
+        both = false;  // of large heads the few rows' code takes more registers: a launch each
+    }
+    if (!both && p.has_row)
+        attend_kernel<DT, DC, Mix::Many, ROWS>
+            <<<row_blocks, many, 0, stream>>>(a, p.key, p.row, row_blocks);
+    if (!both && p.has_key)
+        attend_kernel<DT, DC, Mix::Few, 0><<<key_blocks, few, 0, stream>>>(a, p.key, p.row, 0);
+}
+
 template <int DT, int DC>
 hipError_t run(const AttnArgs& a, const Plan& p, hipStream_t stream) {
     const int64_t row_blocks = p.has_row ? blocks_of(p.row) : 0;
@@ -1238,18 +1267,12 @@ hipError_t run(const AttnArgs& a, const Plan& p, hipStream_t stream) {
         else
             float_kernel<DC, false><<<kb, kThreads, 0, stream>>>(a, p.key);
     } else {
-        constexpr int few = 64 * waves_of(DC, Mix::Few), many = 64 * waves_of(DC, Mix::Many);
-        bool both = p.mix == Mix::Both;
         if constexpr (DC <= 2) {
-            if (both)
-                attend_kernel<DT, DC, Mix::Both><<<rb + kb, many, 0, stream>>>(a, p.key, p.row, rb);
-        } else if (both) {
-            both = false;  // of large heads the few rows' code takes more registers: a launch each
+            if (p.has_row && p.row.rows == 64) attend<DT, DC, 64>(a, p, rb, kb, stream);
+            else attend<DT, DC, 128>(a, p, rb, kb, stream);
+        } else {
+            attend<DT, DC, DC == 3 ? 64 : 128>(a, p, rb, kb, stream);
         }
-        if (!both && p.has_row)
-            attend_kernel<DT, DC, Mix::Many><<<rb, many, 0, stream>>>(a, p.key, p.row, rb);
-        if (!both && p.has_key)
-            attend_kernel<DT, DC, Mix::Few><<<kb, few, 0, stream>>>(a, p.key, p.row, 0);
     }
     const int64_t row_joins = p.has_row ? items_in_parts(p.row) * p.row.joins : 0;
     const int64_t key_joins = p.has_key ? items_in_parts(p.key) : 0;
