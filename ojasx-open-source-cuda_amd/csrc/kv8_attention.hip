@@ -45,7 +45,7 @@ struct Cut {
     int rows;      // rows of a tile
     int tok;       // tokens of a tile
     int subs;      // tiles of one token's heads of a key head
-    int tiles;     // tiles (upper bound), without subs and key heads
+    int64_t tiles; // tiles (upper bound), without subs and key heads
     int each;      // tiles of a request where every one has as many (few rows)
     int small;     // requests of at most so many tokens belong to the launch that splits keys
     int items, whole;
@@ -1080,7 +1080,10 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttnArgs a, Cut key, Cut
 
 // ---------------------------------------------------------------- how a call is cut
 
-constexpr int kFewRows = 32;
+// Rows of a request and key head up to which it is done in tiles of 16 with the keys split over the
+// waves, each tile reading the keys again (50 requests of up to 36 rows over up to 7700 keys: 91 us,
+// 156 with rows split over the waves; at 64 rows of 16 requests over 2000 keys it would be 52 to 36).
+constexpr int kFewRows = 48;
 constexpr int kMaxParts = 64;
 constexpr int kUncut = 1 << 30;
 
@@ -1105,7 +1108,7 @@ void set_cut(Cut& c, const AttnShape& s, int rows, int each) {
     c.subs = group <= rows ? 1 : (group + rows - 1) / rows;
     c.joins = rows < 32 ? 1 : rows / 16;
     c.each = each;
-    c.tiles = each ? s.requests * each : s.requests + s.tokens / c.tok;
+    c.tiles = each ? (int64_t)s.requests * each : (int64_t)s.requests + s.tokens / c.tok;
 }
 
 void set_parts(Cut& c, int kind, int64_t per, int64_t tiles) {
@@ -1128,9 +1131,9 @@ bool plan_of(const AttnShape& s, Plan& p) {
     p.has_key = p.mix != Mix::Many;
     p.has_row = p.mix != Mix::Few;
     auto count = [&](Cut& c) {
-        const int64_t n = (int64_t)c.tiles * c.subs * s.kv_heads;
-        c.items = (int)n;
-        return n <= INT32_MAX;
+        const int64_t n = (int64_t)c.subs * s.kv_heads;
+        c.items = (int)(c.tiles * n);
+        return c.tiles <= INT32_MAX / n;
     };
     if (s.dtype == kF32) {
         // Parts for some waves on every SIMD, of a tile a wave at least.
@@ -1174,7 +1177,7 @@ bool plan_of(const AttnShape& s, Plan& p) {
         // batches of few tiles a slot (7 requests of 62 to 550 tokens: 14.8 us, 30.2 at 128).
         // Around 16 tiles a slot both come out alike.
         int64_t tiles = 0;
-        for (int rows = s.d <= 128 || s.d > 192 ? 128 : 64;; rows = 64) {
+        for (int rows = s.d > 192 || (s.d <= 128 && most > 64) ? 128 : 64;; rows = 64) {
             set_cut(c, s, rows, 0);
             if (!count(c)) return false;
             tiles = key_tiles(s, c.tok);

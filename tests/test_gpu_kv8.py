@@ -318,6 +318,45 @@ def test_several_tokens(dtype, block, hkv, group, d, new):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hkv,group,d,new", [
+    (2, 4, 128, [9, 1, 11, 4]), (1, 1, 64, [17, 33, 48, 2]), (1, 3, 200, [16, 7, 1, 12]),
+    (1, 20, 80, [2, 1, 2, 0]), (2, 7, 96, [6, 5, 3, 1])])
+def test_a_few_rows_of_a_request(dtype, hkv, group, d, new):
+    # up to 48 of a key head: several tiles of a request in one launch, over few and many keys
+    for ctx in ([0, 3, 60, 200], [700, 0, 64, 1500]):
+        tables, lens, starts, total = _batch(ctx, new, 32)
+        cache = _make(32, hkv, d, total)
+        q = torch.randn(starts[-1], hkv * group, d).to(dtype).to(DEV)
+        _check_attention(cache, q, tables, lens, starts, max_query_len=max(new))
+        _check_attention(cache, q, tables, lens, starts, max_query_len=max(new), window=77)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hkv,group,d,new", [
+    (2, 4, 128, [130, 3, 64]), (1, 2, 64, [200, 90, 1]), (2, 5, 40, [70, 26, 51]),
+    (1, 4, 192, [90, 33, 2]), (1, 3, 256, [100, 44, 0]), (2, 1, 96, [256, 128, 129])])
+def test_rows_under_long_bounds(dtype, hkv, group, d, new):
+    # tables of many more columns than the requests use: the launch is sized for long ones
+    tables, lens, starts, total = _batch([0, 300, 70], new, 64, extra=1100)
+    cache = _make(64, hkv, d, total)
+    q = torch.randn(starts[-1], hkv * group, d).to(dtype).to(DEV)
+    _check_attention(cache, q, tables, lens, starts)
+    _check_attention(cache, q, tables, lens, starts, window=100, max_query_len=max(new))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("extra", [0, 500])
+def test_more_tiles_than_workgroups_at_a_time(dtype, extra):
+    # also requests of equal length, which need no place for shorter ones
+    ctx = [(37 * i) % 150 for i in range(90)]
+    for new in ([(7 * i) % 23 + 1 for i in range(90)], [20] * 90):
+        tables, lens, starts, total = _batch(ctx, new, 16, extra=extra)
+        cache = _make(16, 6, 32, total)
+        q = torch.randn(starts[-1], 18, 32).to(dtype).to(DEV)
+        _check_attention(cache, q, tables, lens, starts, max_query_len=max(new))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("window", [1, 2, 15, 16, 17, 63, 64, 65, 100, 1000])
 def test_windows(dtype, window):
     ctx, new = [0, 5, 100, 333], [3, 1, 70, 2]
