@@ -342,7 +342,9 @@ struct Pages {
 // Tile t of the four score products takes 4 keys of each group of 16: a lane then holds the 16
 // scores of one group (one block: one pair of scales), and their weights are the second operand
 // of the value products as they come.  The workgroup's waves take turns at 64 keys of a 16-row tile
-// and join their results in LDS.  (Two tiles of rows for one pass over the keys would need more
+// and join their results in LDS.  Memory bounds it where there are many keys (64 tokens over 500 to
+// 16000 tokens, 631 MB: 124 us and 5 for the join, 4.9 TB/s), launches and latency where there are
+// few (one over 2048 tokens: 6.1 us and 3.5 for the join).  (Two tiles of rows for one pass over the keys would need more
 // than half of a SIMD's registers: two workgroups that share the keys in the L2 cache are faster.)
 template <int DC, int WAVES> struct KeyShared {
     static constexpr int kLd = 64 * DC + 4;
@@ -578,7 +580,9 @@ __device__ __forceinline__ void halves_of(uint32_t codes, uint32_t& a, uint32_t&
 // for the workgroup on their way into LDS: the products then add up in fp32 in the matrix unit,
 // where whole-number products would cost three vector instructions for every result of every 64
 // keys.  The reference of the weights is raised only when one would pass 2^kHeadroom times it, so
-// the sums are scaled again rarely.
+// the sums are scaled again rarely.  Four chunks of 900 to 2048 tokens over up to 8000 (321 GF):
+// 400 us and 10 for the join, 780 Tflop/s of the two products; the matrix unit is busy for a third
+// of the time, q's second byte included, vector instructions for most of the rest: 12 for a score.
 constexpr float kHeadroom = 8.f;
 
 template <int DC> struct RowShared {
@@ -834,7 +838,8 @@ void attend_kernel(AttnArgs a, Cut key, Cut row, int row_blocks) {
 // units.  A workgroup has up to four rows of a key head, so a converted code serves all of them;
 // its waves take every fourth 64-key tile and are joined at the end.  For the scores a lane has a
 // key and q comes from scalar registers; for the values it has up to four d, and the weights pass
-// through LDS.
+// through LDS.  Vector products bound it: 4 x 512 tokens over 2048 (60 GF) 1230 us, 49 Tflop/s; 64
+// tokens over 9000 325 us; one over 32768 42 us.
 constexpr int kFloatRows = kWaves;  // at the end a wave has a row
 constexpr float kLargest = 3e38f;
 
