@@ -339,8 +339,12 @@ __device__ __forceinline__ void take(Best& best, Batch<DT>& x, float lane_max, i
             constexpr int kVec = Batch<DT>::kVec;
             uint32_t equal = 0;
 #pragma unroll
-            for (int i = 0; i < kLaneLogits; ++i) equal |= x.get(i) == cut ? 1u << i : 0u;
-            x.drop_floats();
+            for (int i = 0; i < kLaneLogits; ++i) {
+                // one after the other: all conversions at once would cost a wave of occupancy
+                if constexpr (DT != kF32)
+                    asm volatile("" : "+v"(equal), "+v"((&x.w[i / kVec].x)[i % kVec * 4 / kVec]));
+                equal |= x.get(i) == cut ? 1u << i : 0u;
+            }
             // a lane's logits come by rising token, kVec together
             auto place = [&](int i) { return (i / kVec * 64 + lane) * kVec + i % kVec; };
             __builtin_amdgcn_wave_barrier();
