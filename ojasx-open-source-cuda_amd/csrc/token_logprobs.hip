@@ -192,8 +192,9 @@ __device__ __forceinline__ float kth_of_lanes(float v, int k, int lane, Pool& po
     return -wave_max(above < k ? -v : -INFINITY);
 }
 
-// Takes the first n of the pool into the best k: a few one by one (about 200 cycles each), more
-// by their ranks among all of them and the k.
+// Takes the first n of the pool into the best k: up to four one by one, about 200 cycles each, more
+// by their ranks among all of them and the k (4096 rows of 32000 with 5 alternatives: 72 us, 79 by
+// ranks alone).
 __device__ __forceinline__ void settle(Best& b, Pool& pool, int n, int k, int lane) {
     __builtin_amdgcn_wave_barrier();
     if (n <= 4) {
@@ -450,7 +451,7 @@ struct Parts {
 
 // A workgroup reads a row, or with splits > 1 a part of it, once: every wave keeps its sums and
 // its best k.  Without alternatives memory bounds it (2048 rows of 128256 bf16, 525 MB: 125 us,
-// 4.2 TB/s), with them vector instructions (4096 rows of 32000 fp16 with 5: 77 us, 3.4 TB/s: a
+// 4.2 TB/s), with them vector instructions (4096 rows of 32000 fp16 with 5: 72 us, 3.6 TB/s: a
 // conversion, a maximum, an exponential, two sums and a compare for every logit).
 template <int DT, bool TOP>
 __global__ __launch_bounds__(kThreads) void pass_kernel(LogprobArgs a, Parts p) {
@@ -631,7 +632,7 @@ template <class F> void by_dtype(int dtype, F f) {
 }
 
 // Splits of a row: until the workgroups fill the GPU twice, none under a batch per wave (77 rows of
-// 50021: 17 us, 19.4 with a quarter of them; 4096 rows of 32000: 77 us unsplit, 99 in two).
+// 50021: 17 us, 19.4 with a quarter of them; 4096 rows of 32000: 72 us unsplit, 90 in two).
 int row_splits(int rows, int vocab) {
     const int64_t most = ((int64_t)vocab + kBatch * kGroups - 1) / (kBatch * kGroups);
     int64_t n = rows > 0 ? 2048 / rows : 1;
