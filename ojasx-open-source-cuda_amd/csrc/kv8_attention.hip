@@ -807,6 +807,25 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Cut& c, int bl
     }
 }
 
+// First token past the last request's: read where a kernel begins, beside its other first loads.
+__device__ __forceinline__ int last_start(const AttnArgs& a) {
+    return a.query_starts ? a.query_starts[a.shape.requests] : a.shape.tokens;
+}
+
+// The launch's share of the rows of tokens from `end` on, which belong to no request (a padded
+// batch): zeros, as for rows that see nothing.
+template <int DT> __device__ __forceinline__ void no_request(const AttnArgs& a, int end) {
+    if (end >= a.shape.tokens) return;
+    const int64_t rows = (int64_t)a.shape.tokens * a.shape.heads;
+    const int64_t first = (int64_t)max(end, 0) * a.shape.heads;
+    const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const int64_t step = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t i = first * a.shape.d + at; i < rows * a.shape.d; i += step)
+        store_from_f32<DT>(a.out, i, 0.f);
+    if (a.lse)
+        for (int64_t i = first + at; i < rows; i += step) a.lse[i] = -INFINITY;
+}
+
 // What a launch does: every block of a batch whose requests all have few rows or all have many is
 // of one kind; in a mixed batch the first `row_blocks` take the requests of many rows, the others
 // those of up to 16.
@@ -823,13 +842,15 @@ void attend_kernel(AttnArgs a, Cut key, Cut row, int row_blocks) {
     constexpr size_t few = MIX == Mix::Many ? 0 : sizeof(KeyShared<DC, waves>);
     constexpr size_t many = MIX == Mix::Few ? 0 : sizeof(RowShared<DC>);
     __shared__ __align__(16) char lds[few > many ? few : many];
-    if constexpr (MIX != Mix::Few) {
-        if (MIX == Mix::Many || (int)blockIdx.x < row_blocks)
-            return row_item<DT, DC, ROWS>(a, row, blockIdx.x, *reinterpret_cast<RowShared<DC>*>(lds));
-    }
-    if constexpr (MIX != Mix::Many)
+    const int end = last_start(a);
+    if (MIX == Mix::Many || (MIX == Mix::Both && (int)blockIdx.x < row_blocks)) {
+        if constexpr (MIX != Mix::Few)
+            row_item<DT, DC, ROWS>(a, row, blockIdx.x, *reinterpret_cast<RowShared<DC>*>(lds));
+    } else if constexpr (MIX != Mix::Many) {
         key_item<DT, DC, waves>(a, key, blockIdx.x - row_blocks,
                                 *reinterpret_cast<KeyShared<DC, waves>*>(lds));
+    }
+    no_request<DT>(a, end);
 }
 
 // ---------------------------------------------------------------- fp32 rows
@@ -852,9 +873,8 @@ template <int DC> struct FloatShared {
 typedef const float __attribute__((address_space(4)))* scalar_floats;  // read by all lanes alike
 
 template <int DC, bool ROWS>
-__global__ __launch_bounds__(kThreads) void float_kernel(AttnArgs a, Cut c) {
+__device__ __forceinline__ void float_item(const AttnArgs& a, const Cut& c, FloatShared<DC>& sh) {
     constexpr int DP = 64 * DC, NR = kFloatRows;
-    __shared__ __align__(16) FloatShared<DC> sh;
     const KvCache& kv = a.cache;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1015,6 +1035,14 @@ __global__ __launch_bounds__(kThreads) void float_kernel(AttnArgs a, Cut c) {
             static_cast<float*>(a.out)[mine * a.shape.d + d] = !some ? 0.f : bad ? nan : o[i] / sum;
     }
     if (a.lse && lane == 0) a.lse[mine] = !some ? -INFINITY : bad ? nan : (top + log2f(sum)) * kLn2;
+}
+
+template <int DC, bool ROWS>
+__global__ __launch_bounds__(kThreads) void float_kernel(AttnArgs a, Cut c) {
+    __shared__ __align__(16) FloatShared<DC> sh;
+    const int end = last_start(a);
+    float_item<DC, ROWS>(a, c, sh);
+    no_request<kF32>(a, end);
 }
 
 // ---------------------------------------------------------------- the parts' join

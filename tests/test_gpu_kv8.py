@@ -397,6 +397,25 @@ def test_rows_that_see_nothing(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [[1, 0, 1], [1, 3, 2], [70, 5, 90]])
+@pytest.mark.parametrize("d", [64, 100, 256])
+def test_tokens_of_no_request_are_zero(dtype, new, d):
+    tables, lens, starts, total = _batch([30, 0, 9], new, 16)
+    cache = _make(16, 2, d, total)
+    end = starts[-1]
+    q = torch.randn(end + 300, 6, d).to(dtype).to(DEV)
+
+    def call(_, tables, lens, starts, **kw):
+        torch.full((4 * q.numel(),), math.nan, device=DEV)  # outputs take memory that held NaN
+        out, lse = cache.attention(q, tables, lens, starts, **kw)
+        assert not out[end:].any() and torch.isneginf(lse[end:]).all()
+        return out[:end], lse[:end]
+
+    _check_attention(cache, q[:end], tables, lens, starts, call=call)
+    _check_attention(cache, q[:end], tables, lens, starts, call=call, max_query_len=max(new))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("scale", [0.0, -0.3, 4.0])
 def test_scales_of_the_softmax(dtype, scale):
     tables, lens, starts, total = _batch([100, 20], [1, 9], 16)
