@@ -433,8 +433,9 @@ int ojx_kv8_attention(const void* q, int64_t q_token_stride, int64_t q_head_stri
  * token ids[row] (0 where it is outside [0, vocab)), entropy [rows], lse [rows], stats [rows][2]
  * = (largest logit, log of the sum of exp(logit - largest)), whose sum lse is before rounding, and
  * the top_k (0..64, at most vocab) largest in falling order, equal ones by rising token:
- * top_logprobs, top_ids [rows][top_k].  Everything in fp32.  A row of -inf only has lse -inf, entropy 0 and log
- * probabilities -inf; NaN or +inf in a row makes its results NaN (NaN counts as the largest). */
+ * top_logprobs, top_ids [rows][top_k].  Everything in fp32.  A row of -inf only has lse -inf,
+ * entropy 0 and log probabilities -inf; NaN or +inf in a row makes its results NaN (NaN counts as
+ * the largest). */
 int ojx_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int64_t top_k, int dtype,
                                        size_t* bytes);
 int ojx_token_logprobs(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int dtype,

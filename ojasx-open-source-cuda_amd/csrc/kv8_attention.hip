@@ -342,10 +342,11 @@ struct Pages {
 // Tile t of the four score products takes 4 keys of each group of 16: a lane then holds the 16
 // scores of one group (one block: one pair of scales), and their weights are the second operand
 // of the value products as they come.  The workgroup's waves take turns at 64 keys of a 16-row tile
-// and join their results in LDS.  Memory bounds it where there are many keys (64 tokens over 500 to
-// 16000 tokens, 631 MB: 124 us and 5 for the join, 4.9 TB/s), launches and latency where there are
-// few (one over 2048 tokens: 6.1 us and 3.5 for the join).  (Two tiles of rows for one pass over the keys would need more
-// than half of a SIMD's registers: two workgroups that share the keys in the L2 cache are faster.)
+// and join their results in LDS.  (Two tiles of rows for one pass over the keys would need more
+// than half of a SIMD's registers: two workgroups that share the keys in L2 are faster.)
+// Memory bounds it where there are many keys (64 tokens over 500 to 16000 tokens, 631 MB: 124 us
+// and 5 for the join, 4.9 TB/s), launches and latency where there are few (one over 2048 tokens:
+// 6.1 us and 3.5 for the join).
 template <int DC, int WAVES> struct KeyShared {
     static constexpr int kLd = 64 * DC + 4;
     float joined[WAVES * 16 * kLd];
@@ -574,8 +575,8 @@ __device__ __forceinline__ void halves_of(uint32_t codes, uint32_t& a, uint32_t&
 }
 
 // Many rows: each wave has 32 or 16 of its own, and the workgroup goes through the keys together,
-// 64 at a time through two buffers in LDS.  Vector instructions bound it, so they are what the layout
-// saves: scores as for few rows (no conversion of keys; q's second byte costs matrix
+// 64 at a time through two buffers in LDS.  Vector instructions bound it, so they are what the
+// layout saves: scores as for few rows (no conversion of keys; q's second byte costs matrix
 // instructions, which are not the bound), but the weights as fp16 on fp16 values, converted once
 // for the workgroup on their way into LDS: the products then add up in fp32 in the matrix unit,
 // where whole-number products would cost three vector instructions for every result of every 64
@@ -597,7 +598,8 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Cut& c, int bl
                                          RowShared<DC>& sh) {
     constexpr int NQ = row_columns(DC, ROWS), DP = 64 * DC, DM = DP / 16, kGroup = RowShared<DC>::kGroup;
     constexpr int kStep = 64 * row_waves(DC, ROWS);    // threads
-    // pieces of 16 bytes in 64 keys, a thread's (the last of some threads where they do not come out even)
+    // a thread's pieces of 16 bytes of 64 keys (some threads have one less where they do not come
+    // out even)
     constexpr int kPieces = (4 * DP + kStep - 1) / kStep;
     auto has_piece = [&](int i) {
         return 4 * DP % kStep == 0 || (int)threadIdx.x + kStep * i < 4 * DP;
@@ -1113,9 +1115,9 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttnArgs a, Cut key, Cut
 
 // ---------------------------------------------------------------- how a call is cut
 
-// Rows of a request and key head up to which it is done in tiles of 16 with the keys split over the
-// waves, each tile reading the keys again (50 requests of up to 36 rows over up to 7700 keys: 91 us,
-// 156 with rows split over the waves; at 64 rows of 16 requests over 2000 keys it would be 52 to 36).
+// Rows of a request and key head up to which it is done in tiles of 16 with the keys split over
+// the waves, each tile reading the keys again (50 requests of up to 36 rows over up to 7700 keys:
+// 91 us, 156 with rows split over the waves; 16 requests of 64 rows over 2000 keys: 52 to 36).
 constexpr int kFewRows = 48;
 constexpr int kMaxParts = 64;
 constexpr int kUncut = 1 << 30;
