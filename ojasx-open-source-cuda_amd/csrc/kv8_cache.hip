@@ -791,7 +791,9 @@ hipError_t launch_kv8_plan(const PlanArgs& a, hipStream_t stream) {
 
 hipError_t launch_kv8_append(const KvCache& c, const KvRows& k, const KvRows& v, int dtype,
                              const int64_t* slots, int tokens, hipStream_t stream) {
-    const int64_t held = (int64_t)c.d << c.log_block;
+    // Elements that a run's units cover at most: a key's are whole chunks of 16, so a head of 8
+    // takes as much room as one of 16; values' units are never more.
+    const int64_t held = ((int64_t)c.d + 15) / 16 * 16 << c.log_block;
     const bool vec = rows_vector(k, dtype) && rows_vector(v, dtype);
     // Rows that a run is held in registers of: 16-bit ones on a 16-byte grid (append and read of
     // 21500 tokens of 8 x 80: 43 us, 79 where they are read twice).  The others, fp32 among them,
