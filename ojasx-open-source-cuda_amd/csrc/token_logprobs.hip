@@ -91,12 +91,12 @@ __device__ __forceinline__ void odd_row(const LogprobArgs& a, int row, float* sf
         a.logprob[row] = in ? log_p(load_as_f32<DT>(a.x, x0 + id)) : 0.f;
         a.entropy[row] = bad ? nan : none ? 0.f : ls - u / s;
     }
-    uint64_t last = ~0ull;
+    uint64_t last = ~0ull;  // which is also the key of NaN at token 0: the first pass takes any
     for (int i = 0; i < a.top; ++i) {
         uint64_t best = 0;
         for (int j = threadIdx.x; j < v; j += kThreads) {
             const uint64_t k = key_of(load_as_f32<DT>(a.x, x0 + j), j);
-            if (k < last && k > best) best = k;
+            if ((i == 0 || k < last) && k > best) best = k;
         }
         last = block_reduce(best, sk, [](uint64_t p, uint64_t q) { return p > q ? p : q; });
         if (threadIdx.x == 0) {
