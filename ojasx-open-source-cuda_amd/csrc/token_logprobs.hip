@@ -19,7 +19,10 @@ namespace {
 constexpr int kThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kPlainMax = 1e30f;
+// Largest |logit| that the one pass over a row takes as a reference (struct Sums): its rounding in
+// binary units is an exponent's error, up to 2^3 here (half of the spacing at 1.44e8).  2^(2^3) is
+// harmless in a sum; at 3e9 it would be 2^128, an infinity.
+constexpr float kPlainMax = 1e8f;
 
 // fp32 bits in rising order as unsigned, -0 as +0, NaN above everything.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -50,7 +53,7 @@ template <class T, class F> __device__ T block_reduce(T v, T* shared, F f) {
 // ---------------------------------------------------------------- rows out of the ordinary
 
 // A row with NaN or infinities, or whose largest logit is beyond +-kPlainMax (all of it masked
-// by a type's lowest value, say): one workgroup, one pass for the maximum, one for the sums,
+// by a large negative value, say): one workgroup, one pass for the maximum, one for the sums,
 // one per alternative.
 template <int DT>
 __device__ __forceinline__ void odd_row(const LogprobArgs& a, int row, float* sf, uint64_t* sk) {
@@ -111,7 +114,9 @@ __device__ __forceinline__ void odd_row(const LogprobArgs& a, int row, float* sf
 
 // Sums of some of a row's logits in binary units: r a reference near the largest of them times
 // log2(e), s = sum 2^t and u = sum t 2^t over t = x log2(e) - r.  r is only a reference: its own
-// rounding does not enter.  m is the largest logit itself.
+// rounding is in every t alike and leaves the results, as long as it is small enough for the sums
+// to hold 2^rounding (kPlainMax: lanes of larger masks only have none).  m is the largest logit
+// itself.
 struct Sums {
     float r, s, u, m;
 };
