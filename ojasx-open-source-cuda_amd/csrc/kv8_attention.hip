@@ -307,10 +307,23 @@ __device__ __forceinline__ float largest(const v4f (&x)[4]) {
     return top;
 }
 
-// A reference below every score (and no infinity, whose differences would be NaN), and the least
-// factor of a score: times -inf it stays -inf.
+// A reference below every score (and no infinity, whose differences would be NaN), the score that
+// larger ones count as, and the least and the largest factor of a score: times -inf it stays -inf,
+// times 0 it is 0.
 constexpr float kNone = -1e30f;
+constexpr float kFar = 9e29f;
 constexpr float kLeastFactor = 0x1p-120f;
+constexpr float kLargestFactor = 0x1p120f;
+
+__device__ __forceinline__ float score_factor(float q_unit, float key_scale) {
+    return __builtin_amdgcn_fmed3f(q_unit * key_scale, kLeastFactor, kLargestFactor);
+}
+
+// The exponent of a lane's largest score `top` (-inf: it sees none): top * f + lv, within kFar.
+__device__ __forceinline__ float far_or(float top, float f, float lv) {
+    const float m = __builtin_amdgcn_fmed3f(__builtin_fmaf(top, f, lv), -kFar, kFar);
+    return top == -INFINITY ? top : m;
+}
 
 // The block of a group of 16 keys (-1: none) and its bytes' offset.
 struct Pages {
@@ -447,16 +460,19 @@ __device__ __forceinline__ void key_item(const AttnArgs& a, const Cut& c, int bl
         float beta[NQ];
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
-            const float f = fmaxf(rows.qs[q] * ks, kLeastFactor);
-            const float m = fmaxf(col_max(__builtin_fmaf(largest(x[q]), f, lv)), kNone);
-            const float base = lv - m;
+            // Exponents as differences from the lane's largest score, which are exact: x * f + (lv -
+            // m) is off by m's rounding, and a weight over 1 does not fit its 16 bits.
+            const float f = score_factor(rows.qs[q], ks), top = largest(x[q]);
+            const float mine = far_or(top, f, lv);
+            const float m = fmaxf(col_max(mine), kNone);
+            const float from = fmaxf(top, -0x1p31f), base = mine - m;
             float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float p[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float e = fast_exp2(__builtin_fmaf(x[q][i][r], f, base));
+                    const float e = fast_exp2(__builtin_fmaf(x[q][i][r] - from, f, base));
                     sum += e;
                     p[r] = __builtin_fmaf(e, kFixed, kMagic);
                 }
