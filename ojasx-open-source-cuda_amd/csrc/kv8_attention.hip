@@ -601,6 +601,10 @@ __device__ __forceinline__ void halves_of(uint32_t codes, uint32_t& a, uint32_t&
 // 400 us and 10 for the join, 780 Tflop/s of the two products; the matrix unit is busy for a third
 // of the time, q's second byte included, vector instructions for most of the rest: 12 for a score.
 constexpr float kHeadroom = 8.f;
+// References up to which the weights' exponents are x * f + (lv - ref): that difference's rounding
+// is under 2^-12 then.  Beyond, they are formed from differences of scores, in the step that also
+// raises the reference, so that other rows do not pay an instruction a score for it.
+constexpr float kNearReference = 0x1p12f;
 
 template <int DC> struct RowShared {
     // bytes of 16 keys: groups begin in different banks
@@ -690,10 +694,12 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Cut& c, int bl
     }
 
     v4f o[NQ][DM];
-    float ref[NQ], l_run[NQ];
+    // `step`: exponents above it take the step below
+    float ref[NQ], step[NQ], l_run[NQ];
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
         ref[q] = kNone;
+        step[q] = -INFINITY;
         l_run[q] = 0.f;
 #pragma unroll
         for (int i = 0; i < DM; ++i) o[q][i] = v4f{0.f, 0.f, 0.f, 0.f};
@@ -745,11 +751,13 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Cut& c, int bl
             v8h p[NQ][2];
 #pragma unroll
             for (int q = 0; q < NQ; ++q) {
-                const float f = fmaxf(rows.qs[q] * ks, kLeastFactor);
-                float m = __builtin_fmaf(largest(x[q]), f, lv);
-                if (!__all(m <= ref[q] + kHeadroom)) {
-                    m = col_max(m);
-                    const float next = m > ref[q] + kHeadroom ? m : ref[q];
+                const float f = score_factor(rows.qs[q], ks), top = largest(x[q]);
+                float base = lv - ref[q];
+                if (!__all(__builtin_fmaf(top, f, lv) <= step[q])) {
+                    const float mine = far_or(top, f, lv);
+                    const float m = col_max(mine);
+                    // the difference is exact where the sum may round up to twice the headroom
+                    const float next = m - ref[q] > kHeadroom ? m : ref[q];
                     const float keep = fast_exp2(ref[q] - next);
                     l_run[q] *= keep;
 #pragma unroll
@@ -757,8 +765,15 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Cut& c, int bl
 #pragma unroll
                         for (int r = 0; r < 4; ++r) o[q][i][r] *= keep;
                     ref[q] = next;
+                    const bool near = fabsf(next) < kNearReference;
+                    step[q] = near ? next + kHeadroom : -INFINITY;
+                    const float from = near ? 0.f : fmaxf(top, -0x1p31f);
+                    base = near ? lv - next : mine - next;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) x[q][i][r] -= from;
                 }
-                const float base = lv - ref[q];
                 float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)

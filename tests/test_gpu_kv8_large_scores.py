@@ -78,3 +78,11 @@ def test_few_rows(dtype, size):
     _check([1, 1, 1], 96, 64, size, dtype, 16)
     _check([3, 1, 2], 200, 32, size, dtype, 3)
     _check([5, 2], 64, 64, size, dtype, 6, max_query_len=5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", SIZES)
+def test_many_rows(dtype, size):
+    _check([70, 9, 33], 64, 16, size, dtype, 4)
+    _check([100, 90, 1], 128, 64, size, dtype, 2, max_query_len=100)
+    _check([64, 64], 256, 32, size, dtype, 2)
