@@ -1092,12 +1092,12 @@ __device__ __forceinline__ void join_item(const AttnArgs& a, const Cut& c, int i
     const float nan = __uint_as_float(0x7FC00000u);
     for (int row = first + (threadIdx.x >> 6); row < it.rows; row += step) {
         const int64_t at0 = it.stored + row;
-        float2 ml = make_float2(kNone, 0.f);
+        float2 ml = make_float2(-INFINITY, 0.f);
         if (lane < it.parts) ml = c.ml[at0 + lane * stride];
         const bool some = ml.y > 0.f;
         const bool bad = __any(some && ml.x != ml.x);
-        float m = some && !bad ? ml.x : kNone;
-        m = wave_max(m);
+        // a part with a key has a finite reference, in fp32 also one under kNone
+        const float m = wave_max(some && !bad ? ml.x : -INFINITY);
         const float keep = some && !bad ? fast_exp2(ml.x - m) : 0.f;
         const float l = wave_sum(keep * ml.y);
         float sum[DC];

@@ -86,3 +86,15 @@ def test_many_rows(dtype, size):
     _check([70, 9, 33], 64, 16, size, dtype, 4)
     _check([100, 90, 1], 128, 64, size, dtype, 2, max_query_len=100)
     _check([64, 64], 256, 32, size, dtype, 2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [[1, 1, 1], [70, 40, 3]])
+def test_scores_beyond_32_bits_leave_a_row_its_keys(dtype, new):
+    # no score is a finite float: the row still sees its keys
+    cache, tables, lens, starts, q, _ = _case(new, 64, 16, 1.0, dtype, 4)
+    cache.scales[:, :, 0] = 1e4
+    out, lse = cache.attention(q, _i32(tables), _i32(lens), _i32(starts), scale=1e37,
+                               return_lse=True)
+    assert torch.isfinite(out).all() and not torch.isneginf(lse).any() and not lse.isnan().any()
+    assert (out.abs().amax(-1) > 0).all()
