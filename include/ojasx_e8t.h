@@ -411,10 +411,11 @@ int ojx_kv8_read(const int8_t* k_codes, const int8_t* v_codes, const float* scal
  * request.  q, out: [tokens][heads][head_dim] in dtype (strides of q in elements, out
  * contiguous), heads a multiple of kv_heads, consecutive heads sharing one.  lse (may be NULL):
  * float [tokens][heads], the natural logarithm of the softmax's sum.  A row that sees nothing
- * gets zeros and -inf, and so do tokens past query_starts[requests]; a row of q with NaN or
- * infinities gets NaN.  max_query_len and max_seq_len: no request has more (they size the launch;
- * tokens beyond them are not computed).  The workspace holds partial results of a split over the
- * keys; a smaller one (or none) only lowers the split. */
+ * gets zeros and -inf, and so do tokens before query_starts[0] and past query_starts[requests];
+ * a row of q with NaN or infinities gets NaN.  max_query_len and max_seq_len size the launch: of a
+ * request that has more, the first max_query_len newest tokens are computed (the others get zeros
+ * and -inf), over its first max_seq_len keys.  The workspace holds partial results of a split over
+ * the keys; a smaller one (or none) only lowers the split. */
 int ojx_kv8_attention_workspace_bytes(int64_t tokens, int64_t requests, int64_t heads,
                                       int64_t kv_heads, int64_t head_dim, int64_t window,
                                       int64_t max_query_len, int64_t max_seq_len, int dtype,

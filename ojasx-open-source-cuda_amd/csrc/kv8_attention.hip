@@ -73,8 +73,28 @@ struct Item {
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The item `id` in its part `split`; false: none.
-template <bool ROWS>
+// Zeros in n rows from `first` on, as in rows that see nothing: a thread takes every `step`-th
+// element from `at` on.
+template <int DT>
+__device__ __forceinline__ void clear(const AttnArgs& a, int64_t first, int64_t n, int64_t at,
+                                      int64_t step) {
+    for (int64_t i = first * a.shape.d + at; i < (first + n) * a.shape.d; i += step)
+        store_from_f32<DT>(a.out, i, 0.f);
+    if (a.lse)
+        for (int64_t i = first + at; i < first + n; i += step) a.lse[i] = -INFINITY;
+}
+
+// The workgroup's heads of tokens [from, to).
+template <int DT>
+__device__ __forceinline__ void clear_heads(const AttnArgs& a, const Item& it, int from, int to) {
+    for (int t = from; t < to; ++t)
+        clear<DT>(a, (int64_t)t * a.shape.heads + it.head * it.group, it.group, threadIdx.x, blockDim.x);
+}
+
+// The item `id` in its part `split`; false: none.  CLEAR: rows that no item has are cleared by the
+// workgroup of a first item beside them, which has read where they are: of tokens past a request's
+// max_query, of those before the first request (further loads would cost small calls 0.4 us).
+template <bool ROWS, int DT, bool CLEAR>
 __device__ __forceinline__ bool find_item(const AttnArgs& a, const Cut& c, int id, int split, Item& it) {
     it.id = id;
     it.split = split;
@@ -89,7 +109,6 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, const Cut& c, int i
         q0 = a.query_starts ? a.query_starts[it.r] : it.r;
         q1 = a.query_starts ? a.query_starts[it.r + 1] : it.r + 1;
         it.tok0 = (it.tile - it.r * c.each) * c.tok;
-        if (q1 - q0 > c.small) return false;
     } else {
         // request r's tiles begin at query_starts[r] / tok + r: room for each one's last, partly
         // filled tile without a sum over the requests; 64 requests are looked at at a time
@@ -107,13 +126,19 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, const Cut& c, int i
         q0 = a.query_starts[lo];
         q1 = a.query_starts[lo + 1];
         it.tok0 = (it.tile - (q0 / c.tok + lo)) * c.tok;
-        if (q1 - q0 <= c.small || it.tok0 < 0) return false;
     }
+    const int tokens = a.shape.tokens;
+    const bool first_of = CLEAR && it.sub == 0 && split == 0;
+    if (__builtin_expect(first_of && it.tile == 0 && q0 > 0, 0))
+        clear_heads<DT>(a, it, 0, min(q0, tokens));
     const int newest = q1 - q0;
-    it.ntok = min(min(newest, a.shape.max_query) - it.tok0, c.tok);
-    if (it.ntok <= 0) return false;
+    if (ROWS ? newest <= c.small || it.tok0 < 0 : newest > c.small) return false;
     // no rows outside q, whatever query_starts says
-    if (q0 < 0 || q0 + it.tok0 + it.ntok > a.shape.tokens) return false;
+    if (q0 < 0 || q0 >= tokens) return false;
+    if (__builtin_expect(first_of && it.tok0 == 0 && newest > a.shape.max_query, 0))
+        clear_heads<DT>(a, it, q0 + a.shape.max_query, min(q1, tokens));
+    it.ntok = min(min(min(newest, a.shape.max_query), tokens - q0) - it.tok0, c.tok);
+    if (it.ntok <= 0) return false;
     it.q0 = q0;
     it.rows = c.subs > 1 ? min(it.group - it.sub * c.rows, c.rows) : it.ntok * it.group;
     it.len = max(0, min(a.seq_lens[it.r], a.shape.max_seq));
@@ -135,13 +160,13 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, const Cut& c, int i
 }
 
 // The item and part of a workgroup: parts of an item lie apart, so they run at the same time.
-template <bool ROWS>
+template <bool ROWS, int DT>
 __device__ __forceinline__ bool block_item(const AttnArgs& a, const Cut& c, int block, Item& it) {
     const int first = c.whole * c.parts[0];
-    if (block < first) return find_item<ROWS>(a, c, block % c.whole, block / c.whole, it);
+    if (block < first) return find_item<ROWS, DT, true>(a, c, block % c.whole, block / c.whole, it);
     block -= first;
     const int rest = c.items - c.whole;
-    return find_item<ROWS>(a, c, c.whole + block % rest, block / rest, it);
+    return find_item<ROWS, DT, true>(a, c, c.whole + block % rest, block / rest, it);
 }
 
 // Token (within the tile) and query head of a row of an item.
@@ -372,7 +397,7 @@ __device__ __forceinline__ void key_item(const AttnArgs& a, const Cut& c, int bl
     constexpr int NQ = 1, DP = 64 * DC, DM = DP / 16, LD = KeyShared<DC, WAVES>::kLd;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
     Item it;
-    if (!block_item<false>(a, c, block, it)) return;
+    if (!block_item<false, DT>(a, c, block, it)) return;
     const int t0 = it.t0 + wave, t1 = it.t1;
 
     // the first keys and values are on their way before the queries
@@ -626,7 +651,7 @@ __device__ __forceinline__ void row_item(const AttnArgs& a, const Cut& c, int bl
     };
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
     Item it;
-    if (!block_item<true>(a, c, block, it)) return;
+    if (!block_item<true, DT>(a, c, block, it)) return;
     const int t0 = it.t0, t1 = it.t1;
     const Pages pages(a, it);
 
@@ -845,18 +870,12 @@ __device__ __forceinline__ int last_start(const AttnArgs& a) {
     return a.query_starts ? a.query_starts[a.shape.requests] : a.shape.tokens;
 }
 
-// The launch's share of the rows of tokens from `end` on, which belong to no request (a padded
-// batch): zeros, as for rows that see nothing.
+// The launch's share of the rows of tokens from `end` on, which belong to no request (a padded batch).
 template <int DT> __device__ __forceinline__ void no_request(const AttnArgs& a, int end) {
     if (end >= a.shape.tokens) return;
-    const int64_t rows = (int64_t)a.shape.tokens * a.shape.heads;
     const int64_t first = (int64_t)max(end, 0) * a.shape.heads;
-    const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int64_t step = (int64_t)gridDim.x * blockDim.x;
-    for (int64_t i = first * a.shape.d + at; i < rows * a.shape.d; i += step)
-        store_from_f32<DT>(a.out, i, 0.f);
-    if (a.lse)
-        for (int64_t i = first + at; i < rows; i += step) a.lse[i] = -INFINITY;
+    clear<DT>(a, first, (int64_t)a.shape.tokens * a.shape.heads - first,
+              (int64_t)blockIdx.x * blockDim.x + threadIdx.x, (int64_t)gridDim.x * blockDim.x);
 }
 
 // What a launch does: every block of a batch whose requests all have few rows or all have many is
@@ -912,7 +931,7 @@ __device__ __forceinline__ void float_item(const AttnArgs& a, const Cut& c, Floa
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Item it;
-    if (!block_item<ROWS>(a, c, blockIdx.x, it)) return;
+    if (!block_item<ROWS, kF32>(a, c, blockIdx.x, it)) return;
     const float to_log2 = a.scale * kLog2e;
     int hi[NR], lo[NR];
     scalar_floats q[NR];
@@ -1087,7 +1106,7 @@ __device__ __forceinline__ void join_item(const AttnArgs& a, const Cut& c, int i
     constexpr int DP = 64 * DC;
     const int lane = threadIdx.x & 63;
     Item it;
-    if (!find_item<ROWS>(a, c, id, 0, it) || it.parts <= 1) return;
+    if (!find_item<ROWS, DT, false>(a, c, id, 0, it) || it.parts <= 1) return;
     const int64_t stride = (int64_t)(id < c.whole ? c.whole : c.items - c.whole) * c.rows;
     const float nan = __uint_as_float(0x7FC00000u);
     for (int row = first + (threadIdx.x >> 6); row < it.rows; row += step) {

@@ -87,8 +87,10 @@ def attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, sca
     ``query_starts``), its last tokens; ``seq_lens`` counts them too.  ``window``: only so many
     keys up to the token itself (0: all).  ``scale`` defaults to head size ** -0.5.
     ``max_query_len`` and ``max_seq_len`` are the batch's longest, where the caller knows them:
-    they size the launch, and longer ones are cut off.  A row that sees nothing is zero (log-sum
-    -inf), and so are tokens past the last request's (a padded batch).  With ``return_lse`` also the natural log of each row's softmax sum.
+    they size the launch, and longer ones are cut off: of a request's rows the first
+    ``max_query_len`` are computed, over its first ``max_seq_len`` keys.  A row that sees nothing is
+    zero (log-sum -inf), and so are rows beyond ``max_query_len`` and tokens of no request (a padded
+    batch).  With ``return_lse`` also the natural log of each row's softmax sum.
     """
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])

@@ -1,0 +1,90 @@
+"""Attention under bounds, windows and workspaces that do not fit the batch."""
+
+import ctypes
+
+import pytest
+import torch
+
+from ojasx_amd import _native as N
+from test_gpu_kv8 import DEV, DTYPES, _batch, _i32, _make
+
+pytestmark = pytest.mark.gpu
+
+
+def _code(dtype):
+    return N.DTYPE_CODE[dtype]
+
+
+def _workspace_bytes(q, cache, requests, window, max_query, max_seq):
+    n = ctypes.c_size_t(0)
+    t, heads, d = q.shape
+    N.check(N.lib().ojx_kv8_attention_workspace_bytes(
+        t, requests, heads, cache.k_codes.shape[1], d, window, max_query, max_seq, _code(q.dtype),
+        ctypes.byref(n)), "workspace")
+    return n.value
+
+
+def _call(cache, q, tables, lens, starts, max_query, max_seq, scale, window=0, ws=None, ws_bytes=0):
+    """The C entry point on outputs that held NaN."""
+    t, heads, d = q.shape
+    out = torch.full_like(q, float("nan"), memory_format=torch.contiguous_format)
+    lse = torch.full((t, heads), float("nan"), device=DEV)
+    blocks, kv_heads, block, _ = cache.k_codes.shape
+    N.check(N.lib().ojx_kv8_attention(
+        N.ptr(q), q.stride(0), q.stride(1), t, heads, _code(q.dtype), N.ptr(cache.k_codes),
+        N.ptr(cache.v_codes), N.ptr(cache.scales), blocks, kv_heads, block, d, N.ptr(tables),
+        tables.stride(0), tables.shape[1], N.ptr(lens), N.ptr(starts), lens.numel(), max_query,
+        max_seq, scale, window, N.ptr(out), N.ptr(lse), N.ptr(ws), ws_bytes,
+        N.stream_handle(DEV)), "attention")
+    return out, lse
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,group", [(64, 4), (100, 1), (256, 2)])
+@pytest.mark.parametrize("most", [0, 1, 3, 17, 64, 89])
+def test_rows_past_the_longest_query_are_zero(dtype, d, group, most):
+    new = [5, 1, 90, 0, 70, 2]
+    tables, lens, starts, total = _batch([30, 0, 9, 4, 200, 1], new, 16)
+    cache = _make(16, 2, d, total)
+    q = torch.randn(starts[-1], 2 * group, d).to(dtype).to(DEV)
+    full, full_lse = _call(cache, q, _i32(tables), _i32(lens), _i32(starts), 90, max(lens), 0.1)
+    ws_bytes = _workspace_bytes(q, cache, 6, 0, most, max(lens))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=DEV)
+    for space in ((None, 0), (ws, ws_bytes)):
+        out, lse = _call(cache, q, _i32(tables), _i32(lens), _i32(starts), most, max(lens), 0.1, 0,
+                         *space)
+        for a, b in zip(starts, starts[1:]):
+            cut = min(b, a + most)
+            # what is computed agrees with the call of the right bound (to the forms' roundings)
+            torch.testing.assert_close(out[a:cut], full[a:cut], rtol=2e-2, atol=2e-2)
+            torch.testing.assert_close(lse[a:cut], full_lse[a:cut], rtol=1e-3, atol=1e-3)
+            assert not out[cut:b].any() and torch.isneginf(lse[cut:b]).all()
+    assert torch.isfinite(full).all() and not full_lse.isnan().any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [[1, 2, 1], [40, 1, 70]])
+def test_tokens_before_the_first_request_are_zero(dtype, new):
+    tables, lens, starts, total = _batch([30, 0, 9], new, 16)
+    cache = _make(16, 2, 64, total)
+    q = torch.randn(starts[-1] + 7, 4, 64).to(dtype).to(DEV)
+    t, n = _i32(tables), _i32(lens)
+    want, want_lse = _call(cache, q[7:], t, n, _i32(starts), max(new), max(lens), 0.1)
+    out, lse = _call(cache, q, t, n, _i32([s + 7 for s in starts]), max(new), max(lens), 0.1)
+    assert not out[:7].any() and torch.isneginf(lse[:7]).all()
+    assert torch.equal(out[7:], want) and torch.equal(lse[7:], want_lse)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [[1, 2, 1], [40, 1, 70]])
+def test_rows_outside_q_are_left_out(dtype, new):
+    # the last request's rows go on past q: those that q holds are computed
+    tables, lens, starts, total = _batch([30, 0, 9], new, 16)
+    cache = _make(16, 2, 64, total)
+    q = torch.randn(starts[-1] + 5, 4, 64).to(dtype).to(DEV)
+    t, n = _i32(tables), _i32([*lens[:2], lens[2] + 5])
+    s = _i32([*starts[:3], starts[3] + 5])
+    want, want_lse = _call(cache, q, t, n, s, max(new) + 5, max(lens) + 5, 0.1)
+    out, lse = _call(cache, q[:starts[3]], t, n, s, max(new) + 5, max(lens) + 5, 0.1)
+    assert torch.equal(out, want[:starts[3]]) and torch.equal(lse, want_lse[:starts[3]])
+    assert not lse.isnan().any()
