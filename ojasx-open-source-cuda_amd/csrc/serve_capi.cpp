@@ -79,6 +79,10 @@ int check_attention(int64_t tokens, int64_t requests, int64_t heads, int64_t kv_
     return OJX_OK;
 }
 
+// Of windows that no key seen is outside of, the kernels have none.  One longer than max_seq_len is
+// not one: a request may have more tokens than its table's blocks hold.
+int window_of(int64_t window) { return window > kMaxCount ? 0 : (int)window; }
+
 int check_logits(int64_t ld, int64_t rows, int64_t vocab, int64_t top_k, int dtype) {
     if (!valid_dtype(dtype)) return api_failf(OJX_EDTYPE, "unknown dtype code %d", dtype);
     if (rows < 0 || rows > kMaxCount || vocab < 1 || vocab > kMaxCount)
@@ -209,7 +213,7 @@ OJX_API int ojx_kv8_attention_workspace_bytes(int64_t tokens, int64_t requests, 
     s.heads = (int)heads;
     s.kv_heads = (int)kv_heads;
     s.d = (int)head_dim;
-    s.window = window > max_seq_len ? 0 : (int)window;
+    s.window = window_of(window);
     s.max_query = (int)max_query_len;
     s.max_seq = (int)max_seq_len;
     s.dtype = dtype;
@@ -263,7 +267,7 @@ OJX_API int ojx_kv8_attention(const void* q, int64_t q_token_stride, int64_t q_h
     a.shape.heads = (int)heads;
     a.shape.kv_heads = (int)kv_heads;
     a.shape.d = (int)head_dim;
-    a.shape.window = window > max_seq_len ? 0 : (int)window;
+    a.shape.window = window_of(window);
     a.shape.max_query = query_starts ? (int)max_query_len : 1;
     a.shape.max_seq = (int)(max_seq_len < held ? max_seq_len : held);
     a.shape.dtype = dtype;

@@ -2,11 +2,12 @@
 
 import ctypes
 
+import numpy as np
 import pytest
 import torch
 
 from ojasx_amd import _native as N
-from test_gpu_kv8 import DEV, DTYPES, _batch, _i32, _make
+from test_gpu_kv8 import DEV, DTYPES, _batch, _check_attention, _i32, _make
 
 pytestmark = pytest.mark.gpu
 
@@ -88,3 +89,16 @@ def test_rows_outside_q_are_left_out(dtype, new):
     out, lse = _call(cache, q[:starts[3]], t, n, s, max(new) + 5, max(lens) + 5, 0.1)
     assert torch.equal(out, want[:starts[3]]) and torch.equal(lse, want_lse[:starts[3]])
     assert not lse.isnan().any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("window", [33, 64, 65, 70, 100, 150, 2 ** 31 - 1, 2 ** 40])
+def test_windows_longer_than_what_the_table_holds(dtype, window):
+    # requests of more tokens than their four blocks of 16: the window ends where it does
+    tables, _, starts, total = _batch([60, 60, 60], [4, 4, 4], 16)
+    tables = [row[:4] for row in tables]
+    cache = _make(16, 1, 64, total)
+    for new in ([1, 1, 1], [1, 4, 30]):
+        starts = [0, *np.cumsum(new).tolist()]
+        q = torch.randn(starts[-1], 2, 64).to(dtype).to(DEV)
+        _check_attention(cache, q, tables, [64, 100, 120], starts, window=window)
