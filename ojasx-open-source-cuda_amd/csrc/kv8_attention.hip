@@ -1311,13 +1311,19 @@ size_t cut_bytes(const Cut& c, const AttnShape& s) {
     return stored_rows(c) * (row_bytes(s) + sizeof(float2));
 }
 
-// The cut's part of the workspace, which it moves past; no parts where it does not fit.
+// The cut's part of the workspace, which it moves past; as many parts as fit.  (Fewer than the
+// workspace was asked for may be needed and more: a longer max_seq_len than the table's makes longer
+// parts.  One token over 16128 keys under a max_seq_len of 131072, 64 parts of 4 tiles where 63 fit:
+// 16.0 us, 69.9 uncut.)
 void place(Cut& c, const AttnShape& s, char*& ws, size_t& left) {
-    const size_t need = cut_bytes(c, s);
-    if (need > left) {
-        c.parts[0] = c.parts[1] = 1;
-        c.per[0] = c.per[1] = kUncut;
-        return;
+    size_t need = cut_bytes(c, s);
+    while (need > left && items_in_parts(c) > 0) {
+        const int kind = c.parts[0] > c.parts[1] ? 0 : 1;
+        const int64_t tiles = (int64_t)c.per[kind] * c.parts[kind];
+        const int fewer = c.parts[kind] - 1;
+        c.per[kind] = fewer > 1 ? (int)((tiles + fewer - 1) / fewer) : kUncut;
+        c.parts[kind] = fewer;
+        need = cut_bytes(c, s);
     }
     c.part = reinterpret_cast<float*>(ws);
     c.ml = reinterpret_cast<float2*>(ws + stored_rows(c) * row_bytes(s));

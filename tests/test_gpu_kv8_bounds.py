@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+import kv8_plain as P
 from ojasx_amd import _native as N
 from test_gpu_kv8 import DEV, DTYPES, _batch, _check_attention, _i32, _make
 
@@ -102,3 +103,54 @@ def test_windows_longer_than_what_the_table_holds(dtype, window):
         starts = [0, *np.cumsum(new).tolist()]
         q = torch.randn(starts[-1], 2, 64).to(dtype).to(DEV)
         _check_attention(cache, q, tables, [64, 100, 120], starts, window=window)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [[1] * 3, [9, 3, 1], [70, 5, 130]])
+def test_a_smaller_workspace_lowers_the_split(dtype, new):
+    tables, lens, starts, total = _batch([3000, 2500, 17], new, 64)
+    cache = _make(64, 2, 128, total)
+    q = torch.randn(starts[-1], 4, 128).to(dtype).to(DEV)
+    t, n = _i32(tables), _i32(lens)
+    s = None if max(new) == 1 else _i32(starts)
+    need = _workspace_bytes(q, cache, 3, 0, max(new), max(lens))
+    assert need > 0
+    k, v = P.codes_of(cache)
+    sc = cache.scales.cpu().numpy()
+    want = P.attention(q.float().cpu().numpy(), k, v, sc[:, :, 0], sc[:, :, 1], tables, lens,
+                       starts, 0.1, 0, 64)[0]
+    for share in (0.9, 0.5):
+        size = int(need * share) // 16 * 16
+        ws = torch.full((size + 4096,), 0xA5, dtype=torch.uint8, device=DEV)
+        out, lse = _call(cache, q, t, n, s, max(new), max(lens), 0.1, 0, ws, size)
+        assert (ws[:size] != 0xA5).any()     # it is used
+        assert (ws[size:] == 0xA5).all()
+        # 127 scales of 0.02 e^1.5 at most and rounding to bf16 and 16-bit fixed point: under 0.1
+        assert np.abs(out.double().cpu().numpy() - want).max() < 0.1 and not lse.isnan().any()
+
+
+def test_a_longest_sequence_beyond_the_table_does_not_undo_the_split():
+    """One token over 16128 keys.  Bounds longer than the table ask for other splits than the
+    table's; what the workspace of one holds must not leave the other uncut: one workgroup would
+    go through all 252 tiles of a key head, some 60 times the work of a part."""
+    tables, lens, _, total = _batch([16127], [1], 64)
+    cache = _make(64, 1, 128, total)
+    q = torch.randn(1, 4, 128, dtype=torch.bfloat16, device=DEV)
+    t, n = _i32(tables), _i32(lens)
+    times = {}
+    for bound in (16128, 131072):
+        def call():
+            return cache.attention(q, t, n, max_seq_len=bound)
+        call()
+        a, b = torch.cuda.Event(True), torch.cuda.Event(True)
+        best = float("inf")
+        for _ in range(5):
+            a.record()
+            for _ in range(20):
+                call()
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        times[bound] = best
+    # parts of at most twice as many tiles: twice the time would be a lot
+    assert times[131072] < 2 * times[16128], times
