@@ -428,15 +428,28 @@ PyObject* tuple_of(Tensor* ts, int n) {
     return out;
 }
 
-// Small results of one call, side by side in one allocation: the allocator costs 0.7 us a tensor,
-// as much as a seventh of the kernel of a small call.
+// Results of one call, side by side in an allocation: the allocator costs 0.7 us a tensor, as much as
+// a seventh of the kernel of a small call.  A result that is kept keeps its neighbours, so those of
+// over kTogether bytes are in two allocations, each of results of about the same size (with one for
+// each result a plan of some thousand tokens took 9.4 us, 7.2 in one or two).
 class Results {
   public:
+    static constexpr int64_t kTogether = 64 * 1024;
+
     // Bytes of a result of n elements; all begin at multiples of 16.
     static int64_t room(int64_t n, int64_t element) { return (n * element + 15) / 16 * 16; }
 
-    Results(int64_t bytes, const Tensor& like)
-        : all_(at::empty({bytes}, like.options().dtype(at::kByte))) {}
+    Results(int64_t first, int64_t second, const Tensor& like)
+        : options_(like.options().dtype(at::kByte)),
+          second_(first + second > kTogether ? second : 0),
+          all_(at::empty({second_ ? first : first + second}, options_)) {}
+
+    // The second part's results follow.
+    void second() {
+        if (!second_) return;
+        all_ = at::empty({second_}, options_);
+        used_ = 0;
+    }
 
     Tensor next(at::IntArrayRef shape, at::ScalarType type) {
         const int64_t element = (int64_t)c10::elementSize(type);
@@ -450,6 +463,8 @@ class Results {
     }
 
   private:
+    at::TensorOptions options_;
+    int64_t second_;
     Tensor all_;
     int64_t used_ = 0;
 };
@@ -479,12 +494,15 @@ PyObject* kv8_plan(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     RECORD_FUNCTION("ojasx_e8t::kv8_plan", std::vector<c10::IValue>());
     Unlocked unlocked;
     const c10::DeviceGuard on_device(seq.device());
-    Results all(Results::room(tokens, 8) + 2 * Results::room(tokens, 4) + Results::room(r + 1, 4) +
-                    Results::room(r, 4) + Results::room(1, 4),
-                seq);
-    Tensor out[] = {all.next({tokens}, at::kLong), all.next({tokens}, at::kInt),
-                    all.next({tokens}, at::kInt),  all.next({r + 1}, at::kInt),
-                    all.next({r}, at::kInt),       all.next({1}, at::kInt)};
+    Results all(Results::room(tokens, 8) + 2 * Results::room(tokens, 4),
+                Results::room(r + 1, 4) + Results::room(r, 4) + Results::room(1, 4), seq);
+    Tensor out[6];
+    out[0] = all.next({tokens}, at::kLong);
+    for (int i = 1; i < 3; ++i) out[i] = all.next({tokens}, at::kInt);
+    all.second();
+    out[3] = all.next({r + 1}, at::kInt);
+    out[4] = all.next({r}, at::kInt);
+    out[5] = all.next({1}, at::kInt);
     check(ojx_kv8_plan((const int32_t*)data(seq), (const int32_t*)data(fresh), r,
                        (int32_t*)data(tables), tables.stride(0), tables.size(1),
                        (const int32_t*)data(free), free.numel(), (const int32_t*)data(left), block,
@@ -626,13 +644,13 @@ struct Logprobs {
                              two = shape;
         tops.push_back(top);
         two.push_back(2);
-        Results all(3 * Results::room(rows, 4) + Results::room(rows * top, 4) +
-                        Results::room(rows * top, 8) + Results::room(2 * rows, 4),
-                    x);
+        Results all(3 * Results::room(rows, 4) + Results::room(2 * rows, 4),
+                    Results::room(rows * top, 4) + Results::room(rows * top, 8), x);
         for (int i = 0; i < 3; ++i) out[i] = all.next(shape, at::kFloat);
+        out[5] = all.next(two, at::kFloat);
+        all.second();
         out[3] = all.next(tops, at::kFloat);
         out[4] = all.next(tops, at::kLong);
-        out[5] = all.next(two, at::kFloat);
         size_t bytes = 0;
         check(ojx_token_logprobs_workspace_bytes(rows, v, top, dt, &bytes),
               "token_logprobs_workspace_bytes");

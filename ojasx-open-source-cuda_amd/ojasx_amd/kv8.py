@@ -29,7 +29,10 @@ def _eager(name: str, *args):
 
 
 class KV8Plan(NamedTuple):
-    """Where a step's tokens go (``plan``)."""
+    """Where a step's tokens go (``plan``).
+
+    The results may share allocations: one for up to 64 KiB of them, else one for the three of each
+    token and one for the others.  ``clone()`` what is to be resized in place, or kept alone."""
 
     slots: torch.Tensor         # int64 [tokens]: block * block_size + offset, -1 without a block
     positions: torch.Tensor     # int32 [tokens]: place in the request

@@ -11,6 +11,11 @@ from . import serve_ops as S
 
 
 class TokenLogprobs(NamedTuple):
+    """Results of ``token_logprobs``.
+
+    They may share allocations: one for up to 64 KiB of them, else one for those of each row and one
+    for the alternatives.  ``clone()`` what is to be resized in place, or kept alone."""
+
     logprob: torch.Tensor       # float32 [...]: of the given tokens
     entropy: torch.Tensor       # float32 [...]: of the rows' distributions, in nats
     lse: torch.Tensor           # float32 [...]: log of the sum of exp(logits)
