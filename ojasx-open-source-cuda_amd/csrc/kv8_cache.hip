@@ -369,7 +369,7 @@ __device__ __forceinline__ int quotient(int u, uint32_t inverse, int d) {
 }
 
 // Earlier codes of a block and head for its new scale, a few loads of 16 bytes in flight: keys
-// of `off` tokens, or value words of `quads` 4-token groups.
+// of `off` tokens, or values of whole groups of 16 tokens (units have those of the run's first one).
 __device__ __forceinline__ void recode_keys(int8_t* base, int off, int d, int dp, float ratio,
                                             int first, int step) {
     const int chunks = (d + 15) >> 4, total = off * chunks;
@@ -391,33 +391,24 @@ __device__ __forceinline__ void recode_keys(int8_t* base, int off, int d, int dp
     }
 }
 
-__device__ __forceinline__ void recode_values(int8_t* base, int quads, int d, int dp, float ratio,
+__device__ __forceinline__ void recode_values(int8_t* base, int groups, int d, int dp, float ratio,
                                               int first, int step) {
-    const int groups = (quads + 3) >> 2, total = groups * d;
+    const int total = groups * d;
     const uint32_t inv = inverse_of(d);
     for (int i0 = first; i0 < total; i0 += 4 * step) {
-        uint32_t* p[4];
+        uint4* p[4];
         uint4 o[4];
-        int words[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int i = min(i0 + j * step, total - 1), g = quotient(i, inv, d);
-            p[j] = reinterpret_cast<uint32_t*>(base + g * 16 * dp + (i - g * d) * 16);
-            o[j] = *reinterpret_cast<const uint4*>(p[j]);
-            words[j] = i0 + j * step < total ? quads - 4 * g : 0;
+            p[j] = reinterpret_cast<uint4*>(base + g * 16 * dp + (i - g * d) * 16);
+            o[j] = *p[j];
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint4 v = make_uint4(recode4(o[j].x, ratio), recode4(o[j].y, ratio),
-                                       recode4(o[j].z, ratio), recode4(o[j].w, ratio));
-            if (words[j] >= 4) {
-                *reinterpret_cast<uint4*>(p[j]) = v;
-            } else {  // the rest of the group is written elsewhere
-                if (words[j] > 0) p[j][0] = v.x;
-                if (words[j] > 1) p[j][1] = v.y;
-                if (words[j] > 2) p[j][2] = v.z;
-            }
-        }
+        for (int j = 0; j < 4; ++j)
+            if (i0 + j * step < total)
+                *p[j] = make_uint4(recode4(o[j].x, ratio), recode4(o[j].y, ratio),
+                                   recode4(o[j].z, ratio), recode4(o[j].w, ratio));
     }
 }
 
@@ -539,7 +530,7 @@ __device__ __forceinline__ void append_held(const KvCache& c, const KvRows& src,
         }
         return;
     }
-    if (again) recode_values(base, q0, c.d, c.dp, ratio, first, 64 * WAVES);
+    if (again) recode_values(base, q0 >> 2, c.d, c.dp, ratio, first, 64 * WAVES);
 #pragma unroll
     for (int i = 0; i < HOLD; i += 4) {
         const int u = first + (i >> 2) * 64 * WAVES;
