@@ -386,7 +386,8 @@ int ojx_kv8_plan(const int32_t* seq_lens, const int32_t* new_lens, int64_t reque
 /* Writes keys and values of `tokens` new tokens into the cache.  k, v: [tokens][kv_heads]
  * [head_dim] in dtype, with strides (elements) between tokens and between heads.  Tokens of one
  * block are neighbours in `slots` and at rising offsets without a gap, each block in one run of
- * the call; slots outside the cache are skipped.  A block's scale is the largest |element| of the
+ * the call (two runs of a block race for its scale and codes); slots outside the cache are
+ * skipped.  A block's scale is the largest |element| of the
  * run over 127; where the run begins inside the block, its earlier tokens keep their place: the
  * scale is then not less than the old one and, where it grew, the earlier codes are rounded
  * again.  Infinite elements become +-127 times the scale, NaN 0; neither takes part in the
@@ -414,8 +415,10 @@ int ojx_kv8_read(const int8_t* k_codes, const int8_t* v_codes, const float* scal
  * gets zeros and -inf, and so do tokens before query_starts[0] and past query_starts[requests];
  * a row of q with NaN or infinities gets NaN.  max_query_len and max_seq_len size the launch: of a
  * request that has more, the first max_query_len newest tokens are computed (the others get zeros
- * and -inf), over its first max_seq_len keys.  The workspace holds partial results of a split over
- * the keys; a smaller one (or none) only lowers the split. */
+ * and -inf), over its first max_seq_len keys.  Sums are fp32 or 32-bit integers; 16-bit rows of q
+ * enter as 16-bit fixed point of their largest element, their weights as 16-bit fixed point of the
+ * largest of 64 keys or as fp16; exponents (base 2) beyond +-9e29 count as that.  The workspace
+ * holds partial results of a split over the keys; a smaller one (or none) only lowers the split. */
 int ojx_kv8_attention_workspace_bytes(int64_t tokens, int64_t requests, int64_t heads,
                                       int64_t kv_heads, int64_t head_dim, int64_t window,
                                       int64_t max_query_len, int64_t max_seq_len, int dtype,

@@ -382,9 +382,13 @@ struct Pages {
 // of the value products as they come.  The workgroup's waves take turns at 64 keys of a 16-row tile
 // and join their results in LDS.  (Two tiles of rows for one pass over the keys would need more
 // than half of a SIMD's registers: two workgroups that share the keys in L2 are faster.)
-// Memory bounds it where there are many keys (64 tokens over 500 to 16000 tokens, 631 MB: 124 us
-// and 5 for the join, 4.9 TB/s), launches and latency where there are few (one over 2048 tokens:
-// 6.1 us and 3.5 for the join).
+// The roundings are a choice: 2^-16 of the largest element for q (a bf16 element has 2^-9 of itself;
+// an fp16 one, 2^-11, loses bits of its own from 1/32 of the largest on), 2^-16 of the largest of 64
+// for weights, beside values that are held in 8 bits; all sums are 32-bit.
+// Memory bounds it where there are many keys (64 tokens over 500 to 16000 tokens, 631 MB: 123 us
+// and 5 for the join, 4.9 TB/s; heads off the grid of 64 read their padding too: 132 us for heads of
+// 80, whose own bytes are 409 of 654 MB), launches and latency where there are few (one over 2048
+// tokens: 6.6 us and 3 for the join).
 template <int DC, int WAVES> struct KeyShared {
     static constexpr int kLd = 64 * DC + 4;
     float joined[WAVES * 16 * kLd];
@@ -622,9 +626,11 @@ __device__ __forceinline__ void halves_of(uint32_t codes, uint32_t& a, uint32_t&
 // for the workgroup on their way into LDS: the products then add up in fp32 in the matrix unit,
 // where whole-number products would cost three vector instructions for every result of every 64
 // keys.  The reference of the weights is raised only when one would pass 2^kHeadroom times it, so
-// the sums are scaled again rarely.  Four chunks of 900 to 2048 tokens over up to 8000 (321 GF):
-// 400 us and 10 for the join, 780 Tflop/s of the two products; the matrix unit is busy for a third
-// of the time, q's second byte included, vector instructions for most of the rest: 12 for a score.
+// the sums are scaled again rarely.  A weight's rounding to fp16 is 2^-11 of it, under 2^-14 of
+// the reference 2^-25 of that; the sum takes it unrounded.  Four chunks of 900 to 2048 tokens over
+// up to 8000 (321 GF): 423 us a call with 11 for the join, 760 Tflop/s of the two products; the
+// matrix unit is busy for a third of the time, q's second byte included, vector instructions for
+// most of the rest: 12 for a score.  The two hardly overlap.
 constexpr float kHeadroom = 8.f;
 // References up to which the weights' exponents are x * f + (lv - ref): that difference's rounding
 // is under 2^-12 then.  Beyond, they are formed from differences of scores, in the step that also
@@ -911,8 +917,8 @@ void attend_kernel(AttnArgs a, Cut key, Cut row, int row_blocks) {
 // units.  A workgroup has up to four rows of a key head, so a converted code serves all of them;
 // its waves take every fourth 64-key tile and are joined at the end.  For the scores a lane has a
 // key and q comes from scalar registers; for the values it has up to four d, and the weights pass
-// through LDS.  Vector products bound it: 4 x 512 tokens over 2048 (60 GF) 1230 us, 49 Tflop/s; 64
-// tokens over 9000 325 us; one over 32768 42 us.
+// through LDS.  Vector products bound it: 4 x 512 tokens over 2048 (60 GF) 1191 us, 50 Tflop/s; 64
+// tokens over 9000 315 us (3.7 TB/s); one over 32768 42 us.
 constexpr int kFloatRows = kWaves;  // at the end a wave has a row
 constexpr float kLargest = 3e38f;
 
@@ -1258,8 +1264,9 @@ bool plan_of(const AttnShape& s, Plan& p) {
         // Workgroups at a time: two on each CU, one where a head needs more of its LDS.
         const int64_t slots = s.d <= 192 ? 512 : 256;
         // Tiles of 128 rows read and convert the keys for more rows (four chunks of up to 2048
-        // tokens: 411 us, 535 at 64 rows); those of 64 are through theirs sooner, so they are for
-        // batches of few tiles a slot (7 requests of 62 to 550 tokens: 14.8 us, 30.2 at 128).
+        // tokens: 411 us, 535 at 64 rows, both on inputs used before); those of 64 are through theirs
+        // sooner, so they are for batches of few tiles a slot (7 requests of 62 to 550 tokens: 14.8
+        // us, 30.2 at 128).
         // Around 16 tiles a slot both come out alike.
         int64_t tiles = 0;
         for (int rows = s.d > 192 || (s.d <= 128 && most > 64) ? 128 : 64;; rows = 64) {

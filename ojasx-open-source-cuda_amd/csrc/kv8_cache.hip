@@ -679,8 +679,9 @@ template <int DT> __device__ __forceinline__ void store8(void* p, int64_t i, con
 
 // One block's keys or values per blockIdx.x, a share of its units per blockIdx.y.  The output's
 // order (token, head, d) is the units': 8 d of a token's key, or of 4 tokens' values, whose
-// codes are 8 words of 4 tokens.  WIDE: d a multiple of 8, else a unit is a single element.  Memory
-// bounds it: 23 us for the blocks of 21500 tokens of 8 x 80 fp16 (83 MB read and written, 3.6 TB/s).
+// codes are 8 words of 4 tokens.  WIDE: d a multiple of 8, else a unit is a single element.  23 us
+// for the blocks of 21500 tokens of 8 x 80 fp16 (83 MB read and written, 3.6 TB/s, three quarters of
+// a copy's rate): memory, and two divisions and a scale's load ahead of every unit's.
 template <int DT, bool WIDE>
 __global__ __launch_bounds__(kReadThreads) void read_kernel(KvCache c,
                                                             const int32_t* __restrict__ blocks,

@@ -54,7 +54,7 @@ template <class T, class F> __device__ T block_reduce(T v, T* shared, F f) {
 
 // A row with NaN or infinities, or whose largest logit is beyond +-kPlainMax (all of it masked
 // by a large negative value, say): one workgroup, one pass for the maximum, one for the sums,
-// one per alternative.
+// one per alternative (77 such rows of 50021 fp32 with 20: 683 us, 17 for ordinary ones).
 template <int DT>
 __device__ __forceinline__ void odd_row(const LogprobArgs& a, int row, float* sf, uint64_t* sk) {
     const int v = a.vocab;
@@ -456,8 +456,9 @@ struct Parts {
 
 // A workgroup reads a row, or with splits > 1 a part of it, once: every wave keeps its sums and
 // its best k.  Without alternatives memory bounds it (2048 rows of 128256 bf16, 525 MB: 125 us,
-// 4.2 TB/s), with them vector instructions (4096 rows of 32000 fp16 with 5: 72 us, 3.6 TB/s: a
-// conversion, a maximum, an exponential, two sums and a compare for every logit).
+// 4.2 TB/s), with them vector instructions (4096 rows of 32000 fp16 with 5: 72 us, 3.6 TB/s: 17 for
+// every logit, of which the conversion, maximum, exponential and sums are 8; the others convert it
+// again and look for candidates in every batch that has one).
 template <int DT, bool TOP>
 __global__ __launch_bounds__(kThreads) void pass_kernel(LogprobArgs a, Parts p) {
     __shared__ Sums sums[kGroups];

@@ -63,6 +63,11 @@ def append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_codes: torch
 
     A block's scale covers the largest element it was given; where a later token raises it, the
     codes that are there already are rounded again.  Slots outside the cache (-1) are skipped.
+
+    In one call the tokens of a block have to be neighbours in ``slots``, at rising offsets without
+    a gap, as ``plan`` gives them: one run for each block.  Two runs of a block (slots 5, -1, 6 of
+    one; a slot given twice) are written by different waves at once, and which scale and codes stay
+    is undefined.  Append them in two calls.
     """
     args = (k, v, slots, k_codes, v_codes, scales)
     if _eager("kv8_append", *args) is None:
@@ -94,6 +99,11 @@ def attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, sca
     ``max_query_len`` are computed, over its first ``max_seq_len`` keys.  A row that sees nothing is
     zero (log-sum -inf), and so are rows beyond ``max_query_len`` and tokens of no request (a padded
     batch).  With ``return_lse`` also the natural log of each row's softmax sum.
+
+    Sums are in 32 bits.  float32 queries keep their 24 bits throughout; 16-bit ones enter the
+    products as 16-bit fixed point of their row's largest element (rounded by 2^-16 of it at most).
+    Their weights are rounded to 16 bits of the largest of 64 keys for few rows of a request, to
+    fp16 for many (2^-11 each, denormal under 2^-14 of the row's reference).
     """
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
@@ -123,6 +133,7 @@ class KV8Cache:
         self.scales = torch.zeros((num_blocks, kv_heads, 2), dtype=torch.float32, device=device)
 
     def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+        """``kv8.append`` into this storage: the tokens of a block in one run of ``slots``."""
         append(k, v, slots, self.k_codes, self.v_codes, self.scales)
 
     def read(self, blocks: torch.Tensor, dtype: torch.dtype = torch.bfloat16

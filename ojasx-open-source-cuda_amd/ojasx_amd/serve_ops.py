@@ -1,10 +1,10 @@
 """``torch.library`` custom ops (namespace ``ojasx_e8t``) of the operators around the packed
 linears: the 8-bit paged key / value cache, its attention, token log probabilities.
 
-``kv8_plan``, ``kv8_append`` and ``kv8_read`` move a step's tokens into the cache and blocks out
-of it, ``kv8_attention`` reads it, ``token_logprobs`` (autograd registered, with
-``token_logprobs_bwd``) is what a model answers and trains with.  The reference keeps no
-quantized cache; the layouts and rules are those of ``include/ojasx_e8t.h``.  As for the other
+``kv8_plan``, ``kv8_append`` (a block's tokens in one run of its slots) and ``kv8_read`` move a
+step's tokens into the cache and blocks out of it, ``kv8_attention`` reads it,
+``token_logprobs`` (autograd registered, with ``token_logprobs_bwd``) is what a model answers and
+trains with.  The reference keeps no quantized cache; the layouts and rules are those of ``include/ojasx_e8t.h``.  As for the other
 ops: the current HIP stream of the device, outputs and workspaces from torch's caching
 allocator, ``RuntimeError`` for what does not fit, no fallback.
 """
