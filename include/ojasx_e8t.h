@@ -457,6 +457,41 @@ int ojx_token_logprobs_bwd(const void* logits, int64_t ld, int64_t rows, int64_t
                            const float* grad_entropy, const float* grad_lse,
                            const float* grad_top, void* grad_logits, void* stream);
 
+/* ---- positions rotated into queries and keys ----
+ *
+ * The first 2 * pairs elements of a head are pairs, (i, i + pairs) or, interleaved, (2i, 2i + 1).
+ * Pair i at position p turns by p * rates[i] / 2^64 of a whole turn (the product wraps: exact for
+ * every whole position, negative ones too), and is multiplied by gain:
+ *   y_lo = gain (x_lo cos a - x_hi sin a),  y_hi = gain (x_hi cos a + x_lo sin a);
+ * the head's other elements are copied.  Products in fp32, each output rounded once.  `inverse`
+ * turns by -a (times gain again): the gradient. */
+typedef struct ojx_rotation {
+    const int64_t* rates;   /* [pairs] device */
+    int64_t pairs;          /* 1 .. head_dim / 2 */
+    const void* positions;  /* int32, or int64 when positions64 */
+    int32_t positions64;
+    int32_t interleaved;
+    float gain;
+    int32_t inverse;
+} ojx_rotation;
+
+/* [batches][tokens][heads][head_dim] in x and y, strides in elements (not negative), head_dim
+ * contiguous; y overlaps no input. */
+typedef struct ojx_rotary_rows {
+    const void* x;
+    void* y;
+    int64_t x_batch, x_token, x_head;
+    int64_t y_batch, y_token, y_head;
+    int64_t heads;
+} ojx_rotary_rows;
+
+/* Rotates q and, unless NULL, k (of as many batches and tokens) in one launch.  The position of
+ * token t of batch b is at b * position_batch_stride + t * position_token_stride.  The structs are
+ * read before the call returns. */
+int ojx_rotary(const ojx_rotary_rows* q, const ojx_rotary_rows* k, int64_t batches, int64_t tokens,
+               int64_t head_dim, int dtype, const ojx_rotation* rotation,
+               int64_t position_batch_stride, int64_t position_token_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -34,6 +34,7 @@ SOURCES = [
     "kv8_cache.hip",
     "kv8_attention.hip",
     "token_logprobs.hip",
+    "rotary.hip",
     "e8t_capi.cpp",
     "serve_capi.cpp",
 ]

@@ -8,7 +8,8 @@
 // nothing, for every call that is not plain eager work on tensors it knows: the caller then
 // takes the registered op, which handles (or refuses) it as before.  Plain means: exact
 // Tensor or Parameter objects on one ROCm device; no autograd to record (grad mode off, or
-// nothing requires grad; token_logprobs_recorded brings a node of its own); no tangents; and no
+// nothing requires grad; token_logprobs_recorded and rotary_recorded bring nodes of their own); no
+// tangents; and no
 // dispatch or function mode, functorch transform or tracer active.
 //
 // Measured, us per call among others: one bf16 token through a 4096 x 4096 layer 26.2 -> 6.2
@@ -773,6 +774,173 @@ PyObject* token_logprobs_recorded(PyObject*, PyObject* const* argv, Py_ssize_t n
     END_HANDLE_TH_ERRORS
 }
 
+// Heads [tokens, heads, d] or [batch, tokens, heads, d] as the kernels take them, of q's sizes.
+bool heads_ok(const Tensor& x, const Tensor& q) {
+    const int64_t n = q.dim();
+    return x.dim() == n && x.scalar_type() == q.scalar_type() && x.device() == q.device() &&
+           x.size(0) == q.size(0) && (n == 3 || x.size(1) == q.size(1)) &&
+           x.size(n - 1) == q.size(n - 1) && x.stride(n - 1) == 1;
+}
+
+bool rotation_ok(const Tensor& positions, const Tensor& rates, const Tensor& q) {
+    const int64_t n = q.dim(), tokens = q.size(n - 3);
+    return (positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong) &&
+           positions.device() == q.device() && rates.device() == q.device() &&
+           ((positions.dim() == 1 && positions.size(0) == tokens) ||
+            (positions.dim() == 2 && n == 4 && positions.size(0) == q.size(0) &&
+             positions.size(1) == tokens)) &&
+           rates.scalar_type() == at::kLong && rates.dim() == 1 && rates.is_contiguous() &&
+           rates.numel() >= 1 && 2 * rates.numel() <= q.size(n - 1);
+}
+
+ojx_rotation rotation_of(const Tensor& positions, const Tensor& rates, double gain, bool interleaved,
+                         bool inverse) {
+    ojx_rotation r;
+    r.rates = (const int64_t*)data(rates);
+    r.pairs = rates.numel();
+    r.positions = data(positions);
+    r.positions64 = positions.scalar_type() == at::kLong;
+    r.interleaved = interleaved;
+    r.gain = (float)gain;
+    r.inverse = inverse;
+    return r;
+}
+
+// q and k (undefined: none) rotated; what heads_ok and rotation_ok took.
+void rotate_into(const Tensor& q, const Tensor& k, const Tensor& positions, const ojx_rotation& r,
+                 Tensor* out) {
+    const c10::DeviceGuard on_device(q.device());
+    const int64_t n = q.dim();
+    ojx_rotary_rows rows[2];
+    for (int i = 0; i < 2; ++i) {
+        const Tensor& x = i ? k : q;
+        if (!x.defined()) continue;
+        const Tensor y = out[i] = at::empty_like(x);
+        rows[i] = {data(x), data(y), n == 4 ? x.stride(0) : 0, x.stride(n - 3), x.stride(n - 2),
+                   n == 4 ? y.stride(0) : 0, y.stride(n - 3), y.stride(n - 2), x.size(n - 2)};
+    }
+    check(ojx_rotary(&rows[0], k.defined() ? &rows[1] : nullptr, n == 4 ? q.size(0) : 1, q.size(n - 3),
+                     q.size(n - 1), dtype_code(q.scalar_type()), &r,
+                     positions.dim() == 2 ? positions.stride(0) : 0,
+                     positions.stride(positions.dim() - 1), current_stream(q.device())),
+          "rotary");
+}
+
+// The registered op's autograd formula as a node of the C++ engine (see RecordedLogprobs).
+struct RecordedRotary : torch::autograd::Function<RecordedRotary> {
+    using Context = torch::autograd::AutogradContext;
+    using List = torch::autograd::variable_list;
+
+    static List forward(Context* ctx, const Tensor& q, const std::optional<Tensor>& keys,
+                        const Tensor& positions, const Tensor& rates, double gain, bool interleaved, bool inverse) {
+        ctx->save_for_backward({positions, rates});
+        ctx->saved_data["gain"] = gain;
+        ctx->saved_data["interleaved"] = interleaved;
+        ctx->saved_data["inverse"] = inverse;
+        ctx->set_materialize_grads(false);
+        const Tensor k = keys ? *keys : Tensor();
+        Tensor out[2];
+        rotate_into(q, k, positions, rotation_of(positions, rates, gain, interleaved, inverse), out);
+        if (!k.defined()) return {out[0]};
+        return {out[0], out[1]};
+    }
+
+    static List backward(Context* ctx, List grads) {
+        const List saved = ctx->get_saved_variables();
+        const Tensor &positions = saved[0], &rates = saved[1];
+        const double gain = ctx->saved_data["gain"].toDouble();
+        const bool interleaved = ctx->saved_data["interleaved"].toBool();
+        const bool inverse = !ctx->saved_data["inverse"].toBool();
+        // those that came, in order: queries, keys
+        Tensor g[2];
+        int n = 0, from[2] = {0, 0};
+        for (int i = 0; i < (int)grads.size() && i < 2; ++i)
+            if (grads[i].defined()) {
+                from[n] = i;
+                g[n++] = grads[i];
+            }
+        List result(7);
+        if (n == 0) return result;
+        bool known = plain_state() && plain(positions) && plain(rates), again = false;
+        for (int i = 0; i < n; ++i) {
+            known &= plain(g[i]);
+            again |= g[i].requires_grad();
+        }
+        Tensor out[2];
+        if (known && !(again && c10::GradMode::is_enabled())) {
+            const at::AutoGradMode off(false);
+            for (int i = 0; i < n; ++i)
+                if (g[i].stride(-1) != 1) g[i] = g[i].contiguous();
+            known = rotation_ok(positions, rates, g[0]) && (n == 1 || heads_ok(g[1], g[0]));
+            if (known) {
+                RECORD_FUNCTION("ojasx_e8t::rotary", std::vector<c10::IValue>());
+                rotate_into(g[0], g[1], positions,
+                            rotation_of(positions, rates, gain, interleaved, inverse), out);
+            }
+        } else {
+            known = false;
+        }
+        if (!known) {  // the registered op, which records a gradient of this one where asked
+            static const auto op =
+                c10::Dispatcher::singleton().findSchemaOrThrow("ojasx_e8t::rotary", "");
+            std::vector<c10::IValue> stack{g[0], n > 1 ? c10::IValue(g[1]) : c10::IValue(), positions,
+                                           rates, gain, interleaved, inverse};
+            op.callBoxed(stack);
+            for (int i = 0; i < n; ++i) out[i] = stack[i].toTensor();
+        }
+        for (int i = 0; i < n; ++i) result[from[i]] = out[i];
+        return result;
+    }
+};
+
+// Whether rotary(q, k | None, positions, rates, gain, interleaved, inverse) is a call on tensors as
+// the kernels take them
+bool rotary_ok(PyObject* const* argv, const Args& a) {
+    if (!plain_state() || !plain(argv[0]) || (argv[1] != Py_None && !plain(argv[1])) ||
+        !plain(argv[2]) || !plain(argv[3]))
+        return false;
+    const Tensor& q = a.t(0);
+    return dtype_code(q.scalar_type()) >= 0 && (q.dim() == 3 || q.dim() == 4) && heads_ok(q, q) &&
+           rotation_ok(a.t(2), a.t(3), q) && (argv[1] == Py_None || heads_ok(a.t(1), q));
+}
+
+// rotary(...): (q, k | None)
+PyObject* rotary(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 7, "rotary");
+    const Args a{argv, n};
+    if (!rotary_ok(argv, a)) Py_RETURN_NONE;
+    const Tensor q = a.t(0), k = argv[1] == Py_None ? Tensor() : a.t(1);
+    if (c10::GradMode::is_enabled() && (records(q) || records(k))) Py_RETURN_NONE;
+    const ojx_rotation r = rotation_of(a.t(2), a.t(3), a.f64(4), a.flag(5), a.flag(6));
+    RECORD_FUNCTION("ojasx_e8t::rotary", std::vector<c10::IValue>());
+    Unlocked unlocked;
+    Tensor out[2];
+    rotate_into(q, k, a.t(2), r, out);
+    unlocked.lock();
+    return tuple_of(out, 2);
+    END_HANDLE_TH_ERRORS
+}
+
+// rotary_recorded(...): the same for autograd
+PyObject* rotary_recorded(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 7, "rotary_recorded");
+    const Args a{argv, n};
+    if (!rotary_ok(argv, a)) Py_RETURN_NONE;
+    const Tensor q = a.t(0), k = argv[1] == Py_None ? Tensor() : a.t(1);
+    const double gain = a.f64(4);
+    const bool interleaved = a.flag(5), inverse = a.flag(6);
+    RECORD_FUNCTION("ojasx_e8t::rotary", std::vector<c10::IValue>());
+    Unlocked unlocked;
+    const std::optional<Tensor> keys = k.defined() ? std::optional<Tensor>(k) : std::nullopt;
+    auto got = RecordedRotary::apply(q, keys, a.t(2), a.t(3), gain, interleaved, inverse);
+    unlocked.lock();
+    Tensor out[2] = {got[0], k.defined() ? got[1] : Tensor()};
+    return tuple_of(out, 2);
+    END_HANDLE_TH_ERRORS
+}
+
 // plain(tensor, ...): whether a Function over these tensors is plain eager work (grad aside)
 PyObject* is_plain(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -797,6 +965,8 @@ PyMethodDef kMethods[] = {
     {"token_logprobs", (PyCFunction)(void*)token_logprobs, METH_FASTCALL, nullptr},
     {"token_logprobs_recorded", (PyCFunction)(void*)token_logprobs_recorded, METH_FASTCALL,
      nullptr},
+    {"rotary", (PyCFunction)(void*)rotary, METH_FASTCALL, nullptr},
+    {"rotary_recorded", (PyCFunction)(void*)rotary_recorded, METH_FASTCALL, nullptr},
     {"is_plain", (PyCFunction)(void*)is_plain, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -1,5 +1,6 @@
 // serve.h -- arguments and launchers of the 8-bit paged cache (kv8_cache.hip), its attention
-// (kv8_attention.hip) and token log probabilities (token_logprobs.hip).
+// (kv8_attention.hip), token log probabilities (token_logprobs.hip) and rotated positions
+// (rotary.hip).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -7,6 +8,7 @@
 #include <stdint.h>
 
 #include "e8t_device.h"
+#include "rotary.h"
 
 namespace ojx {
 
@@ -175,6 +177,30 @@ struct LogprobGradArgs {
     void* gx;
 };
 
+// [batch][token][head][d] elements, d contiguous, and where they go rotated.
+struct RotaryRows {
+    const void* x;
+    void* y;
+    int64_t x_batch, x_token, x_head;
+    int64_t y_batch, y_token, y_head;
+    int heads;
+};
+
+struct RotaryArgs {
+    RotaryRows q;
+    RotaryRows k;  // no heads: none
+    Rotation rot;
+    int64_t position_batch;
+    int64_t position_token;
+    int batches;
+    int tokens;  // of a batch
+    int d;
+    // of launch_rotary: chunks of a head, heads of a thread and the groups of such
+    int chunks;
+    int per;
+    int groups;
+};
+
 hipError_t launch_kv8_plan(const PlanArgs& a, hipStream_t stream);
 hipError_t launch_kv8_append(const KvCache& c, const KvRows& k, const KvRows& v, int dtype,
                              const int64_t* slots, int tokens, hipStream_t stream);
@@ -186,5 +212,7 @@ size_t token_logprobs_bytes(int rows, int vocab, int top, int dtype);
 hipError_t launch_token_logprobs(const LogprobArgs& a, void* ws, size_t ws_bytes,
                                  hipStream_t stream);
 hipError_t launch_token_logprobs_bwd(const LogprobGradArgs& a, hipStream_t stream);
+
+hipError_t launch_rotary(RotaryArgs a, int dtype, hipStream_t stream);
 
 }  // namespace ojx

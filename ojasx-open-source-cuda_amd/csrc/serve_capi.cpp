@@ -1,5 +1,5 @@
 // serve_capi.cpp -- extern "C" entry points of the operators around the packed linears: the
-// 8-bit paged cache, its attention and token log probabilities (declared in
+// 8-bit paged cache, its attention, token log probabilities and rotated positions (declared in
 // include/ojasx_e8t.h).  Checks arguments, then enqueues on the caller's stream; allocates
 // nothing.
 
@@ -101,6 +101,52 @@ int check_workspace(const void* ws, size_t bytes) {
         return api_failf(OJX_EINVAL, "workspace_bytes %zu with a null workspace", bytes);
     if (misaligned(ws, 16)) return api_failf(OJX_ELAYOUT, "workspace must be 16-byte aligned");
     return OJX_OK;
+}
+
+// Heads and their size: what 32-bit indexes within one token rely on.
+constexpr int64_t kMaxHeadDim = 4096;
+
+int check_rotation(const ojx_rotation* r, int64_t head_dim, bool tokens) {
+    if (!r) return api_failf(OJX_EINVAL, "null rotation");
+    if (r->pairs < 1 || 2 * r->pairs > head_dim)
+        return api_failf(OJX_ELAYOUT, "%lld rotated pairs in heads of %lld", (long long)r->pairs,
+                        (long long)head_dim);
+    if (!std::isfinite(r->gain)) return api_failf(OJX_EINVAL, "gain is not finite");
+    if (tokens && (!r->rates || !r->positions)) return api_failf(OJX_EINVAL, "null pointer");
+    if (misaligned(r->rates, 8) || misaligned(r->positions, r->positions64 ? 8 : 4))
+        return api_failf(OJX_ELAYOUT, "misaligned rates or positions");
+    return OJX_OK;
+}
+
+ojx::Rotation rotation_of(const ojx_rotation& r) {
+    ojx::Rotation o;
+    o.rates = reinterpret_cast<const uint64_t*>(r.rates);
+    o.positions = r.positions;
+    o.wide = r.positions64 != 0;
+    o.pairs = (int)r.pairs;
+    o.interleaved = r.interleaved != 0;
+    o.cos_gain = r.gain;
+    o.sin_gain = r.inverse ? -r.gain : r.gain;
+    return o;
+}
+
+int check_rows(const ojx_rotary_rows& r, int64_t tokens, int dtype) {
+    if (r.heads < 0 || r.heads > ojx::kKvMaxHeads)
+        return api_failf(OJX_EINVAL, "%lld heads, expected 0..%d", (long long)r.heads,
+                        (int)ojx::kKvMaxHeads);
+    if (r.x_batch < 0 || r.x_token < 0 || r.x_head < 0 || r.y_batch < 0 || r.y_token < 0 ||
+        r.y_head < 0)
+        return api_failf(OJX_EINVAL, "negative stride");
+    if (tokens > 0 && r.heads > 0 && (!r.x || !r.y)) return api_failf(OJX_EINVAL, "null pointer");
+    const uintptr_t unit = dtype == OJX_F32 ? 4 : 2;
+    if (misaligned(r.x, unit) || misaligned(r.y, unit))
+        return api_failf(OJX_ELAYOUT, "misaligned heads");
+    return OJX_OK;
+}
+
+ojx::RotaryRows rows_of(const ojx_rotary_rows& r) {
+    return ojx::RotaryRows{r.x, r.y, r.x_batch, r.x_token, r.x_head, r.y_batch, r.y_token, r.y_head,
+                           (int)r.heads};
 }
 
 }  // namespace
@@ -345,6 +391,37 @@ OJX_API int ojx_token_logprobs_bwd(const void* logits, int64_t ld, int64_t rows,
     a.gx = grad_logits;
     return ojx::api_done(ojx::launch_token_logprobs_bwd(a, (hipStream_t)stream),
                          "token_logprobs_bwd launch");
+}
+
+OJX_API int ojx_rotary(const ojx_rotary_rows* q, const ojx_rotary_rows* k, int64_t batches,
+                       int64_t tokens, int64_t head_dim, int dtype, const ojx_rotation* rotation,
+                       int64_t position_batch_stride, int64_t position_token_stride, void* stream) {
+    if (!valid_dtype(dtype)) return api_failf(OJX_EDTYPE, "unknown dtype code %d", dtype);
+    if (batches < 0 || tokens < 0 || batches > kMaxCount || tokens > kMaxCount ||
+        (tokens > 0 && batches > kMaxCount / tokens))
+        return api_failf(OJX_EINVAL, "%lld batches of %lld tokens", (long long)batches,
+                        (long long)tokens);
+    if (head_dim < 1 || head_dim > kMaxHeadDim)
+        return api_failf(OJX_ELAYOUT, "head_dim %lld is outside 1..%d", (long long)head_dim,
+                        (int)kMaxHeadDim);
+    const int64_t count = batches * tokens;
+    if (int r = check_rotation(rotation, head_dim, count > 0)) return r;
+    if (!q) return api_failf(OJX_EINVAL, "null q");
+    if (int r = check_rows(*q, count, dtype)) return r;
+    if (k)
+        if (int r = check_rows(*k, count, dtype)) return r;
+    if (count == 0) return OJX_OK;
+    if (int r = ojx::api_check_device()) return r;
+    ojx::RotaryArgs a{};
+    a.q = rows_of(*q);
+    if (k) a.k = rows_of(*k);
+    a.rot = rotation_of(*rotation);
+    a.position_batch = position_batch_stride;
+    a.position_token = position_token_stride;
+    a.batches = (int)batches;
+    a.tokens = (int)tokens;
+    a.d = (int)head_dim;
+    return ojx::api_done(ojx::launch_rotary(a, dtype, (hipStream_t)stream), "rotary launch");
 }
 
 }  // extern "C"

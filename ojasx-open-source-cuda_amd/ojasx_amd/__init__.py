@@ -7,7 +7,7 @@ operation runs in hand-written HIP kernels for gfx950 (libojasx_e8t.so, C ABI in
 include/ojasx_e8t.h) registered as ``torch.ops.ojasx_e8t.*``.
 """
 
-from . import grouped, hardware, kv8, ops, optim_state, serve_ops
+from . import grouped, hardware, kv8, ops, optim_state, rotary, serve_ops
 from .lattice import (
     E8LatticeLinear,
     E8QuantizationAwareLinear,
@@ -37,6 +37,7 @@ __all__ = [
     "kv8",
     "ops",
     "optim_state",
+    "rotary",
     "serve_ops",
     "KV8Cache",
     "TokenLogprobs",

@@ -62,6 +62,7 @@ EXPORTS = (
     "ojx_token_logprobs_workspace_bytes",
     "ojx_token_logprobs",
     "ojx_token_logprobs_bwd",
+    "ojx_rotary",
 )
 
 
@@ -87,6 +88,37 @@ class GemvJob(ctypes.Structure):
         ("lora_scaling", ctypes.c_float),
         ("reserved", ctypes.c_int32),
     ]
+
+
+class Rotation(ctypes.Structure):
+    """ojx_rotation of include/ojasx_e8t.h."""
+
+    _fields_ = [
+        ("rates", ctypes.c_void_p),
+        ("pairs", ctypes.c_int64),
+        ("positions", ctypes.c_void_p),
+        ("positions64", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("gain", ctypes.c_float),
+        ("inverse", ctypes.c_int32),
+    ]
+
+
+class RotaryRows(ctypes.Structure):
+    """ojx_rotary_rows of include/ojasx_e8t.h."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("y", ctypes.c_void_p),
+        ("x_batch", ctypes.c_int64),
+        ("x_token", ctypes.c_int64),
+        ("x_head", ctypes.c_int64),
+        ("y_batch", ctypes.c_int64),
+        ("y_token", ctypes.c_int64),
+        ("y_head", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+    ]
+
 
 _lib = None
 _lock = threading.Lock()
@@ -198,7 +230,8 @@ def lib() -> ctypes.CDLL:
                     ("ojx_token_logprobs", [_P, _I64, _I64, _I64, _INT, _P, _I64, _P, _P, _P, _P,
                                             _P, _P, _P, _SZ, _P]),
                     ("ojx_token_logprobs_bwd", [_P, _I64, _I64, _I64, _INT, _P, _P, _P, _I64]
-                     + [_P] * 7)):
+                     + [_P] * 7),
+                    ("ojx_rotary", [_P, _P, _I64, _I64, _I64, _INT, _P, _I64, _I64, _P])):
                 fn = getattr(L, name)
                 fn.restype = _INT
                 fn.argtypes = args

@@ -1,10 +1,10 @@
 """``torch.library`` custom ops (namespace ``ojasx_e8t``) of the operators around the packed
-linears: the 8-bit paged key / value cache, its attention, token log probabilities.
+linears: the 8-bit paged key / value cache, its attention, token log probabilities, rotated positions.
 
 ``kv8_plan``, ``kv8_append`` (a block's tokens in one run of its slots) and ``kv8_read`` move a
 step's tokens into the cache and blocks out of it, ``kv8_attention`` reads it,
 ``token_logprobs`` (autograd registered, with ``token_logprobs_bwd``) is what a model answers and
-trains with.  The reference keeps no quantized cache; the layouts and rules are those of ``include/ojasx_e8t.h``.  As for the other
+trains with; ``rotary`` (its own gradient, turned back) rotates queries and keys.  The reference keeps no quantized cache; the layouts and rules are those of ``include/ojasx_e8t.h``.  As for the other
 ops: the current HIP stream of the device, outputs and workspaces from torch's caching
 allocator, ``RuntimeError`` for what does not fit, no fallback.
 """
@@ -331,3 +331,102 @@ def _logprobs_backward(ctx, g_lp, g_h, g_lse, g_top, *_):
 
 
 token_logprobs.register_autograd(_logprobs_backward, setup_context=_logprobs_setup)
+
+
+# ----------------------------------------------------------------------------- rotated positions
+
+def _rotary_sizes(x: torch.Tensor) -> Tuple[int, int]:
+    """(batches, tokens) of [tokens, heads, d] or [batch, tokens, heads, d]."""
+    return (1, x.shape[0]) if x.dim() == 3 else (x.shape[0], x.shape[1])
+
+
+def _rotary_input(x: torch.Tensor) -> torch.Tensor:
+    """x as it lies, where the elements of a head are neighbours."""
+    return x if x.stride(-1) == 1 else x.contiguous()
+
+
+def _rotary_rows(x: torch.Tensor, y: torch.Tensor) -> "N.RotaryRows":
+    return N.RotaryRows(N.ptr(x), N.ptr(y), x.stride(0) if x.dim() == 4 else 0, x.stride(-3),
+                        x.stride(-2), y.stride(0) if x.dim() == 4 else 0, y.stride(-3),
+                        y.stride(-2), x.shape[-2])
+
+
+def _check_rotation(positions: torch.Tensor, shape: Tuple[int, ...], rates: torch.Tensor,
+                    head_dim: int) -> Tuple[int, int]:
+    """The positions' strides over batches and tokens."""
+    if positions.dtype not in (torch.int32, torch.int64) or \
+            tuple(positions.shape) not in (shape, shape[-1:]):
+        raise RuntimeError(f"positions must be int32 or int64 {list(shape)} or {list(shape[-1:])} "
+                           f"(got {positions.dtype} {list(positions.shape)})")
+    if rates.dtype != torch.int64 or rates.dim() != 1 or not rates.is_contiguous():
+        raise RuntimeError(f"rates must be contiguous int64 [pairs] "
+                           f"(got {rates.dtype} {list(rates.shape)})")
+    if not 1 <= rates.numel() <= head_dim // 2:
+        raise RuntimeError(f"{rates.numel()} rotated pairs do not fit heads of {head_dim}")
+    return (positions.stride(0) if positions.dim() == 2 else 0), positions.stride(-1)
+
+
+@torch.library.custom_op(f"{_NS}::rotary", mutates_args=())
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
+           rates: torch.Tensor, gain: float, interleaved: bool, inverse: bool
+           ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """q and k (None: an empty tensor in its place) rotated, by the negative angles if inverse."""
+    dev = N.require_device(q, k, positions, rates)
+    dt = _dtype_code(q.dtype)
+    if q.dim() not in (3, 4):
+        raise RuntimeError("q must be [tokens, heads, head size] or [batch, tokens, heads, head size] "
+                           f"(got {list(q.shape)})")
+    lead, d = tuple(q.shape[:-2]), q.shape[-1]
+    if k is not None and (k.dtype != q.dtype or k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2]
+                          or k.shape[-1] != d):
+        raise RuntimeError(f"k must be {q.dtype} {[*lead, 'heads', d]} "
+                           f"(got {k.dtype} {list(k.shape)})")
+    pb, pt = _check_rotation(positions, lead, rates, d)
+    rows, out = [], []
+    for x in (q, k):
+        if x is None:
+            out.append(q.new_empty(0))
+            continue
+        x = _rotary_input(x)
+        out.append(torch.empty_like(x))
+        rows.append((x, _rotary_rows(x, out[-1])))
+    rot = N.Rotation(N.ptr(rates), rates.numel(), N.ptr(positions),
+                     positions.dtype == torch.int64, interleaved, gain, inverse)
+    with torch.cuda.device(dev):
+        N.check(N.lib().ojx_rotary(
+            ctypes.byref(rows[0][1]), ctypes.byref(rows[1][1]) if k is not None else None,
+            *_rotary_sizes(q), d, dt, ctypes.byref(rot), pb, pt, N.stream_handle(dev)), "rotary")
+    return out[0], out[1]
+
+
+@rotary.register_fake
+def _(q, k, positions, rates, gain, interleaved, inverse):
+    return (torch.empty_like(_rotary_input(q)),
+            q.new_empty(0) if k is None else torch.empty_like(_rotary_input(k)))
+
+
+def _rotary_setup(ctx, inputs, output):
+    _, k, positions, rates, gain, interleaved, inverse = inputs
+    ctx.save_for_backward(positions, rates)
+    ctx.rest = (gain, interleaved, not inverse)
+    ctx.pair = k is not None
+    ctx.set_materialize_grads(False)
+
+
+def _rotary_backward(ctx, g_q, g_k):
+    positions, rates = ctx.saved_tensors
+    if not ctx.pair or not ctx.needs_input_grad[1]:
+        g_k = None
+    if not ctx.needs_input_grad[0]:
+        g_q = None
+    out = [None, None]
+    if g_q is not None and g_k is not None:
+        out = rotary(g_q, g_k, positions, rates, *ctx.rest)
+    elif g_q is not None:
+        out[0] = rotary(g_q, None, positions, rates, *ctx.rest)[0]
+    elif g_k is not None:
+        out[1] = rotary(g_k, None, positions, rates, *ctx.rest)[0]
+    return out[0], out[1], None, None, None, None, None
+
+
+rotary.register_autograd(_rotary_backward, setup_context=_rotary_setup)
