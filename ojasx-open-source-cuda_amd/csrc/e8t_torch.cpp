@@ -893,6 +893,41 @@ struct RecordedRotary : torch::autograd::Function<RecordedRotary> {
     }
 };
 
+// kv8_rotate_append(q, k, v, positions, slots, rates, gain, interleaved, k_codes, v_codes, scales):
+// q rotated
+PyObject* kv8_rotate_append(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 11, "kv8_rotate_append");
+    const Args a{argv, n};
+    if (!all_plain(argv, 6) || !plain(argv[8]) || !plain(argv[9]) || !plain(argv[10])) Py_RETURN_NONE;
+    const Tensor &q = a.t(0), &k = a.t(1), &v = a.t(2), &positions = a.t(3), &slots = a.t(4),
+                 &rates = a.t(5), &kc = a.t(8), &vc = a.t(9), &scales = a.t(10);
+    const int dt = dtype_code(k.scalar_type());
+    if (dt < 0 || v.scalar_type() != k.scalar_type() || k.dim() != 3 || k.sizes() != v.sizes() ||
+        k.stride(2) != 1 || v.stride(2) != 1 || !cache_ok(kc, vc, scales, k.size(2)) ||
+        k.size(1) != kc.size(1) || !ints(slots, at::kLong, k.size(0)) ||
+        k.device() != kc.device() || v.device() != kc.device() || slots.device() != kc.device() ||
+        !heads_ok(q, k) || !rotation_ok(positions, rates, q) ||
+        !positions.is_contiguous() || (c10::GradMode::is_enabled() && records(q)))
+        Py_RETURN_NONE;
+    const ojx_rotation r = rotation_of(positions, rates, a.f64(6), a.flag(7), false);
+    RECORD_FUNCTION("ojasx_e8t::kv8_rotate_append", std::vector<c10::IValue>());
+    Unlocked unlocked;
+    const c10::DeviceGuard on_device(kc.device());
+    Tensor out = at::empty_like(q);
+    const ojx_rotary_rows rows = {data(q), data(out), 0, q.stride(0), q.stride(1),
+                                  0, out.stride(0), out.stride(1), q.size(1)};
+    check(ojx_kv8_rotate_append((int8_t*)data(kc), (int8_t*)data(vc), (float*)data(scales), kc.size(0),
+                                kc.size(1), kc.size(2), k.size(2), data(k), k.stride(0), k.stride(1),
+                                data(v), v.stride(0), v.stride(1), dt, (const int64_t*)data(slots),
+                                k.size(0), &rows, &r, current_stream(kc.device())),
+          "kv8_rotate_append");
+    for (const Tensor* t : {&kc, &vc, &scales}) torch::autograd::impl::bump_version(*t);
+    unlocked.lock();
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
 // Whether rotary(q, k | None, positions, rates, gain, interleaved, inverse) is a call on tensors as
 // the kernels take them
 bool rotary_ok(PyObject* const* argv, const Args& a) {
@@ -965,6 +1000,7 @@ PyMethodDef kMethods[] = {
     {"token_logprobs", (PyCFunction)(void*)token_logprobs, METH_FASTCALL, nullptr},
     {"token_logprobs_recorded", (PyCFunction)(void*)token_logprobs_recorded, METH_FASTCALL,
      nullptr},
+    {"kv8_rotate_append", (PyCFunction)(void*)kv8_rotate_append, METH_FASTCALL, nullptr},
     {"rotary", (PyCFunction)(void*)rotary, METH_FASTCALL, nullptr},
     {"rotary_recorded", (PyCFunction)(void*)rotary_recorded, METH_FASTCALL, nullptr},
     {"is_plain", (PyCFunction)(void*)is_plain, METH_FASTCALL, nullptr},

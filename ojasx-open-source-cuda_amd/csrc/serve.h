@@ -204,6 +204,9 @@ struct RotaryArgs {
 hipError_t launch_kv8_plan(const PlanArgs& a, hipStream_t stream);
 hipError_t launch_kv8_append(const KvCache& c, const KvRows& k, const KvRows& v, int dtype,
                              const int64_t* slots, int tokens, hipStream_t stream);
+// q: the queries (no heads: none), the rotation and the tokens' positions
+hipError_t launch_kv8_rotate_append(const KvCache& c, const KvRows& k, const KvRows& v, int dtype,
+                                    const int64_t* slots, RotaryArgs q, hipStream_t stream);
 hipError_t launch_kv8_read(const KvCache& c, const int32_t* blocks, int n, int dtype, void* k_out,
                            void* v_out, float* scales_out, hipStream_t stream);
 size_t kv8_attention_bytes(const AttnShape& s);

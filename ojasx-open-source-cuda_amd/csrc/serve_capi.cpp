@@ -223,6 +223,42 @@ OJX_API int ojx_kv8_append(int8_t* k_codes, int8_t* v_codes, float* scales, int6
         "kv8 append launch");
 }
 
+OJX_API int ojx_kv8_rotate_append(int8_t* k_codes, int8_t* v_codes, float* scales,
+                                  int64_t num_blocks, int64_t kv_heads, int64_t block_size,
+                                  int64_t head_dim, const void* k, int64_t k_token_stride,
+                                  int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                                  int64_t v_head_stride, int dtype, const int64_t* slots,
+                                  int64_t tokens, const ojx_rotary_rows* q,
+                                  const ojx_rotation* rotation, void* stream) {
+    if (!valid_dtype(dtype)) return api_failf(OJX_EDTYPE, "unknown dtype code %d", dtype);
+    if (int r = check_cache(k_codes, v_codes, scales, num_blocks, kv_heads, block_size, head_dim))
+        return r;
+    if (tokens < 0 || tokens > kMaxCount)
+        return api_failf(OJX_EINVAL, "%lld tokens", (long long)tokens);
+    if (int r = check_rotation(rotation, head_dim, tokens > 0)) return r;
+    if (rotation->inverse) return api_failf(OJX_EINVAL, "an append rotates forward only");
+    if (q)
+        if (int r = check_rows(*q, tokens, dtype)) return r;
+    if (tokens == 0) return OJX_OK;
+    if (!k || !v || !slots) return api_failf(OJX_EINVAL, "null pointer");
+    if (k_token_stride < 0 || k_head_stride < 0 || v_token_stride < 0 || v_head_stride < 0)
+        return api_failf(OJX_EINVAL, "negative stride");
+    if (int r = ojx::api_check_device()) return r;
+    const ojx::KvCache c = cache_of(k_codes, v_codes, scales, num_blocks, kv_heads, block_size,
+                                    head_dim);
+    const ojx::KvRows kr{k, k_token_stride, k_head_stride}, vr{v, v_token_stride, v_head_stride};
+    ojx::RotaryArgs a{};
+    if (q) a.q = rows_of(*q);
+    a.rot = rotation_of(*rotation);
+    a.position_token = 1;
+    a.batches = 1;
+    a.tokens = (int)tokens;
+    a.d = (int)head_dim;
+    return ojx::api_done(
+        ojx::launch_kv8_rotate_append(c, kr, vr, dtype, slots, a, (hipStream_t)stream),
+        "kv8 rotate_append launch");
+}
+
 OJX_API int ojx_kv8_read(const int8_t* k_codes, const int8_t* v_codes, const float* scales,
                          int64_t num_blocks, int64_t kv_heads, int64_t block_size,
                          int64_t head_dim, const int32_t* blocks, int64_t n, int dtype,

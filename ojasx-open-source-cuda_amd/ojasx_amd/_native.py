@@ -63,6 +63,7 @@ EXPORTS = (
     "ojx_token_logprobs",
     "ojx_token_logprobs_bwd",
     "ojx_rotary",
+    "ojx_kv8_rotate_append",
 )
 
 
@@ -231,7 +232,9 @@ def lib() -> ctypes.CDLL:
                                             _P, _P, _P, _SZ, _P]),
                     ("ojx_token_logprobs_bwd", [_P, _I64, _I64, _I64, _INT, _P, _P, _P, _I64]
                      + [_P] * 7),
-                    ("ojx_rotary", [_P, _P, _I64, _I64, _I64, _INT, _P, _I64, _I64, _P])):
+                    ("ojx_rotary", [_P, _P, _I64, _I64, _I64, _INT, _P, _I64, _I64, _P]),
+                    ("ojx_kv8_rotate_append", [_P, _P, _P] + [_I64] * 4
+                     + [_P, _I64, _I64, _P, _I64, _I64, _INT, _P, _I64, _P, _P, _P])):
                 fn = getattr(L, name)
                 fn.restype = _INT
                 fn.argtypes = args

@@ -4,7 +4,8 @@ Keys and values are held as int8 codes with one float32 scale for each block of 
 (``include/ojasx_e8t.h`` has the layout).  One step of a batch:
 
     p = kv8.plan(seq_lens, new_lens, block_tables, free_blocks, num_free, block_size, num_tokens)
-    cache.append(k, v, p.slots)                      # for each layer
+    cache.append(k, v, p.slots)                      # for each layer; or, with positions rotated
+    q = cache.rotate_append(q, k, v, p.positions, p.slots, rotation)    # in on the way
     o = cache.attention(q, block_tables, p.seq_lens, p.query_starts)
 
 ``plan`` runs on the GPU from the requests' lengths alone, so a step needs no copy to the host;
@@ -21,6 +22,7 @@ import torch
 
 from . import _native as N
 from . import serve_ops as S
+from .rotary import Rotation
 
 
 def _eager(name: str, *args):
@@ -72,6 +74,21 @@ def append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_codes: torch
     args = (k, v, slots, k_codes, v_codes, scales)
     if _eager("kv8_append", *args) is None:
         S.kv8_append(*args)
+
+
+def rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                  slots: torch.Tensor, rotation: Rotation, k_codes: torch.Tensor,
+                  v_codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """``append`` with ``positions`` ``[tokens]`` (int32 or int64) rotated into the keys on the way;
+    returns ``q [tokens, heads, head size]`` rotated alike (``rotary.rotate`` has the rule).
+
+    Rotated keys are not rounded to their type before they become codes: the cache then holds what
+    ``append`` makes of keys that were rotated in float32.  No gradient passes.
+    """
+    args = (q, k, v, positions, slots, rotation.rates, rotation.gain, rotation.interleaved, k_codes,
+            v_codes, scales)
+    out = _eager("kv8_rotate_append", *args)
+    return S.kv8_rotate_append(*args) if out is None else out
 
 
 def read(k_codes: torch.Tensor, v_codes: torch.Tensor, scales: torch.Tensor, blocks: torch.Tensor,
@@ -135,6 +152,13 @@ class KV8Cache:
     def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """``kv8.append`` into this storage: the tokens of a block in one run of ``slots``."""
         append(k, v, slots, self.k_codes, self.v_codes, self.scales)
+
+    def rotate_append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                      positions: torch.Tensor, slots: torch.Tensor, rotation: Rotation
+                      ) -> torch.Tensor:
+        """``kv8.rotate_append`` into this storage; returns the rotated queries."""
+        return rotate_append(q, k, v, positions, slots, rotation, self.k_codes, self.v_codes,
+                             self.scales)
 
     def read(self, blocks: torch.Tensor, dtype: torch.dtype = torch.bfloat16
              ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:

@@ -2,7 +2,8 @@
 linears: the 8-bit paged key / value cache, its attention, token log probabilities, rotated positions.
 
 ``kv8_plan``, ``kv8_append`` (a block's tokens in one run of its slots) and ``kv8_read`` move a
-step's tokens into the cache and blocks out of it, ``kv8_attention`` reads it,
+step's tokens into the cache and blocks out of it (``kv8_rotate_append`` with positions rotated into
+keys and queries on the way), ``kv8_attention`` reads it,
 ``token_logprobs`` (autograd registered, with ``token_logprobs_bwd``) is what a model answers and
 trains with; ``rotary`` (its own gradient, turned back) rotates queries and keys.  The reference keeps no quantized cache; the layouts and rules are those of ``include/ojasx_e8t.h``.  As for the other
 ops: the current HIP stream of the device, outputs and workspaces from torch's caching
@@ -165,6 +166,45 @@ def _(k_codes, v_codes, scales, blocks, head_dim, dtype):
     shape = (blocks.numel(), k_codes.shape[2], k_codes.shape[1], head_dim)
     return (k_codes.new_empty(shape, dtype=dtype), k_codes.new_empty(shape, dtype=dtype),
             scales.new_empty((blocks.numel(), k_codes.shape[1], 2)))
+
+
+@torch.library.custom_op(f"{_NS}::kv8_rotate_append",
+                         mutates_args=("k_codes", "v_codes", "scales"))
+def kv8_rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                      slots: torch.Tensor, rates: torch.Tensor, gain: float, interleaved: bool,
+                      k_codes: torch.Tensor, v_codes: torch.Tensor, scales: torch.Tensor
+                      ) -> torch.Tensor:
+    dev = N.require_device(q, k, v, positions, slots, rates, k_codes, v_codes, scales)
+    dt = _dtype_code(k.dtype)
+    if v.dtype != k.dtype or k.dim() != 3 or v.shape != k.shape:
+        raise RuntimeError(f"k and v must be [tokens, kv heads, head size] of one type "
+                           f"(got {k.dtype} {list(k.shape)} and {v.dtype} {list(v.shape)})")
+    t, _, d = k.shape
+    if q.dtype != k.dtype or q.dim() != 3 or q.shape[0] != t or q.shape[2] != d:
+        raise RuntimeError(f"q must be {k.dtype} {[t, 'heads', d]} (got {q.dtype} {list(q.shape)})")
+    blocks, heads, block_size = _check_cache(k_codes, v_codes, scales, d)
+    kr, vr = _rows("k", k, t, heads), _rows("v", v, t, heads)
+    s = _ints("slots", slots, torch.int64, (t,))
+    if positions.dim() != 1:
+        raise RuntimeError(f"positions must be [{t}] (got {list(positions.shape)})")
+    _check_rotation(positions, (t,), rates, d)
+    qr, p = _rotary_input(q), positions.contiguous()
+    out = torch.empty_like(qr)
+    rot = N.Rotation(N.ptr(rates), rates.numel(), N.ptr(p), p.dtype == torch.int64, interleaved,
+                     gain, False)
+    rows = _rotary_rows(qr, out)
+    with torch.cuda.device(dev):
+        N.check(N.lib().ojx_kv8_rotate_append(
+            N.ptr(k_codes), N.ptr(v_codes), N.ptr(scales), blocks, heads, block_size, d,
+            N.ptr(kr), kr.stride(0), kr.stride(1), N.ptr(vr), vr.stride(0), vr.stride(1), dt,
+            N.ptr(s), t, ctypes.byref(rows), ctypes.byref(rot), N.stream_handle(dev)),
+            "kv8_rotate_append")
+    return out
+
+
+@kv8_rotate_append.register_fake
+def _(q, k, v, positions, slots, rates, gain, interleaved, k_codes, v_codes, scales):
+    return torch.empty_like(_rotary_input(q))
 
 
 # ----------------------------------------------------------------------------- attention
