@@ -503,6 +503,27 @@ int ojx_kv8_rotate_append(int8_t* k_codes, int8_t* v_codes, float* scales, int64
                           const int64_t* slots, int64_t tokens, const ojx_rotary_rows* q,
                           const ojx_rotation* rotation, void* stream);
 
+/* ---- beam search ----
+ *
+ * The best continuations of each of `groups` groups of `beams` (1..64) beams.  logits: rows of
+ * vocab elements at stride ld, row g * beams + b of beam b of group g.  A candidate (b, t) has the
+ * value scores[g][b] + log softmax(row)[t]; of a beam with finished[g][b] (may be NULL) only
+ * (b, pad_id) is possible, with its score.  The `num` (1..64, at most beams * vocab) largest of a
+ * group in falling order, equal ones by rising beam and token:
+ *   out_scores [groups][num], out_parents [groups][num] the row of the beam, out_tokens.
+ * Impossible candidates (masked logits of -inf, a score of -inf) have value -inf and are taken, in
+ * the order of beams and tokens, where a group has fewer than num others.  A beam whose score is
+ * NaN or +inf, or that has such a logit, makes all its candidates NaN, which count as largest; a
+ * finished one's logits are not read.  Values are compared in 64 bits: sums are formed partly in 32,
+ * and again in 64 where two beams' values are closer than 2^-20.  The workspace holds partial results;
+ * one smaller than asked for, but of groups * beams * (16 + 8 * num) bytes, lowers the split of rows. */
+int ojx_beam_select_workspace_bytes(int64_t groups, int64_t beams, int64_t vocab, int64_t num,
+                                    int dtype, size_t* bytes);
+int ojx_beam_select(const void* logits, int64_t ld, int64_t groups, int64_t beams, int64_t vocab,
+                    int dtype, const float* scores, const uint8_t* finished, int64_t pad_id,
+                    int64_t num, float* out_scores, int64_t* out_parents, int64_t* out_tokens,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -35,6 +35,7 @@ SOURCES = [
     "kv8_attention.hip",
     "token_logprobs.hip",
     "rotary.hip",
+    "beam_select.hip",
     "e8t_capi.cpp",
     "serve_capi.cpp",
 ]

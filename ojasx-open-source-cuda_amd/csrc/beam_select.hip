@@ -1,0 +1,347 @@
+// beam_select.hip -- the best continuations of groups of beams: for each group the largest of
+//   value(b, t) = score_b + (x_bt - m_b) - log s_b,   m_b = max x_b,   s_b = sum exp(x_b - m_b),
+// over its beams b and all tokens t of the vocabulary, equal values by rising beam and token.
+//
+// Two launches.  The first reads every beam's logits once: sums, and the largest few of each part of
+// a row (logit_rows.h).  The second joins a group: at most `num` logits of a beam can be among the
+// group's best.
+
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "logit_rows.h"
+
+namespace ojx {
+
+namespace {
+
+// Of a part of a row: s = sum 2^(x log2(e) - r) with r a whole number near the largest exponent, so
+// that sums of different r join without a rounding.
+struct BeamSum {
+    double s;
+    float r, m;
+};
+
+struct BeamParts {
+    BeamSum* sums;   // [rows][splits]
+    uint64_t* keys;  // [rows][splits][num], falling, 0 behind the last
+    int splits;
+};
+
+// Whether a beam's logits matter: not those of a finished one, nor where no finite score leaves them.
+__device__ __forceinline__ bool reads_logits(const BeamArgs& a, int64_t row) {
+    const float score = a.scores[row];
+    return !(a.done && a.done[row]) && score < INFINITY && score > -INFINITY;
+}
+
+__device__ __forceinline__ double scaled(double s, float r, float to) {
+    return ldexp(s, (int)fmaxf(r - to, -2000.f));
+}
+
+// A workgroup reads a row or a part of it once; rows that do not matter not at all.  Four partial
+// sums of 8 terms a batch are held in 32 bits, everything beyond in 64: whole numbers (which beam)
+// hang on these sums, and the join has to settle in 64 bits what they leave open.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void beam_pass_kernel(BeamArgs a, BeamParts p) {
+    __shared__ Pool pool[kGroups];
+    __shared__ uint64_t keys[kGroups * kTopMax];
+    __shared__ BeamSum sums[kGroups];
+    using B = Batch<DT>;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row = blockIdx.x / (unsigned)p.splits;
+    const int split = blockIdx.x - (unsigned)row * p.splits;
+    if (!reads_logits(a, row)) return;
+    const int64_t x0 = row * a.ld;
+    const int size = DT == kF32 ? 4 : 2;
+    const int shift = (int)((((uintptr_t)a.x + x0 * size) & 15) / size);
+    const int batches = (int)(((int64_t)a.vocab + shift + kBatch - 1) / kBatch);
+    const int per = (batches + p.splits - 1) / p.splits;
+    const int end = min(batches, (split + 1) * per);
+    double sum = 0;
+    float ref = -INFINITY, most = -INFINITY;
+    Best best{0, -INFINITY};
+    B x;
+    for (int b = split * per + wave; b < end; b += kGroups) {
+        x.load(a.x, x0, a.vocab, b, lane, shift);
+        float m = x.get(0);
+#pragma unroll
+        for (int i = 1; i < kLaneLogits; ++i) m = or_nan(m, x.get(i));
+        const float r = fmaxf(ref, m < -kPlainMax ? -INFINITY : ceilf(m * kLog2e));
+        const float base = r == -INFINITY ? 0.f : r;
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < kLaneLogits; ++i) s[i & 3] += __builtin_amdgcn_exp2f(term(x.get(i), base));
+        sum = scaled(sum, ref, base) + (((double)s[0] + s[1]) + ((double)s[2] + s[3]));
+        ref = r;
+        most = or_nan(most, m);
+        x.drop_floats();
+        take<DT>(best, x, m, b, a.num, lane, shift, pool[wave]);
+    }
+    // over the wave
+    const bool bad = __any(most != most);
+    const float r = wave_max(ref), base = r == -INFINITY ? 0.f : r;
+    sum = scaled(sum, ref, base);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    most = wave_max(most);
+    if (lane == 0) sums[wave] = BeamSum{sum, r, bad ? __uint_as_float(0x7FC00000u) : most};
+    if (lane < a.num) keys[wave * a.num + lane] = best.key;
+    __syncthreads();
+    const int64_t at = row * p.splits + split;
+    if (threadIdx.x == 0) {
+        BeamSum t = sums[0];
+        for (int w = 1; w < kGroups; ++w) {
+            const float to = fmaxf(t.r, sums[w].r), from = to == -INFINITY ? 0.f : to;
+            t = BeamSum{scaled(t.s, t.r, from) + scaled(sums[w].s, sums[w].r, from), to,
+                        or_nan(t.m, sums[w].m)};
+        }
+        p.sums[at] = t;
+    }
+    for (int i = threadIdx.x; i < kGroups * a.num; i += kThreads) {
+        const uint64_t k = keys[i];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < kGroups * a.num; ++j) rank += keys[j] > k || (keys[j] == k && j < i);
+        if (rank < a.num) p.keys[at * a.num + rank] = k;
+    }
+}
+
+constexpr int kJoinThreads = 512;
+constexpr int kJoinWaves = kJoinThreads / 64;
+constexpr int kJoinBytes = 60 * 1024;  // of LDS for a row's lists and the group's candidates
+// Two values of different beams that are closer than this are compared again with sums in 64 bits.
+// What the first pass is off by: a term that stands alone 2^-23 (its exponential) and 2^-25 (its
+// exponent's rounding, under 1 there); several each up to 17 * 2^-24 for the smallest that count, with
+// both signs, and 7 * 2^-24 for the sum of 8.
+constexpr double kNear = 0x1p-20;
+
+// fp64 bits in rising order as unsigned; NaN above everything.
+__device__ __forceinline__ uint64_t ordered64(double v) {
+    if (v != v) return ~0ull;
+    const uint64_t u = (uint64_t)__double_as_longlong(v + 0.0);
+    return u >> 63 ? ~u : u | 1ull << 63;
+}
+__device__ __forceinline__ double unordered64(uint64_t k) {
+    if (k == ~0ull) return __longlong_as_double(0x7FF8000000000000ll);
+    return __longlong_as_double((int64_t)(k >> 63 ? k & ~(1ull << 63) : ~k));
+}
+
+// A beam in the join.
+struct Beam {
+    double ls;   // log of the sum of exp(x - m)
+    float m, score;
+    int count;   // candidates
+    bool exact;  // ls is a sum in 64 bits, or none is needed
+    bool need;   // such a sum is asked for
+};
+
+// One workgroup a group.
+template <int DT>
+__global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, BeamParts p) {
+    extern __shared__ uint64_t lds[];
+    __shared__ Beam beams[kBeamMax];
+    __shared__ uint64_t top_value[kTopMax + 1];
+    __shared__ int top_at[kTopMax + 1];  // beam * num + place
+    __shared__ double part[kJoinWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n = p.splits * a.num, all = a.beams * a.num;
+    uint64_t* list = lds + wave * n;
+    uint64_t* value = lds + kJoinWaves * n;                        // [beams][num], falling
+    int* token = reinterpret_cast<int*>(value + all);              // [beams][num]
+    const int64_t row0 = (int64_t)blockIdx.x * a.beams;
+
+    for (int b = wave; b < a.beams; b += kJoinWaves) {
+        const int64_t row = row0 + b;
+        const float score = a.scores[row];
+        const bool ended = a.done && a.done[row];
+        Beam t{0.0, 0.f, score, 0, true, false};
+        bool nan = !(score < INFINITY);
+        if (reads_logits(a, row)) {
+            BeamSum s{0.0, -INFINITY, -INFINITY};
+            if (lane < p.splits) s = p.sums[row * p.splits + lane];
+            for (int i = lane; i < n; i += 64) list[i] = p.keys[row * n + i];
+            const float r = wave_max(s.r), base = r == -INFINITY ? 0.f : r;
+            double sum = scaled(s.s, s.r, base);
+#pragma unroll
+            for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+            nan = __any(s.m != s.m);
+            t.m = wave_max(s.m);
+            nan |= t.m == INFINITY;
+            if (!nan && t.m > -INFINITY) {
+                // the pass's own log2(e), so that what it is off by cancels at m
+                t.ls = log(sum) - ((double)t.m * (double)kLog2e - (double)r) * 0.6931471805599453;
+                t.exact = false;
+                t.need = !(t.m > -kPlainMax && t.m < kPlainMax);
+                __builtin_amdgcn_wave_barrier();
+                for (int i0 = 0; i0 < n; i0 += 64) {
+                    const uint64_t mine = i0 + lane < n ? list[i0 + lane] : 0;
+                    int rank = 0;
+#pragma unroll 8
+                    for (int j = 0; j < n; ++j) rank += list[j] > mine;
+                    const bool in = mine != 0 && rank < a.num;
+                    if (in) {
+                        const float x = unordered((uint32_t)(mine >> 32));
+                        value[b * a.num + rank] = ordered64(score + (((double)x - t.m) - t.ls));
+                        token[b * a.num + rank] = (int)(0xFFFFFFFFu - (uint32_t)mine);
+                    }
+                    t.count += __popcll(__ballot(in));
+                }
+                __builtin_amdgcn_wave_barrier();
+            }
+        } else if (ended && !nan && score > -INFINITY) {
+            t.count = 1;
+            if (lane == 0) value[b * a.num] = ordered64(score), token[b * a.num] = (int)a.pad;
+        }
+        if (nan) {  // every token
+            t.count = min(a.num, a.vocab);
+            if (lane < t.count) value[b * a.num + lane] = ~0ull, token[b * a.num + lane] = lane;
+        }
+        if (lane == 0) beams[b] = t;
+    }
+    __syncthreads();
+
+    int total = 0;
+    for (int b = 0; b < a.beams; ++b) total += beams[b].count;
+    for (;;) {
+        // sums in 64 bits of the beams that need one, over tokens in the same order for each beam:
+        // equal rows have equal sums
+        for (int b = 0; b < a.beams; ++b) {
+            if (!beams[b].need) continue;
+            const int64_t x0 = (row0 + b) * a.ld;
+            const double m = beams[b].m;
+            double s = 0;
+#pragma unroll 4
+            for (int j = threadIdx.x; j < a.vocab; j += kJoinThreads)
+                s += exp((double)load_as_f32<DT>(a.x, x0 + j) - m);
+#pragma unroll
+            for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
+            if (lane == 0) part[wave] = s;
+            __syncthreads();
+            s = 0;
+            for (int w = 0; w < kJoinWaves; ++w) s += part[w];
+            const double ls = log(s);
+            for (int i = threadIdx.x; i < beams[b].count; i += kJoinThreads) {
+                const float x = load_as_f32<DT>(a.x, x0 + token[b * a.num + i]);
+                value[b * a.num + i] = ordered64(beams[b].score + (((double)x - m) - ls));
+            }
+            __syncthreads();
+            if (threadIdx.x == 0) beams[b].ls = ls, beams[b].exact = true, beams[b].need = false;
+            __syncthreads();
+        }
+        // a candidate's rank: those before it in its beam, and in the others' lists
+        for (int i = threadIdx.x; i < all; i += kJoinThreads) {
+            const int b = i / a.num, place = i - b * a.num;
+            if (place >= beams[b].count) continue;
+            const uint64_t v = value[i];
+            int rank = place;
+            for (int o = 0; o < a.beams && rank <= a.num; ++o) {
+                if (o == b) continue;
+                // of an earlier beam equal ones come first
+                const uint64_t least = v + (o < b ? 0 : 1);
+                int lo = 0, hi = v == ~0ull && o > b ? 0 : beams[o].count;
+                while (lo < hi) {
+                    const int m = (lo + hi) >> 1;
+                    if (value[o * a.num + m] >= least) lo = m + 1;
+                    else hi = m;
+                }
+                rank += lo;
+            }
+            if (rank <= a.num) {
+                top_value[rank] = v;
+                top_at[rank] = i;
+            }
+        }
+        __syncthreads();
+        const int last = min(total - 1, a.num);
+        bool again = false;
+        if ((int)threadIdx.x < last) {
+            const int i = threadIdx.x, b = top_at[i] / a.num, c = top_at[i + 1] / a.num;
+            if (b != c && !(beams[b].exact && beams[c].exact) &&
+                unordered64(top_value[i]) - unordered64(top_value[i + 1]) < kNear) {
+                again = true;
+                // (lanes that find the same beam write the same)
+                if (!beams[b].exact) beams[b].need = true;
+                if (!beams[c].exact) beams[c].need = true;
+            }
+        }
+        if (!__syncthreads_or(again)) break;
+    }
+
+    const int64_t o0 = (int64_t)blockIdx.x * a.num;
+    if ((int)threadIdx.x < min(total, a.num)) {
+        const int i = threadIdx.x, b = top_at[i] / a.num;
+        a.out_scores[o0 + i] = (float)unordered64(top_value[i]);
+        a.out_parents[o0 + i] = row0 + b;
+        a.out_tokens[o0 + i] = token[top_at[i]];
+    }
+    // Fewer than asked for: impossible ones follow, by rising beam and token.  Those possible are all
+    // in the lists, so the first `num` others are among the group's first total + num.
+    if (total < a.num && wave == 0) {
+        int have = total;
+        for (int64_t f0 = 0; have < a.num; f0 += 64) {
+            const int64_t f = f0 + lane, b = f / a.vocab;
+            const int t = (int)(f - b * a.vocab);
+            bool free = b < a.beams;
+            if (free)
+                for (int i = 0; i < beams[b].count; ++i) free &= token[b * a.num + i] != t;
+            const uint64_t those = __ballot(free);
+            const int rank = have + __popcll(those & ((1ull << lane) - 1));
+            if (free && rank < a.num) {
+                a.out_scores[o0 + rank] = -INFINITY;
+                a.out_parents[o0 + rank] = row0 + b;
+                a.out_tokens[o0 + rank] = t;
+            }
+            have += __popcll(those);
+        }
+    }
+}
+
+size_t join_bytes(int splits, int beams, int num) {
+    return (size_t)kJoinWaves * splits * num * 8 + (size_t)beams * num * 12;
+}
+
+// Parts of a row: until the workgroups fill the GPU twice, none under a batch for each wave, and
+// as many as the join has room for.
+int beam_splits(const BeamArgs& a) {
+    const int64_t rows = (int64_t)a.groups * a.beams;
+    const int64_t most = ((int64_t)a.vocab + kBatch * kGroups - 1) / (kBatch * kGroups);
+    int64_t n = rows > 0 ? 2048 / rows : 1;
+    if (n > most) n = most;
+    if (n > kMaxRowSplits) n = kMaxRowSplits;
+    while (n > 1 && join_bytes((int)n, a.beams, a.num) > kJoinBytes) --n;
+    return n < 1 ? 1 : (int)n;
+}
+
+size_t part_bytes(const BeamArgs& a) {
+    return (size_t)a.groups * a.beams * (sizeof(BeamSum) + a.num * sizeof(uint64_t));
+}
+
+}  // namespace
+
+size_t beam_select_bytes(const BeamArgs& a) { return part_bytes(a) * beam_splits(a); }
+size_t beam_select_least_bytes(const BeamArgs& a) { return part_bytes(a); }
+
+hipError_t launch_beam_select(const BeamArgs& a, void* ws, size_t ws_bytes, hipStream_t stream) {
+    BeamParts p{};
+    p.splits = beam_splits(a);
+    const size_t fit = ws_bytes / part_bytes(a);
+    if (fit < 1) return hipErrorInvalidValue;
+    if ((size_t)p.splits > fit) p.splits = (int)fit;
+    const int64_t rows = (int64_t)a.groups * a.beams, grid = rows * p.splits;
+    if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+    p.sums = static_cast<BeamSum*>(ws);
+    p.keys = reinterpret_cast<uint64_t*>(p.sums + (size_t)rows * p.splits);
+    auto go = [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        beam_pass_kernel<DT><<<(unsigned)grid, kThreads, 0, stream>>>(a, p);
+        beam_join_kernel<DT><<<(unsigned)a.groups, kJoinThreads, join_bytes(p.splits, a.beams, a.num),
+                               stream>>>(a, p);
+    };
+    if (a.dtype == kF32) go(std::integral_constant<int, kF32>{});
+    else if (a.dtype == kF16) go(std::integral_constant<int, kF16>{});
+    else go(std::integral_constant<int, kBF16>{});
+    return hipGetLastError();
+}
+
+}  // namespace ojx

@@ -976,6 +976,47 @@ PyObject* rotary_recorded(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// beam_select(logits, scores, num, finished | None, pad_id): the op's results
+PyObject* beam_select(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 5, "beam_select");
+    const Args a{argv, n};
+    if (!all_plain(argv, 2) || (argv[3] != Py_None && !plain(argv[3]))) Py_RETURN_NONE;
+    const Tensor &x = a.t(0), &scores = a.t(1);
+    const Tensor done = argv[3] == Py_None ? Tensor() : a.t(3);
+    const int64_t num = a.i64(2), pad = a.i64(4);
+    const int dt = dtype_code(x.scalar_type());
+    if (dt < 0 || x.dim() != 3 || x.size(2) < 1 || x.size(1) < 1 || x.size(1) > 64 || num < 1 || num > 64 ||
+        num > x.size(1) * x.size(2) || x.stride(2) != 1 || x.stride(1) < x.size(2) ||
+        (x.size(0) > 1 && x.stride(0) != x.size(1) * x.stride(1)) ||
+        scores.scalar_type() != at::kFloat || scores.dim() != 2 || scores.size(0) != x.size(0) ||
+        scores.size(1) != x.size(1) || !scores.is_contiguous() || scores.device() != x.device() ||
+        (done.defined() && (done.scalar_type() != at::kBool || done.sizes() != scores.sizes() ||
+                            !done.is_contiguous() || done.device() != x.device() || pad < 0 ||
+                            pad >= x.size(2))) ||
+        (c10::GradMode::is_enabled() && (records(x) || records(scores))))
+        Py_RETURN_NONE;
+    RECORD_FUNCTION("ojasx_e8t::beam_select", std::vector<c10::IValue>());
+    Unlocked unlocked;
+    const c10::DeviceGuard on_device(x.device());
+    const int64_t g = x.size(0), k = x.size(1), v = x.size(2);
+    // 20 bytes a result: side by side whatever their number
+    Results all(Results::room(g * num, 4) + 2 * Results::room(g * num, 8), 0, x);
+    Tensor out[] = {all.next({g, num}, at::kFloat), all.next({g, num}, at::kLong),
+                    all.next({g, num}, at::kLong)};
+    size_t bytes = 0;
+    check(ojx_beam_select_workspace_bytes(g, k, v, num, dt, &bytes), "beam_select_workspace_bytes");
+    const Tensor ws = workspace(bytes, x);
+    check(ojx_beam_select(data(x), x.stride(1), g, k, v, dt, (const float*)data(scores),
+                          (const uint8_t*)data(done), pad, num, (float*)data(out[0]),
+                          (int64_t*)data(out[1]), (int64_t*)data(out[2]), data(ws), bytes,
+                          current_stream(x.device())),
+          "beam_select");
+    unlocked.lock();
+    return tuple_of(out, 3);
+    END_HANDLE_TH_ERRORS
+}
+
 // plain(tensor, ...): whether a Function over these tensors is plain eager work (grad aside)
 PyObject* is_plain(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -1003,6 +1044,7 @@ PyMethodDef kMethods[] = {
     {"kv8_rotate_append", (PyCFunction)(void*)kv8_rotate_append, METH_FASTCALL, nullptr},
     {"rotary", (PyCFunction)(void*)rotary, METH_FASTCALL, nullptr},
     {"rotary_recorded", (PyCFunction)(void*)rotary_recorded, METH_FASTCALL, nullptr},
+    {"beam_select", (PyCFunction)(void*)beam_select, METH_FASTCALL, nullptr},
     {"is_plain", (PyCFunction)(void*)is_plain, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

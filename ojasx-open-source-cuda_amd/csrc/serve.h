@@ -1,6 +1,6 @@
 // serve.h -- arguments and launchers of the 8-bit paged cache (kv8_cache.hip), its attention
-// (kv8_attention.hip), token log probabilities (token_logprobs.hip) and rotated positions
-// (rotary.hip).
+// (kv8_attention.hip), token log probabilities (token_logprobs.hip), rotated positions (rotary.hip)
+// and the selection of beams (beam_select.hip).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -67,6 +67,7 @@ int api_done(hipError_t e, const char* what);
 
 constexpr int64_t kKvMaxHeads = 4096;
 constexpr int64_t kTopMax = 64;
+constexpr int64_t kBeamMax = 64;
 
 // A cache; its layout is in include/ojasx_e8t.h.
 struct KvCache {
@@ -177,6 +178,22 @@ struct LogprobGradArgs {
     void* gx;
 };
 
+struct BeamArgs {
+    const void* x;  // [groups][beams] rows of vocab logits
+    int64_t ld;
+    int groups;
+    int beams;
+    int vocab;
+    int dtype;
+    int num;
+    const float* scores;
+    const uint8_t* done;  // null: none
+    int64_t pad;
+    float* out_scores;
+    int64_t* out_parents;
+    int64_t* out_tokens;
+};
+
 // [batch][token][head][d] elements, d contiguous, and where they go rotated.
 struct RotaryRows {
     const void* x;
@@ -216,6 +233,9 @@ hipError_t launch_token_logprobs(const LogprobArgs& a, void* ws, size_t ws_bytes
                                  hipStream_t stream);
 hipError_t launch_token_logprobs_bwd(const LogprobGradArgs& a, hipStream_t stream);
 
+size_t beam_select_bytes(const BeamArgs& a);
+size_t beam_select_least_bytes(const BeamArgs& a);  // what a call needs; more lets it split rows
+hipError_t launch_beam_select(const BeamArgs& a, void* ws, size_t ws_bytes, hipStream_t stream);
 hipError_t launch_rotary(RotaryArgs a, int dtype, hipStream_t stream);
 
 }  // namespace ojx

@@ -1,6 +1,6 @@
 // serve_capi.cpp -- extern "C" entry points of the operators around the packed linears: the
-// 8-bit paged cache, its attention, token log probabilities and rotated positions (declared in
-// include/ojasx_e8t.h).  Checks arguments, then enqueues on the caller's stream; allocates
+// 8-bit paged cache, its attention, token log probabilities, rotated positions and the selection of
+// beams (declared in include/ojasx_e8t.h).  Checks arguments, then enqueues on the caller's stream; allocates
 // nothing.
 
 #include <hip/hip_runtime.h>
@@ -101,6 +101,30 @@ int check_workspace(const void* ws, size_t bytes) {
         return api_failf(OJX_EINVAL, "workspace_bytes %zu with a null workspace", bytes);
     if (misaligned(ws, 16)) return api_failf(OJX_ELAYOUT, "workspace must be 16-byte aligned");
     return OJX_OK;
+}
+
+int check_beams(int64_t ld, int64_t groups, int64_t beams, int64_t vocab, int64_t num, int dtype) {
+    if (beams < 1 || beams > ojx::kBeamMax)
+        return api_failf(OJX_EINVAL, "%lld beams, expected 1..%d", (long long)beams,
+                        (int)ojx::kBeamMax);
+    if (groups < 0 || groups > kMaxCount / beams)
+        return api_failf(OJX_EINVAL, "%lld groups of %lld beams", (long long)groups,
+                        (long long)beams);
+    if (int r = check_logits(ld, groups * beams, vocab, 0, dtype)) return r;
+    if (num < 1 || num > ojx::kTopMax || num > beams * vocab)
+        return api_failf(OJX_EINVAL, "num %lld is outside 1..%lld", (long long)num,
+                        (long long)(beams * vocab < ojx::kTopMax ? beams * vocab : ojx::kTopMax));
+    return OJX_OK;
+}
+
+ojx::BeamArgs beams_of(int64_t groups, int64_t beams, int64_t vocab, int64_t num, int dtype) {
+    ojx::BeamArgs a{};
+    a.groups = (int)groups;
+    a.beams = (int)beams;
+    a.vocab = (int)vocab;
+    a.num = (int)num;
+    a.dtype = dtype;
+    return a;
 }
 
 // Heads and their size: what 32-bit indexes within one token rely on.
@@ -427,6 +451,48 @@ OJX_API int ojx_token_logprobs_bwd(const void* logits, int64_t ld, int64_t rows,
     a.gx = grad_logits;
     return ojx::api_done(ojx::launch_token_logprobs_bwd(a, (hipStream_t)stream),
                          "token_logprobs_bwd launch");
+}
+
+OJX_API int ojx_beam_select_workspace_bytes(int64_t groups, int64_t beams, int64_t vocab,
+                                            int64_t num, int dtype, size_t* bytes) {
+    if (!bytes) return api_failf(OJX_EINVAL, "null pointer");
+    *bytes = 0;
+    if (int r = check_beams(vocab, groups, beams, vocab, num, dtype)) return r;
+    *bytes = ojx::beam_select_bytes(beams_of(groups, beams, vocab, num, dtype));
+    return OJX_OK;
+}
+
+OJX_API int ojx_beam_select(const void* logits, int64_t ld, int64_t groups, int64_t beams,
+                            int64_t vocab, int dtype, const float* scores, const uint8_t* finished,
+                            int64_t pad_id, int64_t num, float* out_scores, int64_t* out_parents,
+                            int64_t* out_tokens, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+    if (int r = check_beams(ld, groups, beams, vocab, num, dtype)) return r;
+    if (finished && (pad_id < 0 || pad_id >= vocab))
+        return api_failf(OJX_EINVAL, "pad_id %lld is outside the vocabulary of %lld",
+                        (long long)pad_id, (long long)vocab);
+    if (int r = check_workspace(workspace, workspace_bytes)) return r;
+    if (groups == 0) return OJX_OK;
+    if (!logits || !scores || !out_scores || !out_parents || !out_tokens)
+        return api_failf(OJX_EINVAL, "null pointer");
+    if (misaligned(logits, dtype == OJX_F32 ? 4 : 2) || misaligned(scores, 4))
+        return api_failf(OJX_ELAYOUT, "misaligned logits or scores");
+    ojx::BeamArgs a = beams_of(groups, beams, vocab, num, dtype);
+    if (workspace_bytes < ojx::beam_select_least_bytes(a))
+        return api_failf(OJX_EINVAL, "workspace of %zu bytes, at least %zu are needed",
+                        workspace_bytes, ojx::beam_select_least_bytes(a));
+    if (int r = ojx::api_check_device()) return r;
+    a.x = logits;
+    a.ld = ld;
+    a.scores = scores;
+    a.done = finished;
+    a.pad = pad_id;
+    a.out_scores = out_scores;
+    a.out_parents = out_parents;
+    a.out_tokens = out_tokens;
+    return ojx::api_done(
+        ojx::launch_beam_select(a, workspace, workspace_bytes, (hipStream_t)stream),
+        "beam_select launch");
 }
 
 OJX_API int ojx_rotary(const ojx_rotary_rows* q, const ojx_rotary_rows* k, int64_t batches,

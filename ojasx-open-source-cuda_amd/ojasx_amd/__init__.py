@@ -25,6 +25,7 @@ from .lattice import (
     fwht_block32,
     pack_model_e8,
 )
+from .beams import BeamStep, beam_select
 from .kv8 import KV8Cache
 from .logprobs import TokenLogprobs, token_logprobs
 from .streaming import StreamingE8LoadReport, load_hf_checkpoint_e8, pack_weight_rowwise
@@ -39,6 +40,8 @@ __all__ = [
     "optim_state",
     "rotary",
     "serve_ops",
+    "BeamStep",
+    "beam_select",
     "KV8Cache",
     "TokenLogprobs",
     "token_logprobs",

@@ -64,6 +64,8 @@ EXPORTS = (
     "ojx_token_logprobs_bwd",
     "ojx_rotary",
     "ojx_kv8_rotate_append",
+    "ojx_beam_select_workspace_bytes",
+    "ojx_beam_select",
 )
 
 
@@ -234,7 +236,10 @@ def lib() -> ctypes.CDLL:
                      + [_P] * 7),
                     ("ojx_rotary", [_P, _P, _I64, _I64, _I64, _INT, _P, _I64, _I64, _P]),
                     ("ojx_kv8_rotate_append", [_P, _P, _P] + [_I64] * 4
-                     + [_P, _I64, _I64, _P, _I64, _I64, _INT, _P, _I64, _P, _P, _P])):
+                     + [_P, _I64, _I64, _P, _I64, _I64, _INT, _P, _I64, _P, _P, _P]),
+                    ("ojx_beam_select_workspace_bytes", [_I64] * 4 + [_INT, _P]),
+                    ("ojx_beam_select", [_P] + [_I64] * 4 + [_INT, _P, _P, _I64, _I64, _P, _P, _P,
+                                                             _P, _SZ, _P])):
                 fn = getattr(L, name)
                 fn.restype = _INT
                 fn.argtypes = args

@@ -1,11 +1,13 @@
 """``torch.library`` custom ops (namespace ``ojasx_e8t``) of the operators around the packed
-linears: the 8-bit paged key / value cache, its attention, token log probabilities, rotated positions.
+linears: the 8-bit paged key / value cache, its attention, token log probabilities, rotated positions,
+beam search.
 
 ``kv8_plan``, ``kv8_append`` (a block's tokens in one run of its slots) and ``kv8_read`` move a
 step's tokens into the cache and blocks out of it (``kv8_rotate_append`` with positions rotated into
 keys and queries on the way), ``kv8_attention`` reads it,
 ``token_logprobs`` (autograd registered, with ``token_logprobs_bwd``) is what a model answers and
-trains with; ``rotary`` (its own gradient, turned back) rotates queries and keys.  The reference keeps no quantized cache; the layouts and rules are those of ``include/ojasx_e8t.h``.  As for the other
+trains with; ``rotary`` (its own gradient, turned back) rotates queries and keys; ``beam_select`` chooses the beams
+that go on.  The reference keeps no quantized cache; the layouts and rules are those of ``include/ojasx_e8t.h``.  As for the other
 ops: the current HIP stream of the device, outputs and workspaces from torch's caching
 allocator, ``RuntimeError`` for what does not fit, no fallback.
 """
@@ -23,6 +25,7 @@ from .ops import _NS, _dtype_code
 BLOCK_SIZES = (16, 32, 64, 128, 256)
 MAX_HEAD_DIM = 256
 MAX_TOP = 64
+MAX_BEAMS = 64
 
 
 def stored_dim(head_dim: int) -> int:
@@ -470,3 +473,54 @@ def _rotary_backward(ctx, g_q, g_k):
 
 
 rotary.register_autograd(_rotary_backward, setup_context=_rotary_setup)
+
+
+# ----------------------------------------------------------------------------- beam search
+
+@torch.library.custom_op(f"{_NS}::beam_select", mutates_args=())
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, num: int,
+                finished: Optional[torch.Tensor], pad_id: int
+                ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(scores, parents, tokens) [groups, num] of logits [groups, beams, V] and scores."""
+    dev = N.require_device(logits, scores, finished)
+    dt = _dtype_code(logits.dtype)
+    if logits.dim() != 3 or logits.shape[2] < 1:
+        raise RuntimeError(f"logits must be [groups, beams, vocabulary] (got {list(logits.shape)})")
+    g, k, v = logits.shape
+    if not 1 <= k <= MAX_BEAMS:
+        raise RuntimeError(f"{k} beams, expected 1..{MAX_BEAMS}")
+    if not 1 <= num <= min(MAX_TOP, k * v):
+        raise RuntimeError(f"num is {num}, expected 1..{min(MAX_TOP, k * v)}")
+    if scores.dtype != torch.float32 or tuple(scores.shape) != (g, k):
+        raise RuntimeError(f"scores must be float32 {[g, k]} (got {scores.dtype} {list(scores.shape)})")
+    if finished is not None:
+        if finished.dtype != torch.bool or tuple(finished.shape) != (g, k):
+            raise RuntimeError(f"finished must be bool {[g, k]} "
+                               f"(got {finished.dtype} {list(finished.shape)})")
+        if not 0 <= pad_id < v:
+            raise RuntimeError(f"pad_id {pad_id} is outside the vocabulary of {v}")
+        finished = finished.contiguous()
+    x = logits.reshape(g * k, v)
+    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < v):
+        x = x.contiguous()
+    s = scores.contiguous()
+    best = torch.empty((g, num), dtype=torch.float32, device=dev)
+    parents = torch.empty((g, num), dtype=torch.int64, device=dev)
+    tokens = torch.empty_like(parents)
+    with torch.cuda.device(dev):
+        nbytes = ctypes.c_size_t(0)
+        N.check(N.lib().ojx_beam_select_workspace_bytes(g, k, v, num, dt, ctypes.byref(nbytes)),
+                "beam_select_workspace_bytes")
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev) if nbytes.value else None
+        N.check(N.lib().ojx_beam_select(
+            N.ptr(x), x.stride(0), g, k, v, dt, N.ptr(s), N.ptr(finished), pad_id, num, N.ptr(best),
+            N.ptr(parents), N.ptr(tokens), N.ptr(ws), nbytes.value, N.stream_handle(dev)),
+            "beam_select")
+    return best, parents, tokens
+
+
+@beam_select.register_fake
+def _(logits, scores, num, finished, pad_id):
+    shape = (logits.shape[0], num)
+    return (scores.new_empty(shape), scores.new_empty(shape, dtype=torch.int64),
+            scores.new_empty(shape, dtype=torch.int64))
