@@ -524,6 +524,45 @@ int ojx_beam_select(const void* logits, int64_t ld, int64_t groups, int64_t beam
                     int64_t num, float* out_scores, int64_t* out_parents, int64_t* out_tokens,
                     void* workspace, size_t workspace_bytes, void* stream);
 
+/* The rows of a cache's batch that go on from others, as beams do: new row c continues old row
+ * parents[c] (outside 0 .. rows: nothing, it is empty).  Old row r holds seq_lens[r] tokens in the
+ * blocks of block_tables [rows][table_ld]; rows may share blocks that are full, a begun one is
+ * one row's alone.  The call shares a parent's full blocks among its children, leaves its begun
+ * block to the first of them and gives each other one a block of its own; blocks that no new row
+ * holds are free again.  Results:
+ *   tables_out [children][table_width]   -1 behind a row's blocks;  seq_lens_out [children]
+ *   sources, targets [children]   the copies that begun blocks need, in every layer's cache
+ *                                 (ojx_kv8_copy_blocks); -1 for none
+ *   free_out [num_blocks], num_free_out [1]   the stack: the old one (a negative num_free is an
+ *       empty one), freed blocks by rising number on top of it, less the blocks taken, by rising
+ *       child from the top; -1 above.  Negative: so many blocks were missing, the last children's
+ *       targets and entries are -1 and what their begun blocks held is lost to them.
+ * All rows that share a block have to be in one call: what other tables hold is not known to it.
+ * Nothing is written in place, so a call may be repeated; no output overlaps an input. */
+int ojx_kv8_reorder_workspace_bytes(int64_t rows, int64_t children, int64_t table_width,
+                                    int64_t block_size, int64_t num_blocks, size_t* bytes);
+int ojx_kv8_reorder(const int64_t* parents, int64_t children, const int32_t* seq_lens, int64_t rows,
+                    const int32_t* block_tables, int64_t table_ld, int64_t table_width,
+                    const int32_t* free_blocks, int64_t free_capacity, const int32_t* num_free,
+                    int64_t block_size, int64_t num_blocks, int32_t* tables_out,
+                    int32_t* seq_lens_out, int32_t* free_out, int32_t* num_free_out,
+                    int32_t* sources, int32_t* targets, void* workspace, size_t workspace_bytes,
+                    void* stream);
+
+/* One layer's cache. */
+typedef struct ojx_kv8_storage {
+    int8_t* k_codes;
+    int8_t* v_codes;
+    float* scales;
+} ojx_kv8_storage;
+
+/* Copies blocks sources[i] to targets[i], codes and scales, in each of `layers` caches of one shape
+ * (host array, read before the call returns), up to 64 in a launch.  Pairs with a block outside the
+ * caches are skipped; no block may be a target twice, or a target and a source. */
+int ojx_kv8_copy_blocks(const ojx_kv8_storage* caches, int64_t layers, int64_t num_blocks,
+                        int64_t kv_heads, int64_t block_size, int64_t head_dim,
+                        const int32_t* sources, const int32_t* targets, int64_t n, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

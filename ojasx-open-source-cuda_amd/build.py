@@ -32,6 +32,7 @@ SOURCES = [
     "e8t_noalloc.hip",
     "e8t_lora.hip",
     "kv8_cache.hip",
+    "kv8_reorder.hip",
     "kv8_attention.hip",
     "token_logprobs.hip",
     "rotary.hip",

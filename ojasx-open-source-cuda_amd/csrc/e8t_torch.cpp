@@ -517,6 +517,82 @@ PyObject* kv8_plan(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// kv8_reorder(parents, seq_lens, tables, free, num_free, block_size, num_blocks): the op's results
+PyObject* kv8_reorder(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 7, "kv8_reorder");
+    const Args a{argv, n};
+    if (!all_plain(argv, 5)) Py_RETURN_NONE;
+    const Tensor &parents = a.t(0), &seq = a.t(1), &tables = a.t(2), &free = a.t(3), &left = a.t(4);
+    const int64_t block = a.i64(5), blocks = a.i64(6), r = seq.numel(), c = parents.numel();
+    if (!ints(parents, at::kLong, c) || !ints(seq, at::kInt, r) ||
+        !ints(free, at::kInt, free.numel()) || !ints(left, at::kInt, 1) ||
+        tables.scalar_type() != at::kInt || tables.dim() != 2 || tables.size(0) != r ||
+        (tables.numel() > 0 && tables.stride(1) != 1) || !kv_block(block) || blocks < 0 ||
+        parents.device() != seq.device() || tables.device() != seq.device() ||
+        free.device() != seq.device() || left.device() != seq.device())
+        Py_RETURN_NONE;
+    RECORD_FUNCTION("ojasx_e8t::kv8_reorder", std::vector<c10::IValue>());
+    Unlocked unlocked;
+    const c10::DeviceGuard on_device(seq.device());
+    const int64_t w = tables.size(1);
+    Results all(Results::room(c * w, 4) + 3 * Results::room(c, 4),
+                Results::room(blocks, 4) + Results::room(1, 4), seq);
+    Tensor out[6];
+    out[0] = all.next({c, w}, at::kInt);
+    for (int i : {1, 4, 5}) out[i] = all.next({c}, at::kInt);
+    all.second();
+    out[2] = all.next({blocks}, at::kInt);
+    out[3] = all.next({1}, at::kInt);
+    size_t bytes = 0;
+    check(ojx_kv8_reorder_workspace_bytes(r, c, w, block, blocks, &bytes),
+          "kv8_reorder_workspace_bytes");
+    const Tensor ws = workspace(bytes, seq);
+    check(ojx_kv8_reorder((const int64_t*)data(parents), c, (const int32_t*)data(seq), r,
+                          (const int32_t*)data(tables), tables.stride(0), w,
+                          (const int32_t*)data(free), free.numel(), (const int32_t*)data(left), block,
+                          blocks, (int32_t*)data(out[0]), (int32_t*)data(out[1]),
+                          (int32_t*)data(out[2]), (int32_t*)data(out[3]), (int32_t*)data(out[4]),
+                          (int32_t*)data(out[5]), data(ws), bytes, current_stream(seq.device())),
+          "kv8_reorder");
+    unlocked.lock();
+    return tuple_of(out, 6);
+    END_HANDLE_TH_ERRORS
+}
+
+// kv8_copy_blocks(sources, targets, k_codes, v_codes, scales, k_codes, ...): True
+PyObject* kv8_copy_blocks(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n < 5 || (n - 2) % 3 != 0) Py_RETURN_NONE;
+    const Args a{argv, n};
+    if (!all_plain(argv, (int)n)) Py_RETURN_NONE;
+    const Tensor &sources = a.t(0), &targets = a.t(1), &first = a.t(2);
+    const int64_t m = sources.numel(), layers = (n - 2) / 3;
+    if (!ints(sources, at::kInt, m) || !ints(targets, at::kInt, m) || first.dim() != 4 ||
+        sources.device() != first.device() || targets.device() != first.device())
+        Py_RETURN_NONE;
+    std::vector<ojx_kv8_storage> caches;
+    caches.reserve(layers);
+    for (int i = 2; i < n; i += 3) {
+        const Tensor &k = a.t(i), &v = a.t(i + 1), &s = a.t(i + 2);
+        if (!cache_ok(k, v, s, first.size(3)) || k.sizes() != first.sizes() ||
+            k.device() != first.device())
+            Py_RETURN_NONE;
+        caches.push_back({(int8_t*)data(k), (int8_t*)data(v), (float*)data(s)});
+    }
+    RECORD_FUNCTION("ojasx_e8t::kv8_copy_blocks", std::vector<c10::IValue>());
+    Unlocked unlocked;
+    const c10::DeviceGuard on_device(first.device());
+    check(ojx_kv8_copy_blocks(caches.data(), layers, first.size(0), first.size(1), first.size(2),
+                              first.size(3), (const int32_t*)data(sources),
+                              (const int32_t*)data(targets), m, current_stream(first.device())),
+          "kv8_copy_blocks");
+    for (int i = 2; i < n; ++i) torch::autograd::impl::bump_version(a.t(i));
+    unlocked.lock();
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
 // kv8_append(k, v, slots, k_codes, v_codes, scales): True
 PyObject* kv8_append(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -1035,6 +1111,8 @@ PyMethodDef kMethods[] = {
     {"encode", (PyCFunction)(void*)encode, METH_FASTCALL, nullptr},
     {"decode", (PyCFunction)(void*)decode, METH_FASTCALL, nullptr},
     {"kv8_plan", (PyCFunction)(void*)kv8_plan, METH_FASTCALL, nullptr},
+    {"kv8_reorder", (PyCFunction)(void*)kv8_reorder, METH_FASTCALL, nullptr},
+    {"kv8_copy_blocks", (PyCFunction)(void*)kv8_copy_blocks, METH_FASTCALL, nullptr},
     {"kv8_append", (PyCFunction)(void*)kv8_append, METH_FASTCALL, nullptr},
     {"kv8_read", (PyCFunction)(void*)kv8_read, METH_FASTCALL, nullptr},
     {"kv8_attention", (PyCFunction)(void*)kv8_attention, METH_FASTCALL, nullptr},

@@ -1,5 +1,5 @@
-// serve.h -- arguments and launchers of the 8-bit paged cache (kv8_cache.hip), its attention
-// (kv8_attention.hip), token log probabilities (token_logprobs.hip), rotated positions (rotary.hip)
+// serve.h -- arguments and launchers of the 8-bit paged cache (kv8_cache.hip, kv8_reorder.hip), its
+// attention (kv8_attention.hip), token log probabilities (token_logprobs.hip), rotated positions (rotary.hip)
 // and the selection of beams (beam_select.hip).
 #pragma once
 
@@ -118,6 +118,44 @@ struct PlanArgs {
     int tokens;
 };
 
+// Old rows and their children; a stack of as many entries as blocks goes out.
+struct ReorderArgs {
+    const int64_t* parents;
+    const int32_t* seq_lens;
+    const int32_t* tables;
+    const int32_t* free_blocks;
+    const int32_t* num_free;
+    int32_t* tables_out;  // [children][width]
+    int32_t* seq_lens_out;
+    int32_t* free_out;  // [blocks]
+    int32_t* num_free_out;
+    int32_t* sources;
+    int32_t* targets;
+    int64_t table_ld;
+    int rows;
+    int children;
+    int width;
+    int capacity;
+    int log_block;
+    int blocks;
+};
+
+constexpr int kCopyLayers = 64;  // of a launch
+
+struct CopyArgs {
+    int8_t* k[kCopyLayers];
+    int8_t* v[kCopyLayers];
+    float* s[kCopyLayers];
+    const int32_t* sources;
+    const int32_t* targets;
+    int64_t bytes;  // of a block's keys
+    int rows;
+    int blocks;
+    int layers;
+    int scales;  // floats of a block
+    int pieces;  // of launch_kv8_copy: of a block's keys and values
+};
+
 struct AttnShape {
     int tokens;
     int requests;
@@ -226,6 +264,9 @@ hipError_t launch_kv8_rotate_append(const KvCache& c, const KvRows& k, const KvR
                                     const int64_t* slots, RotaryArgs q, hipStream_t stream);
 hipError_t launch_kv8_read(const KvCache& c, const int32_t* blocks, int n, int dtype, void* k_out,
                            void* v_out, float* scales_out, hipStream_t stream);
+size_t kv8_reorder_bytes(const ReorderArgs& a);
+hipError_t launch_kv8_reorder(const ReorderArgs& a, void* ws, hipStream_t stream);
+hipError_t launch_kv8_copy(CopyArgs a, hipStream_t stream);
 size_t kv8_attention_bytes(const AttnShape& s);
 hipError_t launch_kv8_attention(const AttnArgs& a, void* ws, size_t ws_bytes, hipStream_t stream);
 size_t token_logprobs_bytes(int rows, int vocab, int top, int dtype);

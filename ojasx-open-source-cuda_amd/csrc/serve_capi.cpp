@@ -5,6 +5,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -124,6 +125,32 @@ ojx::BeamArgs beams_of(int64_t groups, int64_t beams, int64_t vocab, int64_t num
     a.vocab = (int)vocab;
     a.num = (int)num;
     a.dtype = dtype;
+    return a;
+}
+
+bool valid_block(int64_t b) { return b == 16 || b == 32 || b == 64 || b == 128 || b == 256; }
+
+int check_reorder(int64_t rows, int64_t children, int64_t table_width, int64_t block_size,
+                  int64_t num_blocks) {
+    if (rows < 0 || rows > kMaxCount || children < 0 || children > kMaxCount || table_width < 0 ||
+        table_width > kMaxCount || num_blocks < 0 || num_blocks > kMaxCount)
+        return api_failf(OJX_EINVAL, "%lld rows, %lld children, %lld table columns, %lld blocks",
+                        (long long)rows, (long long)children, (long long)table_width,
+                        (long long)num_blocks);
+    if (!valid_block(block_size))
+        return api_failf(OJX_ELAYOUT, "block_size must be 16, 32, 64, 128 or 256 (got %lld)",
+                        (long long)block_size);
+    return OJX_OK;
+}
+
+ojx::ReorderArgs reorder_of(int64_t rows, int64_t children, int64_t table_width,
+                            int64_t block_size, int64_t num_blocks) {
+    ojx::ReorderArgs a{};
+    a.rows = (int)rows;
+    a.children = (int)children;
+    a.width = (int)table_width;
+    a.log_block = __builtin_ctzll((unsigned long long)block_size);
+    a.blocks = (int)num_blocks;
     return a;
 }
 
@@ -451,6 +478,92 @@ OJX_API int ojx_token_logprobs_bwd(const void* logits, int64_t ld, int64_t rows,
     a.gx = grad_logits;
     return ojx::api_done(ojx::launch_token_logprobs_bwd(a, (hipStream_t)stream),
                          "token_logprobs_bwd launch");
+}
+
+OJX_API int ojx_kv8_reorder_workspace_bytes(int64_t rows, int64_t children, int64_t table_width,
+                                            int64_t block_size, int64_t num_blocks,
+                                            size_t* bytes) {
+    if (!bytes) return api_failf(OJX_EINVAL, "null pointer");
+    *bytes = 0;
+    if (int r = check_reorder(rows, children, table_width, block_size, num_blocks)) return r;
+    *bytes = ojx::kv8_reorder_bytes(reorder_of(rows, children, table_width, block_size, num_blocks));
+    return OJX_OK;
+}
+
+OJX_API int ojx_kv8_reorder(const int64_t* parents, int64_t children, const int32_t* seq_lens,
+                            int64_t rows, const int32_t* block_tables, int64_t table_ld,
+                            int64_t table_width, const int32_t* free_blocks, int64_t free_capacity,
+                            const int32_t* num_free, int64_t block_size, int64_t num_blocks,
+                            int32_t* tables_out, int32_t* seq_lens_out, int32_t* free_out,
+                            int32_t* num_free_out, int32_t* sources, int32_t* targets,
+                            void* workspace, size_t workspace_bytes, void* stream) {
+    if (int r = check_reorder(rows, children, table_width, block_size, num_blocks)) return r;
+    if (free_capacity < 0 || free_capacity > kMaxCount || (table_ld < table_width && rows > 1))
+        return api_failf(OJX_EINVAL, "%lld free blocks, table stride %lld of %lld columns",
+                        (long long)free_capacity, (long long)table_ld, (long long)table_width);
+    if (int r = check_workspace(workspace, workspace_bytes)) return r;
+    if (!num_free || !num_free_out || (free_capacity > 0 && !free_blocks) ||
+        (num_blocks > 0 && !free_out) ||
+        (rows > 0 && (!seq_lens || (table_width > 0 && !block_tables))) ||
+        (children > 0 && (!parents || !seq_lens_out || !sources || !targets ||
+                          (table_width > 0 && !tables_out))))
+        return api_failf(OJX_EINVAL, "null pointer");
+    ojx::ReorderArgs a = reorder_of(rows, children, table_width, block_size, num_blocks);
+    if (workspace_bytes < ojx::kv8_reorder_bytes(a))
+        return api_failf(OJX_EINVAL, "workspace of %zu bytes, %zu are needed", workspace_bytes,
+                        ojx::kv8_reorder_bytes(a));
+    if (int r = ojx::api_check_device()) return r;
+    a.parents = parents;
+    a.seq_lens = seq_lens;
+    a.tables = block_tables;
+    a.table_ld = table_ld;
+    a.free_blocks = free_blocks;
+    a.capacity = (int)free_capacity;
+    a.num_free = num_free;
+    a.tables_out = tables_out;
+    a.seq_lens_out = seq_lens_out;
+    a.free_out = free_out;
+    a.num_free_out = num_free_out;
+    a.sources = sources;
+    a.targets = targets;
+    return ojx::api_done(ojx::launch_kv8_reorder(a, workspace, (hipStream_t)stream),
+                         "kv8 reorder launch");
+}
+
+OJX_API int ojx_kv8_copy_blocks(const ojx_kv8_storage* caches, int64_t layers, int64_t num_blocks,
+                                int64_t kv_heads, int64_t block_size, int64_t head_dim,
+                                const int32_t* sources, const int32_t* targets, int64_t n,
+                                void* stream) {
+    if (layers < 0 || layers > kMaxCount || n < 0 || n > kMaxCount)
+        return api_failf(OJX_EINVAL, "%lld caches, %lld copies", (long long)layers, (long long)n);
+    if (layers > 0 && !caches) return api_failf(OJX_EINVAL, "null pointer");
+    for (int64_t i = 0; i < layers; ++i)
+        if (int r = check_cache(caches[i].k_codes, caches[i].v_codes, caches[i].scales, num_blocks,
+                                kv_heads, block_size, head_dim))
+            return r;
+    if (layers == 0 || n == 0 || num_blocks == 0) return OJX_OK;
+    if (!sources || !targets) return api_failf(OJX_EINVAL, "null pointer");
+    if (int r = ojx::api_check_device()) return r;
+    const ojx::KvCache c = cache_of(caches[0].k_codes, caches[0].v_codes, caches[0].scales,
+                                    num_blocks, kv_heads, block_size, head_dim);
+    ojx::CopyArgs a{};
+    a.sources = sources;
+    a.targets = targets;
+    a.bytes = c.at(1, 0);
+    a.rows = (int)n;
+    a.blocks = c.blocks;
+    a.scales = 2 * c.heads;
+    hipError_t e = hipSuccess;
+    for (int64_t l = 0; l < layers && e == hipSuccess; l += a.layers) {
+        a.layers = (int)std::min<int64_t>(layers - l, ojx::kCopyLayers);
+        for (int i = 0; i < a.layers; ++i) {
+            a.k[i] = caches[l + i].k_codes;
+            a.v[i] = caches[l + i].v_codes;
+            a.s[i] = caches[l + i].scales;
+        }
+        e = ojx::launch_kv8_copy(a, (hipStream_t)stream);
+    }
+    return ojx::api_done(e, "kv8 copy_blocks launch");
 }
 
 OJX_API int ojx_beam_select_workspace_bytes(int64_t groups, int64_t beams, int64_t vocab,

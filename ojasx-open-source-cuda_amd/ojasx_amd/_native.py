@@ -66,6 +66,9 @@ EXPORTS = (
     "ojx_kv8_rotate_append",
     "ojx_beam_select_workspace_bytes",
     "ojx_beam_select",
+    "ojx_kv8_reorder_workspace_bytes",
+    "ojx_kv8_reorder",
+    "ojx_kv8_copy_blocks",
 )
 
 
@@ -104,6 +107,16 @@ class Rotation(ctypes.Structure):
         ("interleaved", ctypes.c_int32),
         ("gain", ctypes.c_float),
         ("inverse", ctypes.c_int32),
+    ]
+
+
+class KV8Storage(ctypes.Structure):
+    """ojx_kv8_storage of include/ojasx_e8t.h."""
+
+    _fields_ = [
+        ("k_codes", ctypes.c_void_p),
+        ("v_codes", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
     ]
 
 
@@ -237,6 +250,10 @@ def lib() -> ctypes.CDLL:
                     ("ojx_rotary", [_P, _P, _I64, _I64, _I64, _INT, _P, _I64, _I64, _P]),
                     ("ojx_kv8_rotate_append", [_P, _P, _P] + [_I64] * 4
                      + [_P, _I64, _I64, _P, _I64, _I64, _INT, _P, _I64, _P, _P, _P]),
+                    ("ojx_kv8_reorder_workspace_bytes", [_I64] * 5 + [_P]),
+                    ("ojx_kv8_reorder", [_P, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _I64]
+                     + [_P] * 7 + [_SZ, _P]),
+                    ("ojx_kv8_copy_blocks", [_P] + [_I64] * 5 + [_P, _P, _I64, _P]),
                     ("ojx_beam_select_workspace_bytes", [_I64] * 4 + [_INT, _P]),
                     ("ojx_beam_select", [_P] + [_I64] * 4 + [_INT, _P, _P, _I64, _I64, _P, _P, _P,
                                                              _P, _SZ, _P])):

@@ -9,14 +9,19 @@ Keys and values are held as int8 codes with one float32 scale for each block of 
     o = cache.attention(q, block_tables, p.seq_lens, p.query_starts)
 
 ``plan`` runs on the GPU from the requests' lengths alone, so a step needs no copy to the host;
-``KV8Cache`` is one layer's storage.  The functions take the storage's tensors, for callers that
+``KV8Cache`` is one layer's storage.  Requests that go on from others (beams, several answers to one
+prompt) or are done share and give back blocks:
+
+    r = kv8.reorder(parents, seq_lens, block_tables, free_blocks, num_free, block_size, num_blocks)
+    kv8.copy_blocks(caches, r.sources, r.targets)    # what begun blocks hold, in all layers
+  The functions take the storage's tensors, for callers that
 keep them in tensors of their own.
 """
 
 from __future__ import annotations
 
 import math
-from typing import NamedTuple, Optional, Tuple, Union
+from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -57,6 +62,46 @@ def plan(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torch.Ten
     """
     args = (seq_lens, new_lens, block_tables, free_blocks, num_free, block_size, num_tokens)
     return KV8Plan(*(_eager("kv8_plan", *args) or S.kv8_plan(*args)))
+
+
+class KV8Reorder(NamedTuple):
+    """A batch after ``reorder``.  The results may share allocations (see ``KV8Plan``)."""
+
+    block_tables: torch.Tensor  # int32 [new rows, blocks], -1 behind a row's blocks
+    seq_lens: torch.Tensor      # int32 [new rows]
+    free_blocks: torch.Tensor   # int32 [num_blocks], -1 from num_free on
+    num_free: torch.Tensor      # int32 [1]; negative: so many blocks were missing
+    sources: torch.Tensor       # int32 [new rows]: begun blocks to be copied, -1 for none
+    targets: torch.Tensor       # int32 [new rows]: where to
+
+
+def reorder(parents: torch.Tensor, seq_lens: torch.Tensor, block_tables: torch.Tensor,
+            free_blocks: torch.Tensor, num_free: torch.Tensor, block_size: int, num_blocks: int
+            ) -> KV8Reorder:
+    """The batch whose row i goes on from row ``parents[i]`` (int64; -1: an empty row) of this one.
+
+    There may be more or fewer rows than before: ``[0, 0, 0, 0]`` makes four beams of a prompt.
+    Children of a row share its full blocks.  Its begun block stays with the first of them, the
+    others get one each from the stack: ``copy_blocks`` copies what it holds, in all layers, before
+    the next append.  Blocks that no new row holds go back on the stack, before any is taken.
+
+    All rows that share a block have to be in one call, since blocks are freed by what its rows
+    hold; a begun block is held by one row alone, as this and ``plan`` leave it.  Nothing is written
+    in place.  The stack returned has room for all ``num_blocks``.
+    """
+    args = (parents, seq_lens, block_tables, free_blocks, num_free, block_size, num_blocks)
+    return KV8Reorder(*(_eager("kv8_reorder", *args) or S.kv8_reorder(*args)))
+
+
+def copy_blocks(caches: Sequence, sources: torch.Tensor, targets: torch.Tensor) -> None:
+    """Copies blocks ``sources[i]`` to ``targets[i]`` in every one of ``caches``: ``KV8Cache`` objects,
+    or triples of their tensors, all of one shape.  Pairs with a block outside the cache (-1) are
+    skipped.  No block may be a target twice, or a target and a source."""
+    parts = [(c.k_codes, c.v_codes, c.scales) if isinstance(c, KV8Cache) else tuple(c) for c in caches]
+    if any(len(p) != 3 for p in parts):
+        raise RuntimeError("a cache is a KV8Cache or its three tensors")
+    if _eager("kv8_copy_blocks", sources, targets, *(t for p in parts for t in p)) is None:
+        S.kv8_copy_blocks(*([p[i] for p in parts] for i in range(3)), sources, targets)
 
 
 def append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_codes: torch.Tensor,

@@ -4,7 +4,8 @@ beam search.
 
 ``kv8_plan``, ``kv8_append`` (a block's tokens in one run of its slots) and ``kv8_read`` move a
 step's tokens into the cache and blocks out of it (``kv8_rotate_append`` with positions rotated into
-keys and queries on the way), ``kv8_attention`` reads it,
+keys and queries on the way), ``kv8_reorder`` and ``kv8_copy_blocks`` let requests go on from others,
+``kv8_attention`` reads it,
 ``token_logprobs`` (autograd registered, with ``token_logprobs_bwd``) is what a model answers and
 trains with; ``rotary`` (its own gradient, turned back) rotates queries and keys; ``beam_select`` chooses the beams
 that go on.  The reference keeps no quantized cache; the layouts and rules are those of ``include/ojasx_e8t.h``.  As for the other
@@ -15,7 +16,7 @@ allocator, ``RuntimeError`` for what does not fit, no fallback.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 
@@ -208,6 +209,80 @@ def kv8_rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
 @kv8_rotate_append.register_fake
 def _(q, k, v, positions, slots, rates, gain, interleaved, k_codes, v_codes, scales):
     return torch.empty_like(_rotary_input(q))
+
+
+# ----------------------------------------------------------------------------- reorder
+
+@torch.library.custom_op(f"{_NS}::kv8_reorder", mutates_args=())
+def kv8_reorder(parents: torch.Tensor, seq_lens: torch.Tensor, block_tables: torch.Tensor,
+                free_blocks: torch.Tensor, num_free: torch.Tensor, block_size: int, num_blocks: int
+                ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
+                           torch.Tensor]:
+    """(tables, lengths, stack, its size, sources, targets) of the rows that continue `parents`."""
+    dev = N.require_device(parents, seq_lens, block_tables, free_blocks, num_free)
+    r, c = seq_lens.numel(), parents.numel()
+    par = _ints("parents", parents, torch.int64, (c,))
+    seq = _ints("seq_lens", seq_lens, torch.int32, (r,))
+    free = _ints("free_blocks", free_blocks, torch.int32, (free_blocks.numel(),))
+    nf = _ints("num_free", num_free, torch.int32, (1,))
+    tables = _table(block_tables, r)
+    if tables.numel() and tables.stride(1) != 1:
+        tables = tables.contiguous()
+    _check_block_size(block_size)
+    if num_blocks < 0:
+        raise RuntimeError(f"num_blocks is {num_blocks}")
+    i32 = dict(dtype=torch.int32, device=dev)
+    w = tables.shape[1]
+    out = (torch.empty((c, w), **i32), torch.empty(c, **i32), torch.empty(num_blocks, **i32),
+           torch.empty(1, **i32), torch.empty(c, **i32), torch.empty(c, **i32))
+    with torch.cuda.device(dev):
+        nbytes = ctypes.c_size_t(0)
+        N.check(N.lib().ojx_kv8_reorder_workspace_bytes(r, c, w, block_size, num_blocks,
+                                                        ctypes.byref(nbytes)),
+                "kv8_reorder_workspace_bytes")
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev) if nbytes.value else None
+        N.check(N.lib().ojx_kv8_reorder(
+            N.ptr(par), c, N.ptr(seq), r, N.ptr(tables), tables.stride(0), w, N.ptr(free),
+            free.numel(), N.ptr(nf), block_size, num_blocks, *(N.ptr(t) for t in out), N.ptr(ws),
+            nbytes.value, N.stream_handle(dev)), "kv8_reorder")
+    return out
+
+
+@kv8_reorder.register_fake
+def _(parents, seq_lens, block_tables, free_blocks, num_free, block_size, num_blocks):
+    c = parents.numel()
+    return (block_tables.new_empty((c, block_tables.shape[1])), seq_lens.new_empty(c),
+            seq_lens.new_empty(num_blocks), seq_lens.new_empty(1), seq_lens.new_empty(c),
+            seq_lens.new_empty(c))
+
+
+@torch.library.custom_op(f"{_NS}::kv8_copy_blocks", mutates_args=("k_codes", "v_codes", "scales"))
+def kv8_copy_blocks(k_codes: List[torch.Tensor], v_codes: List[torch.Tensor],
+                    scales: List[torch.Tensor], sources: torch.Tensor, targets: torch.Tensor
+                    ) -> None:
+    dev = N.require_device(*k_codes, *v_codes, *scales, sources, targets)
+    n = sources.numel()
+    src, dst = _ints("sources", sources, torch.int32, (n,)), _ints("targets", targets, torch.int32, (n,))
+    if not len(k_codes) == len(v_codes) == len(scales):
+        raise RuntimeError(f"{len(k_codes)}, {len(v_codes)} and {len(scales)} tensors of caches")
+    if not k_codes:
+        return
+    for k, v, s in zip(k_codes, v_codes, scales):
+        if k.shape != k_codes[0].shape:
+            raise RuntimeError(f"caches of one call must be of one shape (got {list(k.shape)} and "
+                               f"{list(k_codes[0].shape)})")
+        blocks, heads, block_size = _check_cache(k, v, s, k.shape[-1])
+    caches = (N.KV8Storage * len(k_codes))(*((N.ptr(k), N.ptr(v), N.ptr(s))
+                                             for k, v, s in zip(k_codes, v_codes, scales)))
+    with torch.cuda.device(dev):
+        N.check(N.lib().ojx_kv8_copy_blocks(
+            caches, len(k_codes), blocks, heads, block_size, k_codes[0].shape[-1], N.ptr(src),
+            N.ptr(dst), n, N.stream_handle(dev)), "kv8_copy_blocks")
+
+
+@kv8_copy_blocks.register_fake
+def _(k_codes, v_codes, scales, sources, targets):
+    return None
 
 
 # ----------------------------------------------------------------------------- attention
