@@ -5,8 +5,9 @@
 Random weights, synthetic prompts of different lengths.  One batch goes through every operator
 as a serving loop uses them: the cache's plan, append and attention in each step (a step holds
 prompts, single tokens, or both), the prompts' own log probabilities, the most likely next token
-with its log probability, and at the end a few steps of policy training of the head's adapter on
-the answers.  No step waits for the GPU: lengths, tables and tokens stay there.
+with its log probability, a few steps of policy training of the head's adapter on the answers, and at
+the end the prompts again by beam search, whose beams share their blocks and whose positions are
+rotated on the way into the cache.  No step waits for the GPU: lengths, tables and tokens stay there.
 """
 
 from __future__ import annotations
@@ -19,7 +20,8 @@ import torch.nn.functional as F
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
-from ojasx_amd import E8LatticeLinear, KV8Cache, kv8, token_logprobs  # noqa: E402
+from ojasx_amd import (E8LatticeLinear, KV8Cache, beam_select, kv8, rotary,  # noqa: E402
+                       token_logprobs)
 
 
 class Requests:
@@ -38,6 +40,14 @@ class Requests:
                         self.block_size, num_tokens)
         self.lens, self.num_free = plan.seq_lens, plan.num_free
         return plan
+
+    def go_on(self, parents: torch.Tensor, num_blocks: int, caches) -> None:
+        """The batch becomes the rows `parents` of it (-1: none), each with a cache of its own to
+        append to."""
+        r = kv8.reorder(parents, self.lens, self.tables, self.free, self.num_free, self.block_size,
+                        num_blocks)
+        kv8.copy_blocks(caches, r.sources, r.targets)
+        self.tables, self.lens, self.free, self.num_free = r[:4]
 
 
 class Decoder:
@@ -61,6 +71,7 @@ class Decoder:
         self.down = [linear(4 * hidden, hidden) for _ in range(layers)]
         self.head = linear(hidden, vocabulary, rank=8)
         self.rates = 10000.0 ** (-torch.arange(0, head_dim, 2, device=device) / head_dim)
+        self.rotation = rotary.rotation(head_dim, 10000.0, device=device)
 
     def caches(self, num_blocks, block_size):
         return [KV8Cache(num_blocks, self.kv_heads, self.head_dim, block_size,
@@ -71,15 +82,19 @@ class Decoder:
         lo, hi = x.float().chunk(2, dim=-1)
         return torch.cat([lo * a.cos() - hi * a.sin(), hi * a.cos() + lo * a.sin()], -1).to(x.dtype)
 
-    def hidden(self, tokens, plan, tables, caches, **longest):
-        """The tokens' last hidden states; their keys and values go into the caches."""
+    def hidden(self, tokens, plan, tables, caches, rotate_on_append=False, **longest):
+        """The tokens' last hidden states; their keys and values go into the caches, rotated before
+        or on the way (then without a rounding between)."""
         x, t = self.embedding[tokens], len(tokens)
         q_size, kv_size = self.heads * self.head_dim, self.kv_heads * self.head_dim
         for i, cache in enumerate(caches):
             q, k, v = self.qkv[i](F.rms_norm(x, x.shape[-1:])).split([q_size, kv_size, kv_size], -1)
-            q = self.rotate(q.reshape(t, self.heads, -1), plan.positions)
-            k = self.rotate(k.reshape(t, self.kv_heads, -1), plan.positions)
-            cache.append(k, v.reshape(t, self.kv_heads, -1), plan.slots)
+            q, k, v = (y.unflatten(-1, (-1, self.head_dim)) for y in (q, k, v))
+            if rotate_on_append:
+                q = cache.rotate_append(q, k, v, plan.positions, plan.slots, self.rotation)
+            else:
+                q, k = self.rotate(q, plan.positions), self.rotate(k, plan.positions)
+                cache.append(k, v, plan.slots)
             o = cache.attention(q, tables, plan.seq_lens, plan.query_starts, **longest)
             x = x + self.out[i](o.reshape(t, -1))
             x = x + self.down[i](F.silu(self.up[i](F.rms_norm(x, x.shape[-1:]))))
@@ -119,6 +134,41 @@ def answer(model: Decoder, prompts, new_tokens: int, num_blocks=64, block_size=1
             torch.stack(states, 1), batch, caches)
 
 
+@torch.no_grad()
+def beam_answer(model: Decoder, prompts, beams: int, new_tokens: int, end: int, num_blocks=256,
+                block_size=16, watch=None):
+    """The best answers of ``new_tokens`` tokens, less behind the token ``end``, by beam search.
+
+    Returns (tokens [requests, beams, new], their log probabilities [requests, beams], the requests,
+    the caches).  ``watch`` is called with each step's logits, scores, finished beams and choice."""
+    device, n = model.embedding.device, len(prompts)
+    lens = [len(p) for p in prompts]
+    batch = Requests(n, max(lens) + new_tokens, num_blocks, block_size, device)
+    caches = model.caches(num_blocks, block_size)
+    tokens = torch.tensor([t for p in prompts for t in p], device=device)
+    plan = batch.step(torch.tensor(lens, dtype=torch.int32, device=device), len(tokens))
+    h = model.hidden(tokens, plan, batch.tables, caches, True, max_query_len=max(lens),
+                     max_seq_len=max(lens))[plan.query_starts[1:].long() - 1]
+    scores = torch.zeros(n, 1, device=device)
+    done = torch.zeros(n, 1, dtype=torch.bool, device=device)
+    answers = torch.zeros(n, 0, dtype=torch.int64, device=device)
+    one = torch.ones(n * beams, dtype=torch.int32, device=device)
+    for i in range(new_tokens):
+        logits = model.head(h).unflatten(0, scores.shape)
+        best = beam_select(logits, scores, beams, finished=done, pad_id=end)
+        if watch is not None:
+            watch(logits, scores, done, best)
+        rows, scores = best.parents.flatten(), best.scores
+        done = done.flatten()[best.parents] | (best.tokens == end)
+        answers = torch.cat([answers[rows], best.tokens.flatten()[:, None]], 1)
+        batch.go_on(rows, num_blocks, caches)
+        if i + 1 < new_tokens:
+            plan = batch.step(one, n * beams)
+            h = model.hidden(answers[:, -1], plan, batch.tables, caches, True, max_query_len=1,
+                             max_seq_len=max(lens) + i + 1)
+    return answers.unflatten(0, (n, beams)), scores, batch, caches
+
+
 def reinforce(model: Decoder, states, tokens, old_logprobs, rewards, steps=4, rate=1e-2,
               entropy_weight=1e-3):
     """Policy steps on the head's adapter: a clipped ratio of each token's probability now to
@@ -151,6 +201,11 @@ def main() -> None:
     rewards = (tokens % 2 == 0).float().mean(1)
     print("losses", [round(v, 5) for v in reinforce(model, states, tokens, logprobs,
                                                     rewards).tolist()])
+    answers, scores, batch, caches = beam_answer(model, prompts, 4, 12, end=7)
+    print("best of four beams", answers[:, 0, :8].tolist())
+    print("their log probabilities", [round(v, 3) for v in scores[:, 0].tolist()])
+    batch.go_on(torch.full((16,), -1, device=tokens.device), 256, caches)
+    print("blocks given back", batch.num_free.item())
 
 
 if __name__ == "__main__":
