@@ -39,14 +39,36 @@ __device__ __forceinline__ double scaled(double s, float r, float to) {
     return ldexp(s, (int)fmaxf(r - to, -2000.f));
 }
 
+constexpr int kSlots = 16;        // maxima that a lane keeps of the batches it has seen
+constexpr int kCandidates = 192;  // that a wave has room for
+
 // A workgroup reads a row or a part of it once; rows that do not matter not at all.  Four partial
 // sums of 8 terms a batch are held in 32 bits, everything beyond in 64: whole numbers (which beam)
 // hang on these sums, and the join has to settle in 64 bits what they leave open.
+//
+// Nothing is selected on the way, a lane only keeps its batches' maxima.  Of 64 shares of the part,
+// the num-th largest maximum is not over num logits at least, and few more than num are over it: the
+// batches of the few lanes that have one are read again.  Where there are too many (a row of few
+// values, a short one), the part is gone through once more batch by batch.
+//
+// 512 rows of 128256 bf16 (131 MB) take 39 us, 3.4 TB/s: about 5 us until all workgroups run and have
+// their first logits, and 6 for what follows a row's last one, around a stream at 4.9 TB/s (selecting
+// on the way, batch by batch, 51 us; the next batch's loads ahead, no change).
 template <int DT>
 __global__ __launch_bounds__(kThreads) void beam_pass_kernel(BeamArgs a, BeamParts p) {
-    __shared__ Pool pool[kGroups];
-    __shared__ uint64_t keys[kGroups * kTopMax];
+    __shared__ union {
+        struct {
+            float maxima[kSlots * kThreads];
+            uint64_t keys[kGroups][kCandidates];
+        } few;
+        struct {
+            Pool pool[kGroups];
+            uint64_t keys[kGroups * kTopMax];
+        } many;
+    } mem;
     __shared__ BeamSum sums[kGroups];
+    __shared__ float lanes[kThreads], columns[kGroups][64];
+    __shared__ int counts[kGroups];
     using B = Batch<DT>;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t row = blockIdx.x / (unsigned)p.splits;
@@ -57,13 +79,16 @@ __global__ __launch_bounds__(kThreads) void beam_pass_kernel(BeamArgs a, BeamPar
     const int shift = (int)((((uintptr_t)a.x + x0 * size) & 15) / size);
     const int batches = (int)(((int64_t)a.vocab + shift + kBatch - 1) / kBatch);
     const int per = (batches + p.splits - 1) / p.splits;
-    const int end = min(batches, (split + 1) * per);
+    const int first = split * per + wave, end = min(batches, (split + 1) * per);
+    // batches of this wave that share a slot
+    const int share = (per + kGroups * kSlots - 1) / (kGroups * kSlots);
     double sum = 0;
-    float ref = -INFINITY, most = -INFINITY;
-    Best best{0, -INFINITY};
+    float ref = -INFINITY, most = -INFINITY, slot = -INFINITY;
     B x;
-    for (int b = split * per + wave; b < end; b += kGroups) {
+    int s_at = 0, s_left = share, held = -1;
+    for (int b = first; b < end; b += kGroups) {
         x.load(a.x, x0, a.vocab, b, lane, shift);
+        held = b;
         float m = x.get(0);
 #pragma unroll
         for (int i = 1; i < kLaneLogits; ++i) m = or_nan(m, x.get(i));
@@ -71,22 +96,28 @@ __global__ __launch_bounds__(kThreads) void beam_pass_kernel(BeamArgs a, BeamPar
         const float base = r == -INFINITY ? 0.f : r;
         float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < kLaneLogits; ++i) s[i & 3] += __builtin_amdgcn_exp2f(term(x.get(i), base));
+        for (int i = 0; i < kLaneLogits; ++i)
+            s[i & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(x.get(i), kLog2e, -base));
         sum = scaled(sum, ref, base) + (((double)s[0] + s[1]) + ((double)s[2] + s[3]));
         ref = r;
         most = or_nan(most, m);
-        x.drop_floats();
-        take<DT>(best, x, m, b, a.num, lane, shift, pool[wave]);
+        slot = fmaxf(slot, m);
+        if (--s_left == 0 || b + kGroups >= end) {
+            mem.few.maxima[s_at * kThreads + threadIdx.x] = slot;
+            ++s_at, s_left = share, slot = -INFINITY;
+        }
     }
+    lanes[threadIdx.x] = most;
     // over the wave
     const bool bad = __any(most != most);
-    const float r = wave_max(ref), base = r == -INFINITY ? 0.f : r;
-    sum = scaled(sum, ref, base);
+    {
+        const float r = wave_max(ref), base = r == -INFINITY ? 0.f : r;
+        double t = scaled(sum, ref, base);
 #pragma unroll
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-    most = wave_max(most);
-    if (lane == 0) sums[wave] = BeamSum{sum, r, bad ? __uint_as_float(0x7FC00000u) : most};
-    if (lane < a.num) keys[wave * a.num + lane] = best.key;
+        for (int o = 32; o; o >>= 1) t += __shfl_xor(t, o);
+        const float m = wave_max(most);
+        if (lane == 0) sums[wave] = BeamSum{t, r, bad ? __uint_as_float(0x7FC00000u) : m};
+    }
     __syncthreads();
     const int64_t at = row * p.splits + split;
     if (threadIdx.x == 0) {
@@ -98,11 +129,82 @@ __global__ __launch_bounds__(kThreads) void beam_pass_kernel(BeamArgs a, BeamPar
         }
         p.sums[at] = t;
     }
-    for (int i = threadIdx.x; i < kGroups * a.num; i += kThreads) {
-        const uint64_t k = keys[i];
-        int rank = 0;
+    // the num-th largest of the shares' maxima: the least of those that fewer exceed
+    const float share_max = fmaxf(fmaxf(lanes[lane], lanes[lane + 64]),
+                                  fmaxf(lanes[lane + 128], lanes[lane + 192]));
+    columns[wave][lane] = share_max;
+    __builtin_amdgcn_wave_barrier();
+    int over = 0;
+#pragma unroll
+    for (int j = 0; j < 64; j += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(columns[wave] + j);
+        over += f.x > share_max;
+        over += f.y > share_max;
+        over += f.z > share_max;
+        over += f.w > share_max;
+    }
+    const float bound = -wave_max(over < a.num ? -share_max : -INFINITY);
+    int n = 0;
+    if (bound > -INFINITY) {
+        for (int s = 0; s < s_at; ++s) {
+            const bool mine = mem.few.maxima[s * kThreads + threadIdx.x] >= bound;
+            if (!__any(mine)) continue;
+            for (int i = 0; i < share; ++i) {
+                const int b = first + (s * share + i) * kGroups;
+                if (b >= end) break;
+                if (mine && b != held) {
+                    x.load(a.x, x0, a.vocab, b, lane, shift);
+                    held = b;
+                }
+#pragma unroll
+                for (int j = 0; j < kLaneLogits; ++j) {
+                    const float f = x.get(j);
+                    const uint64_t those = __ballot(mine && f >= bound);
+                    if (!those) continue;
+                    const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(those >> 32),
+                                                                 __builtin_amdgcn_mbcnt_lo((uint32_t)those, 0));
+                    if (mine && f >= bound && at < kCandidates)
+                        mem.few.keys[wave][at] = key_of(f, B::index(b, j, lane, shift));
+                    n += __popcll(those);
+                }
+            }
+        }
+    }
+    if (lane == 0) counts[wave] = n;
+    __syncthreads();
+    bool fits = bound > -INFINITY;
+    for (int w = 0; w < kGroups; ++w) fits &= counts[w] <= kCandidates;
+    if (!fits) {
+        Best best{0, -INFINITY};
+        for (int b = first; b < end; b += kGroups) {
+            x.load(a.x, x0, a.vocab, b, lane, shift);
+            float m = x.get(0);
+#pragma unroll
+            for (int i = 1; i < kLaneLogits; ++i) m = or_nan(m, x.get(i));
+            x.drop_floats();
+            take<DT>(best, x, m, b, a.num, lane, shift, mem.many.pool[wave]);
+        }
+        if (lane < a.num) mem.many.keys[wave * a.num + lane] = best.key;
+        __syncthreads();
+        for (int i = threadIdx.x; i < kGroups * a.num; i += kThreads) {
+            const uint64_t k = mem.many.keys[i];
+            int rank = 0;
 #pragma unroll 8
-        for (int j = 0; j < kGroups * a.num; ++j) rank += keys[j] > k || (keys[j] == k && j < i);
+            for (int j = 0; j < kGroups * a.num; ++j)
+                rank += mem.many.keys[j] > k || (mem.many.keys[j] == k && j < i);
+            if (rank < a.num) p.keys[at * a.num + rank] = k;
+        }
+        return;
+    }
+    // at least num of them, all different
+    for (int i = lane; i < n; i += 64) {
+        const uint64_t k = mem.few.keys[wave][i];
+        int rank = 0;
+        for (int w = 0; w < kGroups; ++w) {
+            const int m = counts[w];
+#pragma unroll 4
+            for (int j = 0; j < m; ++j) rank += mem.few.keys[w][j] > k;
+        }
         if (rank < a.num) p.keys[at * a.num + rank] = k;
     }
 }
@@ -142,7 +244,7 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, Bea
     extern __shared__ uint64_t lds[];
     __shared__ Beam beams[kBeamMax];
     __shared__ uint64_t top_value[kTopMax + 1];
-    __shared__ int top_at[kTopMax + 1];  // beam * num + place
+    __shared__ int top_beam[kTopMax + 1], top_token[kTopMax + 1];
     __shared__ double part[kJoinWaves];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n = p.splits * a.num, all = a.beams * a.num;
@@ -155,12 +257,13 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, Bea
         const int64_t row = row0 + b;
         const float score = a.scores[row];
         const bool ended = a.done && a.done[row];
+        // (of a row that does not matter these are not written, nor used)
+        BeamSum s{0.0, -INFINITY, -INFINITY};
+        if (lane < p.splits) s = p.sums[row * p.splits + lane];
+        for (int i = lane; i < n; i += 64) list[i] = p.keys[row * n + i];
         Beam t{0.0, 0.f, score, 0, true, false};
         bool nan = !(score < INFINITY);
-        if (reads_logits(a, row)) {
-            BeamSum s{0.0, -INFINITY, -INFINITY};
-            if (lane < p.splits) s = p.sums[row * p.splits + lane];
-            for (int i = lane; i < n; i += 64) list[i] = p.keys[row * n + i];
+        if (!ended && score < INFINITY && score > -INFINITY) {
             const float r = wave_max(s.r), base = r == -INFINITY ? 0.f : r;
             double sum = scaled(s.s, s.r, base);
 #pragma unroll
@@ -201,6 +304,9 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, Bea
     }
     __syncthreads();
 
+    // lanes for a candidate: a power of two of at most a wave, none without a list to look through
+    int team = 1;
+    while (team < 64 && 2 * team * all <= kJoinThreads && team < a.beams) team *= 2;
     int total = 0;
     for (int b = 0; b < a.beams; ++b) total += beams[b].count;
     for (;;) {
@@ -229,13 +335,14 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, Bea
             if (threadIdx.x == 0) beams[b].ls = ls, beams[b].exact = true, beams[b].need = false;
             __syncthreads();
         }
-        // a candidate's rank: those before it in its beam, and in the others' lists
-        for (int i = threadIdx.x; i < all; i += kJoinThreads) {
+        // a candidate's rank: those before it in its beam, and in the others' lists, which the lanes
+        // of a team share out
+        for (int i = (int)threadIdx.x / team; i < all; i += kJoinThreads / team) {
             const int b = i / a.num, place = i - b * a.num;
             if (place >= beams[b].count) continue;
             const uint64_t v = value[i];
-            int rank = place;
-            for (int o = 0; o < a.beams && rank <= a.num; ++o) {
+            int rank = 0;
+            for (int o = threadIdx.x & (team - 1); o < a.beams; o += team) {
                 if (o == b) continue;
                 // of an earlier beam equal ones come first
                 const uint64_t least = v + (o < b ? 0 : 1);
@@ -247,16 +354,19 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, Bea
                 }
                 rank += lo;
             }
-            if (rank <= a.num) {
+            for (int o = team >> 1; o; o >>= 1) rank += __shfl_xor(rank, o);
+            rank += place;
+            if (rank <= a.num && (threadIdx.x & (team - 1)) == 0) {
                 top_value[rank] = v;
-                top_at[rank] = i;
+                top_beam[rank] = b;
+                top_token[rank] = token[i];
             }
         }
         __syncthreads();
         const int last = min(total - 1, a.num);
         bool again = false;
         if ((int)threadIdx.x < last) {
-            const int i = threadIdx.x, b = top_at[i] / a.num, c = top_at[i + 1] / a.num;
+            const int i = threadIdx.x, b = top_beam[i], c = top_beam[i + 1];
             if (b != c && !(beams[b].exact && beams[c].exact) &&
                 unordered64(top_value[i]) - unordered64(top_value[i + 1]) < kNear) {
                 again = true;
@@ -270,10 +380,10 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, Bea
 
     const int64_t o0 = (int64_t)blockIdx.x * a.num;
     if ((int)threadIdx.x < min(total, a.num)) {
-        const int i = threadIdx.x, b = top_at[i] / a.num;
+        const int i = threadIdx.x;
         a.out_scores[o0 + i] = (float)unordered64(top_value[i]);
-        a.out_parents[o0 + i] = row0 + b;
-        a.out_tokens[o0 + i] = token[top_at[i]];
+        a.out_parents[o0 + i] = row0 + top_beam[i];
+        a.out_tokens[o0 + i] = top_token[i];
     }
     // Fewer than asked for: impossible ones follow, by rising beam and token.  Those possible are all
     // in the lists, so the first `num` others are among the group's first total + num.
@@ -301,12 +411,13 @@ size_t join_bytes(int splits, int beams, int num) {
     return (size_t)kJoinWaves * splits * num * 8 + (size_t)beams * num * 12;
 }
 
-// Parts of a row: until the workgroups fill the GPU twice, none under a batch for each wave, and
-// as many as the join has room for.
+// Parts of a row: until there are four workgroups for each CU, which run at once, none under a batch
+// for each wave, and as many as the join has room for (512 rows of 128256 whole 47.0 us, in two 45.2,
+// in four 49.7; 4 rows of 32000 whole 16.9, in four 12.6).
 int beam_splits(const BeamArgs& a) {
     const int64_t rows = (int64_t)a.groups * a.beams;
     const int64_t most = ((int64_t)a.vocab + kBatch * kGroups - 1) / (kBatch * kGroups);
-    int64_t n = rows > 0 ? 2048 / rows : 1;
+    int64_t n = rows > 0 ? 1024 / rows : 1;
     if (n > most) n = most;
     if (n > kMaxRowSplits) n = kMaxRowSplits;
     while (n > 1 && join_bytes((int)n, a.beams, a.num) > kJoinBytes) --n;
