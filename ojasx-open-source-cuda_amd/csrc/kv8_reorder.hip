@@ -14,12 +14,12 @@ constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
 constexpr int kNone = 0x7FFFFFFF;
 
-// What a call works on: the first child of every old row, and a bit for each block that a row with
+// Of a large call: the first child of every old row, and a byte for each block that a row with
 // children (live) or one without (dead) holds.
 struct Marks {
     int32_t* first;
-    uint32_t* live;
-    uint32_t* dead;
+    uint8_t* live;
+    uint8_t* dead;
 };
 
 __device__ __forceinline__ int parent_of(const ReorderArgs& a, int64_t child) {
@@ -37,37 +37,29 @@ __device__ __forceinline__ int used_of(const ReorderArgs& a, int len) {
     return (int)(n < a.width ? n : a.width);
 }
 
-// Column of a child's begun block that is to be its own, or -1: the first child keeps the parent's.
-__device__ __forceinline__ int copied_column(const ReorderArgs& a, const int32_t* first, int64_t child,
-                                             int parent, int len) {
+// Column of a child's begun block if it is to have one of its own (the first child keeps the
+// parent's), or -1; *block: the parent's.
+template <class First>
+__device__ __forceinline__ int copied_column(const ReorderArgs& a, int parent, int len, First is_first,
+                                             int* block) {
     const int64_t at = len >> a.log_block;
-    if (parent < 0 || (len & ((1 << a.log_block) - 1)) == 0 || at >= a.width || first[parent] == child)
-        return -1;
-    const int block = a.tables[parent * a.table_ld + at];
-    return block >= 0 && block < a.blocks ? (int)at : -1;
+    *block = -1;
+    if (parent < 0 || (len & ((1 << a.log_block) - 1)) == 0 || at >= a.width) return -1;
+    const int b = a.tables[parent * a.table_ld + at];
+    if (b < 0 || b >= a.blocks || is_first()) return -1;
+    *block = b;
+    return (int)at;
 }
 
-__device__ __forceinline__ void mark_row(const ReorderArgs& a, const Marks& m, int row, int lane,
-                                         int step) {
-    const int used = used_of(a, length_of(a, row));
-    uint32_t* bits = m.first[row] != kNone ? m.live : m.dead;
-    const int32_t* t = a.tables + row * a.table_ld;
-    for (int j = lane; j < used; j += step) {
-        const int b = t[j];
-        if (b < 0 || b >= a.blocks) continue;
-        // many rows share a block: a bit that is seen set needs no second time
-        if (!(bits[b >> 5] >> (b & 31) & 1)) atomicOr(bits + (b >> 5), 1u << (b & 31));
-    }
-}
-
-// A new row's entries and length; the entry that copied_column names is write_stack's.
-__device__ __forceinline__ void write_row(const ReorderArgs& a, const int32_t* first, int64_t child,
-                                          int lane, int step) {
+// A new row's entries and length, by a wave; the entry that copied_column names is write_stack's.
+template <class First>
+__device__ __forceinline__ void write_row(const ReorderArgs& a, int64_t child, int lane, First is_first) {
     const int p = parent_of(a, child), len = length_of(a, p), used = p < 0 ? 0 : used_of(a, len);
-    const int skip = copied_column(a, first, child, p, len);
+    int block;
+    const int skip = copied_column(a, p, len, [&] { return is_first(p); }, &block);
     const int32_t* from = a.tables + (p < 0 ? 0 : p) * a.table_ld;
     int32_t* to = a.tables_out + child * a.width;
-    for (int j = lane; j < a.width; j += step)
+    for (int j = lane; j < a.width; j += 64)
         if (j != skip) to[j] = j < used ? from[j] : -1;
     if (lane == 0) a.seq_lens_out[child] = len;
 }
@@ -94,16 +86,34 @@ __device__ __forceinline__ int block_scan(int v, int* totals, int* total) {
     return before;
 }
 
+// A child's begun block that is to be copied: its column and its number, or -1.
+struct Copy {
+    int column, block;
+};
+
+template <class First>
+__device__ __forceinline__ Copy copy_of(const ReorderArgs& a, int64_t child, First is_first) {
+    Copy c{-1, -1};
+    if (child < a.children) {
+        const int p = parent_of(a, child);
+        c.column = copied_column(a, p, length_of(a, p), [&] { return is_first(p, child); }, &c.block);
+    }
+    return c;
+}
+
 // The new stack: what is on the old one, then the freed blocks by rising number, less what children
-// take from its top for begun blocks of their own, by rising child.  One workgroup.
-__device__ __forceinline__ void write_stack(const ReorderArgs& a, const Marks& m, int* totals) {
+// take from its top for begun blocks of their own, by rising child.  One workgroup.  freed(w): those
+// of the blocks 32 w .. 32 w + 31;  `copy`: of the child of the thread's number.
+template <class Freed, class First>
+__device__ __forceinline__ void write_stack(const ReorderArgs& a, int* totals, Copy copy, Freed freed,
+                                            First is_first) {
     int top = max(min(min(*a.num_free, a.capacity), a.blocks), 0);
     const int kept = top;
     for (int i = threadIdx.x; i < kept; i += kThreads) a.free_out[i] = a.free_blocks[i];
     const int words = (a.blocks + 31) >> 5;
     for (int w0 = 0; w0 < words; w0 += kThreads) {
         const int w = w0 + threadIdx.x;
-        uint32_t f = w < words ? m.dead[w] & ~m.live[w] : 0;
+        uint32_t f = w < words ? freed(w) : 0;
         int total, at = top + block_scan(__popc(f), totals, &total);
         for (; f; f &= f - 1, ++at)
             if (at < a.blocks) a.free_out[at] = w * 32 + __builtin_ctz(f);
@@ -113,20 +123,16 @@ __device__ __forceinline__ void write_stack(const ReorderArgs& a, const Marks& m
     __syncthreads();
     for (int64_t c0 = 0; c0 < a.children; c0 += kThreads) {
         const int64_t child = c0 + threadIdx.x;
-        int p = -1, column = -1, total;
+        if (c0) copy = copy_of(a, child, is_first);
+        int total;
+        const int take = top - 1 - block_scan(copy.column >= 0, totals, &total);
         if (child < a.children) {
-            p = parent_of(a, child);
-            column = copied_column(a, m.first, child, p, length_of(a, p));
-        }
-        const int take = top - 1 - block_scan(column >= 0, totals, &total);
-        if (child < a.children) {
-            int source = -1, target = -1;
-            if (column >= 0) {
-                source = a.tables[p * a.table_ld + column];
-                target = take >= 0 ? a.free_out[take] : -1;
-                a.tables_out[child * a.width + column] = target;
+            int target = -1;
+            if (copy.column >= 0) {
+                if (take >= 0) target = a.free_out[take];
+                a.tables_out[child * a.width + copy.column] = target;
             }
-            a.sources[child] = source;
+            a.sources[child] = copy.block;
             a.targets[child] = target;
         }
         top -= total;
@@ -136,47 +142,133 @@ __device__ __forceinline__ void write_stack(const ReorderArgs& a, const Marks& m
     if (threadIdx.x == 0) *a.num_free_out = top;
 }
 
-__device__ __forceinline__ void clear(const ReorderArgs& a, const Marks& m) {
-    for (int i = threadIdx.x; i < a.rows; i += kThreads) m.first[i] = kNone;
-    const int words = (a.blocks + 31) >> 5;
-    for (int i = threadIdx.x; i < words; i += kThreads) m.live[i] = m.dead[i] = 0;
-    __threadfence();  // the atomics below are done in L2
-    __syncthreads();
+__device__ __forceinline__ void first_children(const ReorderArgs& a, int32_t* first) {
     for (int64_t c = threadIdx.x; c < a.children; c += kThreads) {
         const int p = parent_of(a, c);
-        if (p >= 0) atomicMin(m.first + p, (int)c);  // the least, in whatever order
+        if (p >= 0) atomicMin(first + p, (int)c);  // the least, in whatever order
     }
 }
 
-// All of a small call in one workgroup, whose marks are in LDS.
+constexpr int kRowsAhead = 16;  // rows of a wave whose loads are under way together
+
+// A bit for each of 32 bytes that are 0 or 1.
+__device__ __forceinline__ uint32_t bits_of(const uint8_t* bytes) {
+    const uint4* w = reinterpret_cast<const uint4*>(bytes);
+    const uint4 lo = w[0], hi = w[1];
+    const uint32_t u[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) bits |= ((u[i] * 0x10204080u) >> 28) << (4 * i);
+    return bits;
+}
+
+// A call in one launch.  The first workgroup finds the blocks that are free again, by a bit for each in
+// LDS, and writes the stack; the others write rows, and look for themselves whether a child is its
+// parent's first one.  What takes the time is a handful of loads that wait for each other: 16 rows
+// with 8 parents 6.5 us, 512 rows with 23000 entries 13.5 (22.5 in three launches, where the atomics
+// of a prompt's blocks, held by many rows, meet in a few lines of L2; a byte a block in place of a bit
+// and its atomic 13.3 and 6.8).
 __global__ __launch_bounds__(kThreads) void reorder_kernel(ReorderArgs a) {
     extern __shared__ int32_t lds[];
     __shared__ int totals[kWaves];
-    const int words = (a.blocks + 31) >> 5, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Marks m{lds, reinterpret_cast<uint32_t*>(lds) + a.rows,
-                  reinterpret_cast<uint32_t*>(lds) + a.rows + words};
-    clear(a, m);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (blockIdx.x > 0) {
+        const int64_t child = (int64_t)(blockIdx.x - 1) * kWaves + wave;
+        if (child >= a.children) return;
+        return write_row(a, child, lane, [&](int p) {
+            for (int64_t end = child; end > 0; end -= 64 * kRowsAhead) {  // siblings are often near
+                bool same = false;
+#pragma unroll
+                for (int i = 0; i < kRowsAhead; ++i) {
+                    const int64_t c = end - 1 - lane - 64 * i;
+                    same |= a.parents[max(c, (int64_t)0)] == p && c >= 0;
+                }
+                if (__any(same)) return false;
+            }
+            return true;
+        });
+    }
+    const int words = (a.blocks + 31) >> 5;
+    int32_t *first = lds, *used = lds + a.rows;
+    uint32_t *live = reinterpret_cast<uint32_t*>(used + a.rows), *dead = live + words;
+    // the copy that the thread's child may need, whose loads follow each other, under way first
+    Copy copy = copy_of(a, threadIdx.x, [](int, int64_t) { return false; });
+    const int parent = (int)threadIdx.x < a.children ? parent_of(a, threadIdx.x) : -1;
+    for (int i = threadIdx.x; i < a.rows; i += kThreads) {
+        first[i] = kNone;
+        used[i] = used_of(a, length_of(a, i));
+    }
+    for (int i = threadIdx.x; i < words; i += kThreads) live[i] = dead[i] = 0;
     __syncthreads();
-    for (int r = wave; r < a.rows; r += kWaves) mark_row(a, m, r, lane, 64);
-    for (int64_t c = wave; c < a.children; c += kWaves) write_row(a, m.first, c, lane, 64);
+    first_children(a, first);
     __syncthreads();
-    write_stack(a, m, totals);
+    auto is_first = [&](int p, int64_t child) { return first[p] == child; };
+    if (parent >= 0 && is_first(parent, threadIdx.x)) copy = Copy{-1, -1};
+    for (int r0 = wave; r0 < a.rows; r0 += kWaves * kRowsAhead) {
+        int n[kRowsAhead], most = 0;
+#pragma unroll
+        for (int i = 0; i < kRowsAhead; ++i) {
+            n[i] = r0 + kWaves * i < a.rows ? used[r0 + kWaves * i] : 0;
+            most = max(most, n[i]);
+        }
+        for (int j = lane; j < most; j += 64) {
+            int b[kRowsAhead];
+#pragma unroll
+            for (int i = 0; i < kRowsAhead; ++i)
+                b[i] = j < n[i] ? a.tables[(r0 + kWaves * i) * a.table_ld + j] : -1;
+#pragma unroll
+            for (int i = 0; i < kRowsAhead; ++i) {
+                if (b[i] < 0 || b[i] >= a.blocks) continue;
+                uint32_t* bits = first[r0 + kWaves * i] != kNone ? live : dead;
+                // many rows share a block: a bit that is seen set needs no second time
+                if (!(bits[b[i] >> 5] >> (b[i] & 31) & 1)) atomicOr(bits + (b[i] >> 5), 1u << (b[i] & 31));
+            }
+        }
+    }
+    __syncthreads();
+    write_stack(a, totals, copy, [&](int w) { return dead[w] & ~live[w]; }, is_first);
 }
 
 // A large call, in three launches.
-__global__ __launch_bounds__(kThreads) void reorder_clear_kernel(ReorderArgs a, Marks m) { clear(a, m); }
+__global__ __launch_bounds__(kThreads) void reorder_clear_kernel(ReorderArgs a, Marks m) {
+    if (blockIdx.x > 0) {
+        // live and dead lie side by side, in whole words
+        uint32_t* words = reinterpret_cast<uint32_t*>(m.live);
+        const int64_t count = ((int64_t)a.blocks + 31) / 32 * 16;
+        for (int64_t i = (int64_t)(blockIdx.x - 1) * kThreads + threadIdx.x; i < count;
+             i += (int64_t)(gridDim.x - 1) * kThreads)
+            words[i] = 0;
+        return;
+    }
+    for (int i = threadIdx.x; i < a.rows; i += kThreads) m.first[i] = kNone;
+    __threadfence();  // the minima are formed in L2
+    __syncthreads();
+    first_children(a, m.first);
+}
 
 __global__ __launch_bounds__(256) void reorder_mark_kernel(ReorderArgs a, Marks m) {
     const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row < a.rows) mark_row(a, m, row, blockIdx.y * 64 + (threadIdx.x & 63), 64 * gridDim.y);
+    if (row >= a.rows) return;
+    const int used = used_of(a, length_of(a, row));
+    uint8_t* held = m.first[row] != kNone ? m.live : m.dead;
+    const int32_t* t = a.tables + row * a.table_ld;
+    for (int j = blockIdx.y * 64 + (threadIdx.x & 63); j < used; j += 64 * gridDim.y) {
+        const int b = t[j];
+        if (b >= 0 && b < a.blocks) held[b] = 1;
+    }
 }
 
 // The first workgroup writes the stack, the others rows.
 __global__ __launch_bounds__(kThreads) void reorder_write_kernel(ReorderArgs a, Marks m) {
     __shared__ int totals[kWaves];
-    if (blockIdx.x == 0) return write_stack(a, m, totals);
+    auto is_first = [&](int p, int64_t child) { return m.first[p] == child; };
+    if (blockIdx.x == 0)
+        return write_stack(a, totals, copy_of(a, threadIdx.x, is_first),
+                           [&](int w) { return bits_of(m.dead + 32 * (int64_t)w) & ~bits_of(m.live + 32 * (int64_t)w); },
+                           is_first);
     const int64_t child = (int64_t)(blockIdx.x - 1) * kWaves + (threadIdx.x >> 6);
-    if (child < a.children) write_row(a, m.first, child, threadIdx.x & 63, 64);
+    if (child < a.children)
+        write_row(a, child, threadIdx.x & 63, [&](int p) { return is_first(p, child); });
 }
 
 // ---------------------------------------------------------------- copies
@@ -191,9 +283,13 @@ __global__ __launch_bounds__(256) void copy_kernel(CopyArgs a) {
     const uint32_t waves = gridDim.x * 4;
     const uint32_t mine = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint32_t before = 0;  // pieces of earlier rows, modulo the waves
+    int next_from = -1, next_to = -1;
+    if (lane < a.rows) next_from = a.sources[lane], next_to = a.targets[lane];
     for (int64_t r0 = 0; r0 < a.rows; r0 += 64) {
-        int from = -1, to = -1;
-        if (r0 + lane < a.rows) from = a.sources[r0 + lane], to = a.targets[r0 + lane];
+        const int from = next_from, to = next_to;
+        next_from = next_to = -1;
+        if (r0 + 64 + lane < a.rows)
+            next_from = a.sources[r0 + 64 + lane], next_to = a.targets[r0 + 64 + lane];
         const bool on = from >= 0 && from < a.blocks && to >= 0 && to < a.blocks && from != to;
         const uint64_t rows = __ballot(on);
         const int rank = __popcll(rows & ((1ull << lane) - 1));
@@ -225,38 +321,44 @@ __global__ __launch_bounds__(256) void copy_kernel(CopyArgs a) {
     }
 }
 
-// LDS of a call in one workgroup.
-int64_t small_bytes(const ReorderArgs& a) { return (int64_t)a.rows * 4 + ((int64_t)a.blocks + 31) / 32 * 8; }
+// LDS of a call in one launch.
+int64_t lds_bytes(const ReorderArgs& a) { return (int64_t)a.rows * 8 + ((int64_t)a.blocks + 31) / 32 * 8; }
 
-// One workgroup while its loads and stores of all rows cost less than two more launches.
-bool small_call(const ReorderArgs& a) {
-    return small_bytes(a) <= 60 * 1024 && ((int64_t)a.rows + a.children) * a.width <= 32768;
+// One launch while the blocks' bits fit LDS, one workgroup goes through the entries in the time of two
+// more launches, and looking for siblings is short.
+bool one_launch(const ReorderArgs& a) {
+    return lds_bytes(a) <= 60 * 1024 && (int64_t)a.rows * a.width <= 65536 && a.children <= 4096;
 }
+
+int64_t mark_bytes(const ReorderArgs& a) { return ((int64_t)a.blocks + 31) / 32 * 32; }
 
 }  // namespace
 
-size_t kv8_reorder_bytes(const ReorderArgs& a) { return small_call(a) ? 0 : (size_t)small_bytes(a); }
+size_t kv8_reorder_bytes(const ReorderArgs& a) {
+    return one_launch(a) ? 0 : (size_t)(2 * mark_bytes(a) + (int64_t)a.rows * 4);
+}
 
 hipError_t launch_kv8_reorder(const ReorderArgs& a, void* ws, hipStream_t stream) {
-    if (small_call(a)) {
-        reorder_kernel<<<1, kThreads, (size_t)small_bytes(a), stream>>>(a);
+    const unsigned writers = (unsigned)(1 + ((int64_t)a.children + kWaves - 1) / kWaves);
+    if (one_launch(a)) {
+        reorder_kernel<<<writers, kThreads, (size_t)lds_bytes(a), stream>>>(a);
         return hipGetLastError();
     }
     Marks m;
-    m.first = static_cast<int32_t*>(ws);
-    m.live = reinterpret_cast<uint32_t*>(m.first + a.rows);
-    m.dead = m.live + (a.blocks + 31) / 32;
-    reorder_clear_kernel<<<1, kThreads, 0, stream>>>(a, m);
+    m.live = static_cast<uint8_t*>(ws);
+    m.dead = m.live + mark_bytes(a);
+    m.first = reinterpret_cast<int32_t*>(m.dead + mark_bytes(a));
+    const int64_t clearing = (2 * mark_bytes(a) + 65535) / 65536;
+    reorder_clear_kernel<<<(unsigned)(1 + (clearing < 256 ? clearing : 256)), kThreads, 0, stream>>>(a, m);
     if (a.rows > 0) {
         // long tables of few rows by several waves each
         int64_t split = a.rows < 1024 ? 1024 / a.rows : 1;
         const int64_t most = ((int64_t)a.width + 255) / 256;
         split = split < most ? split : most;
-        reorder_mark_kernel<<<dim3((unsigned)((a.rows + 3) / 4), (unsigned)(split < 1 ? 1 : split)), 256, 0,
-                              stream>>>(a, m);
+        reorder_mark_kernel<<<dim3((unsigned)(((int64_t)a.rows + 3) / 4), (unsigned)(split < 1 ? 1 : split)), 256,
+                              0, stream>>>(a, m);
     }
-    reorder_write_kernel<<<(unsigned)(1 + ((int64_t)a.children + kWaves - 1) / kWaves), kThreads, 0,
-                           stream>>>(a, m);
+    reorder_write_kernel<<<writers, kThreads, 0, stream>>>(a, m);
     return hipGetLastError();
 }
 

