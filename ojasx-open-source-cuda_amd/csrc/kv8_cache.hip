@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "rotary_heads.h"
@@ -157,6 +158,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
 constexpr int kAppendWaves = 4;
 constexpr int64_t kAppendBlocks = 1024;
 constexpr float kTinyAmax = 0x1p-100f;
+constexpr int64_t kAngles = 4096;  // of a workgroup that rotates keys
 
 template <int DT> __device__ __forceinline__ float elem(const void* p, int64_t i) {
     return load_as_f32<DT>(p, i);
@@ -589,102 +591,121 @@ __device__ __forceinline__ void append_held(const KvCache& c, const KvRows& src,
     }
 }
 
+// Cosines and sines of the workgroup's tokens t0 .. t0 + n - 1 into angles [n][pairs].
+__device__ __forceinline__ void form_angles(const Rotation& rot, float2* angles, int64_t t0, int n) {
+    const uint32_t inv = inverse_of(rot.pairs);
+    for (int i = threadIdx.x; i < n * rot.pairs; i += kAppendWaves * kWave) {
+        const int t = quotient(i, inv, rot.pairs);
+        float2 a;
+        pair_turn(rot, position_at(rot, t0 + t), rot.rates[i - t * rot.pairs], a.x, a.y);
+        angles[i] = a;
+    }
+}
+
 // Elements d0 .. d0 + 15 of a key (those from n on are zeros), the rotated ones among them turned.
-template <int DT, bool VEC>
-__device__ __forceinline__ void load16_turned(const void* p, int64_t key, int d0, int n,
-                                              const Rotation& rot, uint64_t position, float (&x)[16]) {
+template <int DT, bool VEC, bool INTERLEAVED>
+__device__ __forceinline__ void load16_turned(const void* p, int64_t key, int d0, int n, int pairs,
+                                              const float2* angles, float (&x)[16]) {
     load16<DT, VEC>(p, key + d0, n, x);
-    const int turned = 2 * rot.pairs;
-    if (d0 >= turned) return;
+    if (d0 >= 2 * pairs) return;
 #pragma unroll
-    for (int i = 0; i < 16; i += 2) {
-        if (rot.interleaved) {
-            if (d0 + i >= turned) break;
-            float c, s;
-            pair_turn(rot, position, rot.rates[(d0 + i) >> 1], c, s);
-            turn_pair(c, s, x[i], x[i + 1]);
-            continue;
-        }
-#pragma unroll
-        for (int j = i; j < i + 2; ++j) {
-            const int d = d0 + j;
-            if (d >= turned) break;
-            const bool hi = d >= rot.pairs;
-            const int pair = hi ? d - rot.pairs : d;
-            float c, s, other = elem<DT>(p, key + (hi ? pair : d + rot.pairs));
-            pair_turn(rot, position, rot.rates[pair], c, s);
-            if (hi) turn_pair(c, s, other, x[j]);
-            else turn_pair(c, s, x[j], other);
+    for (int i = 0; i < 16; i += INTERLEAVED ? 2 : 1) {
+        const int d = d0 + i;
+        if (d >= 2 * pairs) break;
+        if constexpr (INTERLEAVED) {
+            const float2 a = angles[d >> 1];
+            turn_pair(a.x, a.y, x[i], x[i + 1]);
+        } else {
+            const bool hi = d >= pairs;
+            const int pair = hi ? d - pairs : d;
+            const float2 a = angles[pair];
+            float other = elem<DT>(p, key + (hi ? pair : d + pairs));
+            if (hi) turn_pair(a.x, a.y, other, x[i]);
+            else turn_pair(a.x, a.y, x[i], other);
         }
     }
 }
 
-// append_run of keys whose positions are rotated into them on the way, in fp32: for rows that
-// append_turned does not take.  Angles are formed in both passes and for each element of a pair.
-template <int DT, bool VEC>
-__device__ void append_run_turned(const KvCache& c, const KvRows& src, const Rotation& rot, int head,
-                                  int64_t t0, int n, int block, int off, int lane) {
-    const void* x0 = src.p;
-    const int64_t e0 = t0 * src.token + head * src.head;
-    const int chunks = (c.d + 15) >> 4;
-    float m = 0.f;
-    for (int i = lane; i < n * chunks; i += kWave) {
-        const int t = i / chunks, ch = i - t * chunks;
-        float x[16];
-        load16_turned<DT, VEC>(x0, e0 + t * src.token, ch * 16, c.d - ch * 16, rot,
-                               position_at(rot, t0 + t), x);
-        m = amax16(m, x);
+// A run's scale from its largest element, whose earlier codes are rounded again where it grew.
+struct RunScale {
+    float inverse;
+    __device__ __forceinline__ RunScale(const KvCache& c, int8_t* base, float* sp, float before, float most,
+                                        int off, int lane) {
+        most = most < kTinyAmax ? 0.f : most;
+        const float scale = fmaxf(before, most * (1.f / 127.f));
+        inverse = scale > 0.f ? 1.f / scale : 0.f;
+        const float ratio = scale > 0.f ? before / scale : 0.f;
+        if (lane == 0) *sp = scale;
+        if (off > 0 && scale > before) recode_keys(base, off, c.d, c.dp, ratio, lane, kWave);
     }
-    m = wave_max(m);
-    m = m < kTinyAmax ? 0.f : m;
-    float* sp = c.scales + c.scale_at(block, head);
-    const float before = off > 0 ? *sp : 0.f;
-    const float scale = fmaxf(before, m * (1.f / 127.f));
-    const float inverse = scale > 0.f ? 1.f / scale : 0.f;
-    const float ratio = scale > 0.f ? before / scale : 0.f;
-    if (lane == 0) *sp = scale;
-    int8_t* base = c.k + c.at(block, head);
-    if (off > 0 && scale > before) recode_keys(base, off, c.d, c.dp, ratio, lane, kWave);
-    for (int i = lane; i < n * chunks; i += kWave) {
-        const int t = i / chunks, ch = i - t * chunks;
-        float x[16];
-        load16_turned<DT, VEC>(x0, e0 + t * src.token, ch * 16, c.d - ch * 16, rot,
-                               position_at(rot, t0 + t), x);
-        const uint2 lo = codes8(x, inverse, false), hi = codes8(x + 8, inverse, false);
-        *reinterpret_cast<uint4*>(base + key_at(off + t, ch, c.dp)) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-    }
-}
+};
 
-// append_held of keys that are rotated on the way: rotated once, and held as floats between the
-// run's maximum and its codes (rounded to 16 bits in between, the largest codes would be a step off
-// in one of five).  A unit is 8 pairs of one token: two chunks of 8 elements, `pairs` apart or
-// neighbours; behind them two chunks that are not rotated.
-template <int DT, int UNITS, int WAVES, bool INTERLEAVED>
+// append_run or append_held of keys that are rotated on the way, one head by each wave of the workgroup
+// (those past the last head only help with the angles).  Rotated keys are not rounded before they
+// become codes: rounded to 16 bits in between, the largest codes would be a step off in one of five.
+//
+// UNITS > 0: rows of 16 bits on a 16-byte grid, rotated once and held as floats between the run's
+// maximum and its codes.  A unit is 8 pairs of one token: two chunks of 8 elements, `pairs` apart or
+// neighbours; behind them two chunks that are not rotated.  Otherwise two passes over the run, and the
+// angles of as many tokens at a time as `room` holds.
+template <int DT, bool VEC, int UNITS, bool INTERLEAVED>
 __device__ __forceinline__ void append_turned(const KvCache& c, const KvRows& src, const Rotation& rot,
-                                              int head, int64_t t0, int n, int block, int off, int lane,
-                                              int wave, uint32_t* shared) {
-    const uint16_t* x0 = static_cast<const uint16_t*>(src.p) + t0 * src.token + head * src.head;
-    const int d8 = c.d >> 3, wide = (d8 + 1) >> 1, first = wave * 64 + lane;
-    const int apart = INTERLEAVED ? 0 : rot.pairs >> 3;  // units of chunks that are not neighbours
-    const int turned = rot.pairs >> 2;                    // chunks that are rotated
-    const uint32_t inv = inverse_of(wide);
-    const int q0 = off >> 2, quads = ((off + n - 1) >> 2) + 1 - q0, units = quads * wide * 4;
-    float* sp = c.scales + c.scale_at(block, head);
-    const float before = off > 0 ? *sp : 0.f;
-    int8_t* base = c.k + c.at(block, head);
-    // unit u: its token of the block, and its chunks (the second may be past the head's end)
-    auto unit_of = [&](int u, int& t, int& a, int& b) {
-        const int w = u >> 2, i = quotient(w, inv, wide), place = w - i * wide;
-        t = 4 * (q0 + i) + (u & 3);
-        a = place < apart ? place : 2 * place;
-        b = place < apart ? place + apart : a + 1;
-    };
-    float x[UNITS][16];
-    {
+                                              float2* angles, int room, int head, int64_t t0, int n,
+                                              int block, int off, int lane) {
+    const bool on = head < c.heads;
+    int8_t* base = c.k + c.at(block, on ? head : 0);
+    float* sp = c.scales + c.scale_at(block, on ? head : 0);
+    const float before = on && off > 0 ? *sp : 0.f;
+    if constexpr (UNITS == 0) {
+        const int64_t e0 = t0 * src.token + head * src.head;
+        const int chunks = (c.d + 15) >> 4, pairs = rot.pairs, some = room / pairs;
+        float m = 0.f, inverse = 0.f;
+        for (int pass = 0; pass < 2; ++pass) {
+            for (int c0 = 0; c0 < n; c0 += some) {
+                const int part = min(some, n - c0);
+                if (pass == 0 || n > some) {
+                    __syncthreads();
+                    form_angles(rot, angles, t0 + c0, part);
+                    __syncthreads();
+                }
+                if (!on) continue;
+                for (int i = lane; i < part * chunks; i += kWave) {
+                    const int t = i / chunks, ch = i - t * chunks;
+                    float x[16];
+                    load16_turned<DT, VEC, INTERLEAVED>(src.p, e0 + (c0 + t) * src.token, ch * 16,
+                                                        c.d - ch * 16, pairs, angles + t * pairs, x);
+                    if (pass == 0) {
+                        m = amax16(m, x);
+                        continue;
+                    }
+                    const uint2 lo = codes8(x, inverse, false), hi = codes8(x + 8, inverse, false);
+                    *reinterpret_cast<uint4*>(base + key_at(off + c0 + t, ch, c.dp)) =
+                        make_uint4(lo.x, lo.y, hi.x, hi.y);
+                }
+            }
+            if (pass == 0 && on) inverse = RunScale(c, base, sp, before, wave_max(m), off, lane).inverse;
+        }
+    } else {
+        const uint16_t* x0 = static_cast<const uint16_t*>(src.p) + t0 * src.token + head * src.head;
+        const int d8 = c.d >> 3, wide = (d8 + 1) >> 1;
+        const int apart = INTERLEAVED ? 0 : rot.pairs >> 3;  // units of chunks that are not neighbours
+        const int turned = rot.pairs >> 2;                    // chunks that are rotated
+        const uint32_t inv = inverse_of(wide);
+        const int q0 = off >> 2, quads = ((off + n - 1) >> 2) + 1 - q0;
+        // the same in all lanes: a short run leaves the unrolled loops early
+        const int units = __builtin_amdgcn_readfirstlane(on ? quads * wide * 4 : 0);
+        // unit u: its token of the block, and its chunks (the second may be past the head's end)
+        auto unit_of = [&](int u, int& t, int& a, int& b) {
+            const int w = u >> 2, i = quotient(w, inv, wide), place = w - i * wide;
+            t = 4 * (q0 + i) + (u & 3);
+            a = place < apart ? place : 2 * place;
+            b = place < apart ? place + apart : a + 1;
+        };
         uint4 w[UNITS][2];
 #pragma unroll
         for (int i = 0; i < UNITS; ++i) {
-            const int u = first + i * 64 * WAVES;
+            if (i * 64 >= units) break;
+            const int u = lane + i * 64;
             int t, a, b;
             unit_of(u, t, a, b);
             const bool in = u < units && t >= off && t < off + n;
@@ -693,8 +714,15 @@ __device__ __forceinline__ void append_turned(const KvCache& c, const KvRows& sr
             if (in) w[i][0] = *reinterpret_cast<const uint4*>(p + 8 * a);
             if (in && b < d8) w[i][1] = *reinterpret_cast<const uint4*>(p + 8 * b);
         }
+        __syncthreads();
+        form_angles(rot, angles, t0, n);
+        __syncthreads();
+        float x[UNITS][16];
+        float m = 0.f;
+        bool plain = true;
 #pragma unroll
         for (int i = 0; i < UNITS; ++i) {
+            if (i * 64 >= units) break;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const uint32_t v[4] = {w[i][h].x, w[i][h].y, w[i][h].z, w[i][h].w};
@@ -704,81 +732,58 @@ __device__ __forceinline__ void append_turned(const KvCache& c, const KvRows& sr
                     x[i][8 * h + 2 * j + 1] = half_to_f32<DT>(v[j] >> 16);
                 }
             }
+            const int u = lane + i * 64;
+            int t, a, b;
+            unit_of(u, t, a, b);
+            if (u < units && t >= off && t < off + n && a < turned) {
+                const float2* g = angles + (t - off) * rot.pairs + (INTERLEAVED ? 4 * a : 8 * a);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (INTERLEAVED && j >= 4 && b >= turned) break;
+                    if constexpr (INTERLEAVED) turn_pair(g[j].x, g[j].y, x[i][2 * j], x[i][2 * j + 1]);
+                    else turn_pair(g[j].x, g[j].y, x[i][j], x[i][8 + j]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float v = fabsf(x[i][j]);
+                plain &= v < INFINITY;
+                m = v < INFINITY ? fmaxf(m, v) : m;
+            }
         }
-    }
+        plain = __all(plain);
+        if (!on) return;
+        const float inverse = RunScale(c, base, sp, before, wave_max(m), off, lane).inverse;
 #pragma unroll
-    for (int i = 0; i < UNITS; ++i) {
-        const int u = first + i * 64 * WAVES;
-        int t, a, b;
-        unit_of(u, t, a, b);
-        if (u >= units || t < off || t >= off + n || a >= turned) continue;
-        const uint64_t position = position_at(rot, t0 + t - off);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (INTERLEAVED && j >= 4 && b >= turned) break;
-            float co, si;
-            pair_turn(rot, position, rot.rates[INTERLEAVED ? 4 * a + j : 8 * a + j], co, si);
-            if constexpr (INTERLEAVED) turn_pair(co, si, x[i][2 * j], x[i][2 * j + 1]);
-            else turn_pair(co, si, x[i][j], x[i][8 + j]);
-        }
-    }
-    float m = 0.f;
-    bool plain = true;
-#pragma unroll
-    for (int i = 0; i < UNITS; ++i)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const float v = fabsf(x[i][j]);
-            plain &= v < INFINITY;
-            m = v < INFINITY ? fmaxf(m, v) : m;
-        }
-    m = wave_max(m);
-    plain = __all(plain);
-    if constexpr (WAVES > 1) {
-        __syncthreads();
-        if (lane == 0) shared[wave] = plain ? __float_as_uint(m) : __float_as_uint(m) | 0x80000000u;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < WAVES; ++i) {
-            m = fmaxf(m, fabsf(__uint_as_float(shared[i])));
-            plain &= !(shared[i] >> 31);
-        }
-    }
-    m = m < kTinyAmax ? 0.f : m;
-    const float scale = fmaxf(before, m * (1.f / 127.f));
-    const float inverse = scale > 0.f ? 1.f / scale : 0.f;
-    const float ratio = scale > 0.f ? before / scale : 0.f;
-    if (lane == 0 && wave == 0) *sp = scale;
-    if (off > 0 && scale > before) recode_keys(base, off, c.d, c.dp, ratio, first, 64 * WAVES);
-#pragma unroll
-    for (int i = 0; i < UNITS; ++i) {
-        const int u = first + i * 64 * WAVES;
-        int t, a, b;
-        unit_of(u, t, a, b);
-        if (u >= units || t < off || t >= off + n) continue;
-        const uint2 lo = codes8(x[i], inverse, plain), hi = codes8(x[i] + 8, inverse, plain);
-        int8_t* pa = base + key_at(t, a >> 1, c.dp);
-        if (!(a & 1) && b == a + 1) {  // a whole place of 16, zeros behind an odd number of chunks
-            *reinterpret_cast<uint4*>(pa) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-        } else {
-            *reinterpret_cast<uint2*>(pa + 8 * (a & 1)) = lo;
-            *reinterpret_cast<uint2*>(base + key_at(t, b >> 1, c.dp) + 8 * (b & 1)) = hi;
+        for (int i = 0; i < UNITS; ++i) {
+            if (i * 64 >= units) break;
+            const int u = lane + i * 64;
+            int t, a, b;
+            unit_of(u, t, a, b);
+            if (u >= units || t < off || t >= off + n) continue;
+            const uint2 lo = codes8(x[i], inverse, plain), hi = codes8(x[i] + 8, inverse, plain);
+            int8_t* pa = base + key_at(t, a >> 1, c.dp);
+            if (!(a & 1) && b == a + 1) {  // a whole place of 16, zeros behind an odd number of chunks
+                *reinterpret_cast<uint4*>(pa) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            } else {
+                *reinterpret_cast<uint2*>(pa + 8 * (a & 1)) = lo;
+                *reinterpret_cast<uint2*>(base + key_at(t, b >> 1, c.dp) + 8 * (b & 1)) = hi;
+            }
         }
     }
 }
 
-// A wave (WAVES > 1: a workgroup) looks for run starts among `window` tokens and writes each run
-// for one head, keys or values.  Runs end where the slots leave the block or skip.  TURN: keys are
-// rotated on the way, by neighbouring pairs or by pairs that lie apart.
-enum Turn { kStill, kApart, kNeighbours };
-template <int DT, bool VEC, int HOLD, int WAVES, Turn TURN = kStill>
-__device__ __forceinline__ void append_unit(const KvCache& c, const KvRows& k, const KvRows& v,
-                                            const int64_t* __restrict__ slots, int tokens, int window,
-                                            int64_t u, int lane, int wave, uint32_t* shared,
-                                            const Rotation& rot = Rotation{}) {
-    const int parts = 2 * c.heads;
-    const int64_t w = u / parts;
-    const int part = (int)(u - w * parts), head = part >> 1;
+// Sizes of append_turned_kernel: its workgroups, windows and the angles that LDS has room for.
+struct AppendTurned {
+    int key_groups, value_groups, window, angles;
+    int64_t windows;
+};
+
+// Calls write(first token, tokens, block, offset) for each run that begins among the `window` tokens from
+// w * window on, by a wave.  Runs end where the slots leave the block or skip.
+template <class F>
+__device__ __forceinline__ void find_runs(const KvCache& c, const int64_t* __restrict__ slots, int tokens,
+                                          int window, int64_t w, int lane, F write) {
     const int64_t end = (int64_t)c.blocks << c.log_block;
     const int block = 1 << c.log_block;
     // lane i has the slot of token base + i - 1: the window's and what may follow it
@@ -807,21 +812,22 @@ __device__ __forceinline__ void append_unit(const KvCache& c, const KvRows& k, c
                 if (miss) break;
             }
         }
-        const int at = (int)(s0 >> c.log_block);
-        if (TURN != kStill && !(part & 1)) {
-            if constexpr (HOLD > 0)
-                append_turned<DT, HOLD / 2, WAVES, TURN == kNeighbours>(
-                    c, k, rot, head, t0, n, at, off, lane, WAVES > 1 ? wave : 0, shared);
-            else
-                append_run_turned<DT, VEC>(c, k, rot, head, t0, n, at, off, lane);
-            continue;
-        }
+        write(t0, n, (int)(s0 >> c.log_block), off);
+    }
+}
+
+// A wave (WAVES > 1: a workgroup) writes the runs of a window for one head, keys or values.
+template <int DT, bool VEC, int HOLD, int WAVES>
+__device__ __forceinline__ void append_unit(const KvCache& c, const KvRows& rows, bool values, int head,
+                                            const int64_t* __restrict__ slots, int tokens, int window,
+                                            int64_t w, int lane, int wave, uint32_t* shared) {
+    find_runs(c, slots, tokens, window, w, lane, [&](int64_t t0, int n, int block, int off) {
         if constexpr (HOLD > 0)
-            append_held<DT, HOLD, WAVES>(c, part & 1 ? v : k, part & 1, head, t0, n, at, off, lane,
+            append_held<DT, HOLD, WAVES>(c, rows, values, head, t0, n, block, off, lane,
                                          WAVES > 1 ? wave : 0, shared);
         else
-            append_run<DT, VEC>(c, part & 1 ? v : k, part & 1, head, t0, n, at, off, lane);
-    }
+            append_run<DT, VEC>(c, rows, values, head, t0, n, block, off, lane);
+    });
 }
 
 // Workgroups start at a few hundred a microsecond at most, so with many units each takes several.
@@ -832,25 +838,53 @@ __global__ __launch_bounds__(kAppendWaves * kWave) void append_kernel(
     __shared__ uint32_t shared[WAVES];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t step = (int64_t)gridDim.x * (WAVES > 1 ? 1 : kAppendWaves);
+    const int parts = 2 * c.heads;
     for (int64_t u = WAVES > 1 ? blockIdx.x : (int64_t)blockIdx.x * kAppendWaves + wave; u < units;
-         u += step)
-        append_unit<DT, VEC, HOLD, WAVES>(c, k, v, slots, tokens, window, u, lane, wave, shared);
+         u += step) {
+        const int64_t w = u / parts;
+        const int part = (int)(u - w * parts);
+        append_unit<DT, VEC, HOLD, WAVES>(c, part & 1 ? v : k, part & 1, part >> 1, slots, tokens, window,
+                                          w, lane, wave, shared);
+    }
 }
 
-// append_kernel with rotated keys in its first workgroups; the others rotate queries.
-template <int DT, bool VEC, int HOLD, int WAVES, Turn TURN>
+// append_kernel with rotated keys: workgroups for keys, for values, and behind them for queries.  A
+// workgroup of keys takes a window's runs for as many heads as it has waves, whose angles it forms
+// once, in LDS: each wave by itself formed them for every head (prompts of 23446 tokens, 8 x 80 fp16
+// half of it rotated FIGURE
+template <int DT, bool VEC, int HOLD, int WAVES, int UNITS, bool INTERLEAVED>
 __global__ __launch_bounds__(kAppendWaves * kWave) void append_turned_kernel(
-    KvCache c, KvRows k, KvRows v, const int64_t* __restrict__ slots, int tokens, int window,
-    int64_t units, int workgroups, RotaryArgs q) {
+    KvCache c, KvRows k, KvRows v, const int64_t* __restrict__ slots, int tokens, AppendTurned p,
+    RotaryArgs q) {
+    extern __shared__ float2 angles[];
     __shared__ uint32_t shared[WAVES];
-    if ((int)blockIdx.x >= workgroups)
-        return rotate_heads<DT, DT == kF32 ? 4 : 8, TURN == kNeighbours>(q, blockIdx.x - workgroups);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t step = (int64_t)workgroups * (WAVES > 1 ? 1 : kAppendWaves);
-    for (int64_t u = WAVES > 1 ? blockIdx.x : (int64_t)blockIdx.x * kAppendWaves + wave; u < units;
-         u += step)
-        append_unit<DT, VEC, HOLD, WAVES, TURN>(c, k, v, slots, tokens, window, u, lane, wave, shared,
-                                                q.rot);
+    int at = blockIdx.x;
+    if (at < p.key_groups) {
+        const int groups = (c.heads + kAppendWaves - 1) / kAppendWaves;
+        const int64_t units = p.windows * groups;
+        for (int64_t u = at; u < units; u += p.key_groups) {
+            const int64_t w = u / groups;
+            const int head = (int)(u - w * groups) * kAppendWaves + wave;
+            find_runs(c, slots, tokens, p.window, w, lane, [&](int64_t t0, int n, int block, int off) {
+                append_turned<DT, VEC, UNITS, INTERLEAVED>(c, k, q.rot, angles, p.angles, head, t0, n, block,
+                                                           off, lane);
+            });
+        }
+        return;
+    }
+    at -= p.key_groups;
+    if (at < p.value_groups) {
+        const int64_t units = p.windows * c.heads;
+        for (int64_t u = WAVES > 1 ? at : (int64_t)at * kAppendWaves + wave; u < units;
+             u += (int64_t)p.value_groups * (WAVES > 1 ? 1 : kAppendWaves)) {
+            const int64_t w = u / c.heads;
+            append_unit<DT, VEC, HOLD, WAVES>(c, v, true, (int)(u - w * c.heads), slots, tokens, p.window, w,
+                                              lane, wave, shared);
+        }
+        return;
+    }
+    rotate_heads<DT, DT == kF32 ? 4 : 8, INTERLEAVED>(q, at - p.value_groups);
 }
 
 // ---------------------------------------------------------------- read
@@ -1004,9 +1038,7 @@ struct AppendPlan {
     int64_t grid;
 };
 
-// `whole_chunks`: rotated elements, if any, are whole chunks of 8.
-AppendPlan append_plan(const KvCache& c, const KvRows& k, const KvRows& v, int dtype, int tokens,
-                       bool whole_chunks) {
+AppendPlan append_plan(const KvCache& c, const KvRows& k, const KvRows& v, int dtype, int tokens) {
     AppendPlan p;
     // Elements that a run's units cover at most: a key's are whole chunks of 16, so a head of 8
     // takes as much room as one of 16; values' units are never more.
@@ -1015,7 +1047,7 @@ AppendPlan append_plan(const KvCache& c, const KvRows& k, const KvRows& v, int d
     // Rows that a run is held in registers of: 16-bit ones on a 16-byte grid (append and read of
     // 21500 tokens of 8 x 80: 43 us, 79 where they are read twice).  The others, fp32 among them,
     // are read twice, the second time from the cache.
-    p.hold = p.vec && dtype != kF32 && c.d % 8 == 0 && p.held <= 32768 && whole_chunks;
+    p.hold = p.vec && dtype != kF32 && c.d % 8 == 0 && p.held <= 32768;
     p.shared = p.hold && p.held > 8192;
     // A window per token fills the GPU for a decode step, whose tokens all begin runs (append and
     // read of 64 tokens 13 us, 47 with windows of 16); with many tokens most of such waves would
@@ -1056,7 +1088,7 @@ template <class F> void by_plan(const AppendPlan& p, int dtype, F go) {
 
 hipError_t launch_kv8_append(const KvCache& c, const KvRows& k, const KvRows& v, int dtype,
                              const int64_t* slots, int tokens, hipStream_t stream) {
-    const AppendPlan p = append_plan(c, k, v, dtype, tokens, true);
+    const AppendPlan p = append_plan(c, k, v, dtype, tokens);
     by_plan(p, dtype, [&](auto dt, auto vec, auto hold, auto waves) {
         append_kernel<decltype(dt)::value, decltype(vec)::value, decltype(hold)::value,
                       decltype(waves)::value>
@@ -1069,9 +1101,20 @@ hipError_t launch_kv8_append(const KvCache& c, const KvRows& k, const KvRows& v,
 hipError_t launch_kv8_rotate_append(const KvCache& c, const KvRows& k, const KvRows& v, int dtype,
                                     const int64_t* slots, RotaryArgs q, hipStream_t stream) {
     const int step = q.rot.interleaved ? 4 : 8;  // pairs of whole chunks of 8 elements
-    const AppendPlan p = append_plan(c, k, v, dtype, q.tokens, q.rot.pairs % step == 0);
-    // Queries go along where they are taken in steps of 16 bytes (a launch less: 64 decode tokens
-    // of 32 + 8 heads of 128, append and read 13.0 us for 16.6), else in a launch of their own.
+    AppendPlan p = append_plan(c, k, v, dtype, q.tokens);
+    // a wave holds a head's run: no more than 8192 elements of it
+    const bool whole = q.rot.pairs % step == 0 && p.held <= 8192;
+    AppendTurned t;
+    t.window = p.window;
+    t.windows = ((int64_t)q.tokens + p.window - 1) / p.window;
+    t.angles = (int)std::min<int64_t>(((int64_t)q.rot.pairs << c.log_block), kAngles);
+    const int64_t keys = t.windows * ((c.heads + kAppendWaves - 1) / kAppendWaves);
+    const int64_t values = p.shared ? t.windows * c.heads
+                                    : (t.windows * c.heads + kAppendWaves - 1) / kAppendWaves;
+    t.key_groups = (int)std::min(keys, kAppendBlocks);
+    t.value_groups = (int)std::min(values, kAppendBlocks);
+    // Queries go along where they are taken in steps of 16 bytes (a launch less: FIGURE), else in a
+    // launch of their own.
     int64_t extra = 0;
     if (q.q.heads > 0) {
         const bool along = rotary_plan(q, dtype, &extra) == (dtype == kF32 ? 4 : 8);
@@ -1080,16 +1123,25 @@ hipError_t launch_kv8_rotate_append(const KvCache& c, const KvRows& k, const KvR
             if (hipError_t e = launch_rotary(q, dtype, stream)) return e;
         }
     }
-    if (p.grid + extra > 0x7FFFFFFF) return hipErrorInvalidValue;
+    const int64_t grid = t.key_groups + t.value_groups + extra;
+    if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
     by_plan(p, dtype, [&](auto dt, auto vec, auto hold, auto waves) {
-        auto go = [&](auto turn) {
-            append_turned_kernel<decltype(dt)::value, decltype(vec)::value, decltype(hold)::value,
-                                 decltype(waves)::value, decltype(turn)::value>
-                <<<dim3((unsigned)(p.grid + extra)), kAppendWaves * kWave, 0, stream>>>(
-                    c, k, v, slots, q.tokens, p.window, p.units, (int)p.grid, q);
+        constexpr int DT = decltype(dt)::value, HOLD = decltype(hold)::value, WAVES = decltype(waves)::value;
+        constexpr bool VEC = decltype(vec)::value;
+        auto go = [&](auto inter, auto held_keys) {
+            append_turned_kernel<DT, VEC, HOLD, WAVES, decltype(held_keys)::value ? HOLD / 2 : 0,
+                                 decltype(inter)::value>
+                <<<(unsigned)grid, kAppendWaves * kWave, (size_t)t.angles * sizeof(float2), stream>>>(
+                    c, k, v, slots, q.tokens, t, q);
         };
-        if (q.rot.interleaved) go(std::integral_constant<Turn, kNeighbours>{});
-        else go(std::integral_constant<Turn, kApart>{});
+        auto by_layout = [&](auto held_keys) {
+            if (q.rot.interleaved) go(std::true_type{}, held_keys);
+            else go(std::false_type{}, held_keys);
+        };
+        if constexpr (HOLD > 0 && WAVES == 1) {
+            if (whole) return by_layout(std::true_type{});
+        }
+        by_layout(std::false_type{});
     });
     return hipGetLastError();
 }
