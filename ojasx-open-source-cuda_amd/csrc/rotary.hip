@@ -34,8 +34,7 @@ int rotary_plan(RotaryArgs& a, int dtype, int64_t* grid) {
     while (v > 1 && (pairs % v != 0 || rest % (2 * v) != 0 || !fits(a.q, v, size) || !fits(a.k, v, size)))
         v >>= 1;
     a.chunks = (a.d + 2 * v - 1) / (2 * v);
-    a.per = kRotaryAhead;
-    a.groups = (heads + a.per - 1) / a.per;
+    a.groups = (heads + kRotaryHeads - 1) / kRotaryHeads;
     const int64_t units = (int64_t)a.batches * a.tokens * a.groups * a.chunks;
     *grid = (units + kRotaryThreads - 1) / kRotaryThreads;
     return v;

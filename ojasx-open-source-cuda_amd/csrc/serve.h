@@ -250,9 +250,8 @@ struct RotaryArgs {
     int batches;
     int tokens;  // of a batch
     int d;
-    // of launch_rotary: chunks of a head, heads of a thread and the groups of such
+    // of rotary_plan: chunks of a head, and threads of a token for each
     int chunks;
-    int per;
     int groups;
 };
 
