@@ -776,6 +776,7 @@ __device__ __forceinline__ void append_turned(const KvCache& c, const KvRows& sr
 // Sizes of append_turned_kernel: its workgroups, windows and the angles that LDS has room for.
 struct AppendTurned {
     int key_groups, value_groups, window, angles;
+    int half_steps;  // queries are taken by 8 bytes, not by 16
     int64_t windows;
 };
 
@@ -884,7 +885,9 @@ __global__ __launch_bounds__(kAppendWaves * kWave) void append_turned_kernel(
         }
         return;
     }
-    rotate_heads<DT, DT == kF32 ? 4 : 8, INTERLEAVED>(q, at - p.value_groups);
+    constexpr int STEP = DT == kF32 ? 4 : 8;
+    if (p.half_steps) rotate_heads<DT, STEP / 2, INTERLEAVED>(q, at - p.value_groups);
+    else rotate_heads<DT, STEP, INTERLEAVED>(q, at - p.value_groups);
 }
 
 // ---------------------------------------------------------------- read
@@ -1113,12 +1116,14 @@ hipError_t launch_kv8_rotate_append(const KvCache& c, const KvRows& k, const KvR
                                     : (t.windows * c.heads + kAppendWaves - 1) / kAppendWaves;
     t.key_groups = (int)std::min(keys, kAppendBlocks);
     t.value_groups = (int)std::min(values, kAppendBlocks);
-    // Queries go along where they are taken in steps of 16 bytes (a launch less: FIGURE), else in a
-    // launch of their own.
+    // Queries go along where they are taken in steps of 16 or 8 bytes, and fill the waits of the
+    // append's loads (FIGURE), else in a launch of their own.
     int64_t extra = 0;
+    t.half_steps = 0;
     if (q.q.heads > 0) {
-        const bool along = rotary_plan(q, dtype, &extra) == (dtype == kF32 ? 4 : 8);
-        if (!along) {
+        const int v = rotary_plan(q, dtype, &extra), most = dtype == kF32 ? 4 : 8;
+        t.half_steps = 2 * v == most;
+        if (v != most && !t.half_steps) {
             extra = 0;
             if (hipError_t e = launch_rotary(q, dtype, stream)) return e;
         }
