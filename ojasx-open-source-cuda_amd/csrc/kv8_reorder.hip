@@ -101,15 +101,18 @@ __device__ __forceinline__ Copy copy_of(const ReorderArgs& a, int64_t child, Fir
     return c;
 }
 
+// Size of the old stack.
+__device__ __forceinline__ int old_top(const ReorderArgs& a) {
+    return max(min(min(*a.num_free, a.capacity), a.blocks), 0);
+}
+
 // The new stack: what is on the old one, then the freed blocks by rising number, less what children
 // take from its top for begun blocks of their own, by rising child.  One workgroup.  freed(w): those
-// of the blocks 32 w .. 32 w + 31;  `copy`: of the child of the thread's number.
+// of the blocks 32 w .. 32 w + 31.
 template <class Freed, class First>
-__device__ __forceinline__ void write_stack(const ReorderArgs& a, int* totals, Copy copy, Freed freed,
-                                            First is_first) {
-    int top = max(min(min(*a.num_free, a.capacity), a.blocks), 0);
-    const int kept = top;
-    for (int i = threadIdx.x; i < kept; i += kThreads) a.free_out[i] = a.free_blocks[i];
+__device__ __forceinline__ void write_stack(const ReorderArgs& a, int* totals, Freed freed, First is_first) {
+    int top = old_top(a);
+    for (int i = threadIdx.x; i < top; i += kThreads) a.free_out[i] = a.free_blocks[i];
     const int words = (a.blocks + 31) >> 5;
     for (int w0 = 0; w0 < words; w0 += kThreads) {
         const int w = w0 + threadIdx.x;
@@ -123,7 +126,7 @@ __device__ __forceinline__ void write_stack(const ReorderArgs& a, int* totals, C
     __syncthreads();
     for (int64_t c0 = 0; c0 < a.children; c0 += kThreads) {
         const int64_t child = c0 + threadIdx.x;
-        if (c0) copy = copy_of(a, child, is_first);
+        const Copy copy = copy_of(a, child, is_first);
         int total;
         const int take = top - 1 - block_scan(copy.column >= 0, totals, &total);
         if (child < a.children) {
@@ -149,7 +152,11 @@ __device__ __forceinline__ void first_children(const ReorderArgs& a, int32_t* fi
     }
 }
 
-constexpr int kRowsAhead = 16;  // rows of a wave whose loads are under way together
+constexpr int kRowsAhead = 8;  // rows of a wave whose loads are under way together
+
+// Bytes of a call's blocks in LDS.
+__host__ __device__ __forceinline__ int lds_room(const ReorderArgs& a) { return (a.blocks + 32) / 32 * 32; }
+
 
 // A bit for each of 32 bytes that are 0 or 1.
 __device__ __forceinline__ uint32_t bits_of(const uint8_t* bytes) {
@@ -162,12 +169,20 @@ __device__ __forceinline__ uint32_t bits_of(const uint8_t* bytes) {
     return bits;
 }
 
-// A call in one launch.  The first workgroup finds the blocks that are free again, by a bit for each in
-// LDS, and writes the stack; the others write rows, and look for themselves whether a child is its
-// parent's first one.  What takes the time is a handful of loads that wait for each other: 16 rows
-// with 8 parents 6.5 us, 512 rows with 23000 entries 13.5 (22.5 in three launches, where the atomics
-// of a prompt's blocks, held by many rows, meet in a few lines of L2; a byte a block in place of a bit
-// and its atomic 13.3 and 6.8).
+// A barrier for what is in LDS: stores to memory go on.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+constexpr int kOneChildren = 1;  // of a thread, in a call in one launch
+
+// A call in one launch.  The first workgroup finds the blocks that are free again, by two bytes for each
+// in LDS, and writes the stack; the others write rows, and look for themselves whether a child is its
+// parent's first one.
+//
+// One workgroup that runs once is bound by what it waits for: loads that follow each other, and its own
+// instructions, which come from memory too (16 rows with 2 KB more of unrolled code 1 us longer).  16
+// rows of 16 blocks 4.9 us, 512 rows with 23000 entries of 2282 blocks 9.5; with a bit a block in place
+// of a byte, set by atomics, 14, and in three launches with those bits in memory, where a prompt's
+// blocks are held by many rows and lie in few lines, 22.5.
 __global__ __launch_bounds__(kThreads) void reorder_kernel(ReorderArgs a) {
     extern __shared__ int32_t lds[];
     __shared__ int totals[kWaves];
@@ -188,45 +203,105 @@ __global__ __launch_bounds__(kThreads) void reorder_kernel(ReorderArgs a) {
             return true;
         });
     }
-    const int words = (a.blocks + 31) >> 5;
-    int32_t *first = lds, *used = lds + a.rows;
-    uint32_t *live = reinterpret_cast<uint32_t*>(used + a.rows), *dead = live + words;
-    // the copy that the thread's child may need, whose loads follow each other, under way first
-    Copy copy = copy_of(a, threadIdx.x, [](int, int64_t) { return false; });
-    const int parent = (int)threadIdx.x < a.children ? parent_of(a, threadIdx.x) : -1;
+    // live and dead: a byte for each block, and one for entries that are none
+    const int room = lds_room(a), words = room / 32;
+    uint8_t *live = reinterpret_cast<uint8_t*>(lds), *dead = live + room;
+    int32_t *first = lds + room / 2, *used = first + a.rows, *fresh = used + a.rows;
+    // The thread's children, and the copies that they may need: three loads that follow each other, each
+    // under way while something else is waited for.
+    const int c0 = threadIdx.x * kOneChildren;
+    int parent[kOneChildren], len[kOneChildren], block[kOneChildren], column[kOneChildren];
+#pragma unroll
+    for (int i = 0; i < kOneChildren; ++i) parent[i] = c0 + i < a.children ? parent_of(a, c0 + i) : -1;
+    const int kept = old_top(a);
     for (int i = threadIdx.x; i < a.rows; i += kThreads) {
         first[i] = kNone;
         used[i] = used_of(a, length_of(a, i));
     }
-    for (int i = threadIdx.x; i < words; i += kThreads) live[i] = dead[i] = 0;
-    __syncthreads();
-    first_children(a, first);
-    __syncthreads();
-    auto is_first = [&](int p, int64_t child) { return first[p] == child; };
-    if (parent >= 0 && is_first(parent, threadIdx.x)) copy = Copy{-1, -1};
+    for (int i = threadIdx.x; i < room / 2; i += kThreads) lds[i] = 0;
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < kOneChildren; ++i) {
+        len[i] = length_of(a, parent[i]);
+        if (parent[i] >= 0) atomicMin(first + parent[i], c0 + i);  // the least, in whatever order
+    }
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < kOneChildren; ++i)
+        column[i] = copied_column(a, parent[i], len[i], [&] { return first[parent[i]] == c0 + i; }, &block[i]);
     for (int r0 = wave; r0 < a.rows; r0 += kWaves * kRowsAhead) {
+        // without a branch: of rows and columns that there are not, the last ones again, to no block
         int n[kRowsAhead], most = 0;
+        uint8_t* held[kRowsAhead];
+        const int32_t* from[kRowsAhead];
 #pragma unroll
         for (int i = 0; i < kRowsAhead; ++i) {
-            n[i] = r0 + kWaves * i < a.rows ? used[r0 + kWaves * i] : 0;
+            const int r = min(r0 + kWaves * i, a.rows - 1);
+            n[i] = used[r];
             most = max(most, n[i]);
+            held[i] = first[r] != kNone ? live : dead;
+            from[i] = a.tables + r * a.table_ld;
         }
         for (int j = lane; j < most; j += 64) {
-            int b[kRowsAhead];
+            uint32_t b[kRowsAhead];
+#pragma unroll
+            for (int i = 0; i < kRowsAhead; ++i) b[i] = from[i][min(j, a.width - 1)];
 #pragma unroll
             for (int i = 0; i < kRowsAhead; ++i)
-                b[i] = j < n[i] ? a.tables[(r0 + kWaves * i) * a.table_ld + j] : -1;
-#pragma unroll
-            for (int i = 0; i < kRowsAhead; ++i) {
-                if (b[i] < 0 || b[i] >= a.blocks) continue;
-                uint32_t* bits = first[r0 + kWaves * i] != kNone ? live : dead;
-                // many rows share a block: a bit that is seen set needs no second time
-                if (!(bits[b[i] >> 5] >> (b[i] & 31) & 1)) atomicOr(bits + (b[i] >> 5), 1u << (b[i] & 31));
-            }
+                held[i][j < n[i] ? min(b[i], (uint32_t)a.blocks) : (uint32_t)a.blocks] = 1;
         }
     }
-    __syncthreads();
-    write_stack(a, totals, copy, [&](int w) { return dead[w] & ~live[w]; }, is_first);
+    lds_barrier();
+    // freed blocks before the thread's 32, and copies before its children
+    uint32_t free_bits = 0;
+    if ((int)threadIdx.x < words) {
+        // the byte past the last block is of none
+        const int w = threadIdx.x, in = a.blocks - 32 * w;
+        free_bits = bits_of(dead + 32 * w) & ~bits_of(live + 32 * w) & (in < 32 ? (1u << in) - 1 : ~0u);
+    }
+    int copies = 0;
+#pragma unroll
+    for (int i = 0; i < kOneChildren; ++i) copies += column[i] >= 0;
+    const int mine = __popc(free_bits) << 16 | copies;  // both sums are under 2^16
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(sum, o);
+        sum += lane >= o ? up : 0;
+    }
+    if (lane == 63) totals[wave] = sum;
+    lds_barrier();
+    int before = sum - mine, all = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        before += w < wave ? totals[w] : 0;
+        all += totals[w];
+    }
+    const int freed = (uint32_t)all >> 16, taken = all & 0xFFFF;
+    const int top = min(kept + freed, a.blocks), left = top - taken;
+    // the stack's new part, and what of it is taken again: the top is fresh[0]
+    for (int at = kept + (int)((uint32_t)before >> 16); free_bits; free_bits &= free_bits - 1, ++at) {
+        const int b = 32 * threadIdx.x + __builtin_ctz(free_bits);
+        if (at < left) a.free_out[at] = b;
+        else if (top - 1 - at >= 0 && top - 1 - at < taken) fresh[top - 1 - at] = b;
+    }
+    lds_barrier();
+    int rank = before & 0xFFFF;
+#pragma unroll
+    for (int i = 0; i < kOneChildren; ++i) {
+        if (c0 + i >= a.children) break;
+        int target = -1;
+        if (column[i] >= 0) {
+            const int at = top - 1 - rank++;
+            target = at >= kept ? fresh[top - 1 - at] : at >= 0 ? a.free_blocks[at] : -1;
+            a.tables_out[(int64_t)(c0 + i) * a.width + column[i]] = target;
+        }
+        a.sources[c0 + i] = block[i];
+        a.targets[c0 + i] = target;
+    }
+    for (int i = threadIdx.x; i < min(kept, left); i += kThreads) a.free_out[i] = a.free_blocks[i];
+    for (int i = max(left, 0) + threadIdx.x; i < a.blocks; i += kThreads) a.free_out[i] = -1;
+    if (threadIdx.x == 0) *a.num_free_out = left;
 }
 
 // A large call, in three launches.
@@ -263,7 +338,7 @@ __global__ __launch_bounds__(kThreads) void reorder_write_kernel(ReorderArgs a, 
     __shared__ int totals[kWaves];
     auto is_first = [&](int p, int64_t child) { return m.first[p] == child; };
     if (blockIdx.x == 0)
-        return write_stack(a, totals, copy_of(a, threadIdx.x, is_first),
+        return write_stack(a, totals,
                            [&](int w) { return bits_of(m.dead + 32 * (int64_t)w) & ~bits_of(m.live + 32 * (int64_t)w); },
                            is_first);
     const int64_t child = (int64_t)(blockIdx.x - 1) * kWaves + (threadIdx.x >> 6);
@@ -322,12 +397,15 @@ __global__ __launch_bounds__(256) void copy_kernel(CopyArgs a) {
 }
 
 // LDS of a call in one launch.
-int64_t lds_bytes(const ReorderArgs& a) { return (int64_t)a.rows * 8 + ((int64_t)a.blocks + 31) / 32 * 8; }
+int64_t lds_bytes(const ReorderArgs& a) {
+    return (int64_t)a.rows * 8 + 2 * (int64_t)lds_room(a) + (int64_t)a.children * 4;
+}
 
-// One launch while the blocks' bits fit LDS, one workgroup goes through the entries in the time of two
+// One launch while the blocks' bytes fit LDS, one workgroup goes through the entries in the time of two
 // more launches, and looking for siblings is short.
 bool one_launch(const ReorderArgs& a) {
-    return lds_bytes(a) <= 60 * 1024 && (int64_t)a.rows * a.width <= 65536 && a.children <= 4096;
+    return lds_bytes(a) <= 60 * 1024 && lds_room(a) <= 32 * kThreads &&
+           (int64_t)a.rows * a.width <= 65536 && a.children <= kThreads * kOneChildren;
 }
 
 int64_t mark_bytes(const ReorderArgs& a) { return ((int64_t)a.blocks + 31) / 32 * 32; }
