@@ -560,26 +560,47 @@ PyObject* kv8_reorder(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// kv8_copy_blocks(sources, targets, k_codes, v_codes, scales, k_codes, ...): True
+// kv8_copy_blocks(caches, sources, targets): True; caches a list or tuple of triples of tensors or of
+// objects that have them as k_codes, v_codes and scales
 PyObject* kv8_copy_blocks(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n < 5 || (n - 2) % 3 != 0) Py_RETURN_NONE;
+    expect(n, 3, "kv8_copy_blocks");
     const Args a{argv, n};
-    if (!all_plain(argv, (int)n)) Py_RETURN_NONE;
-    const Tensor &sources = a.t(0), &targets = a.t(1), &first = a.t(2);
-    const int64_t m = sources.numel(), layers = (n - 2) / 3;
-    if (!ints(sources, at::kInt, m) || !ints(targets, at::kInt, m) || first.dim() != 4 ||
-        sources.device() != first.device() || targets.device() != first.device())
+    if (!(PyList_Check(argv[0]) || PyTuple_Check(argv[0])) || !all_plain(argv + 1, 2)) Py_RETURN_NONE;
+    const Tensor sources = a.t(1), targets = a.t(2);
+    const int64_t m = sources.numel(), layers = PySequence_Fast_GET_SIZE(argv[0]);
+    if (layers == 0 || !ints(sources, at::kInt, m) || !ints(targets, at::kInt, m) ||
+        sources.device() != targets.device())
         Py_RETURN_NONE;
+    static PyObject* const names[] = {PyUnicode_InternFromString("k_codes"),
+                                      PyUnicode_InternFromString("v_codes"),
+                                      PyUnicode_InternFromString("scales")};
+    std::vector<Tensor> parts;
     std::vector<ojx_kv8_storage> caches;
+    parts.reserve(3 * layers);
     caches.reserve(layers);
-    for (int i = 2; i < n; i += 3) {
-        const Tensor &k = a.t(i), &v = a.t(i + 1), &s = a.t(i + 2);
-        if (!cache_ok(k, v, s, first.size(3)) || k.sizes() != first.sizes() ||
-            k.device() != first.device())
+    for (int64_t i = 0; i < layers; ++i) {
+        PyObject* c = PySequence_Fast_GET_ITEM(argv[0], i);
+        const bool triple = PyTuple_CheckExact(c);
+        if (triple && PyTuple_GET_SIZE(c) != 3) Py_RETURN_NONE;
+        for (int j = 0; j < 3; ++j) {
+            PyObject* t = triple ? PyTuple_GET_ITEM(c, j) : PyObject_GetAttr(c, names[j]);
+            if (!t) {
+                PyErr_Clear();
+                Py_RETURN_NONE;
+            }
+            const bool known = plain(t);
+            if (known) parts.push_back(THPVariable_Unpack(t));
+            if (!triple) Py_DECREF(t);
+            if (!known) Py_RETURN_NONE;
+        }
+        const Tensor *t = &parts[3 * i], &k = t[0];
+        if (k.dim() != 4 || !cache_ok(k, t[1], t[2], k.size(3)) || k.sizes() != parts[0].sizes() ||
+            k.device() != sources.device())
             Py_RETURN_NONE;
-        caches.push_back({(int8_t*)data(k), (int8_t*)data(v), (float*)data(s)});
+        caches.push_back({(int8_t*)data(k), (int8_t*)data(t[1]), (float*)data(t[2])});
     }
+    const Tensor& first = parts[0];
     RECORD_FUNCTION("ojasx_e8t::kv8_copy_blocks", std::vector<c10::IValue>());
     Unlocked unlocked;
     const c10::DeviceGuard on_device(first.device());
@@ -587,7 +608,7 @@ PyObject* kv8_copy_blocks(PyObject*, PyObject* const* argv, Py_ssize_t n) {
                               first.size(3), (const int32_t*)data(sources),
                               (const int32_t*)data(targets), m, current_stream(first.device())),
           "kv8_copy_blocks");
-    for (int i = 2; i < n; ++i) torch::autograd::impl::bump_version(a.t(i));
+    for (const Tensor& t : parts) torch::autograd::impl::bump_version(t);
     unlocked.lock();
     Py_RETURN_TRUE;
     END_HANDLE_TH_ERRORS

@@ -97,11 +97,12 @@ def copy_blocks(caches: Sequence, sources: torch.Tensor, targets: torch.Tensor) 
     """Copies blocks ``sources[i]`` to ``targets[i]`` in every one of ``caches``: ``KV8Cache`` objects,
     or triples of their tensors, all of one shape.  Pairs with a block outside the cache (-1) are
     skipped.  No block may be a target twice, or a target and a source."""
+    if _eager("kv8_copy_blocks", caches, sources, targets) is not None:
+        return
     parts = [(c.k_codes, c.v_codes, c.scales) if isinstance(c, KV8Cache) else tuple(c) for c in caches]
     if any(len(p) != 3 for p in parts):
         raise RuntimeError("a cache is a KV8Cache or its three tensors")
-    if _eager("kv8_copy_blocks", sources, targets, *(t for p in parts for t in p)) is None:
-        S.kv8_copy_blocks(*([p[i] for p in parts] for i in range(3)), sources, targets)
+    S.kv8_copy_blocks(*([p[i] for p in parts] for i in range(3)), sources, targets)
 
 
 def append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_codes: torch.Tensor,
