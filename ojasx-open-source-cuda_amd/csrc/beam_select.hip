@@ -213,10 +213,12 @@ constexpr int kJoinThreads = 512;
 constexpr int kJoinWaves = kJoinThreads / 64;
 constexpr int kJoinBytes = 60 * 1024;  // of LDS for a row's lists and the group's candidates
 // Two values of different beams that are closer than this are compared again with sums in 64 bits.
-// What the first pass is off by: a term that stands alone 2^-23 (its exponential) and 2^-25 (its
-// exponent's rounding, under 1 there); several each up to 17 * 2^-24 for the smallest that count, with
-// both signs, and 7 * 2^-24 for the sum of 8.
-constexpr double kNear = 0x1p-20;
+// What a beam's sum in the first pass is off by, of itself: its exponentials 2^-23; their exponents'
+// rounding, under 2^-22 for the terms that count (2^-16 of the largest and more); the constant's,
+// 2^-26 of the distance to the largest, under 2^-22; sums of 8 in 32 bits, 7 * 2^-24 at the most.
+// Together under 2^-20 where all of them lean one way; twice that for two beams.  About one call in a
+// hundred of 64 x 8 beams has such a pair (which takes a workgroup some 80 us).
+constexpr double kNear = 0x1p-19;
 
 // fp64 bits in rising order as unsigned; NaN above everything.
 __device__ __forceinline__ uint64_t ordered64(double v) {

@@ -170,7 +170,9 @@ __device__ __forceinline__ uint32_t bits_of(const uint8_t* bytes) {
 }
 
 // A barrier for what is in LDS: stores to memory go on.
-__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
 
 constexpr int kOneChildren = 1;  // of a thread, in a call in one launch
 
@@ -338,9 +340,9 @@ __global__ __launch_bounds__(kThreads) void reorder_write_kernel(ReorderArgs a, 
     __shared__ int totals[kWaves];
     auto is_first = [&](int p, int64_t child) { return m.first[p] == child; };
     if (blockIdx.x == 0)
-        return write_stack(a, totals,
-                           [&](int w) { return bits_of(m.dead + 32 * (int64_t)w) & ~bits_of(m.live + 32 * (int64_t)w); },
-                           is_first);
+        return write_stack(
+            a, totals,
+            [&](int64_t w) { return bits_of(m.dead + 32 * w) & ~bits_of(m.live + 32 * w); }, is_first);
     const int64_t child = (int64_t)(blockIdx.x - 1) * kWaves + (threadIdx.x >> 6);
     if (child < a.children)
         write_row(a, child, threadIdx.x & 63, [&](int p) { return is_first(p, child); });
@@ -433,8 +435,8 @@ hipError_t launch_kv8_reorder(const ReorderArgs& a, void* ws, hipStream_t stream
         int64_t split = a.rows < 1024 ? 1024 / a.rows : 1;
         const int64_t most = ((int64_t)a.width + 255) / 256;
         split = split < most ? split : most;
-        reorder_mark_kernel<<<dim3((unsigned)(((int64_t)a.rows + 3) / 4), (unsigned)(split < 1 ? 1 : split)), 256,
-                              0, stream>>>(a, m);
+        const dim3 grid((unsigned)(((int64_t)a.rows + 3) / 4), (unsigned)(split < 1 ? 1 : split));
+        reorder_mark_kernel<<<grid, 256, 0, stream>>>(a, m);
     }
     reorder_write_kernel<<<writers, kThreads, 0, stream>>>(a, m);
     return hipGetLastError();

@@ -1,16 +1,16 @@
 """``torch.library`` custom ops (namespace ``ojasx_e8t``) of the operators around the packed
-linears: the 8-bit paged key / value cache, its attention, token log probabilities, rotated positions,
-beam search.
+linears: the 8-bit paged key / value cache, its attention, token log probabilities, rotated
+positions, beam search.
 
 ``kv8_plan``, ``kv8_append`` (a block's tokens in one run of its slots) and ``kv8_read`` move a
 step's tokens into the cache and blocks out of it (``kv8_rotate_append`` with positions rotated into
-keys and queries on the way), ``kv8_reorder`` and ``kv8_copy_blocks`` let requests go on from others,
-``kv8_attention`` reads it,
-``token_logprobs`` (autograd registered, with ``token_logprobs_bwd``) is what a model answers and
-trains with; ``rotary`` (its own gradient, turned back) rotates queries and keys; ``beam_select`` chooses the beams
-that go on.  The reference keeps no quantized cache; the layouts and rules are those of ``include/ojasx_e8t.h``.  As for the other
-ops: the current HIP stream of the device, outputs and workspaces from torch's caching
-allocator, ``RuntimeError`` for what does not fit, no fallback.
+keys and queries on the way), ``kv8_reorder`` and ``kv8_copy_blocks`` let requests go on from
+others, ``kv8_attention`` reads it; ``rotary`` (its own gradient, turned back) rotates queries and
+keys; ``beam_select`` chooses the beams that go on; ``token_logprobs`` (autograd registered, with
+``token_logprobs_bwd``) is what a model answers and trains with.  The reference keeps no quantized
+cache; the layouts and rules are those of ``include/ojasx_e8t.h``.  As for the other ops: the current
+HIP stream of the device, outputs and workspaces from torch's caching allocator, ``RuntimeError`` for
+what does not fit, no fallback.
 """
 
 from __future__ import annotations
