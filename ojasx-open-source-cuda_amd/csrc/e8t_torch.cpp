@@ -136,6 +136,11 @@ struct Args {
         return v;
     }
     bool flag(int i) const { return a[i] == Py_True; }
+    bool truth(int i) const {
+        const int v = PyObject_IsTrue(a[i]);
+        if (v < 0) throw python_error();
+        return v != 0;
+    }
     const Tensor& t(int i) const { return THPVariable_Unpack(a[i]); }
 };
 
@@ -1007,7 +1012,7 @@ PyObject* kv8_rotate_append(PyObject*, PyObject* const* argv, Py_ssize_t n) {
         !heads_ok(q, k) || !rotation_ok(positions, rates, q) ||
         !positions.is_contiguous() || (c10::GradMode::is_enabled() && records(q)))
         Py_RETURN_NONE;
-    const ojx_rotation r = rotation_of(positions, rates, a.f64(6), a.flag(7), false);
+    const ojx_rotation r = rotation_of(positions, rates, a.f64(6), a.truth(7), false);
     RECORD_FUNCTION("ojasx_e8t::kv8_rotate_append", std::vector<c10::IValue>());
     Unlocked unlocked;
     const c10::DeviceGuard on_device(kc.device());
@@ -1044,7 +1049,7 @@ PyObject* rotary(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     if (!rotary_ok(argv, a)) Py_RETURN_NONE;
     const Tensor q = a.t(0), k = argv[1] == Py_None ? Tensor() : a.t(1);
     if (c10::GradMode::is_enabled() && (records(q) || records(k))) Py_RETURN_NONE;
-    const ojx_rotation r = rotation_of(a.t(2), a.t(3), a.f64(4), a.flag(5), a.flag(6));
+    const ojx_rotation r = rotation_of(a.t(2), a.t(3), a.f64(4), a.truth(5), a.truth(6));
     RECORD_FUNCTION("ojasx_e8t::rotary", std::vector<c10::IValue>());
     Unlocked unlocked;
     Tensor out[2];
@@ -1062,7 +1067,7 @@ PyObject* rotary_recorded(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     if (!rotary_ok(argv, a)) Py_RETURN_NONE;
     const Tensor q = a.t(0), k = argv[1] == Py_None ? Tensor() : a.t(1);
     const double gain = a.f64(4);
-    const bool interleaved = a.flag(5), inverse = a.flag(6);
+    const bool interleaved = a.truth(5), inverse = a.truth(6);
     RECORD_FUNCTION("ojasx_e8t::rotary", std::vector<c10::IValue>());
     Unlocked unlocked;
     const std::optional<Tensor> keys = k.defined() ? std::optional<Tensor>(k) : std::nullopt;

@@ -153,6 +153,25 @@ def test_native_call_matches_the_op_and_refusals():
         c.rotate_append(x[:, :2].clone().requires_grad_(True), *good[1:]).float().sum().backward()
 
 
+def test_no_queries_and_compiled_calls():
+    r = rotary.rotation(64, device=DEV)
+    x = torch.randn(20, 4, 96, device=DEV, dtype=torch.bfloat16)
+    pos, slots = torch.arange(20, device=DEV), torch.arange(20, device=DEV) + 3
+    c, d, e = _caches(4, 1, 96, 16, 2, 3)
+    want = c.rotate_append(x[:, :2], x[:, 2:3], x[:, 3:], pos, slots, r)
+    none = d.rotate_append(x[:, :0], x[:, 2:3], x[:, 3:], pos, slots, r)
+    assert none.shape == (20, 0, 96) and torch.equal(c.k_codes, d.k_codes)
+    f = torch.compile(lambda q: kv8.rotate_append(q, x[:, 2:3], x[:, 3:], pos, slots, r, e.k_codes,
+                                                  e.v_codes, e.scales) * 1, backend="eager")
+    assert torch.equal(f(x[:, :2]), want) and torch.equal(c.k_codes, e.k_codes)
+    g = torch.compile(lambda p: kv8.reorder(p, pos[:2].int() + 20, slots[:4].int().view(2, 2),
+                                            slots[:3].int(), slots[:1].int(), 16, 9).block_tables * 1,
+                      backend="eager")
+    rows = torch.tensor([1, 1, 0], device=DEV)
+    assert torch.equal(g(rows), kv8.reorder(rows, pos[:2].int() + 20, slots[:4].int().view(2, 2),
+                                            slots[:3].int(), slots[:1].int(), 16, 9).block_tables)
+
+
 def test_in_a_graph_and_on_a_stream():
     r = rotary.rotation(128, device=DEV)
     x = torch.randn(9, 6, 128, device=DEV, dtype=torch.bfloat16)

@@ -212,6 +212,9 @@ def test_calls_that_are_not_plain():
             rotary.rotate(*args)
     with pytest.raises(RuntimeError):
         rotary.rotate_qk(x, x.half(), pos, r)
+    # a rotation put together by hand
+    by_hand = rotary.Rotation(r.rates, 2, 1)
+    _check(rotary.rotate(x, pos, by_hand), x, by_hand, pos)
     f = torch.compile(lambda t: rotary.rotate(t, pos, r) * 2, backend="eager")
     assert torch.equal(f(x), rotary.rotate(x, pos, r) * 2)
 
