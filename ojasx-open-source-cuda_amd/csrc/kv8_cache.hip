@@ -159,6 +159,7 @@ constexpr int kAppendWaves = 4;
 constexpr int64_t kAppendBlocks = 1024;
 constexpr float kTinyAmax = 0x1p-100f;
 constexpr int64_t kAngles = 4096;  // of a workgroup that rotates keys
+constexpr int kHalfStepHeads = 4;  // of a thread that rotates queries by 8 bytes
 
 template <int DT> __device__ __forceinline__ float elem(const void* p, int64_t i) {
     return load_as_f32<DT>(p, i);
@@ -718,8 +719,7 @@ __device__ __forceinline__ void append_turned(const KvCache& c, const KvRows& sr
         form_angles(rot, angles, t0, n);
         __syncthreads();
         float x[UNITS][16];
-        float m = 0.f;
-        bool plain = true;
+        uint32_t bits = 0;  // of the largest |element|: NaN and infinities are over all others
 #pragma unroll
         for (int i = 0; i < UNITS; ++i) {
             if (i * 64 >= units) break;
@@ -745,13 +745,18 @@ __device__ __forceinline__ void append_turned(const KvCache& c, const KvRows& sr
                 }
             }
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float v = fabsf(x[i][j]);
-                plain &= v < INFINITY;
-                m = v < INFINITY ? fmaxf(m, v) : m;
+            for (int j = 0; j < 16; ++j) bits = max(bits, __float_as_uint(x[i][j]) & 0x7FFFFFFFu);
+        }
+        const bool plain = __all(bits < 0x7F800000u);
+        float m = __uint_as_float(bits);
+        if (!plain) {  // finite elements only
+            m = 0.f;
+#pragma unroll
+            for (int i = 0; i < UNITS; ++i) {
+                if (i * 64 >= units) break;
+                m = amax16(m, x[i]);
             }
         }
-        plain = __all(plain);
         if (!on) return;
         const float inverse = RunScale(c, base, sp, before, wave_max(m), off, lane).inverse;
 #pragma unroll
@@ -888,7 +893,7 @@ __global__ __launch_bounds__(kAppendWaves * kWave) void append_turned_kernel(
         return;
     }
     constexpr int STEP = DT == kF32 ? 4 : 8;
-    if (p.half_steps) rotate_heads<DT, STEP / 2, INTERLEAVED>(q, at - p.value_groups);
+    if (p.half_steps) rotate_heads<DT, STEP / 2, INTERLEAVED, kHalfStepHeads>(q, at - p.value_groups);
     else rotate_heads<DT, STEP, INTERLEAVED>(q, at - p.value_groups);
 }
 
@@ -1125,6 +1130,7 @@ hipError_t launch_kv8_rotate_append(const KvCache& c, const KvRows& k, const KvR
     if (q.q.heads > 0) {
         const int v = rotary_plan(q, dtype, &extra), most = dtype == kF32 ? 4 : 8;
         t.half_steps = 2 * v == most;
+        if (t.half_steps) rotary_plan(q, dtype, &extra, kHalfStepHeads);
         if (v != most && !t.half_steps) {
             extra = 0;
             if (hipError_t e = launch_rotary(q, dtype, stream)) return e;

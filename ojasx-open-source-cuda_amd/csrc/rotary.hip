@@ -27,14 +27,14 @@ bool fits(const RotaryRows& r, int v, int size) {
 
 }  // namespace
 
-int rotary_plan(RotaryArgs& a, int dtype, int64_t* grid) {
+int rotary_plan(RotaryArgs& a, int dtype, int64_t* grid, int heads_of_thread) {
     const int size = dtype == kF32 ? 4 : 2, heads = a.q.heads + a.k.heads;
     const int pairs = a.rot.pairs, rest = a.d - 2 * pairs;
     int v = 16 / size;
     while (v > 1 && (pairs % v != 0 || rest % (2 * v) != 0 || !fits(a.q, v, size) || !fits(a.k, v, size)))
         v >>= 1;
     a.chunks = (a.d + 2 * v - 1) / (2 * v);
-    a.groups = (heads + kRotaryHeads - 1) / kRotaryHeads;
+    a.groups = (heads + heads_of_thread - 1) / heads_of_thread;
     const int64_t units = (int64_t)a.batches * a.tokens * a.groups * a.chunks;
     *grid = (units + kRotaryThreads - 1) / kRotaryThreads;
     return v;

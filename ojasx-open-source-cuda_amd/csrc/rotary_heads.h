@@ -56,10 +56,10 @@ template <int DT, int V> struct Piece {
 };
 
 // A thread has 2 V elements of a head (V pairs, or as many that are copied) and forms their cosines
-// and sines once for kRotaryHeads heads of its token, queries and keys alike.  Memory bounds it, at
+// and sines once for HEADS heads of its token, queries and keys alike.  Memory bounds it, at
 // 5.3 TB/s for large calls (read and written; a large copy reaches 5.2), the latency of a launch, a
 // load, the angles and a store for small ones.
-template <int DT, int V, bool INTERLEAVED>
+template <int DT, int V, bool INTERLEAVED, int HEADS = kRotaryHeads>
 __device__ __forceinline__ void rotate_heads(const RotaryArgs& a, uint32_t workgroup) {
     // (token, group of heads, chunk) of the thread: a division of 64 bits for the workgroup alone
     const uint32_t unit_count = (uint32_t)a.groups * a.chunks;
@@ -78,13 +78,13 @@ __device__ __forceinline__ void rotate_heads(const RotaryArgs& a, uint32_t workg
     const int lo = INTERLEAVED || copy ? 2 * V * chunk : V * chunk;
     int hi = INTERLEAVED || copy ? lo + V : lo + pairs;
     if (V == 1 && copy) hi = min(hi, a.d - 1);  // the last one of an odd head, twice
-    const int h0 = group * kRotaryHeads, heads = a.q.heads + a.k.heads;
+    const int h0 = group * HEADS, heads = a.q.heads + a.k.heads;
     const int64_t qx = b * a.q.x_batch + t * a.q.x_token, qy = b * a.q.y_batch + t * a.q.y_token;
     const int64_t kx = b * a.k.x_batch + t * a.k.x_token, ky = b * a.k.y_batch + t * a.k.y_token;
     // on their way while the angles are formed
-    Piece<DT, V> p[kRotaryHeads], r[kRotaryHeads];
+    Piece<DT, V> p[HEADS], r[HEADS];
 #pragma unroll
-    for (int j = 0; j < kRotaryHeads; ++j) {
+    for (int j = 0; j < HEADS; ++j) {
         const int h = min(h0 + j, heads - 1);
         const bool key = h >= a.q.heads;
         const void* x = key ? a.k.x : a.q.x;
@@ -99,7 +99,7 @@ __device__ __forceinline__ void rotate_heads(const RotaryArgs& a, uint32_t workg
         for (int i = 0; i < V; ++i) pair_turn(a.rot, position, a.rot.rates[chunk * V + i], c[i], s[i]);
     }
 #pragma unroll
-    for (int j = 0; j < kRotaryHeads; ++j) {
+    for (int j = 0; j < HEADS; ++j) {
         const int h = h0 + j;
         if (h >= heads) break;
         if (!copy) {
@@ -132,6 +132,6 @@ __device__ __forceinline__ void rotate_heads(const RotaryArgs& a, uint32_t workg
 // The largest step, up to 16 bytes, that divides pairs, copied elements, strides and addresses, and
 // the launch's sizes for it.  An odd head size leaves one element to copy: it is taken by single
 // elements, two of them a chunk.  Returns the step; *grid: workgroups.
-int rotary_plan(RotaryArgs& a, int dtype, int64_t* grid);
+int rotary_plan(RotaryArgs& a, int dtype, int64_t* grid, int heads_of_thread = kRotaryHeads);
 
 }  // namespace ojx
