@@ -641,15 +641,76 @@ struct RunScale {
     }
 };
 
+// Eight elements, 16 bytes or 32.
+template <int DT> __device__ __forceinline__ void load8(const void* p, int64_t e, float* x) {
+    if constexpr (DT == kF32) {
+        const float4* w = reinterpret_cast<const float4*>(static_cast<const float*>(p) + e);
+        const float4 lo = w[0], hi = w[1];
+        x[0] = lo.x; x[1] = lo.y; x[2] = lo.z; x[3] = lo.w;
+        x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
+    } else {
+        const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + e);
+        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[2 * j] = half_to_f32<DT>(v[j] & 0xFFFFu);
+            x[2 * j + 1] = half_to_f32<DT>(v[j] >> 16);
+        }
+    }
+}
+
+// Units of a run of keys on the 16-byte grid: 8 pairs of one token, as two chunks of 8 elements, `pairs`
+// apart or neighbours; behind them two chunks that are not rotated.
+template <bool INTERLEAVED> struct KeyUnits {
+    int d8, wide, apart, turned, pairs;
+    uint32_t inv;
+    __device__ __forceinline__ KeyUnits(int d, int p)
+        : d8(d >> 3), wide((d8 + 1) >> 1), apart(INTERLEAVED ? 0 : p >> 3), turned(p >> 2), pairs(p),
+          inv(inverse_of(wide)) {}
+    // unit u of the quads from q on: its token of the block, and its chunks (the second may be past the
+    // head's end)
+    __device__ __forceinline__ void place(int u, int q, int& t, int& a, int& b) const {
+        const int w = u >> 2, i = quotient(w, inv, wide), at = w - i * wide;
+        t = 4 * (q + i) + (u & 3);
+        a = at < apart ? at : 2 * at;
+        b = at < apart ? at + apart : a + 1;
+    }
+    // angles: of the unit's token
+    __device__ __forceinline__ void turn(float (&x)[16], int a, int b, const float2* angles) const {
+        if (a >= turned) return;
+        const float2* g = angles + (INTERLEAVED ? 4 * a : 8 * a);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (INTERLEAVED && j >= 4 && b >= turned) break;
+            if constexpr (INTERLEAVED) turn_pair(g[j].x, g[j].y, x[2 * j], x[2 * j + 1]);
+            else turn_pair(g[j].x, g[j].y, x[j], x[8 + j]);
+        }
+    }
+    __device__ __forceinline__ void store(int8_t* base, int t, int a, int b, int dp, const float (&x)[16],
+                                          float inverse, bool plain) const {
+        const uint2 lo = codes8(x, inverse, plain), hi = codes8(x + 8, inverse, plain);
+        int8_t* pa = base + key_at(t, a >> 1, dp);
+        if (!(a & 1) && b == a + 1) {  // a whole place of 16, zeros behind an odd number of chunks
+            *reinterpret_cast<uint4*>(pa) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        } else {
+            *reinterpret_cast<uint2*>(pa + 8 * (a & 1)) = lo;
+            *reinterpret_cast<uint2*>(base + key_at(t, b >> 1, dp) + 8 * (b & 1)) = hi;
+        }
+    }
+};
+
+// How rotated keys are gone through: element by element, by units, or by units that stay in registers.
+enum Keys { kElements, kUnits, kHeldUnits };
+constexpr int kHeld = 2;  // units of a lane then
+
 // append_run or append_held of keys that are rotated on the way, one head by each wave of the workgroup
 // (those past the last head only help with the angles).  Rotated keys are not rounded before they
 // become codes: rounded to 16 bits in between, the largest codes would be a step off in one of five.
-//
-// UNITS > 0: rows of 16 bits on a 16-byte grid, rotated once and held as floats between the run's
-// maximum and its codes.  A unit is 8 pairs of one token: two chunks of 8 elements, `pairs` apart or
-// neighbours; behind them two chunks that are not rotated.  Otherwise two passes over the run, and the
-// angles of as many tokens at a time as `room` holds.
-template <int DT, bool VEC, int UNITS, bool INTERLEAVED>
+// Two passes over the run, one for its maximum, one for its codes, with the angles of as many tokens at
+// a time as `room` holds; a run of at most 128 units is held as floats between them.  (Held by more
+// registers, larger runs left room for two waves a SIMD: 16000 tokens of 8 x 128 bf16 in blocks of 64,
+// FIGURE)
+template <int DT, bool VEC, Keys KEYS, bool INTERLEAVED>
 __device__ __forceinline__ void append_turned(const KvCache& c, const KvRows& src, const Rotation& rot,
                                               float2* angles, int room, int head, int64_t t0, int n,
                                               int block, int off, int lane) {
@@ -657,8 +718,8 @@ __device__ __forceinline__ void append_turned(const KvCache& c, const KvRows& sr
     int8_t* base = c.k + c.at(block, on ? head : 0);
     float* sp = c.scales + c.scale_at(block, on ? head : 0);
     const float before = on && off > 0 ? *sp : 0.f;
-    if constexpr (UNITS == 0) {
-        const int64_t e0 = t0 * src.token + head * src.head;
+    const int64_t e0 = t0 * src.token + head * src.head;
+    if constexpr (KEYS == kElements) {
         const int chunks = (c.d + 15) >> 4, pairs = rot.pairs, some = room / pairs;
         float m = 0.f, inverse = 0.f;
         for (int pass = 0; pass < 2; ++pass) {
@@ -687,92 +748,94 @@ __device__ __forceinline__ void append_turned(const KvCache& c, const KvRows& sr
             if (pass == 0 && on) inverse = RunScale(c, base, sp, before, wave_max(m), off, lane).inverse;
         }
     } else {
-        const uint16_t* x0 = static_cast<const uint16_t*>(src.p) + t0 * src.token + head * src.head;
-        const int d8 = c.d >> 3, wide = (d8 + 1) >> 1;
-        const int apart = INTERLEAVED ? 0 : rot.pairs >> 3;  // units of chunks that are not neighbours
-        const int turned = rot.pairs >> 2;                    // chunks that are rotated
-        const uint32_t inv = inverse_of(wide);
-        const int q0 = off >> 2, quads = ((off + n - 1) >> 2) + 1 - q0;
-        // the same in all lanes: a short run leaves the unrolled loops early
-        const int units = __builtin_amdgcn_readfirstlane(on ? quads * wide * 4 : 0);
-        // unit u: its token of the block, and its chunks (the second may be past the head's end)
-        auto unit_of = [&](int u, int& t, int& a, int& b) {
-            const int w = u >> 2, i = quotient(w, inv, wide), place = w - i * wide;
-            t = 4 * (q0 + i) + (u & 3);
-            a = place < apart ? place : 2 * place;
-            b = place < apart ? place + apart : a + 1;
-        };
-        uint4 w[UNITS][2];
+        const KeyUnits<INTERLEAVED> k(c.d, rot.pairs);
+        const int q0 = off >> 2, q1 = ((off + n - 1) >> 2) + 1;
+        if constexpr (KEYS == kHeldUnits) {
+            // the same in all lanes: a short run leaves the unrolled loops early
+            const int units = __builtin_amdgcn_readfirstlane(on ? (q1 - q0) * k.wide * 4 : 0);
+            float x[kHeld][16];
+            bool in[kHeld];
+            int t[kHeld], a[kHeld], b[kHeld];
 #pragma unroll
-        for (int i = 0; i < UNITS; ++i) {
-            if (i * 64 >= units) break;
-            const int u = lane + i * 64;
-            int t, a, b;
-            unit_of(u, t, a, b);
-            const bool in = u < units && t >= off && t < off + n;
-            const uint16_t* p = x0 + (t - off) * src.token;
-            w[i][0] = w[i][1] = make_uint4(0, 0, 0, 0);
-            if (in) w[i][0] = *reinterpret_cast<const uint4*>(p + 8 * a);
-            if (in && b < d8) w[i][1] = *reinterpret_cast<const uint4*>(p + 8 * b);
-        }
-        __syncthreads();
-        form_angles(rot, angles, t0, n);
-        __syncthreads();
-        float x[UNITS][16];
-        uint32_t bits = 0;  // of the largest |element|: NaN and infinities are over all others
-#pragma unroll
-        for (int i = 0; i < UNITS; ++i) {
-            if (i * 64 >= units) break;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t v[4] = {w[i][h].x, w[i][h].y, w[i][h].z, w[i][h].w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    x[i][8 * h + 2 * j] = half_to_f32<DT>(v[j] & 0xFFFFu);
-                    x[i][8 * h + 2 * j + 1] = half_to_f32<DT>(v[j] >> 16);
-                }
-            }
-            const int u = lane + i * 64;
-            int t, a, b;
-            unit_of(u, t, a, b);
-            if (u < units && t >= off && t < off + n && a < turned) {
-                const float2* g = angles + (t - off) * rot.pairs + (INTERLEAVED ? 4 * a : 8 * a);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    if (INTERLEAVED && j >= 4 && b >= turned) break;
-                    if constexpr (INTERLEAVED) turn_pair(g[j].x, g[j].y, x[i][2 * j], x[i][2 * j + 1]);
-                    else turn_pair(g[j].x, g[j].y, x[i][j], x[i][8 + j]);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) bits = max(bits, __float_as_uint(x[i][j]) & 0x7FFFFFFFu);
-        }
-        const bool plain = __all(bits < 0x7F800000u);
-        float m = __uint_as_float(bits);
-        if (!plain) {  // finite elements only
-            m = 0.f;
-#pragma unroll
-            for (int i = 0; i < UNITS; ++i) {
+            for (int i = 0; i < kHeld; ++i) {
                 if (i * 64 >= units) break;
-                m = amax16(m, x[i]);
-            }
-        }
-        if (!on) return;
-        const float inverse = RunScale(c, base, sp, before, wave_max(m), off, lane).inverse;
+                const int u = lane + i * 64;
+                k.place(u, q0, t[i], a[i], b[i]);
+                in[i] = u < units && t[i] >= off && t[i] < off + n;
+                const int64_t e = e0 + (t[i] - off) * src.token;
 #pragma unroll
-        for (int i = 0; i < UNITS; ++i) {
-            if (i * 64 >= units) break;
-            const int u = lane + i * 64;
-            int t, a, b;
-            unit_of(u, t, a, b);
-            if (u >= units || t < off || t >= off + n) continue;
-            const uint2 lo = codes8(x[i], inverse, plain), hi = codes8(x[i] + 8, inverse, plain);
-            int8_t* pa = base + key_at(t, a >> 1, c.dp);
-            if (!(a & 1) && b == a + 1) {  // a whole place of 16, zeros behind an odd number of chunks
-                *reinterpret_cast<uint4*>(pa) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-            } else {
-                *reinterpret_cast<uint2*>(pa + 8 * (a & 1)) = lo;
-                *reinterpret_cast<uint2*>(base + key_at(t, b >> 1, c.dp) + 8 * (b & 1)) = hi;
+                for (int j = 0; j < 16; ++j) x[i][j] = 0.f;
+                if (in[i]) load8<DT>(src.p, e + 8 * a[i], x[i]);
+                if (in[i] && b[i] < k.d8) load8<DT>(src.p, e + 8 * b[i], x[i] + 8);
+            }
+            __syncthreads();
+            form_angles(rot, angles, t0, n);
+            __syncthreads();
+            uint32_t bits = 0;  // of the largest |element|: NaN and infinities are over all others
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) {
+                if (i * 64 >= units) break;
+                if (in[i]) k.turn(x[i], a[i], b[i], angles + (t[i] - off) * k.pairs);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) bits = max(bits, __float_as_uint(x[i][j]) & 0x7FFFFFFFu);
+            }
+            const bool plain = __all(bits < 0x7F800000u);
+            float m = __uint_as_float(bits);
+            if (!plain) {  // finite elements only
+                m = 0.f;
+#pragma unroll
+                for (int i = 0; i < kHeld; ++i) {
+                    if (i * 64 >= units) break;
+                    m = amax16(m, x[i]);
+                }
+            }
+            if (!on) return;
+            const float inverse = RunScale(c, base, sp, before, wave_max(m), off, lane).inverse;
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) {
+                if (i * 64 >= units) break;
+                if (in[i]) k.store(base, t[i], a[i], b[i], c.dp, x[i], inverse, plain);
+            }
+        } else {
+            const int some = room / k.pairs >> 2;  // quads whose angles fit
+            float m = 0.f, inverse = 0.f;
+            bool plain = true;
+            for (int pass = 0; pass < 2; ++pass) {
+                for (int q = q0; q < q1; q += some) {
+                    const int end = min(q + some, q1), lo = max(4 * q, off), hi = min(4 * end, off + n);
+                    if (pass == 0 || q1 - q0 > some) {
+                        __syncthreads();
+                        form_angles(rot, angles, t0 + lo - off, hi - lo);
+                        __syncthreads();
+                    }
+                    if (!on) continue;
+                    const int units = (end - q) * k.wide * 4;
+#pragma unroll 2
+                    for (int u = lane; u < units; u += kWave) {
+                        int t, a, b;
+                        k.place(u, q, t, a, b);
+                        if (t < lo || t >= hi) continue;
+                        const int64_t e = e0 + (t - off) * src.token;
+                        float x[16] = {};
+                        load8<DT>(src.p, e + 8 * a, x);
+                        if (b < k.d8) load8<DT>(src.p, e + 8 * b, x + 8);
+                        k.turn(x, a, b, angles + (t - lo) * k.pairs);
+                        if (pass == 1) {
+                            k.store(base, t, a, b, c.dp, x, inverse, plain);
+                            continue;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const float v = fabsf(x[j]);
+                            plain &= v < INFINITY;
+                            m = v < INFINITY ? fmaxf(m, v) : m;
+                        }
+                    }
+                }
+                if (pass == 0 && on) {
+                    inverse = RunScale(c, base, sp, before, wave_max(m), off, lane).inverse;
+                    plain = __all(plain);
+                }
             }
         }
     }
@@ -854,13 +917,21 @@ __global__ __launch_bounds__(kAppendWaves * kWave) void append_kernel(
     }
 }
 
+// Another order of each 8 workgroups, which run on 8 XCDs: where a block is several windows only every
+// so many find a run, and in their own order these fell on one XCD or two (16000 tokens of 8 x 128 bf16 in
+// blocks of 64, without queries: 149 us, FIGURE3 spread).
+__device__ __forceinline__ int64_t spread(int64_t i) {
+    const int64_t h = i >> 3;
+    return i ^ ((h ^ (h >> 3) ^ (h >> 6)) & 7);
+}
+
 // append_kernel with rotated keys: workgroups for keys, for values, and behind them for queries.  A
 // workgroup of keys takes a window's runs for as many heads as it has waves, whose angles it forms
 // once, in LDS (prompts of 23446 tokens, 8 x 80 fp16 half of it rotated: 40 us, 50 where each wave formed
 // its own; without a rotation 29).  What bounds it is append_held's chain of a load, a maximum and a store,
 // four waves a SIMD, around which queries' workgroups find room: with 16 heads of them 58 us, 64 in two
 // launches (mixed among the others, so that they start together, 60 to 82).
-template <int DT, bool VEC, int HOLD, int WAVES, int UNITS, bool INTERLEAVED>
+template <int DT, bool VEC, int HOLD, int WAVES, Keys KEYS, bool INTERLEAVED>
 __global__ __launch_bounds__(kAppendWaves * kWave) void append_turned_kernel(
     KvCache c, KvRows k, KvRows v, const int64_t* __restrict__ slots, int tokens, AppendTurned p,
     RotaryArgs q) {
@@ -871,11 +942,13 @@ __global__ __launch_bounds__(kAppendWaves * kWave) void append_turned_kernel(
     if (at < p.key_groups) {
         const int groups = (c.heads + kAppendWaves - 1) / kAppendWaves;
         const int64_t units = p.windows * groups;
-        for (int64_t u = at; u < units; u += p.key_groups) {
+        for (int64_t i = at; i < (units + 7 & ~7); i += p.key_groups) {
+            const int64_t u = spread(i);
+            if (u >= units) continue;
             const int64_t w = u / groups;
             const int head = (int)(u - w * groups) * kAppendWaves + wave;
             find_runs(c, slots, tokens, p.window, w, lane, [&](int64_t t0, int n, int block, int off) {
-                append_turned<DT, VEC, UNITS, INTERLEAVED>(c, k, q.rot, angles, p.angles, head, t0, n, block,
+                append_turned<DT, VEC, KEYS, INTERLEAVED>(c, k, q.rot, angles, p.angles, head, t0, n, block,
                                                            off, lane);
             });
         }
@@ -883,9 +956,11 @@ __global__ __launch_bounds__(kAppendWaves * kWave) void append_turned_kernel(
     }
     at -= p.key_groups;
     if (at < p.value_groups) {
-        const int64_t units = p.windows * c.heads;
-        for (int64_t u = WAVES > 1 ? at : (int64_t)at * kAppendWaves + wave; u < units;
-             u += (int64_t)p.value_groups * (WAVES > 1 ? 1 : kAppendWaves)) {
+        constexpr int EACH = WAVES > 1 ? 1 : kAppendWaves;  // units of a workgroup
+        const int64_t units = p.windows * c.heads, parts = (units + EACH - 1) / EACH;
+        for (int64_t i = at; i < (parts + 7 & ~7); i += p.value_groups) {
+            const int64_t u = spread(i) * EACH + (WAVES > 1 ? 0 : wave);
+            if (u >= units) continue;
             const int64_t w = u / c.heads;
             append_unit<DT, VEC, HOLD, WAVES>(c, v, true, (int)(u - w * c.heads), slots, tokens, p.window, w,
                                               lane, wave, shared);
@@ -1112,26 +1187,27 @@ hipError_t launch_kv8_rotate_append(const KvCache& c, const KvRows& k, const KvR
                                     const int64_t* slots, RotaryArgs q, hipStream_t stream) {
     const int step = q.rot.interleaved ? 4 : 8;  // pairs of whole chunks of 8 elements
     AppendPlan p = append_plan(c, k, v, dtype, q.tokens);
-    // a wave holds a head's run: no more than 8192 elements of it
-    const bool whole = q.rot.pairs % step == 0 && p.held <= 8192;
+    const bool units = p.vec && c.d % 8 == 0 && q.rot.pairs % step == 0;
     AppendTurned t;
-    t.window = p.window;
-    t.windows = ((int64_t)q.tokens + p.window - 1) / p.window;
+    t.window = p.window > 1 && c.log_block >= 6 ? 32 : p.window;
+    t.windows = ((int64_t)q.tokens + t.window - 1) / t.window;
     t.angles = (int)std::min<int64_t>(((int64_t)q.rot.pairs << c.log_block), kAngles);
     const int64_t keys = t.windows * ((c.heads + kAppendWaves - 1) / kAppendWaves);
     const int64_t values = p.shared ? t.windows * c.heads
                                     : (t.windows * c.heads + kAppendWaves - 1) / kAppendWaves;
-    t.key_groups = (int)std::min(keys, kAppendBlocks);
-    t.value_groups = (int)std::min(values, kAppendBlocks);
-    // Queries go along where they are taken in steps of 16 or 8 bytes, else in a launch of their own
-    // (64 decode tokens, append and read: 14.0 us along, 15.8 apart).
+    t.key_groups = (int)std::min((keys + 7) / 8 * 8, kAppendBlocks);
+    t.value_groups = (int)std::min((values + 7) / 8 * 8, kAppendBlocks);
+    // Queries go along where they are taken in steps of 16 or 8 bytes, in a small call (64 decode tokens,
+    // append and read: 14.0 us along, 15.8 apart) and beside runs that take few registers (prompts of
+    // 23446 tokens 51 us, 62 apart), else in a launch of their own: FIGURE2
     int64_t extra = 0;
     t.half_steps = 0;
     if (q.q.heads > 0) {
-        const int v = rotary_plan(q, dtype, &extra), most = dtype == kF32 ? 4 : 8;
-        t.half_steps = 2 * v == most;
+        const int step = rotary_plan(q, dtype, &extra), most = dtype == kF32 ? 4 : 8;
+        t.half_steps = 2 * step == most;
         if (t.half_steps) rotary_plan(q, dtype, &extra, kHalfStepHeads);
-        if (v != most && !t.half_steps) {
+        const bool few = p.hold && p.held <= 2048;
+        if ((step != most && !t.half_steps) || (p.window > 1 && !few)) {
             extra = 0;
             if (hipError_t e = launch_rotary(q, dtype, stream)) return e;
         }
@@ -1141,20 +1217,21 @@ hipError_t launch_kv8_rotate_append(const KvCache& c, const KvRows& k, const KvR
     by_plan(p, dtype, [&](auto dt, auto vec, auto hold, auto waves) {
         constexpr int DT = decltype(dt)::value, HOLD = decltype(hold)::value, WAVES = decltype(waves)::value;
         constexpr bool VEC = decltype(vec)::value;
-        auto go = [&](auto inter, auto held_keys) {
-            append_turned_kernel<DT, VEC, HOLD, WAVES, decltype(held_keys)::value ? HOLD / 2 : 0,
-                                 decltype(inter)::value>
+        auto go = [&](auto inter, auto keys) {
+            append_turned_kernel<DT, VEC, HOLD, WAVES, decltype(keys)::value, decltype(inter)::value>
                 <<<(unsigned)grid, kAppendWaves * kWave, (size_t)t.angles * sizeof(float2), stream>>>(
                     c, k, v, slots, q.tokens, t, q);
         };
-        auto by_layout = [&](auto held_keys) {
-            if (q.rot.interleaved) go(std::true_type{}, held_keys);
-            else go(std::false_type{}, held_keys);
+        auto by_layout = [&](auto keys) {
+            if (q.rot.interleaved) go(std::true_type{}, keys);
+            else go(std::false_type{}, keys);
         };
-        if constexpr (HOLD > 0 && WAVES == 1) {
-            if (whole) return by_layout(std::true_type{});
+        if constexpr (VEC) {
+            // (the runs of HOLD 4, of at most 2048 elements, have 128 units)
+            constexpr Keys KEYS = HOLD == 4 ? kHeldUnits : kUnits;
+            if (units) return by_layout(std::integral_constant<Keys, KEYS>{});
         }
-        by_layout(std::false_type{});
+        by_layout(std::integral_constant<Keys, kElements>{});
     });
     return hipGetLastError();
 }
