@@ -630,14 +630,15 @@ __device__ __forceinline__ void load16_turned(const void* p, int64_t key, int d0
 // A run's scale from its largest element, whose earlier codes are rounded again where it grew.
 struct RunScale {
     float inverse;
+    // first, step: of the lanes that share the run
     __device__ __forceinline__ RunScale(const KvCache& c, int8_t* base, float* sp, float before, float most,
-                                        int off, int lane) {
+                                        int off, int first, int step = kWave) {
         most = most < kTinyAmax ? 0.f : most;
         const float scale = fmaxf(before, most * (1.f / 127.f));
         inverse = scale > 0.f ? 1.f / scale : 0.f;
         const float ratio = scale > 0.f ? before / scale : 0.f;
-        if (lane == 0) *sp = scale;
-        if (off > 0 && scale > before) recode_keys(base, off, c.d, c.dp, ratio, lane, kWave);
+        if (first == 0) *sp = scale;
+        if (off > 0 && scale > before) recode_keys(base, off, c.d, c.dp, ratio, first, step);
     }
 };
 
@@ -707,13 +708,14 @@ constexpr int kHeld = 2;  // units of a lane then
 // (those past the last head only help with the angles).  Rotated keys are not rounded before they
 // become codes: rounded to 16 bits in between, the largest codes would be a step off in one of five.
 // Two passes over the run, one for its maximum, one for its codes, with the angles of as many tokens at
-// a time as `room` holds; a run of at most 128 units is held as floats between them.  (Held by more
-// registers, larger runs left room for two waves a SIMD: 16000 tokens of 8 x 128 bf16 in blocks of 64,
-// FIGURE)
+// a time as `room` holds; a run of at most 128 units is held as floats between them.  (Larger runs held
+// took 256 registers, two waves a SIMD: a decode step of 64 tokens 8.1 us for 7.0.)  Of one or two heads,
+// `share` waves take a run's units by turns.
 template <int DT, bool VEC, Keys KEYS, bool INTERLEAVED>
 __device__ __forceinline__ void append_turned(const KvCache& c, const KvRows& src, const Rotation& rot,
-                                              float2* angles, int room, int head, int64_t t0, int n,
-                                              int block, int off, int lane) {
+                                              float2* angles, int room, int head, int share, int part,
+                                              uint32_t* shared, int64_t t0, int n, int block, int off,
+                                              int lane) {
     const bool on = head < c.heads;
     int8_t* base = c.k + c.at(block, on ? head : 0);
     float* sp = c.scales + c.scale_at(block, on ? head : 0);
@@ -811,7 +813,7 @@ __device__ __forceinline__ void append_turned(const KvCache& c, const KvRows& sr
                     if (!on) continue;
                     const int units = (end - q) * k.wide * 4;
 #pragma unroll 2
-                    for (int u = lane; u < units; u += kWave) {
+                    for (int u = part * kWave + lane; u < units; u += share * kWave) {
                         int t, a, b;
                         k.place(u, q, t, a, b);
                         if (t < lo || t >= hi) continue;
@@ -832,10 +834,21 @@ __device__ __forceinline__ void append_turned(const KvCache& c, const KvRows& sr
                         }
                     }
                 }
-                if (pass == 0 && on) {
-                    inverse = RunScale(c, base, sp, before, wave_max(m), off, lane).inverse;
-                    plain = __all(plain);
+                if (pass == 1) break;
+                m = wave_max(m);
+                plain = __all(plain);
+                if (share > 1) {  // the waves of a head
+                    const int wave = threadIdx.x >> 6;
+                    __syncthreads();
+                    if (lane == 0) shared[wave] = __float_as_uint(m) | (plain ? 0u : 0x80000000u);
+                    __syncthreads();
+                    for (int w = wave - part; w < wave - part + share; ++w) {
+                        m = fmaxf(m, fabsf(__uint_as_float(shared[w])));
+                        plain &= !(shared[w] >> 31);
+                    }
                 }
+                if (on)
+                    inverse = RunScale(c, base, sp, before, m, off, part * kWave + lane, share * kWave).inverse;
             }
         }
     }
@@ -917,9 +930,16 @@ __global__ __launch_bounds__(kAppendWaves * kWave) void append_kernel(
     }
 }
 
+// Waves of a workgroup that share a head's keys, where there are fewer heads than waves, and the
+// workgroups of a window.
+__host__ __device__ __forceinline__ int waves_of_head(int heads) { return heads == 1 ? 4 : heads == 2 ? 2 : 1; }
+__host__ __device__ __forceinline__ int key_groups(int heads, int share) {
+    return (heads * share + kAppendWaves - 1) / kAppendWaves;
+}
+
 // Another order of each 8 workgroups, which run on 8 XCDs: where a block is several windows only every
 // so many find a run, and in their own order these fell on one XCD or two (16000 tokens of 8 x 128 bf16 in
-// blocks of 64, without queries: 149 us, FIGURE3 spread).
+// blocks of 64, without queries: 149 us, 48 spread).
 __device__ __forceinline__ int64_t spread(int64_t i) {
     const int64_t h = i >> 3;
     return i ^ ((h ^ (h >> 3) ^ (h >> 6)) & 7);
@@ -928,28 +948,29 @@ __device__ __forceinline__ int64_t spread(int64_t i) {
 // append_kernel with rotated keys: workgroups for keys, for values, and behind them for queries.  A
 // workgroup of keys takes a window's runs for as many heads as it has waves, whose angles it forms
 // once, in LDS (prompts of 23446 tokens, 8 x 80 fp16 half of it rotated: 40 us, 50 where each wave formed
-// its own; without a rotation 29).  What bounds it is append_held's chain of a load, a maximum and a store,
-// four waves a SIMD, around which queries' workgroups find room: with 16 heads of them 58 us, 64 in two
-// launches (mixed among the others, so that they start together, 60 to 82).
+// its own; without a rotation 29).  What bounds it are vector instructions and append_held's chain of a
+// load, a maximum and a store, four waves a SIMD, around which queries' workgroups find room: with 16
+// heads of them 51 us, 62 in two launches (mixed among the others, so that they start together, slower).
 template <int DT, bool VEC, int HOLD, int WAVES, Keys KEYS, bool INTERLEAVED>
 __global__ __launch_bounds__(kAppendWaves * kWave) void append_turned_kernel(
     KvCache c, KvRows k, KvRows v, const int64_t* __restrict__ slots, int tokens, AppendTurned p,
     RotaryArgs q) {
     extern __shared__ float2 angles[];
-    __shared__ uint32_t shared[WAVES];
+    __shared__ uint32_t shared[kAppendWaves];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int at = blockIdx.x;
     if (at < p.key_groups) {
-        const int groups = (c.heads + kAppendWaves - 1) / kAppendWaves;
+        const int share = KEYS == kUnits ? waves_of_head(c.heads) : 1, part = wave & (share - 1);
+        const int groups = key_groups(c.heads, share);
         const int64_t units = p.windows * groups;
-        for (int64_t i = at; i < (units + 7 & ~7); i += p.key_groups) {
+        for (int64_t i = at; i < ((units + 7) & ~7); i += p.key_groups) {
             const int64_t u = spread(i);
             if (u >= units) continue;
             const int64_t w = u / groups;
-            const int head = (int)(u - w * groups) * kAppendWaves + wave;
+            const int head = ((int)(u - w * groups) * kAppendWaves + wave) / share;
             find_runs(c, slots, tokens, p.window, w, lane, [&](int64_t t0, int n, int block, int off) {
-                append_turned<DT, VEC, KEYS, INTERLEAVED>(c, k, q.rot, angles, p.angles, head, t0, n, block,
-                                                           off, lane);
+                append_turned<DT, VEC, KEYS, INTERLEAVED>(c, k, q.rot, angles, p.angles, head, share, part,
+                                                           shared, t0, n, block, off, lane);
             });
         }
         return;
@@ -958,7 +979,7 @@ __global__ __launch_bounds__(kAppendWaves * kWave) void append_turned_kernel(
     if (at < p.value_groups) {
         constexpr int EACH = WAVES > 1 ? 1 : kAppendWaves;  // units of a workgroup
         const int64_t units = p.windows * c.heads, parts = (units + EACH - 1) / EACH;
-        for (int64_t i = at; i < (parts + 7 & ~7); i += p.value_groups) {
+        for (int64_t i = at; i < ((parts + 7) & ~7); i += p.value_groups) {
             const int64_t u = spread(i) * EACH + (WAVES > 1 ? 0 : wave);
             if (u >= units) continue;
             const int64_t w = u / c.heads;
@@ -1192,14 +1213,15 @@ hipError_t launch_kv8_rotate_append(const KvCache& c, const KvRows& k, const KvR
     t.window = p.window > 1 && c.log_block >= 6 ? 32 : p.window;
     t.windows = ((int64_t)q.tokens + t.window - 1) / t.window;
     t.angles = (int)std::min<int64_t>(((int64_t)q.rot.pairs << c.log_block), kAngles);
-    const int64_t keys = t.windows * ((c.heads + kAppendWaves - 1) / kAppendWaves);
+    // (one head or two make one workgroup a window, whether waves share them or not)
+    const int64_t keys = t.windows * key_groups(c.heads, 1);
     const int64_t values = p.shared ? t.windows * c.heads
                                     : (t.windows * c.heads + kAppendWaves - 1) / kAppendWaves;
     t.key_groups = (int)std::min((keys + 7) / 8 * 8, kAppendBlocks);
     t.value_groups = (int)std::min((values + 7) / 8 * 8, kAppendBlocks);
     // Queries go along where they are taken in steps of 16 or 8 bytes, in a small call (64 decode tokens,
     // append and read: 14.0 us along, 15.8 apart) and beside runs that take few registers (prompts of
-    // 23446 tokens 51 us, 62 apart), else in a launch of their own: FIGURE2
+    // 23446 tokens 51 us, 62 apart), else in a launch of their own, at the rate of a copy.
     int64_t extra = 0;
     t.half_steps = 0;
     if (q.q.heads > 0) {
