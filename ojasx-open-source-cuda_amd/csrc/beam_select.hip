@@ -248,6 +248,7 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, Bea
     __shared__ uint64_t top_value[kTopMax + 1];
     __shared__ int top_beam[kTopMax + 1], top_token[kTopMax + 1];
     __shared__ double part[kJoinWaves];
+    __shared__ int listed;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n = p.splits * a.num, all = a.beams * a.num;
     uint64_t* list = lds + wave * n;
@@ -279,11 +280,33 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, Bea
                 t.exact = false;
                 t.need = !(t.m > -kPlainMax && t.m < kPlainMax);
                 __builtin_amdgcn_wave_barrier();
-                for (int i0 = 0; i0 < n; i0 += 64) {
-                    const uint64_t mine = i0 + lane < n ? list[i0 + lane] : 0;
+                // Parts' lists fall: of all but the last part, which may be short, the (num / parts)-th
+                // keys are a bound that num keys reach; what is under it goes.
+                int m = n;
+                if (p.splits > 2) {
+                    const int parts = p.splits - 1, at = (a.num + parts - 1) / parts - 1;
+                    uint64_t least = lane < parts ? list[lane * a.num + at] : ~0ull;
+#pragma unroll
+                    for (int o = 32; o; o >>= 1) {
+                        const uint64_t other = __shfl_xor(least, o);
+                        least = least < other ? least : other;
+                    }
+                    m = 0;
+                    for (int i0 = 0; i0 < n; i0 += 64) {
+                        const uint64_t mine = i0 + lane < n ? list[i0 + lane] : 0;
+                        const bool in = mine != 0 && mine >= least;
+                        const uint64_t those = __ballot(in);
+                        __builtin_amdgcn_wave_barrier();
+                        if (in) list[m + __popcll(those & ((1ull << lane) - 1))] = mine;
+                        __builtin_amdgcn_wave_barrier();
+                        m += __popcll(those);
+                    }
+                }
+                for (int i0 = 0; i0 < m; i0 += 64) {
+                    const uint64_t mine = i0 + lane < m ? list[i0 + lane] : 0;
                     int rank = 0;
 #pragma unroll 8
-                    for (int j = 0; j < n; ++j) rank += list[j] > mine;
+                    for (int j = 0; j < m; ++j) rank += list[j] > mine;
                     const bool in = mine != 0 && rank < a.num;
                     if (in) {
                         const float x = unordered((uint32_t)(mine >> 32));
@@ -306,15 +329,14 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, Bea
     }
     __syncthreads();
 
-    // lanes for a candidate: a power of two of at most a wave, none without a list to look through
-    int team = 1;
-    while (team < 64 && 2 * team * all <= kJoinThreads && team < a.beams) team *= 2;
-    int total = 0;
-    for (int b = 0; b < a.beams; ++b) total += beams[b].count;
+    int total = lane < a.beams ? beams[lane].count : 0;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o);
+    bool needed = __any(lane < a.beams && beams[lane].need);
     for (;;) {
         // sums in 64 bits of the beams that need one, over tokens in the same order for each beam:
         // equal rows have equal sums
-        for (int b = 0; b < a.beams; ++b) {
+        for (int b = 0; needed && b < a.beams; ++b) {
             if (!beams[b].need) continue;
             const int64_t x0 = (row0 + b) * a.ld;
             const double m = beams[b].m;
@@ -337,9 +359,43 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, Bea
             if (threadIdx.x == 0) beams[b].ls = ls, beams[b].exact = true, beams[b].need = false;
             __syncthreads();
         }
+        // Of many candidates those under a bound have no place: the least of the (q + 1)-th values of
+        // beams that have so many, for the first q where these are num + 1 in all.  The others are listed
+        // (where the parts' lists were), in any order.
+        int count = all;
+        int* alive = reinterpret_cast<int*>(lds);
+        if (all > kJoinThreads) {
+            uint64_t bound = 0;
+            const int mine = lane < a.beams ? beams[lane].count : 0;
+            for (int q = 0; q < a.num; ++q) {
+                const uint64_t those = __ballot(mine > q);
+                if (__popcll(those) * (q + 1) <= a.num) continue;
+                bound = mine > q ? value[lane * a.num + q] : ~0ull;
+#pragma unroll
+                for (int o = 32; o; o >>= 1) {
+                    const uint64_t other = __shfl_xor(bound, o);
+                    bound = bound < other ? bound : other;
+                }
+                break;
+            }
+            if (threadIdx.x == 0) listed = 0;
+            __syncthreads();
+            for (int i = threadIdx.x; i < all; i += kJoinThreads) {
+                const int b = i / a.num;
+                if (i - b * a.num >= beams[b].count || value[i] < bound) continue;
+                const int at = atomicAdd(&listed, 1);
+                if (at < kJoinWaves * n * 2) alive[at] = i;
+            }
+            __syncthreads();
+            if (listed <= kJoinWaves * n * 2) count = listed;
+        }
+        // lanes for a candidate: a power of two of at most a wave, none without a beam to look through
+        int team = 1;
+        while (team < 64 && 2 * team * count <= kJoinThreads && team < a.beams) team *= 2;
         // a candidate's rank: those before it in its beam, and in the others' lists, which the lanes
         // of a team share out
-        for (int i = (int)threadIdx.x / team; i < all; i += kJoinThreads / team) {
+        for (int at = (int)threadIdx.x / team; at < count; at += kJoinThreads / team) {
+            const int i = count < all ? alive[at] : at;
             const int b = i / a.num, place = i - b * a.num;
             if (place >= beams[b].count) continue;
             const uint64_t v = value[i];
@@ -377,7 +433,8 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, Bea
                 if (!beams[c].exact) beams[c].need = true;
             }
         }
-        if (!__syncthreads_or(again)) break;
+        needed = __syncthreads_or(again);
+        if (!needed) break;
     }
 
     const int64_t o0 = (int64_t)blockIdx.x * a.num;

@@ -66,6 +66,24 @@ def test_equal_values_come_by_beam_and_token(dtype, v):
     _check(row, torch.full((1, 4), -3.25, device=DEV), min(30, 4 * v))
 
 
+@pytest.mark.parametrize("num", [1, 9, 64])
+def test_many_beams_alike(num):
+    """More candidates than threads, all or most of them equal at the bound of the places."""
+    gen = torch.Generator().manual_seed(num)
+    for beams, v in ((64, 1001), (33, 70), (64, 20011)):
+        row = torch.randint(-1, 2, (3, 1, v), generator=gen).half().to(DEV)
+        x = row.expand(3, beams, v).contiguous()
+        scores = torch.zeros(3, beams, device=DEV)
+        scores[1, ::3] = -0.5
+        scores[2] = (-torch.rand(beams, generator=gen)).to(DEV)
+        done = torch.rand(3, beams, generator=gen).to(DEV) < 0.7
+        _check(x, scores, num)
+        _check(x, scores, num, done, 5)
+        x[0, 1:] = -math.inf
+        scores[1, 2:] = -math.inf
+        _check(x, scores, num, done, 5)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("v", [1001, 32000, 50021])
 def test_values_closer_than_32_bits_tell(dtype, v):
