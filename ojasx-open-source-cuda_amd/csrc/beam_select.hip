@@ -245,10 +245,11 @@ template <int DT>
 __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, BeamParts p) {
     extern __shared__ uint64_t lds[];
     __shared__ Beam beams[kBeamMax];
-    __shared__ uint64_t top_value[kTopMax + 1];
-    __shared__ int top_beam[kTopMax + 1], top_token[kTopMax + 1];
+    __shared__ uint64_t top_value[kTopMax];
+    __shared__ int top_beam[kTopMax], top_token[kTopMax];
     __shared__ double part[kJoinWaves];
     __shared__ int listed;
+    __shared__ unsigned long long close;  // beams near the last place
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n = p.splits * a.num, all = a.beams * a.num;
     uint64_t* list = lds + wave * n;
@@ -360,7 +361,7 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, Bea
             __syncthreads();
         }
         // Of many candidates those under a bound have no place: the least of the (q + 1)-th values of
-        // beams that have so many, for the first q where these are num + 1 in all.  The others are listed
+        // beams that have so many, for the first q where these are num in all.  The others are listed
         // (where the parts' lists were), in any order.
         int count = all;
         int* alive = reinterpret_cast<int*>(lds);
@@ -369,7 +370,7 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, Bea
             const int mine = lane < a.beams ? beams[lane].count : 0;
             for (int q = 0; q < a.num; ++q) {
                 const uint64_t those = __ballot(mine > q);
-                if (__popcll(those) * (q + 1) <= a.num) continue;
+                if (__popcll(those) * (q + 1) < a.num) continue;
                 bound = mine > q ? value[lane * a.num + q] : ~0ull;
 #pragma unroll
                 for (int o = 32; o; o >>= 1) {
@@ -389,6 +390,7 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, Bea
             __syncthreads();
             if (listed <= kJoinWaves * n * 2) count = listed;
         }
+        if (threadIdx.x == 0) close = 0;  // (the last round's has been seen by all)
         // lanes for a candidate: a power of two of at most a wave, none without a beam to look through
         int team = 1;
         while (team < 64 && 2 * team * count <= kJoinThreads && team < a.beams) team *= 2;
@@ -414,14 +416,17 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, Bea
             }
             for (int o = team >> 1; o; o >>= 1) rank += __shfl_xor(rank, o);
             rank += place;
-            if (rank <= a.num && (threadIdx.x & (team - 1)) == 0) {
+            if (rank < a.num && (threadIdx.x & (team - 1)) == 0) {
                 top_value[rank] = v;
                 top_beam[rank] = b;
                 top_token[rank] = token[i];
             }
         }
         __syncthreads();
-        const int last = min(total - 1, a.num);
+        // Neighbours of different beams that are near, and beams that are near the last place in it or
+        // not: among the former, ranks tell which candidates are next to each other, but those behind the
+        // last place have none.
+        const int last = min(total, a.num) - 1;
         bool again = false;
         if ((int)threadIdx.x < last) {
             const int i = threadIdx.x, b = top_beam[i], c = top_beam[i + 1];
@@ -433,7 +438,21 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, Bea
                 if (!beams[c].exact) beams[c].need = true;
             }
         }
-        needed = __syncthreads_or(again);
+        if (total > a.num) {
+            const double border = unordered64(top_value[a.num - 1]);
+            for (int i = threadIdx.x; i < all; i += kJoinThreads) {
+                const int b = i / a.num;
+                if (i - b * a.num < beams[b].count && fabs(unordered64(value[i]) - border) < kNear)
+                    atomicOr(&close, 1ull << b);
+            }
+            __syncthreads();
+            const uint64_t those = close;
+            if ((int)threadIdx.x < a.beams && __popcll(those) > 1 && (those >> threadIdx.x & 1) &&
+                !beams[threadIdx.x].exact)
+                again = beams[threadIdx.x].need = true;
+        }
+        // (the same in all lanes, which the compiler has to know: they go round together)
+        needed = __builtin_amdgcn_readfirstlane(__syncthreads_or(again));
         if (!needed) break;
     }
 
