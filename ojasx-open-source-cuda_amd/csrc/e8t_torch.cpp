@@ -908,6 +908,12 @@ ojx_rotation rotation_of(const Tensor& positions, const Tensor& rates, double ga
     return r;
 }
 
+// As x lies, where that leaves a head's elements neighbours (not of heads that overlap in x).
+Tensor heads_like(const Tensor& x) {
+    Tensor y = at::empty_like(x);
+    return y.stride(-1) == 1 ? y : at::empty_like(x, at::MemoryFormat::Contiguous);
+}
+
 // q and k (undefined: none) rotated; what heads_ok and rotation_ok took.
 void rotate_into(const Tensor& q, const Tensor& k, const Tensor& positions, const ojx_rotation& r,
                  Tensor* out) {
@@ -917,7 +923,7 @@ void rotate_into(const Tensor& q, const Tensor& k, const Tensor& positions, cons
     for (int i = 0; i < 2; ++i) {
         const Tensor& x = i ? k : q;
         if (!x.defined()) continue;
-        const Tensor y = out[i] = at::empty_like(x);
+        const Tensor y = out[i] = heads_like(x);
         rows[i] = {data(x), data(y), n == 4 ? x.stride(0) : 0, x.stride(n - 3), x.stride(n - 2),
                    n == 4 ? y.stride(0) : 0, y.stride(n - 3), y.stride(n - 2), x.size(n - 2)};
     }
@@ -1016,7 +1022,7 @@ PyObject* kv8_rotate_append(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     RECORD_FUNCTION("ojasx_e8t::kv8_rotate_append", std::vector<c10::IValue>());
     Unlocked unlocked;
     const c10::DeviceGuard on_device(kc.device());
-    Tensor out = at::empty_like(q);
+    Tensor out = heads_like(q);
     const ojx_rotary_rows rows = {data(q), data(out), 0, q.stride(0), q.stride(1),
                                   0, out.stride(0), out.stride(1), q.size(1)};
     check(ojx_kv8_rotate_append((int8_t*)data(kc), (int8_t*)data(vc), (float*)data(scales), kc.size(0),

@@ -193,7 +193,7 @@ def kv8_rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
         raise RuntimeError(f"positions must be [{t}] (got {list(positions.shape)})")
     _check_rotation(positions, (t,), rates, d)
     qr, p = _rotary_input(q), positions.contiguous()
-    out = torch.empty_like(qr)
+    out = _rotary_output(qr)
     rot = N.Rotation(N.ptr(rates), rates.numel(), N.ptr(p), p.dtype == torch.int64, interleaved,
                      gain, False)
     rows = _rotary_rows(qr, out)
@@ -208,7 +208,7 @@ def kv8_rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
 
 @kv8_rotate_append.register_fake
 def _(q, k, v, positions, slots, rates, gain, interleaved, k_codes, v_codes, scales):
-    return torch.empty_like(_rotary_input(q))
+    return _rotary_output(_rotary_input(q))
 
 
 # ----------------------------------------------------------------------------- reorder
@@ -463,6 +463,12 @@ def _rotary_input(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(-1) == 1 else x.contiguous()
 
 
+def _rotary_output(x: torch.Tensor) -> torch.Tensor:
+    """As x lies, where that leaves a head's elements neighbours (not of heads that overlap in x)."""
+    y = torch.empty_like(x)
+    return y if y.stride(-1) == 1 else torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
 def _rotary_rows(x: torch.Tensor, y: torch.Tensor) -> "N.RotaryRows":
     return N.RotaryRows(N.ptr(x), N.ptr(y), x.stride(0) if x.dim() == 4 else 0, x.stride(-3),
                         x.stride(-2), y.stride(0) if x.dim() == 4 else 0, y.stride(-3),
@@ -506,7 +512,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
             out.append(q.new_empty(0))
             continue
         x = _rotary_input(x)
-        out.append(torch.empty_like(x))
+        out.append(_rotary_output(x))
         rows.append((x, _rotary_rows(x, out[-1])))
     rot = N.Rotation(N.ptr(rates), rates.numel(), N.ptr(positions),
                      positions.dtype == torch.int64, interleaved, gain, inverse)
@@ -519,8 +525,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
 
 @rotary.register_fake
 def _(q, k, positions, rates, gain, interleaved, inverse):
-    return (torch.empty_like(_rotary_input(q)),
-            q.new_empty(0) if k is None else torch.empty_like(_rotary_input(k)))
+    return (_rotary_output(_rotary_input(q)),
+            q.new_empty(0) if k is None else _rotary_output(_rotary_input(k)))
 
 
 def _rotary_setup(ctx, inputs, output):

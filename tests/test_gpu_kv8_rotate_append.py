@@ -114,6 +114,24 @@ def test_rows_that_are_views():
     _check(apart[:, :2], apart[:, 2:4], apart[:, 4:], pos.long(), slots, r, 6, 64)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_heads_that_overlap(dtype):
+    """Windows of one tensor as queries, keys and values."""
+    t, d, r = 21, 16, rotary.rotation(16, device=DEV)
+    flat = torch.randn(t, 18, device=DEV).to(dtype)
+    x = flat.unfold(1, d, 1)
+    assert x.shape == (t, 3, d) and x.stride()[1:] == (1, 1)
+    pos, slots = torch.arange(t, device=DEV) * 77, torch.arange(t, device=DEV) + 5
+    _check(x, x[:, :2], x[:, 1:], pos, slots, r, 4, 16)
+    c, e = _caches(4, 2, d, 16, 0)
+    a = c.rotate_append(x, x[:, :2], x[:, 1:], pos, slots, r)
+    b = S.kv8_rotate_append(x, x[:, :2], x[:, 1:], pos, slots, r.rates, r.gain, False, e.k_codes,
+                            e.v_codes, e.scales)
+    assert a.stride(-1) == b.stride(-1) == 1 and torch.equal(a, b)
+    dense = flat.unfold(1, d, 1).contiguous()
+    assert torch.equal(a, rotary.rotate(dense, pos, r))
+
+
 def test_no_tokens_and_padding():
     c, d = _caches(4, 2, 64, 16, 1)
     r = rotary.rotation(64, device=DEV)

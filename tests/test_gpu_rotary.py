@@ -105,6 +105,34 @@ def test_views_are_taken_as_they_lie(dtype, interleaved):
         assert a.stride() == want[0].stride()
 
 
+@pytest.mark.parametrize("dtype", list(EPS))
+def test_heads_that_overlap(dtype):
+    """Windows of one tensor: heads, or tokens, that share elements."""
+    flat = torch.randn(5, 40, device=DEV).to(dtype)
+    r = rotary.rotation(16, device=DEV)
+    pos = torch.arange(5, device=DEV) * 1001
+    few = flat[:, :18].unfold(1, 16, 1)
+    assert few.shape == (5, 3, 16) and few.stride()[1:] == (1, 1)
+    many = flat.unfold(1, 16, 1)
+    along = flat[0, :20].unfold(0, 16, 1)[:, None]
+    across = flat.flatten()[:60].view(20, 3).unfold(0, 16, 1)
+    alike = flat[:1, None, :16].expand(5, 3, 16)
+    for x in (few, many, along, across, alike):
+        got = rotary.rotate(x, pos, r)
+        assert got.stride(-1) == 1
+        _check(got, x, r, pos)
+        assert torch.equal(S.rotary(x, None, pos, r.rates, r.gain, False, False)[0], got)
+        a, b = rotary.rotate_qk(x, few, pos, r)
+        _check(a, x, r, pos)
+        _check(b, few, r, pos)
+    base = flat.clone().requires_grad_()
+    rotary.rotate(base.unfold(1, 16, 1)[:, :3], pos, r).sum().backward()
+    other = flat.clone().requires_grad_()
+    rotary.rotate(other.unfold(1, 16, 1)[:, :3].contiguous(), pos, r).sum().backward()
+    # the heads' parts may be added in another order: 3 terms
+    assert (base.grad - other.grad).abs().max() <= 4 * EPS[dtype] * 6
+
+
 def test_what_is_not_rotated_stays():
     x = torch.randn(4, 2, 40, device=DEV, dtype=torch.float16)
     x[..., 20:] = torch.tensor([math.nan, math.inf, -math.inf, 65504.0] * 5)
