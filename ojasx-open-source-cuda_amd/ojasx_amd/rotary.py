@@ -61,11 +61,16 @@ def frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] 
     rest = dict(scaling or {"kind": None})
     kind = rest.pop("kind", "")
     s = _number(rest, "factor") if kind in ("linear", "base", "ramp", "wavelength") else 1.0
-    b = base * s ** (rotary_dim / (rotary_dim - 2)) if kind == "base" and n > 1 else base
-    f = [b ** (-2 * i / rotary_dim) for i in range(n)]
+    try:
+        b = base * s ** (rotary_dim / (rotary_dim - 2)) if kind == "base" and n > 1 else base
+        f = [b ** (-2 * i / rotary_dim) for i in range(n)]
+    except OverflowError:
+        raise RuntimeError(f"base {base} with scaling {scaling!r} passes float64's range") from None
     if kind == "linear":
         f = [v / s for v in f]
     elif kind == "ramp":
+        if not base > 1:
+            raise RuntimeError(f"base is {base}, expected over 1 for a ramp over slower pairs")
         length, fast, slow = (_number(rest, *a) for a in (("length",), ("fast", 32), ("slow", 1)))
         gain = _number(rest, "gain", 0.1 * math.log(s) + 1 if s > 1 else 1.0)
         lo, hi = (rotary_dim * math.log(length / (2 * math.pi * t)) / (2 * math.log(base))

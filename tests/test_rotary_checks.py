@@ -74,6 +74,8 @@ def test_rates_are_fractions_of_a_turn():
     (8, 1e4, {"kind": "linear"}), (8, 1e4, {"kind": "linear", "factor": -1}),
     (8, 1e4, {"kind": "linear", "factor": 2, "length": 3}), (8, 1e4, {"kind": "ramp", "factor": 2}),
     (8, 1e4, {"kind": "wavelength", "factor": 2, "length": 9, "low": 4, "high": 4}),
+    (8, 1.0, {"kind": "ramp", "factor": 2, "length": 9}), (8, 0.5, {"kind": "ramp", "factor": 2, "length": 9}),
+    (4, 1e4, {"kind": "base", "factor": 1e300}), (512, 1e-320),
     (8, 1e4, {"kind": "list", "factors": [1, 2, 3]}),
     (8, 1e4, {"kind": "list", "factors": [1, 2, 3, 0]})])
 def test_frequencies_that_cannot_be(args):
