@@ -505,9 +505,9 @@ int ojx_kv8_rotate_append(int8_t* k_codes, int8_t* v_codes, float* scales, int64
 
 /* ---- beam search ----
  *
- * The best continuations of each of `groups` groups of `beams` (1..64) beams.  logits: rows of
- * vocab elements at stride ld, row g * beams + b of beam b of group g.  A candidate (b, t) has the
- * value scores[g][b] + log softmax(row)[t]; of a beam with finished[g][b] (may be NULL) only
+ * The best continuations of each of `groups` groups of `beams` (1..64) beams, fewer than 2^23 beams
+ * in all.  logits: rows of vocab elements at stride ld, row g * beams + b of beam b of group g.  A
+ * candidate (b, t) has the value scores[g][b] + log softmax(row)[t]; of a beam with finished[g][b] (may be NULL) only
  * (b, pad_id) is possible, with its score.  The `num` (1..64, at most beams * vocab) largest of a
  * group in falling order, equal ones by rising beam and token:
  *   out_scores [groups][num], out_parents [groups][num] the row of the beam, out_tokens.

@@ -518,19 +518,22 @@ hipError_t launch_beam_select(const BeamArgs& a, void* ws, size_t ws_bytes, hipS
     if (fit < 1) return hipErrorInvalidValue;
     if ((size_t)p.splits > fit) p.splits = (int)fit;
     const int64_t rows = (int64_t)a.groups * a.beams, grid = rows * p.splits;
-    if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+    if (grid > kMaxGroups256 || a.groups > kMaxGroups512) return hipErrorInvalidValue;
     p.sums = static_cast<BeamSum*>(ws);
     p.keys = reinterpret_cast<uint64_t*>(p.sums + (size_t)rows * p.splits);
+    hipError_t pass = hipSuccess;
     auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
         beam_pass_kernel<DT><<<(unsigned)grid, kThreads, 0, stream>>>(a, p);
+        // the join reads logits at the tokens that the pass found: never without it
+        if ((pass = hipGetLastError()) != hipSuccess) return;
         beam_join_kernel<DT><<<(unsigned)a.groups, kJoinThreads, join_bytes(p.splits, a.beams, a.num),
                                stream>>>(a, p);
     };
     if (a.dtype == kF32) go(std::integral_constant<int, kF32>{});
     else if (a.dtype == kF16) go(std::integral_constant<int, kF16>{});
     else go(std::integral_constant<int, kBF16>{});
-    return hipGetLastError();
+    return pass != hipSuccess ? pass : hipGetLastError();
 }
 
 }  // namespace ojx

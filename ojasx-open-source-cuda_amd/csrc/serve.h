@@ -68,6 +68,9 @@ int api_done(hipError_t e, const char* what);
 constexpr int64_t kKvMaxHeads = 4096;
 constexpr int64_t kTopMax = 64;
 constexpr int64_t kBeamMax = 64;
+// Threads of a launch, in one dimension, end under 2^32: workgroups of 256 and of 512 or fewer.
+constexpr int64_t kMaxGroups256 = ((int64_t)1 << 24) - 1;
+constexpr int64_t kMaxGroups512 = ((int64_t)1 << 23) - 1;
 
 // A cache; its layout is in include/ojasx_e8t.h.
 struct KvCache {

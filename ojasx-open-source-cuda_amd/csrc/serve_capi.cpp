@@ -108,9 +108,10 @@ int check_beams(int64_t ld, int64_t groups, int64_t beams, int64_t vocab, int64_
     if (beams < 1 || beams > ojx::kBeamMax)
         return api_failf(OJX_EINVAL, "%lld beams, expected 1..%d", (long long)beams,
                         (int)ojx::kBeamMax);
-    if (groups < 0 || groups > kMaxCount / beams)
-        return api_failf(OJX_EINVAL, "%lld groups of %lld beams", (long long)groups,
-                        (long long)beams);
+    // a workgroup of 256 threads for each beam, one of 512 for each group
+    if (groups < 0 || groups > ojx::kMaxGroups512 / beams)
+        return api_failf(OJX_EINVAL, "%lld groups of %lld beams, expected fewer than 2^23 beams in all",
+                        (long long)groups, (long long)beams);
     if (int r = check_logits(ld, groups * beams, vocab, 0, dtype)) return r;
     if (num < 1 || num > ojx::kTopMax || num > beams * vocab)
         return api_failf(OJX_EINVAL, "num %lld is outside 1..%lld", (long long)num,

@@ -27,8 +27,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num: Optional[int] =
                 finished: Optional[torch.Tensor] = None, pad_id: int = 0) -> BeamStep:
     """The ``num`` (default: as many as beams; up to 64) best continuations of each group.
 
-    ``logits [groups, beams, vocabulary]`` (up to 64 beams), ``scores`` float32 ``[groups, beams]``:
-    the beams' log probabilities so far.  A continuation's value is its beam's score plus the token's
+    ``logits [groups, beams, vocabulary]`` (up to 64 beams, fewer than 2^23 in all groups), ``scores``
+    float32 ``[groups, beams]``: the beams' log probabilities so far.  A continuation's value is its beam's score plus the token's
     log probability; equal ones come by rising beam and token.  A beam that is ``finished`` (bool
     ``[groups, beams]``) goes on by ``pad_id`` alone, at its score, and its logits are not read.
 

@@ -1,0 +1,21 @@
+"""Sizes past what a launch holds (2^32 threads in a dimension) are refused by the operators of a step's
+positions and beams at the C ABI, before anything is launched."""
+
+import ctypes
+
+import pytest
+
+from ojasx_amd import _native as N
+
+P = ctypes.c_void_p(256)  # never read: every call is refused
+
+
+@pytest.mark.parametrize("groups,beams", [(1 << 24, 1), (1 << 23, 1), (1 << 22, 2), (1 << 17, 64),
+                                          ((1 << 30) // 64, 64)])
+def test_beams(groups, beams):
+    lib, n = N.lib(), ctypes.c_size_t(7)
+    size = lib.ojx_beam_select_workspace_bytes
+    assert size(groups, beams, 10, 1, 2, ctypes.byref(n)) == -1 and n.value == 0
+    assert lib.ojx_beam_select(P, 10, groups, beams, 10, 2, P, None, 0, 1, P, P, P, P, 1 << 40, None) == -1
+    # the most that there may be
+    assert size(((1 << 23) - 1) // beams, beams, 10, 1, 2, ctypes.byref(n)) == 0 and n.value > 0
