@@ -538,7 +538,8 @@ int ojx_beam_select(const void* logits, int64_t ld, int64_t groups, int64_t beam
  *       child from the top; -1 above.  Negative: so many blocks were missing, the last children's
  *       targets and entries are -1 and what their begun blocks held is lost to them.
  * All rows that share a block have to be in one call: what other tables hold is not known to it.
- * Nothing is written in place, so a call may be repeated; no output overlaps an input. */
+ * Up to 2^25 rows and as many children.  Nothing is written in place, so a call may be repeated; no
+ * output overlaps an input. */
 int ojx_kv8_reorder_workspace_bytes(int64_t rows, int64_t children, int64_t table_width,
                                     int64_t block_size, int64_t num_blocks, size_t* bytes);
 int ojx_kv8_reorder(const int64_t* parents, int64_t children, const int32_t* seq_lens, int64_t rows,

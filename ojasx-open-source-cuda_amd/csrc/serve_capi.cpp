@@ -133,7 +133,9 @@ bool valid_block(int64_t b) { return b == 16 || b == 32 || b == 64 || b == 128 |
 
 int check_reorder(int64_t rows, int64_t children, int64_t table_width, int64_t block_size,
                   int64_t num_blocks) {
-    if (rows < 0 || rows > kMaxCount || children < 0 || children > kMaxCount || table_width < 0 ||
+    // 64 threads of a launch for each row and child
+    constexpr int64_t most = (int64_t)1 << 25;
+    if (rows < 0 || rows > most || children < 0 || children > most || table_width < 0 ||
         table_width > kMaxCount || num_blocks < 0 || num_blocks > kMaxCount)
         return api_failf(OJX_EINVAL, "%lld rows, %lld children, %lld table columns, %lld blocks",
                         (long long)rows, (long long)children, (long long)table_width,

@@ -19,3 +19,12 @@ def test_beams(groups, beams):
     assert lib.ojx_beam_select(P, 10, groups, beams, 10, 2, P, None, 0, 1, P, P, P, P, 1 << 40, None) == -1
     # the most that there may be
     assert size(((1 << 23) - 1) // beams, beams, 10, 1, 2, ctypes.byref(n)) == 0 and n.value > 0
+
+
+@pytest.mark.parametrize("rows,children", [(1, 1 << 26), (1, (1 << 25) + 1), ((1 << 25) + 1, 1), (1 << 30, 1)])
+def test_reordered_rows(rows, children):
+    lib, n = N.lib(), ctypes.c_size_t(7)
+    size = lib.ojx_kv8_reorder_workspace_bytes
+    assert size(rows, children, 4, 16, 9, ctypes.byref(n)) == -1 and n.value == 0
+    assert lib.ojx_kv8_reorder(P, children, P, rows, P, 4, 4, P, 5, P, 16, 9, *[P] * 7, 1 << 40, None) == -1
+    assert size(min(rows, 1 << 25), min(children, 1 << 25), 4, 16, 9, ctypes.byref(n)) == 0
