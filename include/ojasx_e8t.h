@@ -487,7 +487,8 @@ typedef struct ojx_rotary_rows {
 
 /* Rotates q and, unless NULL, k (of as many batches and tokens) in one launch.  The position of
  * token t of batch b is at b * position_batch_stride + t * position_token_stride.  The structs are
- * read before the call returns. */
+ * read before the call returns.  A call of over 2^32 - 256 threads, which have two heads' pairs of 16
+ * bytes (or of the largest step that divides sizes, strides and addresses), is refused. */
 int ojx_rotary(const ojx_rotary_rows* q, const ojx_rotary_rows* k, int64_t batches, int64_t tokens,
                int64_t head_dim, int dtype, const ojx_rotation* rotation,
                int64_t position_batch_stride, int64_t position_token_stride, void* stream);

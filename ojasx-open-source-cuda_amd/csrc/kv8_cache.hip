@@ -1235,7 +1235,7 @@ hipError_t launch_kv8_rotate_append(const KvCache& c, const KvRows& k, const KvR
         }
     }
     const int64_t grid = t.key_groups + t.value_groups + extra;
-    if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+    if (grid > kMaxGroups256) return hipErrorInvalidValue;
     by_plan(p, dtype, [&](auto dt, auto vec, auto hold, auto waves) {
         constexpr int DT = decltype(dt)::value, HOLD = decltype(hold)::value, WAVES = decltype(waves)::value;
         constexpr bool VEC = decltype(vec)::value;

@@ -40,11 +40,17 @@ int rotary_plan(RotaryArgs& a, int dtype, int64_t* grid, int heads_of_thread) {
     return v;
 }
 
+bool rotary_fits(RotaryArgs a, int dtype) {
+    int64_t grid;
+    rotary_plan(a, dtype, &grid);
+    return grid <= kMaxGroups256;
+}
+
 hipError_t launch_rotary(RotaryArgs a, int dtype, hipStream_t stream) {
     int64_t grid;
     const int v = rotary_plan(a, dtype, &grid);
     if (grid == 0) return hipSuccess;
-    if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+    if (grid > kMaxGroups256) return hipErrorInvalidValue;
     auto go = [&](auto dt, auto step) {
         constexpr int DT = decltype(dt)::value, V = decltype(step)::value;
         if (a.rot.interleaved)

@@ -279,6 +279,7 @@ hipError_t launch_token_logprobs_bwd(const LogprobGradArgs& a, hipStream_t strea
 size_t beam_select_bytes(const BeamArgs& a);
 size_t beam_select_least_bytes(const BeamArgs& a);  // what a call needs; more lets it split rows
 hipError_t launch_beam_select(const BeamArgs& a, void* ws, size_t ws_bytes, hipStream_t stream);
+bool rotary_fits(RotaryArgs a, int dtype);  // in a launch
 hipError_t launch_rotary(RotaryArgs a, int dtype, hipStream_t stream);
 
 }  // namespace ojx

@@ -203,6 +203,13 @@ ojx::RotaryRows rows_of(const ojx_rotary_rows& r) {
                            (int)r.heads};
 }
 
+int check_rotary_size(const ojx::RotaryArgs& a, int dtype) {
+    if (!ojx::rotary_fits(a, dtype))
+        return api_failf(OJX_EINVAL, "%lld tokens of %d heads pass what a launch holds",
+                        (long long)a.batches * a.tokens, a.q.heads + a.k.heads);
+    return OJX_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -297,7 +304,6 @@ OJX_API int ojx_kv8_rotate_append(int8_t* k_codes, int8_t* v_codes, float* scale
     if (!k || !v || !slots) return api_failf(OJX_EINVAL, "null pointer");
     if (k_token_stride < 0 || k_head_stride < 0 || v_token_stride < 0 || v_head_stride < 0)
         return api_failf(OJX_EINVAL, "negative stride");
-    if (int r = ojx::api_check_device()) return r;
     const ojx::KvCache c = cache_of(k_codes, v_codes, scales, num_blocks, kv_heads, block_size,
                                     head_dim);
     const ojx::KvRows kr{k, k_token_stride, k_head_stride}, vr{v, v_token_stride, v_head_stride};
@@ -308,6 +314,8 @@ OJX_API int ojx_kv8_rotate_append(int8_t* k_codes, int8_t* v_codes, float* scale
     a.batches = 1;
     a.tokens = (int)tokens;
     a.d = (int)head_dim;
+    if (int r = check_rotary_size(a, dtype)) return r;
+    if (int r = ojx::api_check_device()) return r;
     return ojx::api_done(
         ojx::launch_kv8_rotate_append(c, kr, vr, dtype, slots, a, (hipStream_t)stream),
         "kv8 rotate_append launch");
@@ -629,7 +637,6 @@ OJX_API int ojx_rotary(const ojx_rotary_rows* q, const ojx_rotary_rows* k, int64
     if (k)
         if (int r = check_rows(*k, count, dtype)) return r;
     if (count == 0) return OJX_OK;
-    if (int r = ojx::api_check_device()) return r;
     ojx::RotaryArgs a{};
     a.q = rows_of(*q);
     if (k) a.k = rows_of(*k);
@@ -639,6 +646,8 @@ OJX_API int ojx_rotary(const ojx_rotary_rows* q, const ojx_rotary_rows* k, int64
     a.batches = (int)batches;
     a.tokens = (int)tokens;
     a.d = (int)head_dim;
+    if (int r = check_rotary_size(a, dtype)) return r;
+    if (int r = ojx::api_check_device()) return r;
     return ojx::api_done(ojx::launch_rotary(a, dtype, (hipStream_t)stream), "rotary launch");
 }
 

@@ -28,3 +28,25 @@ def test_reordered_rows(rows, children):
     assert size(rows, children, 4, 16, 9, ctypes.byref(n)) == -1 and n.value == 0
     assert lib.ojx_kv8_reorder(P, children, P, rows, P, 4, 4, P, 5, P, 16, 9, *[P] * 7, 1 << 40, None) == -1
     assert size(min(rows, 1 << 25), min(children, 1 << 25), 4, 16, 9, ctypes.byref(n)) == 0
+
+
+def _heads(heads, d, at=256):
+    return N.RotaryRows(x=at, y=at, x_batch=0, x_token=heads * d, x_head=d, y_batch=0, y_token=heads * d,
+                        y_head=d, heads=heads)
+
+
+@pytest.mark.parametrize("dtype,d,pairs,heads,tokens", [
+    (2, 64, 32, 2, 1 << 30),    # 16 bytes of two heads by two a thread: 2^32 threads
+    (1, 33, 16, 4, 1 << 27),    # single elements: 17 chunks, two threads each
+    (0, 128, 64, 64, 1 << 23)])
+def test_rotated_tokens(dtype, d, pairs, heads, tokens):
+    lib = N.lib()
+    rows, few = _heads(heads, d), _heads(heads, d)
+    rot = N.Rotation(256, pairs, 256, False, False, 1.0, False)
+    for batches, t in ((1, tokens), (2, tokens // 2)):
+        assert lib.ojx_rotary(ctypes.byref(rows), None, batches, t, d, dtype, ctypes.byref(rot), 0, 1,
+                              None) == -1
+        assert lib.ojx_rotary(ctypes.byref(few), ctypes.byref(rows), batches, t, d, dtype, ctypes.byref(rot),
+                              0, 1, None) == -1
+    assert lib.ojx_kv8_rotate_append(P, P, P, 4, heads, 16, d, P, heads * d, d, P, heads * d, d, dtype, P,
+                                     tokens, ctypes.byref(rows), ctypes.byref(rot), None) == -1
