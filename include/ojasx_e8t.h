@@ -516,7 +516,7 @@ int ojx_kv8_rotate_append(int8_t* k_codes, int8_t* v_codes, float* scales, int64
  * the order of beams and tokens, where a group has fewer than num others.  A beam whose score is
  * NaN or +inf, or that has such a logit, makes all its candidates NaN, which count as largest; a
  * finished one's logits are not read.  Values are compared in 64 bits: sums are formed partly in 32,
- * and again in 64 where two beams' values are closer than 2^-19.  The workspace holds partial results;
+ * and again in 64 where two beams' values are closer than 2^-18.  The workspace holds partial results;
  * one smaller than asked for, but of groups * beams * (16 + 8 * num) bytes, lowers the split of rows. */
 int ojx_beam_select_workspace_bytes(int64_t groups, int64_t beams, int64_t vocab, int64_t num,
                                     int dtype, size_t* bytes);

@@ -213,12 +213,17 @@ constexpr int kJoinThreads = 512;
 constexpr int kJoinWaves = kJoinThreads / 64;
 constexpr int kJoinBytes = 60 * 1024;  // of LDS for a row's lists and the group's candidates
 // Two values of different beams that are closer than this are compared again with sums in 64 bits.
-// What a beam's sum in the first pass is off by, of itself: its exponentials 2^-23; their exponents'
-// rounding, under 2^-22 for the terms that count (2^-16 of the largest and more); the constant's,
-// 2^-26 of the distance to the largest, under 2^-22; sums of 8 in 32 bits, 7 * 2^-24 at the most.
-// Together under 2^-20 where all of them lean one way; twice that for two beams.  About one call in a
-// hundred of 64 x 8 beams has such a pair (which takes a workgroup some 80 us).
-constexpr double kNear = 0x1p-19;
+// What a beam's sum in the first pass is off by at most, of itself, in units of 2^-20:
+//   0.125  its exponentials, 2^-23 each;
+//   0.70   their exponents' rounding, half a step: 2^-20 ln 2 from 16 to 32 binary places under the lane's
+//          largest so far, less above; a lane's 2^22 terms (of 2^30 logits) that are further under weigh
+//          2^-10 together;
+//   0.30   the constant's error, 2^-26.1 of the terms' mean distance from the largest, which is under
+//          ln 2^30;
+//   0.44   sums of 8 in 32 bits, 7 * 2^-24.
+// Together 1.57, under 2^-19; two beams' may lean apart.  Two calls of 60 of 64 x 8 beams had such a
+// pair (which takes a workgroup some 80 us).
+constexpr double kNear = 0x1p-18;
 
 // fp64 bits in rising order as unsigned; NaN above everything.
 __device__ __forceinline__ uint64_t ordered64(double v) {

@@ -38,7 +38,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num: Optional[int] =
     or a logit of NaN or +inf has NaN continuations, which come first.
 
     Values are compared in 64 bits, so the choice does not hang on the rounding of 32-bit sums (they
-    are formed again in 64 where two beams' values are closer than 2^-19); they are returned rounded
+    are formed again in 64 where two beams' values are closer than 2^-18); they are returned rounded
     to float32.  No gradient passes.
     """
     if num is None:
