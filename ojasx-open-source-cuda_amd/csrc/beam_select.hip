@@ -1,6 +1,7 @@
 // beam_select.hip -- the best continuations of groups of beams: for each group the largest of
 //   value(b, t) = score_b + (x_bt - m_b) - log s_b,   m_b = max x_b,   s_b = sum exp(x_b - m_b),
-// over its beams b and all tokens t of the vocabulary, equal values by rising beam and token.
+// over its beams b and all tokens t of the vocabulary, equal values by rising beam, of one
+// beam by falling logit, then by rising token.
 //
 // Two launches.  The first reads every beam's logits once: sums, and the largest few of each part of
 // a row (logit_rows.h).  The second joins a group: at most `num` logits of a beam can be among the

@@ -28,14 +28,15 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num: Optional[int] =
     """The ``num`` (default: as many as beams; up to 64) best continuations of each group.
 
     ``logits [groups, beams, vocabulary]`` (up to 64 beams, fewer than 2^23 in all groups), ``scores``
-    float32 ``[groups, beams]``: the beams' log probabilities so far.  A continuation's value is its beam's score plus the token's
-    log probability; equal ones come by rising beam and token.  A beam that is ``finished`` (bool
+    float32 ``[groups, beams]``: the beams' log probabilities so far.  A continuation's value is its
+    beam's score plus the token's log probability; equal ones come by rising beam, of one beam by falling logit (beside a score like
+    -1e30 all of a beam's values are one), then by rising token.  A beam that is ``finished`` (bool
     ``[groups, beams]``) goes on by ``pad_id`` alone, at its score, and its logits are not read.
 
     A group's first step, with all beams alike, is chosen from one: scores of -inf for the others.
     Impossible continuations (masked logits of -inf, such scores) are taken, in the order of beams
     and tokens at a score of -inf, where a group has fewer than ``num`` others.  A beam with a score
-    or a logit of NaN or +inf has NaN continuations, which come first.
+    or a logit of NaN or +inf has NaN continuations, which come first, by rising token.
 
     Values are compared in 64 bits, so the choice does not hang on the rounding of 32-bit sums (they
     are formed again in 64 where two beams' values are closer than 2^-18); they are returned rounded
