@@ -508,17 +508,19 @@ int ojx_kv8_rotate_append(int8_t* k_codes, int8_t* v_codes, float* scales, int64
  *
  * The best continuations of each of `groups` groups of `beams` (1..64) beams, fewer than 2^23 beams
  * in all.  logits: rows of vocab elements at stride ld, row g * beams + b of beam b of group g.  A
- * candidate (b, t) has the value scores[g][b] + log softmax(row)[t]; of a beam with finished[g][b] (may be NULL) only
- * (b, pad_id) is possible, with its score.  The `num` (1..64, at most beams * vocab) largest of a
- * group in falling order, equal ones by rising beam, of one beam by falling logit (beside a large score
- * or a far larger logit, values of different logits are one in 64 bits), then by rising token:
+ * candidate (b, t) has the value scores[g][b] + log softmax(row)[t]; of a beam with finished[g][b]
+ * (may be NULL) only (b, pad_id) is possible, with its score.  The `num` (1..64, at most
+ * beams * vocab) largest of a group in falling order, equal ones by rising beam, of one beam by
+ * falling logit (beside a large score or a far larger logit, values of different logits are one in
+ * 64 bits), then by rising token:
  *   out_scores [groups][num], out_parents [groups][num] the row of the beam, out_tokens.
  * Impossible candidates (masked logits of -inf, a score of -inf) have value -inf and are taken, in
  * the order of beams and tokens, where a group has fewer than num others.  A beam whose score is
  * NaN or +inf, or that has such a logit, makes all its candidates NaN, which count as largest, by
- * rising token; a finished one's logits are not read.  Values are compared in 64 bits: sums are formed partly in 32,
- * and again in 64 where two beams' values are closer than 2^-18.  The workspace holds partial results;
- * one smaller than asked for, but of groups * beams * (16 + 8 * num) bytes, lowers the split of rows. */
+ * rising token; a finished one's logits are not read.  Values are compared in 64 bits: sums are formed
+ * partly in 32, and again in 64 where two beams' values are closer than 2^-18 or than 2^-50 of
+ * themselves.  The workspace holds partial results; one smaller than asked for, but of
+ * groups * beams * (16 + 8 * num) bytes, lowers the split of rows. */
 int ojx_beam_select_workspace_bytes(int64_t groups, int64_t beams, int64_t vocab, int64_t num,
                                     int dtype, size_t* bytes);
 int ojx_beam_select(const void* logits, int64_t ld, int64_t groups, int64_t beams, int64_t vocab,

@@ -29,9 +29,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num: Optional[int] =
 
     ``logits [groups, beams, vocabulary]`` (up to 64 beams, fewer than 2^23 in all groups), ``scores``
     float32 ``[groups, beams]``: the beams' log probabilities so far.  A continuation's value is its
-    beam's score plus the token's log probability; equal ones come by rising beam, of one beam by falling logit (beside a score like
-    -1e30 all of a beam's values are one), then by rising token.  A beam that is ``finished`` (bool
-    ``[groups, beams]``) goes on by ``pad_id`` alone, at its score, and its logits are not read.
+    beam's score plus the token's log probability; equal ones come by rising beam, of one beam by
+    falling logit (beside a score like -1e30 all of a beam's values are one), then by rising token.  A
+    beam that is ``finished`` (bool ``[groups, beams]``) goes on by ``pad_id`` alone, at its score, and
+    its logits are not read.
 
     A group's first step, with all beams alike, is chosen from one: scores of -inf for the others.
     Impossible continuations (masked logits of -inf, such scores) are taken, in the order of beams
@@ -39,8 +40,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num: Optional[int] =
     or a logit of NaN or +inf has NaN continuations, which come first, by rising token.
 
     Values are compared in 64 bits, so the choice does not hang on the rounding of 32-bit sums (they
-    are formed again in 64 where two beams' values are closer than 2^-18); they are returned rounded
-    to float32.  No gradient passes.
+    are formed again in 64 where two beams' values are closer than 2^-18, or than 2^-50 of
+    themselves); they are returned rounded to float32.  No gradient passes.
     """
     if num is None:
         num = logits.shape[1]
