@@ -959,11 +959,11 @@ struct RecordedRotary : torch::autograd::Function<RecordedRotary> {
         const double gain = ctx->saved_data["gain"].toDouble();
         const bool interleaved = ctx->saved_data["interleaved"].toBool();
         const bool inverse = !ctx->saved_data["inverse"].toBool();
-        // those that came, in order: queries, keys
+        // those that came for what needs one, in order: queries, keys
         Tensor g[2];
         int n = 0, from[2] = {0, 0};
         for (int i = 0; i < (int)grads.size() && i < 2; ++i)
-            if (grads[i].defined()) {
+            if (grads[i].defined() && ctx->needs_input_grad(i)) {
                 from[n] = i;
                 g[n++] = grads[i];
             }
