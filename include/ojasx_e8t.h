@@ -494,9 +494,11 @@ int ojx_rotary(const ojx_rotary_rows* q, const ojx_rotary_rows* k, int64_t batch
                int64_t position_batch_stride, int64_t position_token_stride, void* stream);
 
 /* ojx_kv8_append of keys that are rotated on the way, in fp32 with no rounding but that to their
- * codes, and the rotation of the tokens' queries (q NULL: none), in one launch where heads and
- * strides are steps of 16 bytes.  Positions are [tokens]; `inverse` has to be 0; of q the strides
- * between batches are not used. */
+ * codes, and the rotation of the tokens' queries (q NULL: none).  Queries whose sizes, strides and
+ * addresses are steps of 16 or 8 bytes go along in the same launch in a small call (2 * tokens *
+ * kv_heads up to 16384), and where keys and values of 16 bits are steps of 16 bytes and a head's block
+ * has up to 2048 elements; others take a launch of their own.  Positions are [tokens]; `inverse` has to be 0; of q the strides between
+ * batches are not used. */
 int ojx_kv8_rotate_append(int8_t* k_codes, int8_t* v_codes, float* scales, int64_t num_blocks,
                           int64_t kv_heads, int64_t block_size, int64_t head_dim, const void* k,
                           int64_t k_token_stride, int64_t k_head_stride, const void* v,
