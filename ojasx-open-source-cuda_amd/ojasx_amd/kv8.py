@@ -9,13 +9,12 @@ Keys and values are held as int8 codes with one float32 scale for each block of 
     o = cache.attention(q, block_tables, p.seq_lens, p.query_starts)
 
 ``plan`` runs on the GPU from the requests' lengths alone, so a step needs no copy to the host;
-``KV8Cache`` is one layer's storage.  Requests that go on from others (beams, several answers to one
+``KV8Cache`` is one layer's storage.  The functions take the storage's tensors, for callers that keep
+them in tensors of their own.  Requests that go on from others (beams, several answers to one
 prompt) or are done share and give back blocks:
 
     r = kv8.reorder(parents, seq_lens, block_tables, free_blocks, num_free, block_size, num_blocks)
     kv8.copy_blocks(caches, r.sources, r.targets)    # what begun blocks hold, in all layers
-  The functions take the storage's tensors, for callers that
-keep them in tensors of their own.
 """
 
 from __future__ import annotations
