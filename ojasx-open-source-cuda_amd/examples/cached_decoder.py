@@ -70,17 +70,11 @@ class Decoder:
         self.up = [linear(hidden, 4 * hidden) for _ in range(layers)]
         self.down = [linear(4 * hidden, hidden) for _ in range(layers)]
         self.head = linear(hidden, vocabulary, rank=8)
-        self.rates = 10000.0 ** (-torch.arange(0, head_dim, 2, device=device) / head_dim)
         self.rotation = rotary.rotation(head_dim, 10000.0, device=device)
 
     def caches(self, num_blocks, block_size):
         return [KV8Cache(num_blocks, self.kv_heads, self.head_dim, block_size,
                          self.embedding.device) for _ in self.qkv]
-
-    def rotate(self, x, positions):
-        a = positions[:, None, None] * self.rates
-        lo, hi = x.float().chunk(2, dim=-1)
-        return torch.cat([lo * a.cos() - hi * a.sin(), hi * a.cos() + lo * a.sin()], -1).to(x.dtype)
 
     def hidden(self, tokens, plan, tables, caches, rotate_on_append=False, **longest):
         """The tokens' last hidden states; their keys and values go into the caches, rotated before
@@ -93,7 +87,7 @@ class Decoder:
             if rotate_on_append:
                 q = cache.rotate_append(q, k, v, plan.positions, plan.slots, self.rotation)
             else:
-                q, k = self.rotate(q, plan.positions), self.rotate(k, plan.positions)
+                q, k = rotary.rotate_qk(q, k, plan.positions, self.rotation)
                 cache.append(k, v, plan.slots)
             o = cache.attention(q, tables, plan.seq_lens, plan.query_starts, **longest)
             x = x + self.out[i](o.reshape(t, -1))
