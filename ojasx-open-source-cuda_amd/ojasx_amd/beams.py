@@ -44,7 +44,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num: Optional[int] =
     themselves); they are returned rounded to float32.  No gradient passes.
     """
     if num is None:
-        num = logits.shape[1]
+        num = logits.shape[1] if logits.dim() == 3 else 1  # (others are refused)
     if not torch.compiler.is_compiling():
         out = N.eager().beam_select(logits, scores, num, finished, pad_id)
         if out is not None:
