@@ -502,8 +502,8 @@ size_t join_bytes(int splits, int beams, int num) {
 }
 
 // Parts of a row: until there are four workgroups for each CU, which run at once, none under a batch
-// for each wave, and as many as the join has room for (512 rows of 128256 whole 47.0 us, in two 45.2,
-// in four 49.7; 4 rows of 32000 whole 16.9, in four 12.6).
+// for each wave, and as many as the join has room for (512 rows of 128256 whole 48.4 us, in two 46.3;
+// 4 rows of 32000 whole 17.2, in two 15.4, in four 13.5).
 int beam_splits(const BeamArgs& a) {
     const int64_t rows = (int64_t)a.groups * a.beams;
     const int64_t most = ((int64_t)a.vocab + kBatch * kGroups - 1) / (kBatch * kGroups);
