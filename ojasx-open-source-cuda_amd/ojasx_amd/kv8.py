@@ -80,9 +80,8 @@ def reorder(parents: torch.Tensor, seq_lens: torch.Tensor, block_tables: torch.T
     """The batch whose row i goes on from row ``parents[i]`` (int64; -1: an empty row) of this one.
 
     There may be more or fewer rows than before (up to 2^25): ``[0, 0, 0, 0]`` makes four beams of a
-    prompt.
-    Children of a row share its full blocks.  Its begun block stays with the first of them, the
-    others get one each from the stack: ``copy_blocks`` copies what it holds, in all layers, before
+    prompt.  Children of a row share its full blocks.  Its begun block stays with the first of them,
+    the others get one each from the stack: ``copy_blocks`` copies what it holds, in all layers, before
     the next append.  Blocks that no new row holds go back on the stack, before any is taken.
 
     All rows that share a block have to be in one call, since blocks are freed by what its rows
